@@ -90,11 +90,26 @@ EXPORTED_SYMBOLS = [
     "aitamd_elementwise",
     "aitamd_elementwise_supported",
     "aitamd_copy_rows",
+    "aitamd_quantize_rows",
+    "aitamd_rotary_embedding",
+    "aitamd_paged_kv_append",
     "aitamd_gemm_workspace_bytes",
     "aitamd_gemm_rcr_ws",
     "aitamd_gemm_rcr_noalloc",
     "aitamd_gemm_noalloc_scratch_bytes",
 ]
+
+
+
+class PagedCache(ctypes.Structure):
+    """aitamd_paged_cache of the C ABI."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v")]
+                + [(n, ctypes.c_int64) for n in ("pages", "page_size", "kv_heads", "head_dim", "k_page_stride", "k_slot_stride",
+                                                 "k_head_stride", "v_page_stride", "v_slot_stride", "v_head_stride")]
+                + [("table", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ("table_pitch", "max_pages")]
+                + [(n, ctypes.c_void_p) for n in ("lengths", "offsets")] + [(n, ctypes.c_int64) for n in ("batch", "tokens")])
+
 
 _lock = threading.Lock()
 _lib: Optional[ctypes.CDLL] = None
@@ -171,6 +186,14 @@ def load() -> ctypes.CDLL:
         lib.aitamd_elementwise_supported.argtypes = [i32]
         lib.aitamd_copy_rows.restype = i32
         lib.aitamd_copy_rows.argtypes = [vp, vp, i64, i64, i64, i64, vp]
+        lib.aitamd_quantize_rows.restype = i32
+        lib.aitamd_quantize_rows.argtypes = [i32, vp, vp, vp, i64, i64, i64, i64, vp]
+        lib.aitamd_rotary_embedding.restype = i32
+        lib.aitamd_rotary_embedding.argtypes = [i32, vp, vp, vp, i32, vp] + [i64] * 13 + [ctypes.c_float, i32, i32, vp]
+        cache = ctypes.POINTER(PagedCache)
+        lib.aitamd_paged_kv_append.restype = i32
+        lib.aitamd_paged_kv_append.argtypes = [i32, cache, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, i64, vp, i64, i64,
+                                               ctypes.c_float, i32, vp]
         _lib = lib
         return lib
 

@@ -463,3 +463,227 @@ def concatenate(tensors, dim: int) -> torch.Tensor:
         _kernels.check(rc, "concatenate")
         start += n
     return out
+
+
+# ---- the attention block of a decoder that is being served ------------------------------------------------------
+# Launches go to the stream that is current on the operands' device; every tensor has to be on that device.
+
+def _operands(*named) -> torch.device:
+    """The device of the tensors in (name, tensor or None, dtypes or None) triples, checked: one GPU, the types given."""
+    device = None
+    for name, t, dtypes in named:
+        if t is None:
+            continue
+        _check(t, name)
+        if dtypes is not None and t.dtype not in dtypes:
+            raise ValueError(f"{name}: dtype {t.dtype} is not {' or '.join(str(d) for d in dtypes)}")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+    return device
+
+
+def _dense_heads(t: torch.Tensor, name: str) -> torch.Tensor:
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    return t
+
+
+def quantize_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
+                  scale: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows of `x` [..., columns] (fp16 / bf16) as 8-bit integers, and one fp32 scale a row ([...]): scale = max|x| / 127 and
+    the whole number nearest to x / scale (of 127 x / max|x|, exactly; ties to even).  A row of zeros has scale 0; a row
+    with an infinity or a NaN has scale NaN and zeros.  `x` may be a 2-D view with row pitch."""
+    device = _operands(("x", x, tuple(_TORCH_DTYPE_ID)), ("out", out, (torch.int8,)), ("scale", scale, (torch.float32,)))
+    if x.dim() < 1:
+        raise ValueError("x must have at least one dimension")
+    lead, columns = x.shape[:-1], x.shape[-1]
+    rows = 1
+    for d in lead:
+        rows *= d
+    ldx = _row_pitch(x, "x") if x.dim() == 2 else columns
+    if x.dim() != 2 and not x.is_contiguous():
+        raise ValueError("x must be contiguous, or 2-D with a contiguous last dimension")
+    if rows > 1 and ldx < columns:
+        raise ValueError("x: rows overlap")
+    if out is None:
+        out = torch.empty(x.shape, dtype=torch.int8, device=device)
+    else:
+        _check_out(out, rows * columns, "x.numel()")
+    if scale is None:
+        scale = torch.empty(lead, dtype=torch.float32, device=device)
+    else:
+        _check_out(scale, rows, "rows")
+    with torch.cuda.device(device):
+        rc = _kernels.load().aitamd_quantize_rows(_TORCH_DTYPE_ID[x.dtype], _p(x), _p(out), _p(scale), rows, columns, ldx, columns,
+                                                  _stream_ptr())
+    _kernels.check(rc, "quantize_rows")
+    return out, scale
+
+
+def rotary_frequencies(rotated: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
+                       original_length: Optional[int] = None, low: float = 1.0, high: float = 32.0,
+                       device="cuda") -> Tuple[torch.Tensor, float]:
+    """(freqs, scale) for `rotary_embedding`: base ** (-2 i / rotated) for pair i, in fp32 on `device`, and the factor of the result.
+
+    `scaling` stretches them for contexts `factor` times as long as the `original_length` that a model was trained on:
+
+    * None: as they are;
+    * "linear": every frequency divided by `factor`;
+    * "base": the base raised to base * factor ** (rotated / (rotated - 2)), which divides the lowest frequency by `factor`
+      and leaves the highest;
+    * "bands": frequencies that turn fewer than `low` times over `original_length` are divided by `factor`, those that turn
+      more than `high` times stay, and in between the share that stays grows evenly with the number of turns;
+    * "yarn": likewise, but the share grows evenly with the pair's index, between the pairs of `high` and of `low` turns
+      (rounded outwards), and the result is scaled by 0.1 ln(factor) + 1."""
+    import math
+
+    if rotated < 2 or rotated % 2:
+        raise ValueError(f"rotated must be an even number of at least 2, got {rotated}")
+    if scaling not in (None, "linear", "base", "bands", "yarn"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    if not base > 1.0 or (scaling is not None and not factor >= 1.0):
+        raise ValueError(f"base {base} must be above 1 and factor {factor} at least 1")
+    if scaling in ("bands", "yarn") and (not original_length or original_length <= 0 or not 0.0 < low < high):
+        raise ValueError(f"{scaling!r} needs original_length and 0 < low < high")
+    if scaling == "base" and rotated == 2:
+        raise ValueError("'base' needs more than one pair")
+    pair = torch.arange(rotated // 2, dtype=torch.float64, device="cpu")
+    if scaling == "base":
+        base = base * factor ** (rotated / (rotated - 2))
+    freqs = base ** (pair * (-2.0 / rotated))
+    scale = 1.0
+    if scaling == "linear":
+        freqs = freqs / factor
+    elif scaling in ("bands", "yarn"):
+        if scaling == "bands":
+            turns = original_length * freqs / (2.0 * math.pi)
+            stays = ((turns - low) / (high - low)).clamp(0.0, 1.0)
+        else:
+            def pair_of(turns):  # the (fractional) pair that turns so often
+                return rotated / 2.0 * math.log(original_length / (turns * 2.0 * math.pi)) / math.log(base)
+
+            first = max(math.floor(pair_of(high)), 0)
+            last = min(math.ceil(pair_of(low)), rotated - 1)
+            stays = 1.0 - ((pair - first) / max(last - first, 0.001)).clamp(0.0, 1.0)
+            scale = 0.1 * math.log(factor) + 1.0
+        freqs = freqs * stays + freqs / factor * (1.0 - stays)
+    return freqs.float().to(device), scale
+
+
+def _check_freqs(freqs: torch.Tensor, head_dim: int) -> int:
+    if freqs.dim() != 1 or not freqs.is_contiguous() or 2 * freqs.numel() > head_dim:
+        raise ValueError(f"freqs must be a contiguous 1-D tensor of at most head_dim / 2 = {head_dim // 2} numbers, got shape {tuple(freqs.shape)}")
+    return 2 * freqs.numel()
+
+
+def rotary_embedding(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, interleaved: bool = False, scale: float = 1.0,
+                     inverse: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotary positions: `x` [tokens, heads, head_dim] or [batch, seq, heads, head_dim] (any strides, contiguous head dims) with the
+    first 2 len(freqs) dims of every head turned by positions * freqs: dims i and len(freqs) + i, or with `interleaved` 2 i and
+    2 i + 1, become scale * (x1 cos - x2 sin, x2 cos + x1 sin); the other dims are handed through.
+
+    `positions`: int32 or int64 [tokens], [batch, seq], or [seq] for every batch entry.  `freqs`: fp32, see `rotary_frequencies`
+    (whose second result is `scale`).  `inverse` turns back: the gradient with respect to `x` of the same call without it.
+    `out` may be `x` itself and must not overlap it otherwise."""
+    device = _operands(("x", x, tuple(_TORCH_DTYPE_ID)), ("positions", positions, (torch.int32, torch.int64)),
+                       ("freqs", freqs, (torch.float32,)), ("out", out, (x.dtype,)))
+    if x.dim() not in (3, 4):
+        raise ValueError("x must be [tokens, heads, head_dim] or [batch, seq, heads, head_dim]")
+    rotated = _check_freqs(freqs, x.shape[-1])
+    if tuple(positions.shape) not in (tuple(x.shape[:-2]), tuple(x.shape[-3:-2])):
+        raise ValueError(f"positions of shape {tuple(positions.shape)} do not fit x of shape {tuple(x.shape)}")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=device)
+    elif out.shape != x.shape:
+        raise ValueError(f"out must be {tuple(x.shape)}, got {tuple(out.shape)}")
+    _dense_heads(x, "x"), _dense_heads(out, "out")
+    flat = x.dim() == 3
+    batch, seq = (1, x.shape[0]) if flat else (x.shape[0], x.shape[1])
+    xs, os = ((0,) + t.stride() if flat else t.stride() for t in (x, out))
+    ps = (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()
+    with torch.cuda.device(device):
+        rc = _kernels.load().aitamd_rotary_embedding(
+            _TORCH_DTYPE_ID[x.dtype], _p(x), _p(out), _p(positions), int(positions.dtype == torch.int64), _p(freqs), batch, seq,
+            x.shape[-2], x.shape[-1], rotated, *xs[:3], *os[:3], *ps, float(scale), int(bool(interleaved)), int(bool(inverse)),
+            _stream_ptr())
+    _kernels.check(rc, "rotary_embedding")
+    return out
+
+
+def _paged_cache(k_cache, v_cache, block_table, lengths, offsets, tokens, head_dim) -> "_kernels.PagedCache":
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+        raise ValueError(f"k_cache and v_cache must be [pages, page_size, kv_heads, head_dim], got {tuple(k_cache.shape)} and "
+                         f"{tuple(v_cache.shape)}")
+    pages, page_size, kv_heads, dim = k_cache.shape
+    if dim != head_dim:
+        raise ValueError(f"head_dim of the cache is {dim}, of the operands {head_dim}")
+    _dense_heads(k_cache, "k_cache"), _dense_heads(v_cache, "v_cache")
+    if lengths.dim() != 1 or not lengths.is_contiguous():
+        raise ValueError("lengths must be a contiguous 1-D tensor")
+    batch = lengths.numel()
+    if block_table.dim() != 2 or block_table.shape[0] != batch or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError(f"block_table must be [batch = {batch}, pages of a sequence] with contiguous rows, got {tuple(block_table.shape)}")
+    if offsets is not None and (offsets.dim() != 1 or not offsets.is_contiguous() or offsets.numel() != batch + 1):
+        raise ValueError(f"offsets must be a contiguous 1-D tensor of batch + 1 = {batch + 1} entries")
+    if offsets is None and tokens != batch:
+        raise ValueError(f"without offsets every sequence has one row: {tokens} rows, {batch} sequences")
+    return _kernels.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, kv_heads, dim, *k_cache.stride()[:3],
+                               *v_cache.stride()[:3], block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+                               lengths.data_ptr(), None if offsets is None else offsets.data_ptr(), batch, tokens)
+
+
+def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                    lengths: torch.Tensor, offsets: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
+                    freqs: Optional[torch.Tensor] = None, interleaved: bool = False, scale: float = 1.0, first_position: int = 0,
+                    q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """One step's keys and values `k`, `v` [tokens, kv_heads, head_dim] into the pages of their sequences, in one launch with the
+    rotation of the keys and of the queries `q` [tokens, heads, head_dim]; returns the rotated queries (None without `q`).
+
+    `k_cache`, `v_cache` [pages, page_size, kv_heads, head_dim], any strides with contiguous head dims: a cache that lies head by
+    head is passed transposed.  `block_table` [batch, n] int32: the pages of each sequence in order; entries outside [0, pages)
+    are no page.  `lengths` [batch] int32: tokens that the sequences have in their pages before the step.  `offsets` [batch + 1]
+    int32: sequence i has the rows offsets[i] to offsets[i + 1]; without it, row i.  Row j of a sequence goes to its place
+    lengths[i] + j, rotated (with `freqs`, as by `rotary_embedding`) for position first_position + lengths[i] + j.
+
+    Rows from offsets[batch] on are left as they were, in `q_out` too; keys and values that no page is there for are dropped.
+    Pages that are written must not be shared between sequences.  `lengths` stay as they are: the attention of the same step
+    takes them as they are too.  `q_out` may be `q`."""
+    types = tuple(_TORCH_DTYPE_ID)
+    device = _operands(("k", k, types), ("v", v, (k.dtype,)), ("k_cache", k_cache, (k.dtype,)), ("v_cache", v_cache, (k.dtype,)),
+                       ("block_table", block_table, (torch.int32,)), ("lengths", lengths, (torch.int32,)),
+                       ("offsets", offsets, (torch.int32,)), ("q", q, (k.dtype,)), ("freqs", freqs, (torch.float32,)),
+                       ("q_out", q_out, (k.dtype,)))
+    if k.dim() != 3 or k.shape != v.shape:
+        raise ValueError(f"k and v must be [tokens, kv_heads, head_dim], got {tuple(k.shape)} and {tuple(v.shape)}")
+    tokens, kv_heads, head_dim = k.shape
+    cache = _paged_cache(k_cache, v_cache, block_table, lengths, offsets, tokens, head_dim)
+    if cache.kv_heads != kv_heads:
+        raise ValueError(f"the cache has {cache.kv_heads} heads, k {kv_heads}")
+    _dense_heads(k, "k"), _dense_heads(v, "v")
+    rotated = 0 if freqs is None else _check_freqs(freqs, head_dim)
+    q_in, heads, qs, os = None, 0, (0, 0), (0, 0)
+    if q is None:
+        if q_out is not None:
+            raise ValueError("q_out without q")
+    else:
+        if q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != head_dim:
+            raise ValueError(f"q must be [{tokens}, heads, {head_dim}], got {tuple(q.shape)}")
+        _dense_heads(q, "q")
+        if q_out is None and rotated == 0:
+            q_out = q  # (nothing is done to it)
+        elif q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        elif q_out.shape != q.shape:
+            raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
+        _dense_heads(q_out, "q_out")
+        if q_out is not q or rotated:
+            q_in, heads, qs, os = q, q.shape[1], q.stride(), q_out.stride()
+    with torch.cuda.device(device):
+        rc = _kernels.load().aitamd_paged_kv_append(
+            _TORCH_DTYPE_ID[k.dtype], cache, _p(k), *k.stride()[:2], _p(v), *v.stride()[:2], _p(q_in), *qs[:2],
+            _p(q_out) if q_in is not None else None, *os[:2], heads, _p(freqs) if rotated else None, rotated, int(first_position),
+            float(scale), int(bool(interleaved)), _stream_ptr())
+    _kernels.check(rc, "paged_kv_append")
+    return q_out

@@ -291,6 +291,56 @@ AITAMD_API int aitamd_elementwise_supported(int func);
 AITAMD_API int aitamd_copy_rows(const void* src, void* dst, int64_t rows, int64_t row_bytes, int64_t src_pitch_bytes,
                                 int64_t dst_pitch_bytes, void* stream);
 
+/* ---- the attention block of a decoder that is being served -----------------
+ * Rows in 8-bit integers and their product, rotary positions, a cache of keys and values in pages and attention over it.
+ * No counterpart in the reference. ---- */
+
+/* Rows of fp16 / bf16 to 8-bit integers: scale[r] = max_c |x[r, c]| / 127 and q[r, c] = the whole number nearest to
+ * 127 x[r, c] / max_c |x[r, c]|, ties to even.  A row of zeros gets scale 0 and zeros; a row that holds an infinity or a
+ * NaN gets scale NaN and zeros.  ldx / ldq: row pitches in elements. */
+AITAMD_API int aitamd_quantize_rows(int dtype, const void* x, int8_t* q, float* scale, int64_t rows, int64_t columns,
+                                    int64_t ldx, int64_t ldq, void* stream);
+
+/* out[b, s, h, :] = x[b, s, h, :] with its first `rotated` dims turned by the position: with n = rotated / 2 and
+ * angle = position(b, s) * freqs[i], the pair (x[i], x[n + i]), or (x[2 i], x[2 i + 1]) with `interleaved`, becomes
+ * scale * (x1 cos - x2 sin, x2 cos + x1 sin); the other dims are handed through.  `inverse` turns the other way, which
+ * is the gradient with respect to x of the forward call (same scale).  Dims of a head are contiguous, x_* and out_* are
+ * strides in elements; positions are int32, or int64 with positions_64, pos_* their strides (0 broadcasts).
+ * freqs: n fp32 numbers on the device.  `out` may be `x` with the same strides; it must not overlap it otherwise. */
+AITAMD_API int aitamd_rotary_embedding(int dtype, const void* x, void* out, const void* positions, int positions_64,
+                                       const float* freqs, int64_t batch, int64_t seq, int64_t heads, int64_t head_dim,
+                                       int64_t rotated, int64_t x_batch, int64_t x_seq, int64_t x_head, int64_t out_batch,
+                                       int64_t out_seq, int64_t out_head, int64_t pos_batch, int64_t pos_seq, float scale,
+                                       int interleaved, int inverse, void* stream);
+
+/* Keys and values of a batch of sequences in pages, and the rows of one step.
+ * Page g holds the keys of `page_size` consecutive tokens of one sequence: token s of the page and head h at
+ * k + g * k_page_stride + s * k_slot_stride + h * k_head_stride (elements; head_dim contiguous ones), values likewise.
+ * Row i of `table` ([batch, max_pages], table_pitch entries apart) lists sequence i's pages in order; entries that are
+ * not in [0, pages) are no page.  lengths[i]: tokens that sequence i has in its pages BEFORE the step.  The step's rows
+ * offsets[i] .. offsets[i + 1] (offsets: [batch + 1], not descending) are sequence i's next tokens; without offsets
+ * sequence i has row i alone, and `tokens`, the number of rows, equals `batch`.  Rows from offsets[batch] on belong to
+ * nobody and are left alone.  table, lengths and offsets are int32 and stay on the device. */
+typedef struct {
+  void *k, *v;
+  int64_t pages, page_size, kv_heads, head_dim;
+  int64_t k_page_stride, k_slot_stride, k_head_stride, v_page_stride, v_slot_stride, v_head_stride;
+  const int32_t* table;
+  int64_t table_pitch, max_pages;
+  const int32_t *lengths, *offsets;
+  int64_t batch, tokens;
+} aitamd_paged_cache;
+
+/* A step's keys and values into the cache: row r of sequence i, the j-th of its rows, goes to token lengths[i] + j, its
+ * key rotated for position first_position + lengths[i] + j (rotated = 0: as it is; otherwise as aitamd_rotary_embedding).
+ * q: null, or the step's queries [tokens, heads, head_dim], rotated likewise into q_out (which may be q with the same
+ * strides).  Keys and values that no page is there for are dropped.  Two rows must not go to the same place. */
+AITAMD_API int aitamd_paged_kv_append(int dtype, const aitamd_paged_cache* cache, const void* k, int64_t k_token,
+                                      int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const void* q,
+                                      int64_t q_token, int64_t q_head, void* q_out, int64_t q_out_token, int64_t q_out_head,
+                                      int64_t heads, const float* freqs, int64_t rotated, int64_t first_position, float scale,
+                                      int interleaved, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

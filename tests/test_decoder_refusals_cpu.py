@@ -1,0 +1,118 @@
+"""Calls that the decoder operators refuse, at the C ABI and in the eager calls; nothing here launches anything."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from aitemplate_amd import _kernels, eager
+
+P = ctypes.c_void_p(64)  # never followed: every call below is refused or has nothing to do
+
+
+def refused(rc, *words):
+    message = _kernels.last_error()
+    assert rc != 0 and all(w in message for w in words), (rc, message)
+
+
+def quantize(dtype=0, x=P, q=P, scale=P, rows=2, columns=64, ldx=64, ldq=64):
+    return _kernels.load().aitamd_quantize_rows(dtype, x, q, scale, rows, columns, ldx, ldq, None)
+
+
+def test_quantize_rows():
+    refused(quantize(dtype=2), "dtype")
+    refused(quantize(rows=-1), "negative")
+    refused(quantize(x=None), "null")
+    refused(quantize(scale=None), "null")
+    refused(quantize(ldx=63), "pitch")
+    refused(quantize(columns=1 << 31, ldx=1 << 31, ldq=1 << 31), "large")
+    assert quantize(rows=0, x=None, q=None, scale=None) == 0
+
+
+def rotary(dtype=0, x=P, out=P, positions=P, freqs=P, batch=1, seq=2, heads=2, head_dim=64, rotated=64):
+    return _kernels.load().aitamd_rotary_embedding(dtype, x, out, positions, 0, freqs, batch, seq, heads, head_dim, rotated, 0, 128, 64, 0,
+                                                   128, 64, 0, 1, 1.0, 0, 0, None)
+
+
+def test_rotary_embedding():
+    refused(rotary(dtype=-1), "dtype")
+    refused(rotary(seq=-1), "negative")
+    refused(rotary(rotated=63), "rotated")
+    refused(rotary(rotated=66), "rotated")
+    refused(rotary(head_dim=1026, rotated=0), "head_dim")
+    refused(rotary(x=None), "null")
+    refused(rotary(freqs=None), "freqs")
+    refused(rotary(batch=1 << 20, seq=1 << 20), "large")
+    refused(rotary(heads=1 << 30), "large")
+    assert rotary(seq=0, x=None, out=None, positions=None) == 0
+
+
+def cache(**changed):
+    c = _kernels.PagedCache(64, 64, 8, 16, 2, 64, 2048, 128, 64, 2048, 128, 64, 64, 4, 4, 64, None, 3, 3)
+    for name, value in changed.items():
+        setattr(c, name, value)
+    return c
+
+
+def append(c=None, dtype=0, k=P, v=P, q=P, q_out=P, heads=4, freqs=P, rotated=64):
+    return _kernels.load().aitamd_paged_kv_append(dtype, c, k, 128, 64, v, 128, 64, q, 256, 64, q_out, 256, 64, heads, freqs, rotated, 0,
+                                                  1.0, 0, None)
+
+
+def test_paged_kv_append():
+    refused(append(None), "null", "cache")
+    refused(append(cache(), dtype=7), "dtype")
+    refused(append(cache(page_size=0)), "page_size")
+    refused(append(cache(batch=-1)), "negative")
+    refused(append(cache(tokens=4)), "without offsets")
+    refused(append(cache(lengths=None)), "null")
+    refused(append(cache(table=None)), "null")
+    refused(append(cache(k=None)), "null")
+    refused(append(cache(max_pages=1 << 28)), "large")
+    refused(append(cache(), k=None), "null")
+    refused(append(cache(), q_out=None), "q_out")
+    refused(append(cache(), freqs=None), "freqs")
+    refused(append(cache(), rotated=65), "rotated")
+    refused(append(cache(), heads=1 << 30), "large")
+    assert append(cache(tokens=0, batch=0)) == 0
+
+
+def test_eager_calls_take_gpu_tensors_only():
+    x = torch.zeros(2, 4, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="GPU"):
+        eager.quantize_rows(x)
+    with pytest.raises(ValueError, match="GPU"):
+        eager.rotary_embedding(x, torch.zeros(2, dtype=torch.int64), torch.zeros(32))
+    with pytest.raises(ValueError, match="GPU"):
+        eager.paged_kv_append(x, x, x, x, x, x)
+
+
+def test_frequencies():
+    freqs, scale = eager.rotary_frequencies(64, device="cpu")
+    want = 10000.0 ** (torch.arange(0, 64, 2, dtype=torch.float64) / -64)
+    assert scale == 1.0 and freqs.dtype == torch.float32 and torch.equal(freqs, want.float())
+    assert torch.equal(eager.rotary_frequencies(64, scaling="linear", factor=4.0, device="cpu")[0], (want / 4).float())
+    # the base raised: the highest frequency stays, the lowest is divided by the factor
+    raised, _ = eager.rotary_frequencies(64, scaling="base", factor=4.0, device="cpu")
+    assert raised[0] == 1.0 and abs(raised[-1].item() / (want[-1].item() / 4) - 1) < 1e-6
+    for scaling in ("bands", "yarn"):
+        got, scale = eager.rotary_frequencies(128, base=500000.0, scaling=scaling, factor=8.0, original_length=8192, low=1.0, high=4.0,
+                                              device="cpu")
+        plain = 500000.0 ** (torch.arange(0, 128, 2, dtype=torch.float64) / -128)
+        turns = 8192 * plain / (2 * math.pi)
+        share = (got.double() / plain - 1 / 8) / (1 - 1 / 8)
+        # (yarn's bounds are whole pairs, rounded outwards)
+        edge = 1e-6
+        assert (share >= -edge).all() and (share <= 1 + edge).all() and (share[1:] <= share[:-1] + edge).all()
+        slow, fast = torch.nonzero(turns < 1.0)[:, 0], torch.nonzero(turns > 4.0)[:, 0]
+        assert (share[slow[1:]].abs() < edge).all() and ((share[fast[:-1]] - 1).abs() < edge).all()
+        assert abs(scale - (1.0 if scaling == "bands" else 0.1 * math.log(8.0) + 1.0)) < 1e-12
+
+
+@pytest.mark.parametrize("arguments", [dict(rotated=63), dict(rotated=0), dict(rotated=64, scaling="other"), dict(rotated=64, base=1.0),
+                                       dict(rotated=64, scaling="linear", factor=0.5), dict(rotated=64, scaling="yarn", factor=2.0),
+                                       dict(rotated=2, scaling="base", factor=2.0),
+                                       dict(rotated=64, scaling="bands", factor=2.0, original_length=2048, low=4.0, high=4.0)])
+def test_frequencies_refused(arguments):
+    with pytest.raises(ValueError):
+        eager.rotary_frequencies(device="cpu", **arguments)
