@@ -93,6 +93,8 @@ EXPORTED_SYMBOLS = [
     "aitamd_quantize_rows",
     "aitamd_rotary_embedding",
     "aitamd_paged_kv_append",
+    "aitamd_prefix_attention_workspace_bytes",
+    "aitamd_prefix_attention",
     "aitamd_gemm_workspace_bytes",
     "aitamd_gemm_rcr_ws",
     "aitamd_gemm_rcr_noalloc",
@@ -194,6 +196,10 @@ def load() -> ctypes.CDLL:
         lib.aitamd_paged_kv_append.restype = i32
         lib.aitamd_paged_kv_append.argtypes = [i32, cache, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, i64, vp, i64, i64,
                                                ctypes.c_float, i32, vp]
+        lib.aitamd_prefix_attention_workspace_bytes.restype = i64
+        lib.aitamd_prefix_attention_workspace_bytes.argtypes = [cache, i64, i64]
+        lib.aitamd_prefix_attention.restype = i32
+        lib.aitamd_prefix_attention.argtypes = [i32, cache, vp, i64, i64, vp, i64, i64, i64, vp, i64, i64, ctypes.c_float, vp, i64, vp]
         _lib = lib
         return lib
 

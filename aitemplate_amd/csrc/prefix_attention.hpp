@@ -1,0 +1,535 @@
+// Attention of a batch's new rows over a paged cache: each row sees a prefix that the whole batch shares and its own
+// sequence's pages up to itself,
+//     out[r] = sum_n exp(c s[r, n]) v[n] / sum_n exp(c s[r, n]),   s[r, n] = q[r] . k[n],
+// taken in one pass over the keys with the running maximum m and sum l of each row.  Parts of the keys that different
+// workgroups take leave (m, l, sum exp(c (s - m)) v) each and are joined afterwards: with M the largest m,
+// the weights are exp(c (m - M)).
+//
+// A wave owns 32 rows (a row is one query head of one token; the query heads of a key head are neighbours) and takes the
+// scores in transposed form, S^T = K Q^T, whose accumulator layout is that of the second product's operand, O^T += V^T P^T:
+// the probabilities never leave the registers.  WR waves stand side by side over rows and share every tile of keys; WK waves
+// take 32 keys of a tile each, for themselves, and join at the end.
+//
+// Keys and values go from their pages straight to LDS: 16 consecutive keys lie in one page (page sizes are multiples of
+// 16), so the page is one scalar per 16 keys and the bounds of its buffer descriptor cut off what is past the last key:
+// what lies there may be anything, and is not read.
+#pragma once
+
+#include "attention_kernel.hpp"
+#include "paged.hpp"
+
+namespace aitamd {
+
+struct PrefixParams {
+  PagedCache cache;
+  const void* q;
+  void* out;
+  float* part_o;   // [slot, token, head, head_dim]
+  float2* part_ml; // [slot, token, head]: c * m and l
+  const int32_t* prefix_table;
+  int64_t q_token, q_head, out_token, out_head;
+  int32_t heads, group, head_dim, prefix;
+  int32_t row_tiles, prefix_slots, own_slots, prefix_wgs;
+  float scale_log2e;
+  Divisor by_group, by_row_tiles, by_own_slots, by_kv_heads;
+};
+
+// HD: head dims, padded; a row takes the next power of two in LDS
+template <int HD_, int WR_, int WK_, int KB_, int NS_, int OCC_>
+struct PagedTile {
+  static constexpr int HD = HD_, WR = WR_, WK = WK_, KB = KB_, NS = NS_, OCC = OCC_;
+  static constexpr int KP = HD <= 64 ? 64 : (HD <= 128 ? 128 : 256);
+  static constexpr int KS = HD / 16, OT = HD / 32;
+  static constexpr int NW = WR * WK, NT = 64 * NW;
+  static constexpr int ROWS = 32 * WR;
+  static constexpr int BN = 32 * KB * WK;     // keys of a tile
+  static constexpr int KPW = BN / NW;         // keys a wave loads
+  static constexpr int GROUPS = KPW / 16;
+  static constexpr int CHUNKS = KP / 8;       // 16-byte pieces of a row in LDS
+  static constexpr int RPL = 64 / CHUNKS;     // rows of a wave-load
+  static constexpr int LPG = 16 / RPL;        // wave-loads of 16 keys
+  static constexpr int LOADS = 2 * GROUPS * LPG;
+  static constexpr int STAGE = 2 * BN * KP;   // elements: K, then V
+  static constexpr int kRing = NS * STAGE * 2;
+  static constexpr int kMerge = WK > 1 ? WK * (16 * OT + 2) * 64 * 4 : 0;
+  static constexpr int kLdsBytes = kRing > kMerge ? kRing : kMerge;
+  // 16-byte piece c of row r lies at piece c ^ swizzle(r).  K: 32 rows' piece at a time; V: see AttnTile::v_swz.
+  static constexpr int k_swz(int row) { return CHUNKS == 8 ? (row / 2) % 8 : row % 16; }
+  static constexpr int v_swz(int row) { return CHUNKS == 8 ? 4 * ((row / 2) % 2) : 4 * (row % 4); }
+  static_assert(WK == 1 || (WR == 1 && KPW == 32 * KB), "waves side by side over keys load what they multiply");
+  static_assert(NS > 1 || WR == 1, "one stage: a wave waits for its own loads only");
+  static_assert(KPW % 16 == 0, "a wave loads whole groups of 16 keys");
+  static_assert(kLdsBytes <= 160 * 1024, "LDS budget");
+};
+
+// What one workgroup does: rows [row0, rows) of the `rows` that start at token `token0`, for key head `kv_head`, over tiles
+// [t_lo, t_hi): the first `prefix_tiles` of all are the prefix's, the others the sequence's own (`own_keys` of them, of which the
+// rows of the j-th token see seen + j).
+struct PagedWork {
+  const int32_t* table;
+  int kv_head, token0, row0, rows, t_lo, t_hi, prefix_tiles, own_keys, seen, slot;
+};
+
+// 16 bytes a lane from memory to LDS: lane l's to dst + 16 l.  (The host pass does not know the builtin, and gives up a function
+// template that holds it where two kernels call it.)
+AITAMD_DEVICE void load_to_lds(__amdgpu_buffer_rsrc_t r, void* dst, uint32_t off) {
+#ifdef __HIP_DEVICE_COMPILE__
+  typedef __attribute__((address_space(3))) void lds_void;
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)dst, 16, off, 0, 0, 0);
+#endif
+}
+
+template <class T, class Tile>
+AITAMD_DEVICE void attend(const PrefixParams& p, const PagedWork& w, unsigned char* smem_raw) {
+  using Tr = ElemTraits<T>;
+  using vec8 = typename Tr::vec8;
+  using vec4 = typename Tr::vec4;
+  typedef __attribute__((address_space(3))) const T lds_T;
+  typedef __attribute__((address_space(3))) const vec8 lds_vec8;
+  typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
+  constexpr int KP = Tile::KP, KS = Tile::KS, OT = Tile::OT, KB = Tile::KB, WR = Tile::WR, WK = Tile::WK, BN = Tile::BN;
+  constexpr int D = Tile::NS - 1;  // tiles asked for ahead
+  static_assert((D > 0 ? D - 1 : 0) * Tile::LOADS <= 63, "vmcnt field is 6 bits");
+  T* const smem = reinterpret_cast<T*>(smem_raw);
+  const PagedCache& c = p.cache;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = WK == 1 ? wave : 0, wk = WK == 1 ? 0 : wave;
+  const int r32 = lane & 31, h = lane >> 5;
+
+  // lane offsets of the loads of 16 keys
+  uint32_t k_off[Tile::LPG], v_off[Tile::LPG];
+#pragma unroll
+  for (int i = 0; i < Tile::LPG; ++i) {
+    const int row = i * Tile::RPL + lane / Tile::CHUNKS, slot = lane % Tile::CHUNKS;
+    const int kc = slot ^ Tile::k_swz(row), vc = slot ^ Tile::v_swz(row);
+    k_off[i] = kc * 8 < p.head_dim ? (uint32_t)row * (uint32_t)(c.k_slot * 2) + (uint32_t)kc * 16u : kOobOffset;
+    v_off[i] = vc * 8 < p.head_dim ? (uint32_t)row * (uint32_t)(c.v_slot * 2) + (uint32_t)vc * 16u : kOobOffset;
+  }
+  // first key of group g of tile t that this wave loads, and the keys there are in the tile's part
+  auto first_key = [&](int t, int g) { return (t < w.prefix_tiles ? t : t - w.prefix_tiles) * BN + wave * Tile::KPW + g * 16; };
+  auto keys_of = [&](int t) { return t < w.prefix_tiles ? p.prefix : w.own_keys; };
+  auto entry = [&](int t, int g) {
+    const int key = first_key(t, g), last = keys_of(t) - 1;
+    scalar_ptr table = (scalar_ptr) reinterpret_cast<uintptr_t>(t < w.prefix_tiles ? p.prefix_table : w.table);
+    return table[quotient(key < last ? key : last, c.by_page)];
+  };
+  int pages[Tile::GROUPS];  // of the tile that is to be loaded next
+  auto fetch_pages = [&](int t) {
+#pragma unroll
+    for (int g = 0; g < Tile::GROUPS; ++g) pages[g] = t < w.t_hi ? entry(t, g) : 0;
+  };
+  auto issue = [&](int t, int stage) {
+#pragma unroll
+    for (int g = 0; g < Tile::GROUPS; ++g) {
+      const int key = first_key(t, g), page = __builtin_amdgcn_readfirstlane(pages[g]);
+      int rows = keys_of(t) - key;
+      rows = rows < 0 || (uint32_t)page >= (uint32_t)c.pages ? 0 : (rows < 16 ? rows : 16);
+      const int within = key - quotient(key, c.by_page) * c.page_size;
+      const T* kb = reinterpret_cast<const T*>(c.k) + page * c.k_page + within * c.k_slot + w.kv_head * c.k_head;
+      const T* vb = reinterpret_cast<const T*>(c.v) + page * c.v_page + within * c.v_slot + w.kv_head * c.v_head;
+      const __amdgpu_buffer_rsrc_t rk = make_rsrc(kb, rows > 0 ? (uint32_t)(((rows - 1) * (int)c.k_slot + p.head_dim) * 2) : 0u);
+      const __amdgpu_buffer_rsrc_t rv = make_rsrc(vb, rows > 0 ? (uint32_t)(((rows - 1) * (int)c.v_slot + p.head_dim) * 2) : 0u);
+      T* dk = smem + stage * Tile::STAGE + (wave * Tile::KPW + g * 16) * KP;
+      T* dv = dk + BN * KP;
+#pragma unroll
+      for (int i = 0; i < Tile::LPG; ++i)
+        load_to_lds(rk, dk + i * 512, k_off[i]);
+#pragma unroll
+      for (int i = 0; i < Tile::LPG; ++i)
+        load_to_lds(rv, dv + i * 512, v_off[i]);
+    }
+  };
+
+  // Q fragments (B operand of S^T = K Q^T): lane (row = r32, k = 16 ks + 8 h + j)
+  const int row = w.row0 + wr * 32 + r32;
+  const int ahead = quotient(row, p.by_group);                   // the row's token, from token0
+  const int head = w.kv_head * p.group + row - ahead * p.group;
+  const int64_t token = w.token0 + ahead;
+  const bool live = row < w.rows;
+  const uint32_t flip = p.scale_log2e < 0.0f ? 0x80008000u : 0u;  // a negative scale changes sides: (-Q) K^T, exact
+  const float cs = fmaxf(__builtin_fabsf(p.scale_log2e), 1e-37f); // (a scale of zero counts as one that makes every score the same)
+  vec8 qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    const int k0 = ks * 16 + h * 8;
+    u32x4 raw = {};
+    if (live && k0 < p.head_dim) raw = load_vec<u32x4>(reinterpret_cast<const T*>(p.q) + token * p.q_token + head * p.q_head + k0);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) raw[d] ^= flip;
+    qf[ks] = __builtin_bit_cast(vec8, raw);
+  }
+  // own keys that this row sees
+  int seen = w.seen + ahead;
+  seen = seen < w.own_keys ? seen : w.own_keys;
+  // ... and that every row of the wave does
+  const int wave_seen = __builtin_amdgcn_readfirstlane(seen);
+
+  // LDS offsets of the fragment reads
+  int k_rd[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) k_rd[ks] = (wk * 32 * KB + r32) * KP + ((2 * ks + h) ^ Tile::k_swz(r32)) * 8;
+  const int tr_row = (lane & 15) >> 2;
+  const int tr_col = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+  int v_rd[OT];
+#pragma unroll
+  for (int ot = 0; ot < OT; ++ot)
+    v_rd[ot] = BN * KP + (wk * 32 * KB + h * 4 + tr_row) * KP + ((ot * 32) ^ (Tile::v_swz(tr_row) * 8)) + tr_col;
+
+  f32x16 oacc[OT];
+#pragma unroll
+  for (int ot = 0; ot < OT; ++ot) oacc[ot] = f32x16{};
+  float m_run = -INFINITY, l_run = 0.0f;
+
+  fetch_pages(w.t_lo);
+#pragma unroll
+  for (int t = 0; t < D; ++t) {
+    if (w.t_lo + t < w.t_hi) issue(w.t_lo + t, t);
+    fetch_pages(w.t_lo + t + 1);
+  }
+  int stage = 0, stage_in = D;
+  for (int t = w.t_lo; t < w.t_hi; ++t) {
+    if constexpr (D == 0) {
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave has read the last tile
+      issue(t, 0);
+      fetch_pages(t + 1);
+      attn_wait_vmcnt<0>();
+    } else {
+      // tile t has landed once only the younger ones are out; past the barrier everybody's part has, and nobody reads the
+      // stage that tile t + D goes to any more
+      if (t + D <= w.t_hi)
+        attn_wait_vmcnt<(D - 1) * Tile::LOADS>();
+      else
+        attn_wait_vmcnt<0>();
+      if constexpr (WR > 1) {
+        __builtin_amdgcn_s_barrier();
+      } else {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+      if (t + D < w.t_hi) {
+        issue(t + D, stage_in);
+        fetch_pages(t + D + 1);
+      }
+    }
+    const T* st = smem + stage * Tile::STAGE;
+    stage = stage + 1 == Tile::NS ? 0 : stage + 1;
+    stage_in = stage_in + 1 == Tile::NS ? 0 : stage_in + 1;
+    const bool shared = t < w.prefix_tiles;
+    const int first = (shared ? t : t - w.prefix_tiles) * BN + wk * 32 * KB;  // this wave's first key
+    const int limit = shared ? p.prefix : seen;                               // keys the row sees
+    const int some = shared ? p.prefix : w.own_keys;
+    if (first >= some) continue;
+    f32x16 s[KB];
+    {
+      lds_T* kb_ptr = (lds_T*)st;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const vec8 kf = *(lds_vec8*)(kb_ptr + kb * 32 * KP + k_rd[ks]);
+          s[kb] = Tr::mfma32(kf, qf[ks], ks == 0 ? f32x16{} : s[kb]);
+        }
+    }
+    float most = -INFINITY;
+    // (wave-uniform) keys that some row does not see
+    if (first + 32 * KB > (shared ? p.prefix : wave_seen)) {
+      const int left = limit - first - h * 4;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (kb * 32 + (e >> 2) * 8 + (e & 3) >= left) s[kb][e] = -INFINITY;
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) most = fmaxf(most, s[kb][e]);
+    most = max_across_halves(most);
+    // The reference point moves only when the row maximum has grown by more than kLazyLog2 binary orders since it was last
+    // taken: until then P may exceed 1 by at most 2^kLazyLog2, harmless in fp32 sums and in P.
+    constexpr float kLazyLog2 = 8.0f;
+    const float m_cand = fmaxf(m_run, most);
+    const float drift = (m_run - m_cand) * cs;  // <= 0; -inf (or NaN for inf - inf) on the first live tile
+    const bool move = !(drift >= -kLazyLog2);
+    const float m_new = move ? m_cand : m_run;
+    const float m_safe = __builtin_isinf(m_new) ? 0.0f : m_new;  // every key so far masked
+    const float alpha = !move ? 1.0f : (__builtin_isinf(m_run) ? 0.0f : __builtin_amdgcn_exp2f(drift));
+    const float mc = -m_safe * cs;
+    l_run *= alpha;
+    vec8 pf[2 * KB];
+#pragma unroll
+    for (int i = 0; i < 2 * KB; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        pf[i][j] = Tr::from_float(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][(i & 1) * 8 + j], cs, mc)));
+      l_run = add_elements(pf[i], l_run);
+    }
+    m_run = m_new;
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+#pragma unroll
+      for (int ot = 0; ot < OT; ++ot)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) oacc[ot][e] *= alpha;
+    }
+    lds_T* vb = (lds_T*)st;
+#pragma unroll
+    for (int i = 0; i < 2 * KB; ++i)
+#pragma unroll
+      for (int ot = 0; ot < OT; ++ot) {
+        const vec4 lo = AttnVec<T>::tr_read(vb + v_rd[ot] + i * 16 * KP);
+        const vec4 hi = AttnVec<T>::tr_read(vb + v_rd[ot] + (i * 16 + 8) * KP);
+        oacc[ot] = Tr::mfma32(join_halves<T>(lo, hi), pf[i], oacc[ot]);
+      }
+  }
+  l_run = sum_across_halves(l_run);
+
+  // ---- waves side by side over keys: each takes some of the dims of all
+  if constexpr (WK > 1) {
+    __syncthreads();
+    constexpr int NVAL = 16 * OT + 2;
+    float* const xch = reinterpret_cast<float*>(smem_raw) + lane;
+#pragma unroll
+    for (int ot = 0; ot < OT; ++ot)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) xch[(wk * NVAL + ot * 16 + e) * 64] = oacc[ot][e];
+    xch[(wk * NVAL + NVAL - 2) * 64] = m_run;
+    xch[(wk * NVAL + NVAL - 1) * 64] = l_run;
+    __syncthreads();
+    float m[WK], m_all = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < WK; ++i) {
+      m[i] = xch[(i * NVAL + NVAL - 2) * 64];
+      m_all = fmaxf(m_all, m[i]);
+    }
+    m_run = m_all;
+    l_run = 0.0f;
+#pragma unroll
+    for (int i = 0; i < WK; ++i) {
+      m[i] = __builtin_isinf(m[i]) ? 0.0f : __builtin_amdgcn_exp2f((m[i] - m_all) * cs);
+      l_run += m[i] * xch[(i * NVAL + NVAL - 1) * 64];
+    }
+#pragma unroll
+    for (int ot = 0; ot < OT; ++ot) {
+      if (ot % WK != wk) continue;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < WK; ++i) sum += m[i] * xch[(i * NVAL + ot * 16 + e) * 64];
+        oacc[ot][e] = sum;
+      }
+    }
+  }
+  if (!live) return;
+  // ---- store: the result, or this part of it
+  if (p.part_o == nullptr) {
+    const float inv = l_run > 0.0f ? 1.0f / l_run : (l_run == 0.0f ? 0.0f : l_run);  // (NaN stays)
+    T* const o = reinterpret_cast<T*>(p.out) + token * p.out_token + head * p.out_head;
+#pragma unroll
+    for (int ot = 0; ot < OT; ++ot) {
+      if (ot % WK != wk) continue;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = ot * 32 + g * 8 + h * 4;
+        vec4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = Tr::from_float(oacc[ot][g * 4 + j] * inv);
+        if (d < p.head_dim) store_vec(o + d, v);
+      }
+    }
+  } else {
+    const int64_t at = ((int64_t)w.slot * c.tokens + token) * p.heads + head;
+    if (wk == 0 && h == 0) p.part_ml[at] = make_float2(l_run == 0.0f ? -INFINITY : m_run * cs, l_run);
+    float* const o = p.part_o + at * p.head_dim;
+#pragma unroll
+    for (int ot = 0; ot < OT; ++ot) {
+      if (ot % WK != wk) continue;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = ot * 32 + g * 8 + h * 4;
+        f32x4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = oacc[ot][g * 4 + j];
+        if (d < p.head_dim) *reinterpret_cast<f32x4*>(o + d) = v;
+      }
+    }
+  }
+}
+
+// Rows of tokens [first, last) of sequence `s`, within the buffers whatever the offsets are
+AITAMD_DEVICE void rows_of(const PagedCache& c, int s, int& first, int& last) {
+  if (c.offsets == nullptr) {
+    first = s;
+    last = s + 1;
+    return;
+  }
+  first = c.offsets[s];
+  last = c.offsets[s + 1];
+  first = first < 0 ? 0 : (first < c.tokens ? first : c.tokens);
+  last = last < first ? first : (last < c.tokens ? last : c.tokens);
+}
+
+// Keys of its own that a sequence's first new row sees, and how many its last one does
+AITAMD_DEVICE void keys_of_sequence(const PagedCache& c, int s, int count, int& seen, int& keys) {
+  // (lengths below zero: a sequence that is not there; its rows see no key of their own until they are counted up)
+  const int len = c.lengths[s];
+  seen = len >= c.most_keys ? c.most_keys : len + 1;
+  const int64_t all = (int64_t)len + count;
+  keys = all <= 0 ? 0 : (all < c.most_keys ? (int)all : c.most_keys);
+}
+
+// [lo, hi) of `tiles` that part `i` of `parts` takes
+AITAMD_DEVICE void part_of(int tiles, int i, int parts, int& lo, int& hi) {
+  lo = (int)((int64_t)tiles * i / parts);
+  hi = (int)((int64_t)tiles * (i + 1) / parts);
+}
+
+// The sequence that the `tile`-th row tile of all sequences belongs to (-1: there are fewer), and which of its tiles that is:
+// 64 sequences at a time, their tiles added up.
+AITAMD_DEVICE int sequence_of_tile(const PrefixParams& p, int tile_rows, int& tile) {
+  const PagedCache& c = p.cache;
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int base = 0; base < c.batch; base += 64) {
+    int mine = 0;
+    if (base + lane < c.batch) {
+      int first, last;
+      rows_of(c, base + lane, first, last);
+      mine = ((last - first) * p.group + tile_rows - 1) / tile_rows;
+    }
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int other = __shfl_up(upto, d);
+      if (lane >= d) upto += other;
+    }
+    const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before + upto <= tile));
+    if (n < 64) {
+      // (lanes past the last sequence have no tiles, so lane n is a sequence)
+      tile = __builtin_amdgcn_readfirstlane(tile - before - (n > 0 ? __shfl(upto, n - 1) : 0));
+      return __builtin_amdgcn_readfirstlane(base + n);
+    }
+    before += __shfl(upto, 63);
+  }
+  return -1;
+}
+
+// Few rows a sequence (decoding).  The first workgroups take the prefix, for the rows of all sequences together; the others
+// one sequence's own keys each.
+template <class T, class Shared, class Own>
+__global__ void __launch_bounds__(Shared::NT, Shared::OCC) prefix_decode_kernel(const PrefixParams p) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
+  static_assert(Shared::NT == Own::NT, "one workgroup size");
+  const PagedCache& c = p.cache;
+  PagedWork w{};
+  if ((int)blockIdx.x < p.prefix_wgs) {
+    // consecutive workgroups go to the 8 XCDs in turn: the row tiles of one (head, part) follow each other on one of them
+    const int id = blockIdx.x, xcd = id % kNumXcd, local = id / kNumXcd;
+    const int nth = quotient(local, p.by_row_tiles), tile = local - nth * p.row_tiles;
+    const int pair = nth * kNumXcd + xcd;
+    const int part = quotient(pair, p.by_kv_heads);
+    w.kv_head = pair - part * c.kv_heads;
+    if (part >= p.prefix_slots) return;
+    int tokens = c.tokens;
+    if (c.offsets != nullptr) {
+      const int last = c.offsets[c.batch];
+      tokens = last < 0 ? 0 : (last < tokens ? last : tokens);
+    }
+    w.rows = tokens * p.group;
+    w.row0 = tile * Shared::ROWS;
+    if (w.row0 >= w.rows) return;
+    w.prefix_tiles = (p.prefix + Shared::BN - 1) / Shared::BN;
+    part_of(w.prefix_tiles, part, p.prefix_slots, w.t_lo, w.t_hi);
+    w.slot = part;
+    attend<T, Shared>(p, w, smem_raw);
+  } else {
+    const int id = blockIdx.x - p.prefix_wgs;
+    const int pair = quotient(id, p.by_own_slots), part = id - pair * p.own_slots;
+    int s = quotient(pair, p.by_kv_heads);
+    w.kv_head = pair - s * c.kv_heads;
+    int first, last, tile = 0;
+    if (c.offsets != nullptr || p.group > Own::ROWS) {
+      tile = s;
+      s = sequence_of_tile(p, Own::ROWS, tile);
+      if (s < 0) return;
+    }
+    rows_of(c, s, first, last);
+    w.token0 = first;
+    w.rows = (last - first) * p.group;
+    w.row0 = tile * Own::ROWS;
+    if (w.row0 >= w.rows) return;
+    keys_of_sequence(c, s, last - first, w.seen, w.own_keys);
+    w.table = c.table + s * c.table_pitch;
+    part_of((w.own_keys + Own::BN - 1) / Own::BN, part, p.own_slots, w.t_lo, w.t_hi);
+    w.slot = p.prefix_slots + part;
+    attend<T, Own>(p, w, smem_raw);
+  }
+}
+
+// Many rows a sequence (prompts, pieces of them).  A workgroup takes a tile of one sequence's rows over the prefix and then over
+// the sequence's own keys.
+template <class T, class Tile>
+__global__ void __launch_bounds__(Tile::NT, Tile::OCC) prefix_prompt_kernel(const PrefixParams p) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
+  const PagedCache& c = p.cache;
+  // an XCD takes a run of (key head, part) pairs' row tiles, so that the keys they share come to one L2
+  const int per_xcd = gridDim.x / kNumXcd;
+  const int id = (int)(blockIdx.x % kNumXcd) * per_xcd + (int)(blockIdx.x / kNumXcd);
+  const int pair = quotient(id, p.by_row_tiles);
+  int tile = id - pair * p.row_tiles, first, last;
+  const int part = quotient(pair, p.by_kv_heads);
+  if (part >= p.own_slots) return;
+  const int s = sequence_of_tile(p, Tile::ROWS, tile);
+  if (s < 0) return;
+  PagedWork w{};
+  rows_of(c, s, first, last);
+  w.kv_head = pair - part * c.kv_heads;
+  w.token0 = first;
+  w.rows = (last - first) * p.group;
+  w.row0 = tile * Tile::ROWS;
+  if (w.row0 >= w.rows) return;
+  keys_of_sequence(c, s, last - first, w.seen, w.own_keys);
+  // (no further than the tile's last row sees)
+  const int last_row = w.row0 + Tile::ROWS < w.rows ? w.row0 + Tile::ROWS - 1 : w.rows - 1;
+  const int last_seen = w.seen + quotient(last_row, p.by_group);
+  w.own_keys = last_seen < 0 ? 0 : (last_seen < w.own_keys ? last_seen : w.own_keys);
+  w.table = c.table + s * c.table_pitch;
+  w.prefix_tiles = (p.prefix + Tile::BN - 1) / Tile::BN;
+  part_of(w.prefix_tiles + (w.own_keys + Tile::BN - 1) / Tile::BN, part, p.own_slots, w.t_lo, w.t_hi);
+  w.slot = part;
+  attend<T, Tile>(p, w, smem_raw);
+}
+
+// The parts of a row joined: D / 4 lanes a row
+template <class T>
+__global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p, int slots, int lanes, Divisor by_lanes, Divisor by_heads) {
+  const int64_t rows = (int64_t)p.cache.tokens * p.heads;
+  const int per_wg = quotient(256, by_lanes);
+  const int in_wg = quotient(threadIdx.x, by_lanes), d = (threadIdx.x - in_wg * lanes) * 4;
+  const int64_t row = (int64_t)blockIdx.x * per_wg + in_wg;
+  if (in_wg >= per_wg || row >= rows) return;
+  const int64_t token = row / p.heads;
+  if (p.cache.offsets != nullptr && (token < p.cache.offsets[0] || token >= p.cache.offsets[p.cache.batch])) return;
+  float most = -INFINITY;
+  for (int s = 0; s < slots; ++s) most = fmaxf(most, p.part_ml[s * rows + row].x);
+  f32x4 o = {};
+  float sum = 0.0f;
+  for (int s = 0; s < slots; ++s) {
+    const float2 ml = p.part_ml[s * rows + row];
+    if (ml.y == 0.0f) continue;  // (no key)
+    const float weight = __builtin_amdgcn_exp2f(ml.x - most);
+    sum += ml.y * weight;
+    const f32x4 v = *reinterpret_cast<const f32x4*>(p.part_o + (s * rows + row) * p.head_dim + d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] += v[j] * weight;
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+  typename ElemTraits<T>::vec4 y;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) y[j] = ElemTraits<T>::from_float(o[j] * inv);
+  store_vec(reinterpret_cast<T*>(p.out) + token * p.out_token + (row - token * p.heads) * p.out_head + d, y);
+}
+
+}  // namespace aitamd

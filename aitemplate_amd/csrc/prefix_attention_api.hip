@@ -1,0 +1,201 @@
+// C ABI launcher of aitamd_prefix_attention.
+#include <mutex>
+
+#include "../../include/aitemplate_amd_kernels.h"
+#include "device.hpp"
+#include "errors.hpp"
+#include "paged.hpp"
+#include "prefix_attention.hpp"
+
+namespace aitamd {
+namespace {
+
+constexpr int kMaxDevices = 64;
+
+template <int HD>
+struct Tiles {
+  using Shared = PagedTile<HD, 4, 1, 2, 2, HD <= 128 ? 2 : 1>;  // the prefix for the rows of all sequences
+  using Own = PagedTile<HD, 1, 4, 1, 1, HD <= 128 ? 2 : 1>;     // few rows over their own keys
+  using Prompt = PagedTile<HD, 4, 1, 2, 2, HD <= 128 ? 2 : 1>;  // many rows of one sequence
+};
+
+// How a call is dealt to workgroups (the same for every head dim: the tiles have the same rows and about the same keys)
+struct Plan {
+  bool prompts;         // tiles of one sequence's rows over prefix and own keys; otherwise the prefix for all rows together
+  int64_t row_tiles;    // of the prefix (decoding), of all sequences at most (prompts)
+  int64_t own_tiles;    // decoding: row tiles of all sequences at most
+  int64_t prefix_slots, own_slots;
+  int64_t slots() const { return prefix_slots + own_slots; }
+};
+
+// parts that `items` workgroups' keys are split into: about two workgroups a CU, of at least `least` keys each
+int64_t parts(int64_t items, int64_t keys, int64_t least, int cus) {
+  int64_t n = 2 * (int64_t)cus / (items > 0 ? items : 1);
+  if (n > keys / least) n = keys / least;
+  return n < 1 ? 1 : (n > 64 ? 64 : n);
+}
+
+Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t prefix, int64_t most_keys, bool ragged, int cus) {
+  const int64_t group = heads / kv_heads, rows = tokens * group;
+  Plan n{};
+  n.prompts = ragged && rows > 32 * batch;
+  const int64_t tile = n.prompts ? 128 : 32;
+  // (every sequence has one tile that is not full at most)
+  const int64_t at_most = ragged ? rows / tile + batch : batch * ((group + tile - 1) / tile);
+  if (n.prompts) {
+    n.row_tiles = at_most;
+    n.own_slots = parts(rows / tile * kv_heads, prefix + most_keys, 256, cus);
+  } else {
+    n.own_tiles = at_most;
+    n.row_tiles = (rows + 127) / 128;
+    n.prefix_slots = prefix > 0 ? parts(n.row_tiles * kv_heads, prefix, 256, cus) : 0;
+    n.own_slots = parts(at_most * kv_heads, most_keys, 256, cus);
+  }
+  return n;
+}
+
+struct LdsOptIn {
+  std::once_flag once[kMaxDevices];
+  hipError_t err[kMaxDevices];
+  hipError_t operator()(const void* kernel, int bytes) {
+    int dev = 0;
+    const hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    dev %= kMaxDevices;
+    std::call_once(once[dev], [&] { err[dev] = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+    return err[dev];
+  }
+};
+
+template <class T, int HD>
+hipError_t launch_attention(PrefixParams& p, const Plan& plan, int64_t wgs, hipStream_t stream) {
+  using S = typename Tiles<HD>::Shared;
+  using O = typename Tiles<HD>::Own;
+  using M = typename Tiles<HD>::Prompt;
+  constexpr int kDecodeLds = S::kLdsBytes > O::kLdsBytes ? S::kLdsBytes : O::kLdsBytes;
+  static LdsOptIn decode_opt_in, prompt_opt_in;
+  if (plan.prompts) {
+    auto kernel = prefix_prompt_kernel<T, M>;
+    const hipError_t e = prompt_opt_in(reinterpret_cast<const void*>(kernel), M::kLdsBytes);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(M::NT), M::kLdsBytes, stream, p);
+  } else {
+    auto kernel = prefix_decode_kernel<T, S, O>;
+    const hipError_t e = decode_opt_in(reinterpret_cast<const void*>(kernel), kDecodeLds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(S::NT), kDecodeLds, stream, p);
+  }
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t launch_all(PrefixParams& p, const Plan& plan, int64_t wgs, hipStream_t stream) {
+  const int d = p.head_dim;
+  hipError_t e = d <= 64 ? launch_attention<T, 64>(p, plan, wgs, stream)
+      : d <= 96          ? launch_attention<T, 96>(p, plan, wgs, stream)
+      : d <= 128         ? launch_attention<T, 128>(p, plan, wgs, stream)
+                         : launch_attention<T, 256>(p, plan, wgs, stream);
+  if (e != hipSuccess || plan.slots() == 1) return e;
+  const int lanes = (d + 3) / 4, per_wg = 256 / lanes;
+  const int64_t rows = (int64_t)p.cache.tokens * p.heads;
+  hipLaunchKernelGGL(prefix_join_kernel<T>, dim3((unsigned)((rows + per_wg - 1) / per_wg)), dim3(256), 0, stream, p, (int)plan.slots(), lanes,
+                     make_divisor(lanes), make_divisor(p.heads));
+  return hipGetLastError();
+}
+
+// the sizes that both entry points take
+int check_sizes(const char* who, const aitamd_paged_cache* cache, int64_t heads, int64_t prefix_length, PagedCache* c) {
+  if (paged_cache(who, cache, 16, c)) return 1;
+  if (heads < 0 || prefix_length < 0) return fail("%s: negative dimension", who);
+  if (cache->kv_heads == 0 ? heads != 0 : heads % cache->kv_heads != 0)
+    return fail("%s: %lld query heads are not a multiple of %lld key heads", who, (long long)heads, (long long)cache->kv_heads);
+  if (cache->head_dim > 256 || cache->head_dim % 8 != 0)
+    return fail("%s: head_dim %lld: a multiple of 8 up to 256 is wanted", who, (long long)cache->head_dim);
+  if (heads > 0 && (cache->tokens > 0x3fffffffll / heads || cache->batch > 0x3fffffffll / heads)) return fail("%s: dimension too large", who);
+  if (prefix_length > 0x3fffffffll || c->most_keys > 0x3fffffff) return fail("%s: too many keys", who);
+  return 0;
+}
+
+int64_t workspace_of(const Plan& plan, int64_t tokens, int64_t heads, int64_t head_dim) {
+  if (plan.slots() <= 1) return 0;
+  const int64_t rows = plan.slots() * tokens * heads;
+  return rows * head_dim * 4 + rows * 8;
+}
+
+}  // namespace
+}  // namespace aitamd
+
+using namespace aitamd;
+
+extern "C" int64_t aitamd_prefix_attention_workspace_bytes(const aitamd_paged_cache* cache, int64_t heads, int64_t prefix_length) {
+  const char* who = "aitamd_prefix_attention_workspace_bytes";
+  PagedCache c{};
+  if (check_sizes(who, cache, heads, prefix_length, &c)) return -1;
+  if (cache->tokens == 0 || heads == 0 || cache->batch == 0 || cache->head_dim == 0) return 0;
+  const Plan plan = make_plan(cache->tokens, cache->batch, heads, cache->kv_heads, prefix_length, c.most_keys, cache->offsets != nullptr,
+                              current_device_cus());
+  return workspace_of(plan, cache->tokens, heads, cache->head_dim);
+}
+
+extern "C" int aitamd_prefix_attention(int dtype, const aitamd_paged_cache* cache, const void* q, int64_t q_token, int64_t q_head, void* out,
+                                       int64_t out_token, int64_t out_head, int64_t heads, const int32_t* prefix_table,
+                                       int64_t prefix_pages, int64_t prefix_length, float scale, void* workspace, int64_t workspace_bytes,
+                                       void* stream) {
+  const char* who = "aitamd_prefix_attention";
+  if (dtype != AITAMD_F16 && dtype != AITAMD_BF16) return fail("%s: bad dtype %d", who, dtype);
+  PrefixParams p{};
+  if (check_sizes(who, cache, heads, prefix_length, &p.cache)) return 1;
+  const int64_t tokens = cache->tokens, batch = cache->batch, kv_heads = cache->kv_heads, head_dim = cache->head_dim;
+  if (tokens == 0 || heads == 0 || batch == 0 || head_dim == 0) return 0;
+  if (!q || !out || !cache->k || !cache->v || (prefix_length > 0 && !prefix_table)) return fail("%s: null pointer", who);
+  if (prefix_pages < 0 || prefix_length > prefix_pages * cache->page_size)
+    return fail("%s: a prefix of %lld keys does not lie in %lld pages of %lld", who, (long long)prefix_length, (long long)prefix_pages,
+                (long long)cache->page_size);
+  // 16-byte loads, and 16 keys of a page within 32-bit offsets, one after the other
+  if ((reinterpret_cast<uintptr_t>(cache->k) | reinterpret_cast<uintptr_t>(cache->v)) & 15)
+    return fail("%s: the cache has to be 16-byte aligned", who);
+  const int64_t strides[6] = {cache->k_page_stride, cache->k_slot_stride, cache->k_head_stride,
+                              cache->v_page_stride, cache->v_slot_stride, cache->v_head_stride};
+  for (int i = 0; i < 6; ++i)
+    if (strides[i] % 8 != 0) return fail("%s: the cache's strides have to be multiples of 8 elements", who);
+  for (int i = 1; i < 6; i += 3)
+    if (strides[i] < head_dim || strides[i] > (1 << 24))
+      return fail("%s: a token's stride of %lld in the cache: head_dim = %lld to 2^24 is wanted", who, (long long)strides[i], (long long)head_dim);
+  const Plan plan = make_plan(tokens, batch, heads, kv_heads, prefix_length, p.cache.most_keys, cache->offsets != nullptr, current_device_cus());
+  const int64_t need = workspace_of(plan, tokens, heads, head_dim);
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need)
+      return fail("%s: %lld bytes of workspace are wanted, got %lld", who, (long long)need, (long long)(workspace ? workspace_bytes : 0));
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail("%s: the workspace has to be 16-byte aligned", who);
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + plan.slots() * tokens * heads * head_dim);
+  }
+  p.q = q;
+  p.out = out;
+  p.prefix_table = prefix_table;
+  p.q_token = q_token, p.q_head = q_head, p.out_token = out_token, p.out_head = out_head;
+  p.heads = (int32_t)heads;
+  p.group = (int32_t)(heads / kv_heads);
+  p.head_dim = (int32_t)head_dim;
+  p.prefix = (int32_t)prefix_length;
+  p.row_tiles = (int32_t)plan.row_tiles;
+  p.prefix_slots = (int32_t)plan.prefix_slots;
+  p.own_slots = (int32_t)plan.own_slots;
+  p.scale_log2e = scale * 1.4426950408889634f;
+  p.by_group = make_divisor(p.group);
+  p.by_row_tiles = make_divisor(plan.row_tiles > 0 ? plan.row_tiles : 1);
+  p.by_own_slots = make_divisor(plan.own_slots);
+  p.by_kv_heads = make_divisor(kv_heads);
+  int64_t wgs;
+  if (plan.prompts) {
+    wgs = (plan.row_tiles * kv_heads * plan.own_slots + kNumXcd - 1) / kNumXcd * kNumXcd;
+  } else {
+    p.prefix_wgs = (int32_t)((plan.prefix_slots * kv_heads + kNumXcd - 1) / kNumXcd * kNumXcd * plan.row_tiles);
+    wgs = p.prefix_wgs + plan.own_tiles * kv_heads * plan.own_slots;
+  }
+  if (wgs > 0x7fffffffll || tokens * heads > 0x7fffffffll) return fail("%s: dimension too large", who);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const hipError_t e = dtype == AITAMD_F16 ? launch_all<f16>(p, plan, wgs, s) : launch_all<bf16>(p, plan, wgs, s);
+  if (e != hipSuccess) return fail("%s: launch failed: %s", who, hipGetErrorString(e));
+  return 0;
+}

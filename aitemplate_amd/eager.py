@@ -687,3 +687,61 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
             float(scale), int(bool(interleaved)), _stream_ptr())
     _kernels.check(rc, "paged_kv_append")
     return q_out
+
+
+def prefix_attention_workspace_bytes(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                                     lengths: torch.Tensor, offsets: Optional[torch.Tensor] = None, prefix_length: int = 0) -> int:
+    """Bytes of scratch memory that `prefix_attention` of these arguments needs."""
+    cache = _paged_cache(k_cache, v_cache, block_table, lengths, offsets, q.shape[0], q.shape[-1])
+    with torch.cuda.device(q.device):
+        need = int(_kernels.load().aitamd_prefix_attention_workspace_bytes(cache, q.shape[1], int(prefix_length)))
+    if need < 0:
+        raise RuntimeError(f"prefix_attention failed: {_kernels.last_error()}")
+    return need
+
+
+def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+                     offsets: Optional[torch.Tensor] = None, prefix_table: Optional[torch.Tensor] = None, prefix_length: int = 0,
+                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                     workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one step's queries `q` [tokens, heads, head_dim] over a paged cache, after `paged_kv_append` of the same step
+    (`k_cache`, `v_cache`, `block_table`, `lengths`, `offsets` as there, `lengths` still those from before the step).
+
+    Every row sees the first `prefix_length` keys of the pages `prefix_table` [n] int32, which the whole batch shares and which
+    are read once for all of its rows, and those of its own sequence's pages up to itself.  Query head h reads key head
+    h // (heads / kv_heads).  `scale` is head_dim ** -0.5 unless given.  Rows that see no key are zeros; rows of `out` from
+    offsets[batch] on are left as they were.
+
+    page_size has to be a multiple of 16, head_dim one of 8 up to 256.  `workspace`: a buffer from `new_workspace` of
+    `prefix_attention_workspace_bytes`, allocated for the call otherwise; calls that may overlap in time need one each."""
+    device = _operands(("q", q, tuple(_TORCH_DTYPE_ID)), ("k_cache", k_cache, (q.dtype,)), ("v_cache", v_cache, (q.dtype,)),
+                       ("block_table", block_table, (torch.int32,)), ("lengths", lengths, (torch.int32,)),
+                       ("offsets", offsets, (torch.int32,)), ("prefix_table", prefix_table, (torch.int32,)), ("out", out, (q.dtype,)),
+                       ("workspace", workspace, (torch.uint8,)))
+    if q.dim() != 3:
+        raise ValueError(f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
+    tokens, heads, head_dim = q.shape
+    cache = _paged_cache(k_cache, v_cache, block_table, lengths, offsets, tokens, head_dim)
+    if prefix_table is not None and (prefix_table.dim() != 1 or not prefix_table.is_contiguous()):
+        raise ValueError("prefix_table must be a contiguous 1-D tensor")
+    if prefix_length and prefix_table is None:
+        raise ValueError("prefix_length without prefix_table")
+    _dense_heads(q, "q")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    elif out.shape != q.shape:
+        raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    _dense_heads(out, "out")
+    lib = _kernels.load()
+    with torch.cuda.device(device):
+        if workspace is None:
+            need = int(lib.aitamd_prefix_attention_workspace_bytes(cache, heads, int(prefix_length)))
+            workspace = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+        elif not workspace.is_contiguous():
+            raise ValueError("workspace must be a contiguous uint8 GPU tensor (see new_workspace)")
+        rc = lib.aitamd_prefix_attention(
+            _TORCH_DTYPE_ID[q.dtype], cache, _p(q), *q.stride()[:2], _p(out), *out.stride()[:2], heads, _p(prefix_table),
+            0 if prefix_table is None else prefix_table.numel(), int(prefix_length),
+            float(head_dim ** -0.5 if scale is None else scale), _p(workspace), 0 if workspace is None else workspace.numel(), _stream_ptr())
+    _kernels.check(rc, "prefix_attention")
+    return out

@@ -341,6 +341,26 @@ AITAMD_API int aitamd_paged_kv_append(int dtype, const aitamd_paged_cache* cache
                                       int64_t heads, const float* freqs, int64_t rotated, int64_t first_position, float scale,
                                       int interleaved, void* stream);
 
+/* Attention of a step's rows over the cache.  Row r, the j-th of sequence i, sees the first `prefix_length` keys of the
+ * pages in prefix_table ([prefix_pages] entries), which the whole batch shares, and the first lengths[i] + j + 1 of its
+ * sequence's own pages (the step's keys are in the cache already, lengths are those from before the step; none where
+ * that is not positive, all that the table has room for where there are not as many):
+ *   out[r, h, :] = sum_n softmax_n(scale * q[r, h, :] . k[n, h / (heads / kv_heads), :]) v[n, h / (heads / kv_heads), :]
+ * Rows that see no key are written as zeros.  A table entry that a row's keys need and that is not in [0, pages) counts as
+ * a page of zeros.  What lies behind a sequence's last key is not read.  Keys that only later rows of the step see do not
+ * count for a row, as long as their values are finite.
+ * page_size a multiple of 16; head_dim a multiple of 8 up to 256; heads a multiple of kv_heads; cache 16-byte aligned, its
+ * strides multiples of 8; q and out with contiguous head dims, their strides in elements.
+ * workspace: device memory, 16-byte aligned, of aitamd_prefix_attention_workspace_bytes() bytes (may be null where that is
+ * 0; -1: the sizes are refused); nothing in it has to be set and nothing is kept in it.  Launches that overlap in time
+ * need one each. */
+AITAMD_API int64_t aitamd_prefix_attention_workspace_bytes(const aitamd_paged_cache* cache, int64_t heads,
+                                                           int64_t prefix_length);
+AITAMD_API int aitamd_prefix_attention(int dtype, const aitamd_paged_cache* cache, const void* q, int64_t q_token,
+                                       int64_t q_head, void* out, int64_t out_token, int64_t out_head, int64_t heads,
+                                       const int32_t* prefix_table, int64_t prefix_pages, int64_t prefix_length, float scale,
+                                       void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -77,6 +77,46 @@ def test_paged_kv_append():
     assert append(cache(tokens=0, batch=0)) == 0
 
 
+def attention(c=None, dtype=0, q=P, out=P, heads=4, table=P, pages=4, length=0, workspace=None, nbytes=0):
+    return _kernels.load().aitamd_prefix_attention(dtype, c, q, 256, 64, out, 256, 64, heads, table, pages, length, 0.125, workspace,
+                                                   nbytes, None)
+
+
+def workspace_bytes(c, heads=4, length=0):
+    return _kernels.load().aitamd_prefix_attention_workspace_bytes(c, heads, length)
+
+
+def test_prefix_attention():
+    refused(attention(None), "null", "cache")
+    refused(attention(cache(), dtype=2), "dtype")
+    refused(attention(cache(page_size=24)), "page_size", "16")
+    refused(attention(cache(head_dim=60)), "head_dim")
+    refused(attention(cache(head_dim=264)), "head_dim")
+    refused(attention(cache(), heads=5), "multiple")
+    refused(attention(cache(kv_heads=0)), "multiple")
+    refused(attention(cache(), q=None), "null")
+    refused(attention(cache(v=None)), "null")
+    refused(attention(cache(), length=5, table=None), "null")
+    refused(attention(cache(), length=65), "prefix", "pages")
+    refused(attention(cache(), length=-1), "negative")
+    refused(attention(cache(k=72)), "aligned")
+    refused(attention(cache(v_head_stride=65)), "strides")
+    refused(attention(cache(k_slot_stride=56)), "stride")
+    refused(attention(cache(k_slot_stride=1 << 25)), "stride")
+    refused(attention(cache(tokens=2)), "without offsets")
+    refused(attention(cache(max_pages=1 << 27)), "large")
+    refused(attention(cache(max_pages=1 << 26)), "keys")
+    refused(attention(cache(tokens=1 << 29, offsets=64)), "large")
+    refused(attention(cache(), length=50), "workspace")
+    refused(attention(cache(), length=50, workspace=P, nbytes=workspace_bytes(cache(), length=50) - 1), "workspace")
+    refused(attention(cache(), length=50, workspace=ctypes.c_void_p(72), nbytes=1 << 30), "workspace", "aligned")
+    assert attention(cache(tokens=0, batch=0)) == 0
+    assert workspace_bytes(cache(page_size=8)) == -1 and "page_size" in _kernels.last_error()
+    assert workspace_bytes(cache(tokens=0, batch=0)) == 0
+    # one part of a row: (m, l) and head_dim numbers in 32 bits
+    assert workspace_bytes(cache(), length=16) % (3 * 4 * (64 * 4 + 8)) == 0 < workspace_bytes(cache(), length=16)
+
+
 def test_eager_calls_take_gpu_tensors_only():
     x = torch.zeros(2, 4, 64, dtype=torch.float16)
     with pytest.raises(ValueError, match="GPU"):
@@ -85,6 +125,8 @@ def test_eager_calls_take_gpu_tensors_only():
         eager.rotary_embedding(x, torch.zeros(2, dtype=torch.int64), torch.zeros(32))
     with pytest.raises(ValueError, match="GPU"):
         eager.paged_kv_append(x, x, x, x, x, x)
+    with pytest.raises(ValueError, match="GPU"):
+        eager.prefix_attention(x, x, x, x, x)
 
 
 def test_frequencies():
