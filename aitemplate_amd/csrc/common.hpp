@@ -65,6 +65,29 @@ struct ElemTraits<bf16> {
   static AITAMD_DEVICE float to_float_plus(bf16 v, float one, float c) { (void)one; return (float)v + c; }
 };
 
+// Two 8-bit integers, the 2-byte element of their products: K, pitches and slabs are counted in pairs, so that tiles, loads
+// and LDS layouts are those of the 16-bit types.  A matrix instruction takes 16 bytes a lane of either, in the same time;
+// which byte of the 16 is which k does not matter, as both operands have them alike.  The accumulators are 32-bit integers,
+// kept in registers declared as floats.
+struct i8x2 {
+  uint16_t pair;
+};
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
+template <>
+struct ElemTraits<i8x2> {
+  typedef uint16_t vec8 __attribute__((ext_vector_type(8)));
+  typedef uint16_t vec4 __attribute__((ext_vector_type(4)));
+  static AITAMD_DEVICE f32x16 mfma32(vec8 a, vec8 b, f32x16 c) {
+    return __builtin_bit_cast(f32x16, __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b),
+                                                                            __builtin_bit_cast(i32x16, c), 0, 0, 0));
+  }
+  static AITAMD_DEVICE f32x4 mfma16(vec8 a, vec8 b, f32x4 c) {
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b),
+                                                                           __builtin_bit_cast(i32x4, c), 0, 0, 0));
+  }
+};
+
 // LDS transpose read: 4 x 16-bit per lane, gathered across the 16 lanes of a block.
 // __restrict__ is for the compiler's wait insertion: without alias information on the read it assumes that any
 // direct-to-LDS load on its way may be the data and drains them all (s_waitcnt vmcnt(0)) in front of every read, which

@@ -108,6 +108,25 @@ AITAMD_DEF_EPI(kEpiAdd, false, 1, 1, acc + d0)
 
 #undef AITAMD_DEF_EPI
 
+// Operands of 8-bit integers: the accumulators are 32-bit integers, and the expression is of each of them times the scales of
+// its row and of its column (GemmParams::scale_a, scale_b); results and bias are OUT.
+template <int ID, class OUT>
+struct ScaledEpilogue : Epilogue<ID> {};
+
+// the type of results, bias and residuals, and whether the accumulators are integers that are scaled first
+template <class T, class Epi>
+struct OutElem {
+  using type = T;
+  static constexpr bool scaled = false;
+};
+template <class T, int ID, class OUT>
+struct OutElem<T, ScaledEpilogue<ID, OUT>> {
+  using type = OUT;
+  static constexpr bool scaled = true;
+};
+// an integer accumulator that stands in a float's place, scaled (the one rounding to 32 bits that it does not have in 24)
+AITAMD_DEVICE float scaled_sum(float acc, float scale) { return (float)__float_as_int(acc) * scale; }
+
 // Epi applied to xb = acc (+ bias, already added) and the residuals as stored, with the residual adds that lead
 // the expression folded into the residuals' conversion (see LEAD above).
 template <class Epi, class T>

@@ -16,7 +16,7 @@
 #error "compile with -DAITAMD_EPI=<id>"
 #endif
 #ifndef AITAMD_DT
-#error "compile with -DAITAMD_DT=<0|1>"
+#error "compile with -DAITAMD_DT=<0|1|2|3>"
 #endif
 
 namespace aitamd {
@@ -25,22 +25,36 @@ namespace {
 #if AITAMD_DT == 0
 using Elem = f16;
 #define AITAMD_DT_NAME "f16"
-#else
+#elif AITAMD_DT == 1
 using Elem = bf16;
 #define AITAMD_DT_NAME "bf16"
+#else
+// 8-bit integers, results in fp16 or bf16
+using Elem = i8x2;
+#if AITAMD_DT == 2
+using Scaled = f16;
+#define AITAMD_DT_NAME "i8_f16"
+#else
+using Scaled = bf16;
+#define AITAMD_DT_NAME "i8_bf16"
+#endif
 #endif
 
 constexpr int kMaxDevices = 64;
 
+#if AITAMD_DT < 2
 using Epi = Epilogue<AITAMD_EPI>;
+#else
+using Epi = ScaledEpilogue<AITAMD_EPI, Scaled>;
+#endif
 
 // Kernels with the permuted store exist for the two epilogues the permuting ops use.
-constexpr bool kHasPermutedStore = AITAMD_EPI == kEpiNone || AITAMD_EPI == kEpiBias;
+constexpr bool kHasPermutedStore = AITAMD_DT < 2 && (AITAMD_EPI == kEpiNone || AITAMD_EPI == kEpiBias);
 
 // Kernels for operands that are not K-contiguous exist on the direct-to-LDS tiles whose edges allow it, for the
 // epilogues the reference's ops in those layouts use: plain and residual-add in all of rrr, ccr, crr; bias for
 // rrr with the permuted store (gemm_rrr_bias_permute).  kLayoutBits: bit L set when layout L is compiled.
-constexpr int kLayoutBits = (AITAMD_EPI == kEpiNone || AITAMD_EPI == kEpiAdd) ? 0xf : (AITAMD_EPI == kEpiBias ? 0x3 : 0x1);
+constexpr int kLayoutBits = AITAMD_DT >= 2 ? 0x1 : (AITAMD_EPI == kEpiNone || AITAMD_EPI == kEpiAdd) ? 0xf : (AITAMD_EPI == kEpiBias ? 0x3 : 0x1);
 constexpr bool kLayoutsArePermuted = AITAMD_EPI == kEpiBias;  // the bias kernels of the other layouts store permuted
 
 constexpr int kShortK = 4;
@@ -236,12 +250,16 @@ hipError_t launch_tile(const GemmParams& p, hipStream_t stream) {
     if (p.layout != 0) return hipErrorInvalidValue;
     const bool multiplies = four_waves_multiply(Tile::KVEC, p.K) && (p.N & 7) == 0;
     if (multiplies && four_waves_store(p)) return launch_kernel<Tile, false>(p, stream);
+#if AITAMD_DT >= 2
+    return launch_tile<GemmTileDma<128, 128, 64, 2, 4, 4, 1, 1, 32, 0, Tile::KTAIL != 0 ? 2 : 0>>(p, stream);
+#else
     // Asked for by name with others: an instance that takes the same operands, any K and any output.  For a permuted store
     // the one of the same matrix instructions, whose results are those of the plain store.
     if (multiplies && p.perm_on) return launch_tile<GemmTileDma<32, 32, 128, 2, 2, 4, 2, 0, 16, 0, Tile::KTAIL != 0 ? 2 : 0>>(p, stream);
     using Other = std::conditional_t<Tile::KTAIL != 0, GemmTileDma<128, 128, 64, 2, 4, 4, 1, 1, 32, 0, 2>,
                                      GemmTilePersist<256, 256, 32, 2, 4, 4, 16, 256>>;
     return launch_tile<Other>(p, stream);
+#endif
   } else {
   if (p.layout != 0) {
     constexpr int mask = LayoutMask<Tile>::value;
@@ -317,9 +335,22 @@ const GemmAlgo kAlgos[] = {
 #define AITAMD_GEMM_TILE_DMA(BM, BN, BK, WM, WN, NS, OCC, PIPE, MT, AUX, ...)                                        \
   entry<GemmTileDma<BM, BN, BK, WM, WN, NS, OCC, PIPE, MT, AUX>, 1, OCC>(                                            \
       AITAMD_NAME #BM "x" #BN "x" #BK "_w" #WM "x" #WN "_dma" #NS "_o" #OCC "_p" #PIPE "_m" #MT "_c" #AUX, {__VA_ARGS__}),
+#if AITAMD_DT >= 2
+// (the persistent kernel on eight waves rounds its accumulators to the operands' type ahead of the epilogue; rows at any
+// byte have a kernel of their own)
+#define AITAMD_GEMM_TILE_PERSIST(...)
+#define AITAMD_GEMM_TILE_STAGED(...)
+#define AITAMD_GEMM_ROWS_ELEM(...)
+#else
 #define AITAMD_GEMM_TILE_PERSIST(BM, BN, BK, WM, WN, NS, MT, LBM, ...)                                               \
   entry<GemmTilePersist<BM, BN, BK, WM, WN, NS, MT, LBM>, 2, 1>(                                                     \
       AITAMD_NAME #BM "x" #BN "x" #BK "_w" #WM "x" #WN "_persist" #NS "_m" #MT, {__VA_ARGS__}),
+#define AITAMD_GEMM_TILE_STAGED(BM, BN, BK, WM, WN, NS, OCC, MT, ...)                                                \
+  entry<GemmTileDma<BM, BN, BK, WM, WN, NS, OCC, 0, MT, 0, 4>, 0, OCC>(                                              \
+      AITAMD_NAME #BM "x" #BN "x" #BK "_w" #WM "x" #WN "_reg" #NS "_o" #OCC "_v1", {__VA_ARGS__}),
+#define AITAMD_GEMM_ROWS_ELEM(NW, NS, ...)                                                                           \
+  entry<GemmTileRows<NW, NS, 1>, 8, 2>(AITAMD_NAME "rows16x16_n" #NW "_s" #NS "_v1", {__VA_ARGS__}),
+#endif
 #define AITAMD_GEMM_TILE_WIDE(MI, NI, BM, BN, ...)                                                                   \
   entry<GemmTileWide<MI, NI, 0>, 16, 1>(AITAMD_NAME #BM "x" #BN "x32_w2x2_wide", {__VA_ARGS__}),
 #define AITAMD_GEMM_TILE_WIDE_K2(MI, NI, BM, BN, ...)                                                                \
@@ -333,13 +364,8 @@ const GemmAlgo kAlgos[] = {
 #define AITAMD_GEMM_TILE_DMA_SPLITK_K2(BM, BN, BK, WM, WN, NS, OCC, PIPE, MT, ...)                                   \
   entry<GemmTileDma<BM, BN, BK, WM, WN, NS, OCC, PIPE, MT, 0, 3>, 4, OCC>(                                           \
       AITAMD_NAME #BM "x" #BN "x" #BK "_w" #WM "x" #WN "_dma" #NS "_o" #OCC "_p" #PIPE "_m" #MT "_k2_splitk", {__VA_ARGS__}),
-#define AITAMD_GEMM_TILE_STAGED(BM, BN, BK, WM, WN, NS, OCC, MT, ...)                                                \
-  entry<GemmTileDma<BM, BN, BK, WM, WN, NS, OCC, 0, MT, 0, 4>, 0, OCC>(                                              \
-      AITAMD_NAME #BM "x" #BN "x" #BK "_w" #WM "x" #WN "_reg" #NS "_o" #OCC "_v1", {__VA_ARGS__}),
 #define AITAMD_GEMM_ROWS(NW, NS, ...)                                                                                \
   entry<GemmTileRows<NW, NS, 0>, 8, 2>(AITAMD_NAME "rows16x16_n" #NW "_s" #NS "_k2", {__VA_ARGS__}),
-#define AITAMD_GEMM_ROWS_ELEM(NW, NS, ...)                                                                           \
-  entry<GemmTileRows<NW, NS, 1>, 8, 2>(AITAMD_NAME "rows16x16_n" #NW "_s" #NS "_v1", {__VA_ARGS__}),
 #include "gemm_tiles.inc"
 #undef AITAMD_GEMM_TILE_DMA
 #undef AITAMD_GEMM_TILE_PERSIST

@@ -60,6 +60,8 @@ struct GemmParams {
   void* ws;
   int64_t ws_bytes;
   int32_t split_k;  // number of workgroups that share a tile along K (set by the launcher of a split-K instance)
+  // Operands of 8-bit integers (i8x2: K, lda, ldb, sa and sb count pairs): fp32 scales of the M rows of A and of the N rows of B
+  const float *scale_a, *scale_b;
 };
 
 // The launcher's part of the walk over tiles of bm x bn.  xcd_shift: see GemmParams; -1 for the grouped walk.

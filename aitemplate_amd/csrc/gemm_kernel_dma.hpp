@@ -186,6 +186,9 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
   using Tr = ElemTraits<T>;
   using vec8 = typename Tr::vec8;
   using vec4 = typename Tr::vec4;
+  using Out = typename OutElem<T, Epi>::type;
+  using out8 = typename ElemTraits<Out>::vec8;
+  constexpr bool kScaled = OutElem<T, Epi>::scaled;
   constexpr bool A_T = (LAYOUT & 2) != 0, B_T = (LAYOUT & 1) != 0;
   static_assert(LAYOUT == 0 || Tile::kTransposable, "this tile has no transposed-operand form");
   using Mfma = MfmaOp<T, Tile::MT>;
@@ -354,23 +357,39 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
     const int rd_row = lane / LANES_PER_ROW;
     const int rd_col = (lane % LANES_PER_ROW) * 8;
     const int n_epi = n0 + wn * Tile::WTN + rd_col;          // the lane's 8 columns, the same in every pass
-    const T* D0b = Epi::kNumD >= 1 ? reinterpret_cast<const T*>(p.d0) + (int64_t)batch * p.sd : nullptr;
-    const T* D1b = Epi::kNumD >= 2 ? reinterpret_cast<const T*>(p.d1) + (int64_t)batch * p.sd : nullptr;
-    const T* bias = reinterpret_cast<const T*>(p.bias);
+    const Out* D0b = Epi::kNumD >= 1 ? reinterpret_cast<const Out*>(p.d0) + (int64_t)batch * p.sd : nullptr;
+    const Out* D1b = Epi::kNumD >= 2 ? reinterpret_cast<const Out*>(p.d1) + (int64_t)batch * p.sd : nullptr;
+    const Out* bias = reinterpret_cast<const Out*>(p.bias);
     auto epi_row = [&](int mi, int ps) { return m0 + wm * Tile::WTM + mi * MT + ps * ROWS_PER_PASS + rd_row; };
     constexpr bool kEarlyBias = Epi::kHasBias && BM * BN <= 128 * 128;
     constexpr int kEarlyD = MI * PASSES <= 2 ? MI * PASSES : 0;
-    vec8 bias_v = {}, d0_e[kEarlyD > 0 ? kEarlyD : 1] = {}, d1_e[kEarlyD > 0 ? kEarlyD : 1] = {};
+    out8 bias_v = {}, d0_e[kEarlyD > 0 ? kEarlyD : 1] = {}, d1_e[kEarlyD > 0 ? kEarlyD : 1] = {};
     if constexpr (kEarlyBias) {
-      if (n_epi + 8 <= p.N) bias_v = load_vec<vec8>(bias + n_epi);
+      if (n_epi + 8 <= p.N) bias_v = load_vec<out8>(bias + n_epi);
+    }
+    // scales of the lane's columns and of its rows, likewise
+    constexpr bool kEarlyScale = kScaled && BM * BN <= 128 * 128;
+    f32x4 scale_lo = {}, scale_hi = {};
+    float scale_e[kEarlyD > 0 ? kEarlyD : 1] = {};
+    auto load_scales = [&]() {
+      if (n_epi + 8 <= p.N) {
+        scale_lo = load_vec<f32x4>(p.scale_b + n_epi);
+        scale_hi = load_vec<f32x4>(p.scale_b + n_epi + 4);
+      }
+    };
+    if constexpr (kEarlyScale) {
+      load_scales();
+#pragma unroll
+      for (int i = 0; i < kEarlyD; ++i)
+        if (epi_row(i / PASSES, i % PASSES) < p.M) scale_e[i] = p.scale_a[epi_row(i / PASSES, i % PASSES)];
     }
     if constexpr (kEarlyD > 0 && Epi::kNumD >= 1) {
 #pragma unroll
       for (int i = 0; i < kEarlyD; ++i) {
         const int m = epi_row(i / PASSES, i % PASSES);
         if (m < p.M && n_epi + 8 <= p.N) {
-          d0_e[i] = load_vec<vec8>(D0b + (int64_t)m * p.ldd + n_epi);
-          if constexpr (Epi::kNumD >= 2) d1_e[i] = load_vec<vec8>(D1b + (int64_t)m * p.ldd + n_epi);
+          d0_e[i] = load_vec<out8>(D0b + (int64_t)m * p.ldd + n_epi);
+          if constexpr (Epi::kNumD >= 2) d1_e[i] = load_vec<out8>(D1b + (int64_t)m * p.ldd + n_epi);
         }
       }
     }
@@ -678,7 +697,11 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
               const f32x4 v4 = __builtin_bit_cast(f32x4, part[s][q]);
               constexpr int Q = ACC_N / 4;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) acc[q / Q / NI][q / Q % NI][q % Q * 4 + j] += v4[j];
+              for (int j = 0; j < 4; ++j) {
+                acc_t& sum = acc[q / Q / NI][q / Q % NI];
+                const float was = sum[q % Q * 4 + j];
+                sum[q % Q * 4 + j] = kScaled ? __int_as_float(__float_as_int(was) + __float_as_int(v4[j])) : was + v4[j];
+              }
             }
         }
         // the counter is zero again for the next launch (which starts after this kernel has ended)
@@ -688,8 +711,9 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
     }
 
     // ---------------- epilogue: acc -> LDS (fp32, per-wave strip) -> 16-byte stores --------
-    T* Cb = reinterpret_cast<T*>(p.c) + out_batch_offset(p, batch);
+    Out* Cb = reinterpret_cast<Out*>(p.c) + out_batch_offset(p, batch);
     const __amdgpu_buffer_rsrc_t rc = make_rsrc(Cb, kStoreRecords);
+    if constexpr (kScaled && !kEarlyScale) load_scales();
     // vector form for the lanes whose 8 columns lie inside the row, at any alignment (element by element, an odd N
     // took 29 us where its even neighbour took 18: 2000 x 3001 x 500); the streaming stores need even pitches and a
     // dword-aligned pointer
@@ -730,22 +754,29 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
           float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
           const int64_t c_idx = out_index<PERM>(p, m, n);
           const int64_t d_idx = (int64_t)m * p.ldd + n;
+          float scale = 1.0f;  // (of the row)
+          if constexpr (kScaled) scale = kEarlyScale && kEarlyD > 0 ? scale_e[kEarlyD > 0 ? mi * PASSES + ps : 0] : p.scale_a[m];
           if (vec_ok && n + 8 <= p.N) {
-            vec8 bv = bias_v, d0v = d0_e[kEarlyD > 0 ? mi * PASSES + ps : 0], d1v = d1_e[kEarlyD > 0 ? mi * PASSES + ps : 0];
-            if constexpr (Epi::kHasBias && !kEarlyBias) bv = load_vec<vec8>(bias + n);
-            if constexpr (Epi::kNumD >= 1 && kEarlyD == 0) d0v = load_vec<vec8>(D0b + d_idx);
-            if constexpr (Epi::kNumD >= 2 && kEarlyD == 0) d1v = load_vec<vec8>(D1b + d_idx);
-            const vec8 o = epilogue8<Epi, T>(v, bv, d0v, d1v, one);
+            if constexpr (kScaled) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = scaled_sum(v[j], scale * (j < 4 ? scale_lo[j & 3] : scale_hi[j & 3]));
+            }
+            out8 bv = bias_v, d0v = d0_e[kEarlyD > 0 ? mi * PASSES + ps : 0], d1v = d1_e[kEarlyD > 0 ? mi * PASSES + ps : 0];
+            if constexpr (Epi::kHasBias && !kEarlyBias) bv = load_vec<out8>(bias + n);
+            if constexpr (Epi::kNumD >= 1 && kEarlyD == 0) d0v = load_vec<out8>(D0b + d_idx);
+            if constexpr (Epi::kNumD >= 2 && kEarlyD == 0) d1v = load_vec<out8>(D1b + d_idx);
+            const out8 o = epilogue8<Epi, Out>(v, bv, d0v, d1v, one);
             store_out(Cb, c_idx, o, stream_ok, rc);
           } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               if (n + j < p.N) {
-                T bj = T{}, d0j = T{}, d1j = T{};
+                Out bj = Out{}, d0j = Out{}, d1j = Out{};
+                if constexpr (kScaled) v[j] = scaled_sum(v[j], scale * p.scale_b[n + j]);
                 if constexpr (Epi::kHasBias) bj = bias[n + j];
                 if constexpr (Epi::kNumD >= 1) d0j = D0b[d_idx + j];
                 if constexpr (Epi::kNumD >= 2) d1j = D1b[d_idx + j];
-                Cb[out_index<PERM>(p, m, n + j)] = epilogue1<Epi, T>(v[j], bj, d0j, d1j, one);
+                Cb[out_index<PERM>(p, m, n + j)] = epilogue1<Epi, Out>(v[j], bj, d0j, d1j, one);
               }
             }
           }

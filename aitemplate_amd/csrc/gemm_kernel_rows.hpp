@@ -61,6 +61,8 @@ template <class T, class Tile, class Epi, bool PERM = false>
 __global__ void __launch_bounds__(Tile::NT) gemm_rcr_rows_kernel(const GemmParams p) {
   using Tr = ElemTraits<T>;
   using vec8 = typename Tr::vec8;
+  using Out = typename OutElem<T, Epi>::type;
+  constexpr bool kScaled = OutElem<T, Epi>::scaled;
   constexpr int NW = Tile::NW, NS = Tile::NS, BM = Tile::BM, BN = Tile::BN, GROUP = Tile::GROUP, ELEM = Tile::ELEM;
   typedef __attribute__((address_space(3))) void lds_void;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
@@ -119,7 +121,8 @@ __global__ void __launch_bounds__(Tile::NT) gemm_rcr_rows_kernel(const GemmParam
   // a thread's outputs, and what the epilogue reads for them
   const int out_m = tid / BN, out_n = tid % BN;
   constexpr int OUTS = (BM * BN + Tile::NT - 1) / Tile::NT;
-  T bias_v[OUTS], d0_v[OUTS], d1_v[OUTS];
+  Out bias_v[OUTS], d0_v[OUTS], d1_v[OUTS];
+  float scale_v[OUTS];
   // (for an output that does not exist, of one that does: a branch around the loads would wait for them)
   auto read_epilogue = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -127,10 +130,11 @@ __global__ void __launch_bounds__(Tile::NT) gemm_rcr_rows_kernel(const GemmParam
       const int m = out_m + o * (Tile::NT / BN);
       const int mc = m0 + (m < rows_a ? m : rows_a - 1), nc = n0 + (out_n < rows_b ? out_n : rows_b - 1);
       const int64_t at = (int64_t)batch * p.sd + (int64_t)mc * p.ldd + nc;
-      bias_v[o] = d0_v[o] = d1_v[o] = T{};
-      if constexpr (Epi::kHasBias) bias_v[o] = reinterpret_cast<const T*>(p.bias)[nc];
-      if constexpr (Epi::kNumD >= 1) d0_v[o] = reinterpret_cast<const T*>(p.d0)[at];
-      if constexpr (Epi::kNumD >= 2) d1_v[o] = reinterpret_cast<const T*>(p.d1)[at];
+      bias_v[o] = d0_v[o] = d1_v[o] = Out{};
+      if constexpr (Epi::kHasBias) bias_v[o] = reinterpret_cast<const Out*>(p.bias)[nc];
+      if constexpr (Epi::kNumD >= 1) d0_v[o] = reinterpret_cast<const Out*>(p.d0)[at];
+      if constexpr (Epi::kNumD >= 2) d1_v[o] = reinterpret_cast<const Out*>(p.d1)[at];
+      if constexpr (kScaled) scale_v[o] = p.scale_a[mc] * p.scale_b[nc];
     }
   };
 
@@ -228,15 +232,19 @@ __global__ void __launch_bounds__(Tile::NT) gemm_rcr_rows_kernel(const GemmParam
   __syncthreads();
   float one = 1.0f;
   asm volatile("" : "+s"(one));  // (opaque to the optimizer: see to_float_plus)
-  T* Cb = reinterpret_cast<T*>(p.c) + out_batch_offset(p, batch);
+  Out* Cb = reinterpret_cast<Out*>(p.c) + out_batch_offset(p, batch);
 #pragma unroll
   for (int o = 0; o < OUTS; ++o) {
     const int m = out_m + o * (Tile::NT / BN);
     if (m < rows_a && out_n < rows_b) {
       float v = 0.0f;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) v += part[(w * BM + m) * BN + out_n];
-      Cb[out_index<PERM>(p, m0 + m, n0 + out_n)] = epilogue1<Epi, T>(v, bias_v[o], d0_v[o], d1_v[o], one);
+      for (int w = 0; w < NW; ++w) {
+        const float more = part[(w * BM + m) * BN + out_n];
+        v = kScaled ? __int_as_float(__float_as_int(v) + __float_as_int(more)) : v + more;
+      }
+      if constexpr (kScaled) v = scaled_sum(v, scale_v[o]);
+      Cb[out_index<PERM>(p, m0 + m, n0 + out_n)] = epilogue1<Epi, Out>(v, bias_v[o], d0_v[o], d1_v[o], one);
     }
   }
 }

@@ -69,6 +69,17 @@ struct AccMfma<bf16> {
   }
 };
 
+template <>
+struct AccMfma<i8x2> {
+  using vec8 = ElemTraits<i8x2>::vec8;
+  static AITAMD_DEVICE void run(f32x4& c, vec8 a, vec8 b) {
+    asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  }
+  static AITAMD_DEVICE void first(f32x4& c, vec8 a, vec8 b) {
+    asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, 0" : "=a"(c) : "v"(a), "v"(b));
+  }
+};
+
 template <int OFF, class V>
 AITAMD_DEVICE void lds_read16(V& v, uint32_t addr) {
   asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "n"(OFF));
@@ -93,6 +104,9 @@ template <class T, class Tile, class Epi>
 __global__ void __launch_bounds__(Tile::NT, 1) gemm_rcr_wide_kernel(const GemmParams p) {
   using Tr = ElemTraits<T>;
   using vec8 = typename Tr::vec8;
+  using Out = typename OutElem<T, Epi>::type;
+  using out8 = typename ElemTraits<Out>::vec8;
+  constexpr bool kScaled = OutElem<T, Epi>::scaled;
   constexpr int BM = Tile::BM, BN = Tile::BN, NS = Tile::NS, MI = Tile::MI, NI = Tile::NI;
   constexpr int STAGE = Tile::STAGE_BYTES;
   constexpr int SLAB = Tile::BK * 2;  // bytes of a row in one slab
@@ -254,7 +268,7 @@ __global__ void __launch_bounds__(Tile::NT, 1) gemm_rcr_wide_kernel(const GemmPa
   };
 
   // ---- epilogue ----
-  const T* bias = reinterpret_cast<const T*>(p.bias);
+  const Out* bias = reinterpret_cast<const Out*>(p.bias);
   // A lane's place in a pair of column blocks and in a pair of row blocks (the last column block of an odd number)
   const int sub = fq & 1, half8 = (fq >> 1) * 8;
   constexpr int NP = NI / 2;
@@ -279,17 +293,26 @@ __global__ void __launch_bounds__(Tile::NT, 1) gemm_rcr_wide_kernel(const GemmPa
     const int n_w = c.n0 + wn * Tile::WTN;
     const int rows_left = p.M - m_w;
     const uint32_t rows_valid = rows_left <= 0 ? 0u : (uint32_t)(rows_left < Tile::WTM ? rows_left : Tile::WTM);
-    T* Cw = reinterpret_cast<T*>(p.c) + out_batch_offset(p, c.batch) + (int64_t)m_w * p.ldc + n_w;
+    Out* Cw = reinterpret_cast<Out*>(p.c) + out_batch_offset(p, c.batch) + (int64_t)m_w * p.ldc + n_w;
     const __amdgpu_buffer_rsrc_t rc = make_rsrc(Cw, rows_valid * (uint32_t)p.ldc * 2u);
     __amdgpu_buffer_rsrc_t rd0 = rc, rd1 = rc;
     if constexpr (Epi::kNumD >= 1)
-      rd0 = make_rsrc(reinterpret_cast<const T*>(p.d0) + (int64_t)c.batch * p.sd + (int64_t)m_w * p.ldd + n_w, rows_valid * (uint32_t)p.ldd * 2u);
+      rd0 = make_rsrc(reinterpret_cast<const Out*>(p.d0) + (int64_t)c.batch * p.sd + (int64_t)m_w * p.ldd + n_w, rows_valid * (uint32_t)p.ldd * 2u);
     if constexpr (Epi::kNumD >= 2)
-      rd1 = make_rsrc(reinterpret_cast<const T*>(p.d1) + (int64_t)c.batch * p.sd + (int64_t)m_w * p.ldd + n_w, rows_valid * (uint32_t)p.ldd * 2u);
+      rd1 = make_rsrc(reinterpret_cast<const Out*>(p.d1) + (int64_t)c.batch * p.sd + (int64_t)m_w * p.ldd + n_w, rows_valid * (uint32_t)p.ldd * 2u);
     // byte offsets of the lane's first row in each unit, out of range where its columns are; of a pair of units the
     // lane's share behind the exchange (below)
     uint32_t off_c[NU], off_d[NU];
-    vec8 bv[NU];
+    out8 bv[NU];
+    // scales of the lane's columns in each unit, and of its row in each row block
+    float scale_n[kScaled ? NU : 1][8], scale_m[kScaled ? MI : 1];
+    if constexpr (kScaled) {
+#pragma unroll
+      for (int mi = 0; mi < MI; ++mi) {
+        const int m = m_w + mi * 16 + fr;
+        scale_m[mi] = p.scale_a[m < p.M ? m : p.M - 1];
+      }
+    }
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const bool row_pair = u == NP;
@@ -301,9 +324,19 @@ __global__ void __launch_bounds__(Tile::NT, 1) gemm_rcr_wide_kernel(const GemmPa
       const int col_c = joined ? (u / 2 * 2 + (fr >> 3)) * 32 + sub * 16 + half8 : col;
       const int row_c = joined ? (fr & 7) + (u & 1) * 8 : row;
       off_c[u] = n_w + col_c < p.N ? (uint32_t)((row_c * (int)p.ldc + col_c) * 2) : kOobOffset;
-      bv[u] = vec8{};
+      bv[u] = out8{};
       if constexpr (Epi::kHasBias) {
-        if (ok) bv[u] = load_vec<vec8>(bias + n_w + col);
+        if (ok) bv[u] = load_vec<out8>(bias + n_w + col);
+      }
+      if constexpr (kScaled) {
+        // (of columns that are not there, of the last ones that are: N is a multiple of 8)
+        const float* at = p.scale_b + (ok ? n_w + col : p.N - 8);
+        const f32x4 lo = load_vec<f32x4>(at), hi = load_vec<f32x4>(at + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          scale_n[u][j] = lo[j];
+          scale_n[u][4 + j] = hi[j];
+        }
       }
     }
     float one = 1.0f;
@@ -311,14 +344,14 @@ __global__ void __launch_bounds__(Tile::NT, 1) gemm_rcr_wide_kernel(const GemmPa
     // (one residual: a row pair ahead of its use, and ahead of the stores of the pair before - loads and stores complete
     // in order, a load behind them waits for them; two of them held so spill)
     constexpr int AHEAD = Epi::kNumD == 1 ? 1 : 0;
-    vec8 d0r[1 + AHEAD][2 * NU], d1r[1 + AHEAD][2 * NU];
+    out8 d0r[1 + AHEAD][2 * NU], d1r[1 + AHEAD][2 * NU];
     auto load_d = [&](auto mp_c) __attribute__((always_inline)) {
       constexpr int mp = decltype(mp_c)::value;
       if constexpr (Epi::kNumD >= 1 && mp < MI / 2) {
         for_units(mp_c, [&](const f32x4&, const f32x4&, auto s_c, int row, auto u_c) __attribute__((always_inline)) {
           const uint32_t off = off_d[decltype(u_c)::value] + (uint32_t)(row * (int)p.ldd * 2);
-          d0r[mp % (1 + AHEAD)][decltype(s_c)::value] = __builtin_bit_cast(vec8, buffer_load_16B(rd0, off));
-          if constexpr (Epi::kNumD >= 2) d1r[mp % (1 + AHEAD)][decltype(s_c)::value] = __builtin_bit_cast(vec8, buffer_load_16B(rd1, off));
+          d0r[mp % (1 + AHEAD)][decltype(s_c)::value] = __builtin_bit_cast(out8, buffer_load_16B(rd0, off));
+          if constexpr (Epi::kNumD >= 2) d1r[mp % (1 + AHEAD)][decltype(s_c)::value] = __builtin_bit_cast(out8, buffer_load_16B(rd1, off));
         });
       }
     };
@@ -326,7 +359,7 @@ __global__ void __launch_bounds__(Tile::NT, 1) gemm_rcr_wide_kernel(const GemmPa
     static_for<0, MI / 2>([&](auto mp_c) __attribute__((always_inline)) {
       load_d(std::integral_constant<int, decltype(mp_c)::value + AHEAD>{});
       u32x4 held = {};
-      const vec8 *d0v = d0r[decltype(mp_c)::value % (1 + AHEAD)], *d1v = d1r[decltype(mp_c)::value % (1 + AHEAD)];
+      const out8 *d0v = d0r[decltype(mp_c)::value % (1 + AHEAD)], *d1v = d1r[decltype(mp_c)::value % (1 + AHEAD)];
       for_units(mp_c, [&](const f32x4& x, const f32x4& y, auto s_c, int row, auto u_c) __attribute__((always_inline)) {
         constexpr int u = decltype(u_c)::value, s = decltype(s_c)::value;
         float v[8];
@@ -336,7 +369,14 @@ __global__ void __launch_bounds__(Tile::NT, 1) gemm_rcr_wide_kernel(const GemmPa
           v[4 + j] = y[j];
           swap_rows16(v[j], v[4 + j]);
         }
-        const vec8 o = epilogue8<Epi, T>(v, bv[u], d0v[s], d1v[s], one);
+        if constexpr (kScaled) {
+          // (the last unit of an odd number of column blocks: the odd 16 lanes have the row block below)
+          constexpr int mp2 = 2 * decltype(mp_c)::value;
+          const float scale = u == NP ? (sub ? scale_m[mp2 + 1] : scale_m[mp2]) : scale_m[s < NU ? mp2 : mp2 + 1];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = scaled_sum(v[j], scale * scale_n[u][j]);
+        }
+        const out8 o = epilogue8<Epi, Out>(v, bv[u], d0v[s], d1v[s], one);
         auto store = [&](u32x4 v, uint32_t off) __attribute__((always_inline)) {
           __builtin_amdgcn_raw_buffer_store_b128(v, rc, off + (uint32_t)(row * (int)p.ldc * 2), 0, NT_BITS);
         };

@@ -522,6 +522,53 @@ def quantize_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
     return out, scale
 
 
+def gemm_int8_workspace_bytes(M: int, N: int, K: int, bias: bool = False, dtype=torch.float16, algo: int = -1) -> int:
+    """Bytes of scratch memory with which `gemm_rcr_int8` may choose any of its instances for this problem (0: none takes any)."""
+    return int(_kernels.load().aitamd_gemm_int8_workspace_bytes(_TORCH_DTYPE_ID[dtype], algo, int(bool(bias)), M, N, K))
+
+
+def gemm_rcr_int8(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                  dtype=torch.float16, out: Optional[torch.Tensor] = None, algo: int = -1,
+                  workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out = a_scale * b_scale * (a @ b.T) (+ bias) of 8-bit integers `a` [..., K] with a fp32 scale for each row ([...], see
+    `quantize_rows`) and `b` [N, K] with one for each of its rows ([N]: a layer's output channels); `out` and `bias` [N] are of
+    type `dtype`.  The sums are exact, K goes up to 131071, rows may lie at any byte.  `a` and `b` may have row pitch (2-D views);
+    `algo` and `workspace` as of `gemm` (sizes from `gemm_int8_workspace_bytes`)."""
+    if dtype not in _TORCH_DTYPE_ID:
+        raise ValueError(f"unsupported dtype {dtype}")
+    device = _operands(("a", a, (torch.int8,)), ("b", b, (torch.int8,)), ("a_scale", a_scale, (torch.float32,)),
+                       ("b_scale", b_scale, (torch.float32,)), ("bias", bias, (dtype,)), ("out", out, (dtype,)),
+                       ("workspace", workspace, (torch.uint8,)))
+    if a.dim() < 1:
+        raise ValueError("a must have at least one dimension")
+    lead, K = a.shape[:-1], a.shape[-1]
+    M = 1
+    for d in lead:
+        M *= d
+    if b.dim() != 2 or b.shape[1] != K:
+        raise ValueError(f"b must be [N, K={K}], got {tuple(b.shape)}")
+    N = b.shape[0]
+    a2 = a if a.dim() == 2 else a.reshape(M, K)
+    for t, n, name in ((a_scale, M, "a_scale"), (b_scale, N, "b_scale")) + (((bias, N, "bias"),) if bias is not None else ()):
+        if t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous with {n} elements, got shape {tuple(t.shape)}")
+    if out is None:
+        out = torch.empty(*lead, N, dtype=dtype, device=device)
+    if out.dim() == 2 and out.shape == (M, N) and (out.stride(1) == 1 or N == 1) and out.stride(0) >= N:
+        out2 = out  # (rows of a wider buffer: written in place)
+    else:
+        _check_out(out, M * N, "M*N")
+        out2 = out.view(M, N)
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous uint8 GPU tensor (see new_workspace)")
+    with torch.cuda.device(device):
+        rc = _kernels.load().aitamd_gemm_rcr_int8(
+            _TORCH_DTYPE_ID[dtype], algo, _p(a2), _p(b), _p(a_scale), _p(b_scale), _p(bias), _p(out2), M, N, K, _row_pitch(a2, "a"),
+            _row_pitch(b, "b"), _row_pitch(out2, "out"), _p(workspace), 0 if workspace is None else workspace.numel(), _stream_ptr())
+    _kernels.check(rc, "gemm_rcr_int8")
+    return out
+
+
 def rotary_frequencies(rotated: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
                        original_length: Optional[int] = None, low: float = 1.0, high: float = 32.0,
                        device="cuda") -> Tuple[torch.Tensor, float]:

@@ -301,6 +301,19 @@ AITAMD_API int aitamd_copy_rows(const void* src, void* dst, int64_t rows, int64_
 AITAMD_API int aitamd_quantize_rows(int dtype, const void* x, int8_t* q, float* scale, int64_t rows, int64_t columns,
                                     int64_t ldx, int64_t ldq, void* stream);
 
+/* C[m, n] = scale_a[m] * scale_b[n] * sum_k A[m, k] B[n, k] (+ bias[n]): A [M, K] and B [N, K] 8-bit integers, rows
+ * K-contiguous, lda / ldb bytes apart; scales fp32 (a token's, a channel's); C and bias (may be null) of type `dtype`.
+ * The sums are exact (32-bit integers, K up to 131071); each is rounded to fp32, scaled, biased and rounded to `dtype`.
+ * Any K, pitch and address; rows of whole dwords, and more so of whole 16-byte pieces, are faster.  algo = -1: the
+ * heuristic instance; otherwise an instance of aitamd_gemm_num_algos(bias ? AITAMD_EPI_BIAS : AITAMD_EPI_NONE, 2 + dtype),
+ * for rows of whole dwords (queries about them count K, lda and ldb in pairs of bytes).  workspace: as of
+ * aitamd_gemm_rcr_ws, aitamd_gemm_int8_workspace_bytes() bytes (algo = -1: enough for any instance) or null. */
+AITAMD_API int aitamd_gemm_rcr_int8(int dtype, int algo, const int8_t* a, const int8_t* b, const float* scale_a,
+                                    const float* scale_b, const void* bias, void* c, int64_t M, int64_t N, int64_t K,
+                                    int64_t lda, int64_t ldb, int64_t ldc, void* workspace, int64_t workspace_bytes,
+                                    void* stream);
+AITAMD_API int64_t aitamd_gemm_int8_workspace_bytes(int dtype, int algo, int bias, int64_t M, int64_t N, int64_t K);
+
 /* out[b, s, h, :] = x[b, s, h, :] with its first `rotated` dims turned by the position: with n = rotated / 2 and
  * angle = position(b, s) * freqs[i], the pair (x[i], x[n + i]), or (x[2 i], x[2 i + 1]) with `interleaved`, becomes
  * scale * (x1 cos - x2 sin, x2 cos + x1 sin); the other dims are handed through.  `inverse` turns the other way, which

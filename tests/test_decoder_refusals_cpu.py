@@ -29,6 +29,32 @@ def test_quantize_rows():
     assert quantize(rows=0, x=None, q=None, scale=None) == 0
 
 
+def int8(dtype=0, algo=-1, a=P, b=P, scale_a=P, scale_b=P, bias=None, c=P, M=2, N=8, K=64, lda=64, ldb=64, ldc=8):
+    return _kernels.load().aitamd_gemm_rcr_int8(dtype, algo, a, b, scale_a, scale_b, bias, c, M, N, K, lda, ldb, ldc, None, 0, None)
+
+
+def test_gemm_rcr_int8():
+    lib = _kernels.load()
+    refused(int8(dtype=2), "dtype")
+    refused(int8(M=-1), "negative")
+    refused(int8(M=1 << 31), "large")
+    refused(int8(K=131072, lda=131072, ldb=131072), "131071")
+    refused(int8(a=None), "null")
+    refused(int8(scale_b=None), "null")
+    refused(int8(c=None), "null")
+    refused(int8(lda=63), "pitch")
+    refused(int8(ldc=7), "pitch")
+    refused(int8(scale_a=ctypes.c_void_p(66)), "aligned")
+    refused(int8(algo=0, K=63), "dwords")
+    refused(int8(algo=999), "range")
+    assert int8(M=0, a=None, c=None) == 0
+    # the tables of 8-bit integers take scales: not through the other entry points
+    assert lib.aitamd_gemm_num_algos(0, 2) > 0 and lib.aitamd_gemm_num_algos(3, 2) == 0
+    refused(lib.aitamd_gemm_rcr(0, 2, -1, P, P, None, None, None, P, 2, 8, 64, 64, 64, 8, 8, None), "dtype")
+    for name in _kernels.gemm_algo_names(1, 3):
+        assert name.startswith("gemm_rcr_i8_bf16_")
+
+
 def rotary(dtype=0, x=P, out=P, positions=P, freqs=P, batch=1, seq=2, heads=2, head_dim=64, rotated=64):
     return _kernels.load().aitamd_rotary_embedding(dtype, x, out, positions, 0, freqs, batch, seq, heads, head_dim, rotated, 0, 128, 64, 0,
                                                    128, 64, 0, 1, 1.0, 0, 0, None)
@@ -121,6 +147,8 @@ def test_eager_calls_take_gpu_tensors_only():
     x = torch.zeros(2, 4, 64, dtype=torch.float16)
     with pytest.raises(ValueError, match="GPU"):
         eager.quantize_rows(x)
+    with pytest.raises(ValueError, match="GPU"):
+        eager.gemm_rcr_int8(x.to(torch.int8), x.to(torch.int8), x.float(), x.float())
     with pytest.raises(ValueError, match="GPU"):
         eager.rotary_embedding(x, torch.zeros(2, dtype=torch.int64), torch.zeros(32))
     with pytest.raises(ValueError, match="GPU"):
