@@ -11,6 +11,7 @@ callers for device memory and streams.
 from __future__ import annotations
 
 import ctypes
+import importlib
 import os
 import threading
 import warnings
@@ -218,23 +219,24 @@ class _NoNative:
         return lambda *args: NotImplemented
 
 
-def load_native():
-    """The extension module of the eager calls and model runs (csrc/native_calls.cpp).  It holds no kernels and only
+def load_native(name: str = "_native"):
+    """The extension module `name`: of the eager calls and model runs ("_native", csrc/native_calls.cpp), or of the eager calls of
+    the decoder operators ("_native_decoder", csrc/native_decoder.cpp).  It holds no kernels and only
     saves host time, so where it was not built, or was built for another torch, a warning says so and the Python code
     behind every one of its calls takes them."""
     import torch  # (its libraries have to be in the process first)
 
     try:
-        from . import _native
+        module = importlib.import_module("." + name, __package__)
 
         # (the headers' version has no pre-release part: a module built for one of those names it beside that)
-        built_for = getattr(_native, "torch_build", getattr(_native, "torch_version", "unknown"))
+        built_for = getattr(module, "torch_build", getattr(module, "torch_version", "unknown"))
         if built_for.split("+")[0] == torch.__version__.split("+")[0]:
-            return _native
+            return module
         why = f"it was built for torch {built_for}, this is {torch.__version__}"
     except ImportError as e:
         why = str(e)
-    warnings.warn(f"the extension module aitemplate_amd._native is not used ({why}): eager calls and model runs take 10 to 50 us "
+    warnings.warn(f"the extension module aitemplate_amd.{name} is not used ({why}): eager calls and model runs take 10 to 50 us "
                   "longer; build it with `make -C aitemplate_amd/csrc -j8` (or __graft_entry__.build())", RuntimeWarning)
     return _NoNative()
 

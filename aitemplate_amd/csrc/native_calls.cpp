@@ -64,105 +64,7 @@ const OpInfo kOps[] = {
     {"gemm_rcr_bias_mul_tanh", AITAMD_EPI_BIAS_MUL_TANH, 1},
 };
 
-PyObject* not_ordinary() { Py_RETURN_NOTIMPLEMENTED; }
-
-// A plain tensor on the GPU, or null (also for None and for subclasses, which may intercept what is done to them).
-// The wrappers of torch.func and of functionalization are of the exact type torch.Tensor and report the device of what
-// they wrap, but have no memory of their own.
-const at::Tensor* gpu_tensor(PyObject* o) {
-  if (!THPVariable_CheckExact(o)) return nullptr;
-  const at::Tensor& t = THPVariable_Unpack(o);
-  constexpr c10::DispatchKeySet wrappers(
-      {c10::DispatchKey::Functionalize, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper});
-  return on_device(t) && t.layout() == at::kStrided && t.has_storage() && !t.key_set().has_any(wrappers) ? &t : nullptr;
-}
-
-int dtype_id(const at::Tensor& t) {
-  const at::ScalarType s = t.scalar_type();
-  return s == at::kHalf ? 0 : (s == at::kBFloat16 ? 1 : -1);
-}
-
-// The class of the function mode behind `with torch.device(...)` and torch.set_default_device (null where torch has none)
-PyTypeObject* device_context_type() {
-  // (not an initializer of the static: the import may give up the interpreter lock, and others would wait with it held)
-  static PyTypeObject* type = nullptr;
-  if (type == nullptr) {
-    THPObjectPtr from(PyImport_ImportModule("torch.utils._device"));
-    PyObject* found = from ? PyObject_GetAttrString(from, "DeviceContext") : nullptr;
-    if (found == nullptr)
-      PyErr_Clear();
-    else if (type == nullptr && PyType_Check(found))
-      type = reinterpret_cast<PyTypeObject*>(found);  // (kept for good)
-    else
-      Py_DECREF(found);
-  }
-  return type;
-}
-
-// Whether every function mode gives new tensors a default device and no more: what is allocated here names its device
-bool device_contexts_only() {
-  for (int64_t i = at::impl::PythonTorchFunctionTLS::stack_len(); i-- > 0;)
-    if (Py_TYPE(at::impl::PythonTorchFunctionTLS::get_stack_at(i)->ptr(getPyInterpreter())) != device_context_type()) return false;
-  return true;
-}
-
-// False under a mode that sees, changes, records or refuses what the Python path does through torch (its allocation,
-// reshapes and views): dispatch modes, fake tensors among them, function modes other than those of a default device,
-// torch.func transforms, functionalization, tracing.  All but the function modes put a key of theirs into the thread's
-// dispatch keys; autocast, no_grad and inference mode put none.
-bool ordinary_context() {
-  return (c10::impl::tls_local_dispatch_key_set().included_ - c10::default_included_set).empty() && device_contexts_only();
-}
-
-// results of torch.empty that torch would have to fill are not ordinary
-bool plain_allocation() {
-  return !(at::globalContext().deterministicAlgorithms() && at::globalContext().deterministicFillUninitializedMemory());
-}
-
-// Row pitch of a [rows, cols] view with contiguous rows; false where the rows are not contiguous.
-bool row_pitch(const at::Tensor& t, int64_t* pitch) {
-  const int64_t rows = t.size(0), cols = t.size(1);
-  if (cols > 1 && t.stride(1) != 1) return false;
-  *pitch = rows > 1 ? t.stride(0) : std::max(cols, t.stride(0));
-  return true;
-}
-
-// The same for an operand whose leading dims are flattened into `rows`.
-bool flat_row_pitch(const at::Tensor& t, int64_t rows, int64_t cols, int64_t* pitch) {
-  if (t.dim() == 2 && t.size(0) == rows && t.size(1) == cols) return row_pitch(t, pitch);
-  if (!t.is_contiguous() || t.numel() != rows * cols) return false;
-  *pitch = cols;
-  return true;
-}
-
-PyObject* finish(int rc, const char* what, const at::Tensor* made, PyObject* out) {
-  if (rc != 0) return PyErr_Format(PyExc_RuntimeError, "%s failed: %s", what, aitamd_last_error());
-  if (made != nullptr) return THPVariable_Wrap(*made);
-  Py_INCREF(out);
-  return out;
-}
-
-// torch's own translation of C++ exceptions: the types and texts that its bindings raise
-template <class F>
-PyObject* guarded(F&& body) {
-  HANDLE_TH_ERRORS
-  return ordinary_context() ? body() : not_ordinary();
-  END_HANDLE_TH_ERRORS
-}
-
-// The launch itself runs without the interpreter lock, as it does through ctypes.  What it takes is plain pointers and
-// numbers, read beforehand: a tensor's accessors may throw, and the error is raised with the lock held.
-struct Unlocked {
-  PyThreadState* const save = PyEval_SaveThread();
-  ~Unlocked() { PyEval_RestoreThread(save); }
-};
-template <class F>
-int unlocked(F&& launch) {
-  const Unlocked here;
-  return launch();
-}
-
-const void* pointer(const at::Tensor* t) { return t == nullptr ? nullptr : t->data_ptr(); }
+#include "native_common.inc"
 
 // gemm(op, a, b, bias, d0, d1, out, algo, workspace)
 PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {

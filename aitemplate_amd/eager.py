@@ -22,6 +22,7 @@ import torch
 from . import _kernels
 
 _native = _kernels.load_native()
+_native_decoder = _kernels.load_native("_native_decoder")
 
 _TORCH_DTYPE_ID = {torch.float16: 0, torch.bfloat16: 1}
 
@@ -495,6 +496,10 @@ def quantize_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
     """Rows of `x` [..., columns] (fp16 / bf16) as 8-bit integers, and one fp32 scale a row ([...]): scale = max|x| / 127 and
     the whole number nearest to x / scale (of 127 x / max|x|, exactly; ties to even).  A row of zeros has scale 0; a row
     with an infinity or a NaN has scale NaN and zeros.  `x` may be a 2-D view with row pitch."""
+    if out is None and scale is None:
+        result = _native_decoder.quantize_rows(x)
+        if result is not NotImplemented:
+            return result
     device = _operands(("x", x, tuple(_TORCH_DTYPE_ID)), ("out", out, (torch.int8,)), ("scale", scale, (torch.float32,)))
     if x.dim() < 1:
         raise ValueError("x must have at least one dimension")
@@ -536,6 +541,9 @@ def gemm_rcr_int8(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_sca
     `algo` and `workspace` as of `gemm` (sizes from `gemm_int8_workspace_bytes`)."""
     if dtype not in _TORCH_DTYPE_ID:
         raise ValueError(f"unsupported dtype {dtype}")
+    result = _native_decoder.gemm_rcr_int8(a, b, a_scale, b_scale, bias, dtype is torch.bfloat16, out, algo, workspace)
+    if result is not NotImplemented:
+        return result
     device = _operands(("a", a, (torch.int8,)), ("b", b, (torch.int8,)), ("a_scale", a_scale, (torch.float32,)),
                        ("b_scale", b_scale, (torch.float32,)), ("bias", bias, (dtype,)), ("out", out, (dtype,)),
                        ("workspace", workspace, (torch.uint8,)))
@@ -634,6 +642,9 @@ def rotary_embedding(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tens
     `positions`: int32 or int64 [tokens], [batch, seq], or [seq] for every batch entry.  `freqs`: fp32, see `rotary_frequencies`
     (whose second result is `scale`).  `inverse` turns back: the gradient with respect to `x` of the same call without it.
     `out` may be `x` itself and must not overlap it otherwise."""
+    result = _native_decoder.rotary_embedding(x, positions, freqs, interleaved, scale, inverse, out)
+    if result is not NotImplemented:
+        return result
     device = _operands(("x", x, tuple(_TORCH_DTYPE_ID)), ("positions", positions, (torch.int32, torch.int64)),
                        ("freqs", freqs, (torch.float32,)), ("out", out, (x.dtype,)))
     if x.dim() not in (3, 4):
@@ -697,6 +708,10 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     Rows from offsets[batch] on are left as they were, in `q_out` too; keys and values that no page is there for are dropped.
     Pages that are written must not be shared between sequences.  `lengths` stay as they are: the attention of the same step
     takes them as they are too.  `q_out` may be `q`."""
+    result = _native_decoder.paged_kv_append(k, v, k_cache, v_cache, block_table, lengths, offsets, q, freqs, interleaved, scale,
+                                             first_position, q_out)
+    if result is not NotImplemented:
+        return result
     types = tuple(_TORCH_DTYPE_ID)
     device = _operands(("k", k, types), ("v", v, (k.dtype,)), ("k_cache", k_cache, (k.dtype,)), ("v_cache", v_cache, (k.dtype,)),
                        ("block_table", block_table, (torch.int32,)), ("lengths", lengths, (torch.int32,)),
@@ -761,6 +776,10 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
     page_size has to be a multiple of 16, head_dim one of 8 up to 256.  `workspace`: a buffer from `new_workspace` of
     `prefix_attention_workspace_bytes`, allocated for the call otherwise; calls that may overlap in time need one each."""
+    result = _native_decoder.prefix_attention(q, k_cache, v_cache, block_table, lengths, offsets, prefix_table, prefix_length, scale, out,
+                                              workspace)
+    if result is not NotImplemented:
+        return result
     device = _operands(("q", q, tuple(_TORCH_DTYPE_ID)), ("k_cache", k_cache, (q.dtype,)), ("v_cache", v_cache, (q.dtype,)),
                        ("block_table", block_table, (torch.int32,)), ("lengths", lengths, (torch.int32,)),
                        ("offsets", offsets, (torch.int32,)), ("prefix_table", prefix_table, (torch.int32,)), ("out", out, (q.dtype,)),
