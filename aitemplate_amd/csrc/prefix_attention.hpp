@@ -502,34 +502,61 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) prefix_prompt_kernel(cons
   attend<T, Tile>(p, w, smem_raw);
 }
 
-// The parts of a row joined: D / 4 lanes a row
-template <class T>
-__global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p, int slots, int lanes, Divisor by_lanes, Divisor by_heads) {
+// The parts of a row joined.  A workgroup takes one row: LANES lanes of 4 dims each, and 256 / LANES groups of those that take
+// every so manieth part; the parts' weights are computed once, by as many lanes.  Bound: latency, of three trips to memory (offsets,
+// (m, l), parts) one after the other.  64 x 32 rows of 33 parts of 128 dims: 28 us with one lane going through a row's parts, <JOIN> so.
+constexpr int kMostSlots = 128;
+template <class T, int LANES>
+__global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p, int slots, Divisor by_heads) {
+  constexpr int GROUPS = 256 / LANES;
+  __shared__ float weight[kMostSlots];
+  __shared__ float sums[4];
+  __shared__ __attribute__((aligned(16))) f32x4 part[GROUPS][LANES];
+  const int row = blockIdx.x, token = quotient(row, by_heads), head = row - token * p.heads;
   const int64_t rows = (int64_t)p.cache.tokens * p.heads;
-  const int per_wg = quotient(256, by_lanes);
-  const int in_wg = quotient(threadIdx.x, by_lanes), d = (threadIdx.x - in_wg * lanes) * 4;
-  const int64_t row = (int64_t)blockIdx.x * per_wg + in_wg;
-  if (in_wg >= per_wg || row >= rows) return;
-  const int64_t token = row / p.heads;
+  const int tid = threadIdx.x, lane = tid % LANES, group = tid / LANES, d = lane * 4;
+  float2 ml = make_float2(-INFINITY, 0.0f);
+  if (tid < slots) ml = p.part_ml[tid * rows + row];
   if (p.cache.offsets != nullptr && (token < p.cache.offsets[0] || token >= p.cache.offsets[p.cache.batch])) return;
-  float most = -INFINITY;
-  for (int s = 0; s < slots; ++s) most = fmaxf(most, p.part_ml[s * rows + row].x);
-  f32x4 o = {};
-  float sum = 0.0f;
-  for (int s = 0; s < slots; ++s) {
-    const float2 ml = p.part_ml[s * rows + row];
-    if (ml.y == 0.0f) continue;  // (no key)
-    const float weight = __builtin_amdgcn_exp2f(ml.x - most);
-    sum += ml.y * weight;
-    const f32x4 v = *reinterpret_cast<const f32x4*>(p.part_o + (s * rows + row) * p.head_dim + d);
+  // (the first two waves hold all parts)
+  float most = ml.x;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] += v[j] * weight;
+  for (int s = 32; s > 0; s >>= 1) most = fmaxf(most, __shfl_xor(most, s));
+  if ((tid & 63) == 0 && tid < kMostSlots) sums[tid >> 6] = most;
+  __syncthreads();
+  most = fmaxf(sums[0], sums[1]);
+  // (no key: no weight, whatever lies in its place)
+  const float w = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - most);
+  if (tid < kMostSlots) weight[tid] = w;
+  float sum = ml.y == 0.0f ? 0.0f : ml.y * w;
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
+  if ((tid & 63) == 0 && tid < kMostSlots) sums[2 + (tid >> 6)] = sum;
+  __syncthreads();
+  sum = sums[2] + sums[3];
+  f32x4 o = {};
+  if (d < p.head_dim) {
+    const float* at = p.part_o + (int64_t)row * p.head_dim + d;
+    const int64_t step = rows * p.head_dim;
+#pragma unroll 4
+    for (int s = group; s < slots; s += GROUPS) {
+      const float by = weight[s];
+      const f32x4 v = *reinterpret_cast<const f32x4*>(at + s * step);
+      // (a part without keys is not written)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] += by == 0.0f ? 0.0f : v[j] * by;
+    }
   }
+  part[group][lane] = o;
+  __syncthreads();
+  if (group != 0 || d >= p.head_dim) return;
+#pragma unroll
+  for (int g = 1; g < GROUPS; ++g) o += part[g][lane];
   const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
   typename ElemTraits<T>::vec4 y;
 #pragma unroll
   for (int j = 0; j < 4; ++j) y[j] = ElemTraits<T>::from_float(o[j] * inv);
-  store_vec(reinterpret_cast<T*>(p.out) + token * p.out_token + (row - token * p.heads) * p.out_head + d, y);
+  store_vec(reinterpret_cast<T*>(p.out) + token * p.out_token + head * p.out_head + d, y);
 }
 
 }  // namespace aitamd

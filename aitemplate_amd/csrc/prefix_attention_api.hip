@@ -32,7 +32,7 @@ struct Plan {
 int64_t parts(int64_t items, int64_t keys, int64_t least, int cus) {
   int64_t n = 2 * (int64_t)cus / (items > 0 ? items : 1);
   if (n > keys / least) n = keys / least;
-  return n < 1 ? 1 : (n > 64 ? 64 : n);
+  return n < 1 ? 1 : (n > kMostSlots / 2 ? kMostSlots / 2 : n);
 }
 
 Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t prefix, int64_t most_keys, bool ragged, int cus) {
@@ -96,10 +96,9 @@ hipError_t launch_all(PrefixParams& p, const Plan& plan, int64_t wgs, hipStream_
       : d <= 128         ? launch_attention<T, 128>(p, plan, wgs, stream)
                          : launch_attention<T, 256>(p, plan, wgs, stream);
   if (e != hipSuccess || plan.slots() == 1) return e;
-  const int lanes = (d + 3) / 4, per_wg = 256 / lanes;
-  const int64_t rows = (int64_t)p.cache.tokens * p.heads;
-  hipLaunchKernelGGL(prefix_join_kernel<T>, dim3((unsigned)((rows + per_wg - 1) / per_wg)), dim3(256), 0, stream, p, (int)plan.slots(), lanes,
-                     make_divisor(lanes), make_divisor(p.heads));
+  const unsigned rows = (unsigned)(p.cache.tokens * p.heads);
+  const auto join = d <= 64 ? prefix_join_kernel<T, 16> : (d <= 128 ? prefix_join_kernel<T, 32> : prefix_join_kernel<T, 64>);
+  hipLaunchKernelGGL(join, dim3(rows), dim3(256), 0, stream, p, (int)plan.slots(), make_divisor(p.heads));
   return hipGetLastError();
 }
 
