@@ -34,10 +34,12 @@ struct PrefixParams {
   Divisor by_group, by_row_tiles, by_own_slots, by_kv_heads;
 };
 
-// HD: head dims, padded; a row takes the next power of two in LDS
-template <int HD_, int WR_, int WK_, int KB_, int NS_, int OCC_>
+// HD: head dims, padded; a row takes the next power of two in LDS.  WR > 1: waves side by side over rows, the second product a
+// tile behind the first (K(t) and V(t - 1) are multiplied while K(t + 1) and V(t + 1) land: two stages for K, three for V).
+// WK > 1: over keys, a wave loads a tile, waits and multiplies; the CU's other waves have theirs on the way meanwhile.
+template <int HD_, int WR_, int WK_, int KB_, int OCC_>
 struct PagedTile {
-  static constexpr int HD = HD_, WR = WR_, WK = WK_, KB = KB_, NS = NS_, OCC = OCC_;
+  static constexpr int HD = HD_, WR = WR_, WK = WK_, KB = KB_, OCC = OCC_;
   static constexpr int KP = HD <= 64 ? 64 : (HD <= 128 ? 128 : 256);
   static constexpr int KS = HD / 16, OT = HD / 32;
   static constexpr int NW = WR * WK, NT = 64 * NW;
@@ -48,16 +50,16 @@ struct PagedTile {
   static constexpr int CHUNKS = KP / 8;       // 16-byte pieces of a row in LDS
   static constexpr int RPL = 64 / CHUNKS;     // rows of a wave-load
   static constexpr int LPG = 16 / RPL;        // wave-loads of 16 keys
-  static constexpr int LOADS = 2 * GROUPS * LPG;
-  static constexpr int STAGE = 2 * BN * KP;   // elements: K, then V
-  static constexpr int kRing = NS * STAGE * 2;
+  static constexpr bool PIPED = WR > 1;
+  static constexpr int NK = PIPED ? 2 : 1, NV = PIPED ? 3 : 1;
+  static constexpr int STAGE = BN * KP;       // elements
+  static constexpr int kRing = (NK + NV) * STAGE * 2;
   static constexpr int kMerge = WK > 1 ? WK * (16 * OT + 2) * 64 * 4 : 0;
   static constexpr int kLdsBytes = kRing > kMerge ? kRing : kMerge;
   // 16-byte piece c of row r lies at piece c ^ swizzle(r).  K: 32 rows' piece at a time; V: see AttnTile::v_swz.
   static constexpr int k_swz(int row) { return CHUNKS == 8 ? (row / 2) % 8 : row % 16; }
   static constexpr int v_swz(int row) { return CHUNKS == 8 ? 4 * ((row / 2) % 2) : 4 * (row % 4); }
   static_assert(WK == 1 || (WR == 1 && KPW == 32 * KB), "waves side by side over keys load what they multiply");
-  static_assert(NS > 1 || WR == 1, "one stage: a wave waits for its own loads only");
   static_assert(KPW % 16 == 0, "a wave loads whole groups of 16 keys");
   static_assert(kLdsBytes <= 160 * 1024, "LDS budget");
 };
@@ -86,11 +88,10 @@ AITAMD_DEVICE void attend(const PrefixParams& p, const PagedWork& w, unsigned ch
   using vec4 = typename Tr::vec4;
   typedef __attribute__((address_space(3))) const T lds_T;
   typedef __attribute__((address_space(3))) const vec8 lds_vec8;
-  typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
   constexpr int KP = Tile::KP, KS = Tile::KS, OT = Tile::OT, KB = Tile::KB, WR = Tile::WR, WK = Tile::WK, BN = Tile::BN;
-  constexpr int D = Tile::NS - 1;  // tiles asked for ahead
-  static_assert((D > 0 ? D - 1 : 0) * Tile::LOADS <= 63, "vmcnt field is 6 bits");
-  T* const smem = reinterpret_cast<T*>(smem_raw);
+  constexpr int V_LOADS = Tile::GROUPS * Tile::LPG;  // of a wave and a tile
+  T* const sK = reinterpret_cast<T*>(smem_raw);
+  T* const sV = sK + Tile::NK * Tile::STAGE;
   const PagedCache& c = p.cache;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -106,39 +107,61 @@ AITAMD_DEVICE void attend(const PrefixParams& p, const PagedWork& w, unsigned ch
     k_off[i] = kc * 8 < p.head_dim ? (uint32_t)row * (uint32_t)(c.k_slot * 2) + (uint32_t)kc * 16u : kOobOffset;
     v_off[i] = vc * 8 < p.head_dim ? (uint32_t)row * (uint32_t)(c.v_slot * 2) + (uint32_t)vc * 16u : kOobOffset;
   }
-  // first key of group g of tile t that this wave loads, and the keys there are in the tile's part
-  auto first_key = [&](int t, int g) { return (t < w.prefix_tiles ? t : t - w.prefix_tiles) * BN + wave * Tile::KPW + g * 16; };
-  auto keys_of = [&](int t) { return t < w.prefix_tiles ? p.prefix : w.own_keys; };
-  auto entry = [&](int t, int g) {
-    const int key = first_key(t, g), last = keys_of(t) - 1;
-    scalar_ptr table = (scalar_ptr) reinterpret_cast<uintptr_t>(t < w.prefix_tiles ? p.prefix_table : w.table);
-    return table[quotient(key < last ? key : last, c.by_page)];
+  // The tile that is to be loaded next, of this wave's 16 keys at a time: their page, where in it they begin and how many
+  // there are.  All scalars, prepared a tile ahead: the page is a trip to memory.
+  typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
+  int next_t = w.t_lo, next_key, next_keys;
+  scalar_ptr next_table;
+  auto enter = [&](bool shared) {  // the prefix's tiles, or the sequence's own
+    next_key = (next_t - (shared ? 0 : w.prefix_tiles)) * BN + wave * Tile::KPW;
+    next_keys = shared ? p.prefix : w.own_keys;
+    next_table = (scalar_ptr) reinterpret_cast<uintptr_t>(shared ? p.prefix_table : w.table);
   };
-  int pages[Tile::GROUPS];  // of the tile that is to be loaded next
-  auto fetch_pages = [&](int t) {
-#pragma unroll
-    for (int g = 0; g < Tile::GROUPS; ++g) pages[g] = t < w.t_hi ? entry(t, g) : 0;
-  };
-  auto issue = [&](int t, int stage) {
+  enter(next_t < w.prefix_tiles);
+  int page[Tile::GROUPS], within[Tile::GROUPS], rows[Tile::GROUPS];
+  auto prepare = [&]() {
+    if (next_t >= w.t_hi) return;
+    if (next_t == w.prefix_tiles) enter(false);
 #pragma unroll
     for (int g = 0; g < Tile::GROUPS; ++g) {
-      const int key = first_key(t, g), page = __builtin_amdgcn_readfirstlane(pages[g]);
-      int rows = keys_of(t) - key;
-      rows = rows < 0 || (uint32_t)page >= (uint32_t)c.pages ? 0 : (rows < 16 ? rows : 16);
-      const int within = key - quotient(key, c.by_page) * c.page_size;
-      const T* kb = reinterpret_cast<const T*>(c.k) + page * c.k_page + within * c.k_slot + w.kv_head * c.k_head;
-      const T* vb = reinterpret_cast<const T*>(c.v) + page * c.v_page + within * c.v_slot + w.kv_head * c.v_head;
-      const __amdgpu_buffer_rsrc_t rk = make_rsrc(kb, rows > 0 ? (uint32_t)(((rows - 1) * (int)c.k_slot + p.head_dim) * 2) : 0u);
-      const __amdgpu_buffer_rsrc_t rv = make_rsrc(vb, rows > 0 ? (uint32_t)(((rows - 1) * (int)c.v_slot + p.head_dim) * 2) : 0u);
-      T* dk = smem + stage * Tile::STAGE + (wave * Tile::KPW + g * 16) * KP;
-      T* dv = dk + BN * KP;
-#pragma unroll
-      for (int i = 0; i < Tile::LPG; ++i)
-        load_to_lds(rk, dk + i * 512, k_off[i]);
-#pragma unroll
-      for (int i = 0; i < Tile::LPG; ++i)
-        load_to_lds(rv, dv + i * 512, v_off[i]);
+      const int key = next_key + g * 16, left = next_keys - key;
+      const int at = left > 0 ? key : 0, which = quotient(at, c.by_page);
+      page[g] = next_table[which];
+      within[g] = at - which * c.page_size;
+      rows[g] = left > 0 ? (left < 16 ? left : 16) : 0;
     }
+    next_key += BN;
+    ++next_t;
+  };
+  const char* const k_base = reinterpret_cast<const char*>(reinterpret_cast<const T*>(c.k) + w.kv_head * c.k_head);
+  const char* const v_base = reinterpret_cast<const char*>(reinterpret_cast<const T*>(c.v) + w.kv_head * c.v_head);
+  const uint32_t k_page16 = (uint32_t)(c.k_page / 8), v_page16 = (uint32_t)(c.v_page / 8);  // in 16-byte units
+  const uint32_t k_slot = (uint32_t)(c.k_slot * 2), v_slot = (uint32_t)(c.v_slot * 2);      // in bytes
+  const uint32_t row_bytes = (uint32_t)p.head_dim * 2u;
+  // the prepared tile into stage k_in, v_in (offsets in elements)
+  int k_in = 0, v_in = 0;
+  auto issue = [&]() {
+    T* const dk = sK + k_in + wave * Tile::KPW * KP;
+    T* const dv = sV + v_in + wave * Tile::KPW * KP;
+    __amdgpu_buffer_rsrc_t rv[Tile::GROUPS];
+#pragma unroll
+    for (int g = 0; g < Tile::GROUPS; ++g) {
+      // (a page that is none: nothing in bounds, so zeros)
+      const uint32_t pg = (uint32_t)__builtin_amdgcn_readfirstlane(page[g]);
+      const uint32_t n = (uint32_t)__builtin_amdgcn_readfirstlane(pg < (uint32_t)c.pages ? rows[g] : 0);
+      const uint32_t in = (uint32_t)__builtin_amdgcn_readfirstlane(within[g]);
+      const __amdgpu_buffer_rsrc_t rk = make_rsrc(k_base + (((uint64_t)pg * k_page16) << 4) + in * k_slot, n > 0 ? (n - 1) * k_slot + row_bytes : 0u);
+      rv[g] = make_rsrc(v_base + (((uint64_t)pg * v_page16) << 4) + in * v_slot, n > 0 ? (n - 1) * v_slot + row_bytes : 0u);
+#pragma unroll
+      for (int i = 0; i < Tile::LPG; ++i) load_to_lds(rk, dk + g * 16 * KP + i * 512, k_off[i]);
+    }
+    // (behind all of K: a wait for the last V_LOADS leaves them out)
+#pragma unroll
+    for (int g = 0; g < Tile::GROUPS; ++g)
+#pragma unroll
+      for (int i = 0; i < Tile::LPG; ++i) load_to_lds(rv[g], dv + g * 16 * KP + i * 512, v_off[i]);
+    k_in = k_in == (Tile::NK - 1) * Tile::STAGE ? 0 : k_in + Tile::STAGE;
+    v_in = v_in == (Tile::NV - 1) * Tile::STAGE ? 0 : v_in + Tile::STAGE;
   };
 
   // Q fragments (B operand of S^T = K Q^T): lane (row = r32, k = 16 ks + 8 h + j)
@@ -162,8 +185,8 @@ AITAMD_DEVICE void attend(const PrefixParams& p, const PagedWork& w, unsigned ch
   // own keys that this row sees
   int seen = w.seen + ahead;
   seen = seen < w.own_keys ? seen : w.own_keys;
-  // ... and that every row of the wave does
-  const int wave_seen = __builtin_amdgcn_readfirstlane(seen);
+  // ... that every row of the wave does, and that some row does (rows are in order)
+  const int every = __builtin_amdgcn_readfirstlane(seen), some_own = __builtin_amdgcn_readlane(seen, 31);
 
   // LDS offsets of the fragment reads
   int k_rd[KS];
@@ -174,67 +197,44 @@ AITAMD_DEVICE void attend(const PrefixParams& p, const PagedWork& w, unsigned ch
   int v_rd[OT];
 #pragma unroll
   for (int ot = 0; ot < OT; ++ot)
-    v_rd[ot] = BN * KP + (wk * 32 * KB + h * 4 + tr_row) * KP + ((ot * 32) ^ (Tile::v_swz(tr_row) * 8)) + tr_col;
+    v_rd[ot] = (wk * 32 * KB + h * 4 + tr_row) * KP + ((ot * 32) ^ (Tile::v_swz(tr_row) * 8)) + tr_col;
 
   f32x16 oacc[OT];
 #pragma unroll
   for (int ot = 0; ot < OT; ++ot) oacc[ot] = f32x16{};
   float m_run = -INFINITY, l_run = 0.0f;
 
-  fetch_pages(w.t_lo);
+  vec8 pf[2 * KB];  // P^T fragments (of the tile whose second product is due)
+
+  auto read_v = [&](lds_T* base, int i, int ot) {
+    const vec4 lo = AttnVec<T>::tr_read(base + v_rd[ot] + i * 16 * KP);
+    const vec4 hi = AttnVec<T>::tr_read(base + v_rd[ot] + (i * 16 + 8) * KP);
+    return join_halves<T>(lo, hi);
+  };
+  auto second_product = [&](lds_T* base) {
 #pragma unroll
-  for (int t = 0; t < D; ++t) {
-    if (w.t_lo + t < w.t_hi) issue(w.t_lo + t, t);
-    fetch_pages(w.t_lo + t + 1);
-  }
-  int stage = 0, stage_in = D;
-  for (int t = w.t_lo; t < w.t_hi; ++t) {
-    if constexpr (D == 0) {
-      __builtin_amdgcn_sched_barrier(0);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave has read the last tile
-      issue(t, 0);
-      fetch_pages(t + 1);
-      attn_wait_vmcnt<0>();
-    } else {
-      // tile t has landed once only the younger ones are out; past the barrier everybody's part has, and nobody reads the
-      // stage that tile t + D goes to any more
-      if (t + D <= w.t_hi)
-        attn_wait_vmcnt<(D - 1) * Tile::LOADS>();
-      else
-        attn_wait_vmcnt<0>();
-      if constexpr (WR > 1) {
-        __builtin_amdgcn_s_barrier();
-      } else {
-        __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      }
-      if (t + D < w.t_hi) {
-        issue(t + D, stage_in);
-        fetch_pages(t + D + 1);
-      }
-    }
-    const T* st = smem + stage * Tile::STAGE;
-    stage = stage + 1 == Tile::NS ? 0 : stage + 1;
-    stage_in = stage_in + 1 == Tile::NS ? 0 : stage_in + 1;
-    const bool shared = t < w.prefix_tiles;
-    const int first = (shared ? t : t - w.prefix_tiles) * BN + wk * 32 * KB;  // this wave's first key
-    const int limit = shared ? p.prefix : seen;                               // keys the row sees
-    const int some = shared ? p.prefix : w.own_keys;
-    if (first >= some) continue;
-    f32x16 s[KB];
-    {
-      lds_T* kb_ptr = (lds_T*)st;
+    for (int i = 0; i < 2 * KB; ++i)
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+      for (int ot = 0; ot < OT; ++ot) oacc[ot] = Tr::mfma32(read_v(base, i, ot), pf[i], oacc[ot]);
+  };
+  auto scores = [&](const T* st, f32x16* s) {
+    lds_T* kb_ptr = (lds_T*)st;
+    // (all reads first: left to itself the compiler fetches a pair and waits for it in front of every second product)
+    vec8 kf[KB][KS];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const vec8 kf = *(lds_vec8*)(kb_ptr + kb * 32 * KP + k_rd[ks]);
-          s[kb] = Tr::mfma32(kf, qf[ks], ks == 0 ? f32x16{} : s[kb]);
-        }
-    }
-    float most = -INFINITY;
-    // (wave-uniform) keys that some row does not see
-    if (first + 32 * KB > (shared ? p.prefix : wave_seen)) {
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) kf[kb][ks] = *(lds_vec8*)(kb_ptr + kb * 32 * KP + k_rd[ks]);
+    __builtin_amdgcn_sched_barrier(0x6);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s[kb] = Tr::mfma32(kf[kb][ks], qf[ks], ks == 0 ? f32x16{} : s[kb]);
+  };
+  // Probabilities of a tile in the full form: masks, the row's maximum, a moved reference point, rescaled accumulators.
+  // first: this wave's first key; limit: keys the row sees; whole: every row sees all of the tile's
+  auto full_form = [&](f32x16* s, int first, int limit, bool whole) {
+    if (!whole) {
       const int left = limit - first - h * 4;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
@@ -242,6 +242,7 @@ AITAMD_DEVICE void attend(const PrefixParams& p, const PagedWork& w, unsigned ch
         for (int e = 0; e < 16; ++e)
           if (kb * 32 + (e >> 2) * 8 + (e & 3) >= left) s[kb][e] = -INFINITY;
     }
+    float most = -INFINITY;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -258,7 +259,6 @@ AITAMD_DEVICE void attend(const PrefixParams& p, const PagedWork& w, unsigned ch
     const float alpha = !move ? 1.0f : (__builtin_isinf(m_run) ? 0.0f : __builtin_amdgcn_exp2f(drift));
     const float mc = -m_safe * cs;
     l_run *= alpha;
-    vec8 pf[2 * KB];
 #pragma unroll
     for (int i = 0; i < 2 * KB; ++i) {
 #pragma unroll
@@ -273,15 +273,87 @@ AITAMD_DEVICE void attend(const PrefixParams& p, const PagedWork& w, unsigned ch
 #pragma unroll
         for (int e = 0; e < 16; ++e) oacc[ot][e] *= alpha;
     }
-    lds_T* vb = (lds_T*)st;
-#pragma unroll
-    for (int i = 0; i < 2 * KB; ++i)
-#pragma unroll
-      for (int ot = 0; ot < OT; ++ot) {
-        const vec4 lo = AttnVec<T>::tr_read(vb + v_rd[ot] + i * 16 * KP);
-        const vec4 hi = AttnVec<T>::tr_read(vb + v_rd[ot] + (i * 16 + 8) * KP);
-        oacc[ot] = Tr::mfma32(join_halves<T>(lo, hi), pf[i], oacc[ot]);
+  };
+
+  prepare();
+  if constexpr (Tile::PIPED) {
+    bool due = false;     // (wave-uniform) pf holds a tile's probabilities
+    bool ref_ok = false;  // (wave-uniform) every row of the wave has a finite reference point
+    int k_at = 0, v_at = 0;  // stages of K(t) and V(t - 1)
+    if (w.t_lo < w.t_hi) {
+      issue();
+      prepare();
+    }
+    int first = (w.t_lo < w.prefix_tiles ? w.t_lo : w.t_lo - w.prefix_tiles) * BN;  // the tile's first key
+    for (int t = w.t_lo; t < w.t_hi; ++t, first += BN) {
+      // K(t) and V(t - 1) have landed once only V(t) is out; past the barrier everybody's have, and nobody reads the stages of
+      // K(t - 1) and V(t - 2) any more
+      attn_wait_vmcnt<V_LOADS>();
+      __builtin_amdgcn_s_barrier();
+      if (t + 1 < w.t_hi) {
+        issue();
+        prepare();
       }
+      const bool shared = t < w.prefix_tiles;
+      if (t == w.prefix_tiles) first = 0;
+      lds_T* const vb = (lds_T*)(sV + v_at);
+      if (first < (shared ? p.prefix : some_own)) {
+        f32x16 s[KB];
+        scores(sK + k_at, s);
+        const bool whole = first + 32 * KB <= (shared ? p.prefix : every);
+        bool full = !ref_ok || !whole;
+        if (!full) {
+          // The probabilities against the reference point the row has (exact whatever it is, as long as nothing leaves its range),
+          // between the matrix instructions of the tile before.
+          const float l_before = l_run, mc = -m_run * cs;
+#pragma unroll
+          for (int i = 0; i < 2 * KB; ++i) {
+#pragma unroll
+            for (int ot = 0; ot < OT; ++ot) oacc[ot] = Tr::mfma32(read_v(vb, i, ot), pf[i], oacc[ot]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              pf[i][j] = Tr::from_float(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][(i & 1) * 8 + j], cs, mc)));
+            l_run = add_elements(pf[i], l_run);
+          }
+          if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(l_run <= kMaxRowSum)) != 0, 0)) {
+            l_run = l_before;  // (NaN, or a maximum far above the reference point: again, in the full form)
+            full = true;
+            due = false;
+          }
+        }
+        if (full) {
+          if (due) second_product(vb);
+          due = true;
+          full_form(s, first, shared ? p.prefix : seen, whole);
+          ref_ok = __builtin_amdgcn_ballot_w64(__builtin_isinf(m_run)) == 0;
+        }
+      } else if (due) {
+        second_product(vb);
+        due = false;
+      }
+      k_at = k_at == (Tile::NK - 1) * Tile::STAGE ? 0 : k_at + Tile::STAGE;
+      if (t > w.t_lo) v_at = v_at == (Tile::NV - 1) * Tile::STAGE ? 0 : v_at + Tile::STAGE;  // (V(t): behind V(t - 1)'s, which for the first is none)
+    }
+    attn_wait_vmcnt<0>();
+    __builtin_amdgcn_s_barrier();
+    if (due) second_product((lds_T*)(sV + v_at));
+  } else {
+    for (int t = w.t_lo; t < w.t_hi; ++t) {
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave has read the last tile
+      issue();
+      prepare();
+      const bool shared = t < w.prefix_tiles;
+      const int first = (shared ? t : t - w.prefix_tiles) * BN + wk * 32 * KB;  // this wave's first key
+      const bool there = first < (shared ? p.prefix : some_own);
+      attn_wait_vmcnt<V_LOADS>();
+      f32x16 s[KB];
+      if (there) scores(sK, s);
+      attn_wait_vmcnt<0>();
+      if (!there) continue;
+      full_form(s, first, shared ? p.prefix : seen, first + 32 * KB <= (shared ? p.prefix : every));
+      second_product((lds_T*)sV);
+    }
   }
   l_run = sum_across_halves(l_run);
 
@@ -323,10 +395,11 @@ AITAMD_DEVICE void attend(const PrefixParams& p, const PagedWork& w, unsigned ch
     }
   }
   if (!live) return;
-  // ---- store: the result, or this part of it
-  if (p.part_o == nullptr) {
+  // ---- store: the result, or this part of it (its arguments fetched here and not held over the loop)
+  const PrefixParams& a = arguments_anew<PrefixParams>();
+  if (a.part_o == nullptr) {
     const float inv = l_run > 0.0f ? 1.0f / l_run : (l_run == 0.0f ? 0.0f : l_run);  // (NaN stays)
-    T* const o = reinterpret_cast<T*>(p.out) + token * p.out_token + head * p.out_head;
+    T* const o = reinterpret_cast<T*>(a.out) + token * a.out_token + head * a.out_head;
 #pragma unroll
     for (int ot = 0; ot < OT; ++ot) {
       if (ot % WK != wk) continue;
@@ -336,13 +409,13 @@ AITAMD_DEVICE void attend(const PrefixParams& p, const PagedWork& w, unsigned ch
         vec4 v;
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = Tr::from_float(oacc[ot][g * 4 + j] * inv);
-        if (d < p.head_dim) store_vec(o + d, v);
+        if (d < a.head_dim) store_vec(o + d, v);
       }
     }
   } else {
-    const int64_t at = ((int64_t)w.slot * c.tokens + token) * p.heads + head;
-    if (wk == 0 && h == 0) p.part_ml[at] = make_float2(l_run == 0.0f ? -INFINITY : m_run * cs, l_run);
-    float* const o = p.part_o + at * p.head_dim;
+    const int64_t at = ((int64_t)w.slot * a.cache.tokens + token) * a.heads + head;
+    if (wk == 0 && h == 0) a.part_ml[at] = make_float2(l_run == 0.0f ? -INFINITY : m_run * cs, l_run);
+    float* const o = a.part_o + at * a.head_dim;
 #pragma unroll
     for (int ot = 0; ot < OT; ++ot) {
       if (ot % WK != wk) continue;
@@ -352,7 +425,7 @@ AITAMD_DEVICE void attend(const PrefixParams& p, const PagedWork& w, unsigned ch
         f32x4 v;
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = oacc[ot][g * 4 + j];
-        if (d < p.head_dim) *reinterpret_cast<f32x4*>(o + d) = v;
+        if (d < a.head_dim) *reinterpret_cast<f32x4*>(o + d) = v;
       }
     }
   }

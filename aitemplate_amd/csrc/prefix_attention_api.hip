@@ -14,9 +14,9 @@ constexpr int kMaxDevices = 64;
 
 template <int HD>
 struct Tiles {
-  using Shared = PagedTile<HD, 4, 1, 2, 2, HD <= 128 ? 2 : 1>;  // the prefix for the rows of all sequences
-  using Own = PagedTile<HD, 1, 4, 1, 1, HD <= 128 ? 2 : 1>;     // few rows over their own keys
-  using Prompt = PagedTile<HD, 4, 1, 2, 2, HD <= 128 ? 2 : 1>;  // many rows of one sequence
+  using Shared = PagedTile<HD, 4, 1, 2, HD <= 128 ? 2 : 1>;  // the prefix for the rows of all sequences
+  using Own = PagedTile<HD, 1, 4, 1, HD <= 128 ? 2 : 1>;     // few rows over their own keys
+  using Prompt = PagedTile<HD, 4, 1, 2, HD <= 128 ? 2 : 1>;  // many rows of one sequence
 };
 
 // How a call is dealt to workgroups (the same for every head dim: the tiles have the same rows and about the same keys)
@@ -28,9 +28,9 @@ struct Plan {
   int64_t slots() const { return prefix_slots + own_slots; }
 };
 
-// parts that `items` workgroups' keys are split into: about two workgroups a CU, of at least `least` keys each
-int64_t parts(int64_t items, int64_t keys, int64_t least, int cus) {
-  int64_t n = 2 * (int64_t)cus / (items > 0 ? items : 1);
+// parts that `items` workgroups' keys are split into: about `wgs` workgroups in all, of at least `least` keys each
+int64_t parts(int64_t items, int64_t keys, int64_t least, int64_t wgs) {
+  int64_t n = wgs / (items > 0 ? items : 1);
   if (n > keys / least) n = keys / least;
   return n < 1 ? 1 : (n > kMostSlots / 2 ? kMostSlots / 2 : n);
 }
@@ -44,12 +44,16 @@ Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, i
   const int64_t at_most = ragged ? rows / tile + batch : batch * ((group + tile - 1) / tile);
   if (n.prompts) {
     n.row_tiles = at_most;
-    n.own_slots = parts(rows / tile * kv_heads, prefix + most_keys, 256, cus);
+    n.own_slots = parts(rows / tile * kv_heads, prefix + most_keys, 256, 2 * cus);
   } else {
+    // Two workgroups fit a CU.  The prefix takes one place on each, and the sequences' own keys, which memory bounds where the
+    // prefix is bound by its matrix instructions, go on beside it.  us with 128 / 192 / 256 / 512 workgroups for the prefix: 64
+    // sequences behind 8192 keys with 516 of their own on average 47.6 / 48.8 / 50.9 / 61.0, with one 35 / 29 / 28 / 33, behind
+    // 32768 108 / 78 / 64 / 63, eight sequences 21.5 / 19.6 / 19.0 / 18.6.
     n.own_tiles = at_most;
     n.row_tiles = (rows + 127) / 128;
     n.prefix_slots = prefix > 0 ? parts(n.row_tiles * kv_heads, prefix, 256, cus) : 0;
-    n.own_slots = parts(at_most * kv_heads, most_keys, 256, cus);
+    n.own_slots = parts(at_most * kv_heads, most_keys, 256, 2 * cus);
   }
   return n;
 }
@@ -160,6 +164,12 @@ extern "C" int aitamd_prefix_attention(int dtype, const aitamd_paged_cache* cach
   for (int i = 1; i < 6; i += 3)
     if (strides[i] < head_dim || strides[i] > (1 << 24))
       return fail("%s: a token's stride of %lld in the cache: head_dim = %lld to 2^24 is wanted", who, (long long)strides[i], (long long)head_dim);
+  // ... pages apart by less than 2^32 of those 16 bytes, and within one of them by less than 2 GiB
+  for (int i = 0; i < 6; i += 3)
+    if (strides[i] < 0 || strides[i] / 8 > 0xffffffffll) return fail("%s: a page's stride of %lld in the cache is too large", who, (long long)strides[i]);
+  for (int i = 1; i < 6; i += 3)
+    if (strides[i] * cache->page_size * 2 > 0x7fffffffll) return fail("%s: pages of %lld tokens %lld elements apart are too large", who,
+                                                                    (long long)cache->page_size, (long long)strides[i]);
   const Plan plan = make_plan(tokens, batch, heads, kv_heads, prefix_length, p.cache.most_keys, cache->offsets != nullptr, current_device_cus());
   const int64_t need = workspace_of(plan, tokens, heads, head_dim);
   if (need > 0) {
