@@ -286,6 +286,9 @@ int64_t aitamd_gemm_workspace_bytes(int epilogue, int dtype, int algo, int64_t b
   return t.algos[algo].workspace_bytes(p);
 }
 
+// (of the scratch memory: what its users leave zero)
+constexpr int64_t kCounterBytes = 4096;
+
 int aitamd_gemm_rcr_int8(int dtype, int algo, const int8_t* a, const int8_t* b, const float* scale_a, const float* scale_b, const void* bias,
                          void* c, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldc, void* workspace,
                          int64_t workspace_bytes, void* stream) {
@@ -307,12 +310,25 @@ int aitamd_gemm_rcr_int8(int dtype, int algo, const int8_t* a, const int8_t* b, 
   p.lda = lda, p.ldb = ldb, p.ldc = ldc;
   p.ws = workspace, p.ws_bytes = workspace ? workspace_bytes : 0;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const uintptr_t bytes = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | (uintptr_t)K | (M > 1 ? (uintptr_t)lda : 0) |
-      (N > 1 ? (uintptr_t)ldb : 0);
-  if (bytes & 3) {
+  // rows that are no whole dwords
+  const bool odd_k = (K & 3) != 0;
+  const bool odd_a = odd_k || ((reinterpret_cast<uintptr_t>(a) | (M > 1 ? (uintptr_t)lda : 0)) & 3) != 0;
+  const bool odd_b = odd_k || ((reinterpret_cast<uintptr_t>(b) | (N > 1 ? (uintptr_t)ldb : 0)) & 3) != 0;
+  if (odd_a || odd_b) {
     if (algo >= 0) return fail("%s: instance %d takes rows of whole dwords only", who, algo);
-    const hipError_t e = launch_gemm_int8_any(p, dtype == AITAMD_BF16, current_device_cus(), s);
-    return e == hipSuccess ? 0 : fail("%s: launch failed: %s", who, hipGetErrorString(e));
+    // to the scratch memory, behind the counters of the instances that share tiles, which are zero and stay zero
+    const int64_t row = (K + 15) / 16 * 16, bytes_a = odd_a ? M * row : 0, bytes_b = odd_b ? N * row : 0;
+    if (!int8_align_pays(K) || kCounterBytes + bytes_a + bytes_b > p.ws_bytes || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) {
+      const hipError_t e = launch_gemm_int8_any(p, dtype == AITAMD_BF16, current_device_cus(), s);
+      return e == hipSuccess ? 0 : fail("%s: launch failed: %s", who, hipGetErrorString(e));
+    }
+    unsigned char* const at = static_cast<unsigned char*>(workspace) + kCounterBytes;
+    const hipError_t e = launch_int8_align(a, lda, odd_a ? M : 0, at, b, ldb, odd_b ? N : 0, at + bytes_a, K, s);
+    if (e != hipSuccess) return fail("%s: launch failed: %s", who, hipGetErrorString(e));
+    if (odd_a) p.a = at, lda = row;
+    if (odd_b) p.b = at + bytes_a, ldb = row;
+    if (odd_k) K = row;
+    p.ws = nullptr, p.ws_bytes = 0;
   }
   p.K = (int32_t)(K / 2), p.lda = M > 1 ? lda / 2 : K / 2, p.ldb = N > 1 ? ldb / 2 : K / 2;
   return run_gemm(bias ? kEpiBias : kEpiNone, dtype + kNumDTypes, algo, p, s);
@@ -327,6 +343,8 @@ int64_t aitamd_gemm_int8_workspace_bytes(int dtype, int algo, int bias, int64_t 
     const int64_t n = aitamd_gemm_workspace_bytes(epilogue, dtype + kNumDTypes, i, 1, M, N, K / 2);
     most = n > most ? n : most;
   }
+  if ((K & 3) != 0 && int8_align_pays(K) && M > 0 && N > 0 && K <= 131071 && M <= 0x7fffffffll && N <= 0x7fffffffll)
+    most = kCounterBytes + (M + N) * ((K + 15) / 16 * 16);  // (no instance shares tiles of such rows)
   return most;
 }
 

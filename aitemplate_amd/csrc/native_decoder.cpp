@@ -116,6 +116,14 @@ PyObject* gemm_rcr_int8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     c10::SmallVector<int64_t, 6> sizes(a->sizes().begin(), a->sizes().end());
     sizes.back() = N;
     at::Tensor out = make(sizes, type, *a);
+    at::Tensor scratch;  // (rows that are no whole dwords are laid out there first)
+    if (ws == nullptr && K % 4 != 0 && algo < 0) {
+      const int64_t need = aitamd_gemm_int8_workspace_bytes(dt, -1, bias != nullptr, M, N, K);
+      if (need > 0) {
+        scratch = make({need}, at::kByte, *a);
+        ws = &scratch;
+      }
+    }
     const int8_t *pa = static_cast<const int8_t*>(a->data_ptr()), *pb = static_cast<const int8_t*>(b->data_ptr());
     const float *sa = static_cast<const float*>(a_scale->data_ptr()), *sb = static_cast<const float*>(b_scale->data_ptr());
     const void* pbias = pointer(bias);

@@ -570,6 +570,10 @@ def gemm_rcr_int8(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_sca
     if workspace is not None and not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous uint8 GPU tensor (see new_workspace)")
     with torch.cuda.device(device):
+        if workspace is None and K % 4 != 0 and algo < 0:
+            # (rows that are no whole dwords are laid out there first; nothing in it has to be zero for that)
+            need = gemm_int8_workspace_bytes(M, N, K, bias is not None, dtype)
+            workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         rc = _kernels.load().aitamd_gemm_rcr_int8(
             _TORCH_DTYPE_ID[dtype], algo, _p(a2), _p(b), _p(a_scale), _p(b_scale), _p(bias), _p(out2), M, N, K, _row_pitch(a2, "a"),
             _row_pitch(b, "b"), _row_pitch(out2, "out"), _p(workspace), 0 if workspace is None else workspace.numel(), _stream_ptr())
