@@ -541,8 +541,8 @@ __global__ void __launch_bounds__(Shared::NT, Shared::OCC) prefix_decode_kernel(
   }
 }
 
-// Many rows a sequence (prompts, pieces of them).  A workgroup takes a tile of one sequence's rows over the prefix and then over
-// the sequence's own keys.
+// Many rows a sequence (prompts, pieces of them), or one sequence alone.  A workgroup takes a tile of one sequence's rows over the
+// prefix and then over the sequence's own keys.
 template <class T, class Tile>
 __global__ void __launch_bounds__(Tile::NT, Tile::OCC) prefix_prompt_kernel(const PrefixParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
@@ -554,8 +554,11 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) prefix_prompt_kernel(cons
   int tile = id - pair * p.row_tiles, first, last;
   const int part = quotient(pair, p.by_kv_heads);
   if (part >= p.own_slots) return;
-  const int s = sequence_of_tile(p, Tile::ROWS, tile);
-  if (s < 0) return;
+  int s = 0;
+  if (c.batch > 1) {
+    s = sequence_of_tile(p, Tile::ROWS, tile);
+    if (s < 0) return;
+  }
   PagedWork w{};
   rows_of(c, s, first, last);
   w.kv_head = pair - part * c.kv_heads;

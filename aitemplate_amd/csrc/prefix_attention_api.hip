@@ -14,16 +14,16 @@ constexpr int kMaxDevices = 64;
 
 template <int HD>
 struct Tiles {
-  using Shared = PagedTile<HD, 4, 1, 2, HD <= 128 ? 2 : 1>;  // the prefix for the rows of all sequences
-  using Own = PagedTile<HD, 1, 4, 1, HD <= 128 ? 2 : 1>;     // few rows over their own keys
-  using Prompt = PagedTile<HD, 4, 1, 2, HD <= 128 ? 2 : 1>;  // many rows of one sequence
+  using Many = PagedTile<HD, 4, 1, 2, HD <= 128 ? 2 : 1>;  // 128 rows
+  using Few = PagedTile<HD, 1, 4, 1, HD <= 128 ? 2 : 1>;   // 32
 };
 
 // How a call is dealt to workgroups (the same for every head dim: the tiles have the same rows and about the same keys)
 struct Plan {
-  bool prompts;         // tiles of one sequence's rows over prefix and own keys; otherwise the prefix for all rows together
-  int64_t row_tiles;    // of the prefix (decoding), of all sequences at most (prompts)
-  int64_t own_tiles;    // decoding: row tiles of all sequences at most
+  bool each;            // tiles of one sequence's rows over prefix and own keys; otherwise the prefix for all rows together
+  bool many;            // tiles of 128 rows (not each: the prefix's), otherwise 32
+  int64_t row_tiles;    // of all sequences at most (each), of the prefix
+  int64_t own_tiles;    // not each: row tiles of all sequences at most
   int64_t prefix_slots, own_slots;
   int64_t slots() const { return prefix_slots + own_slots; }
 };
@@ -38,20 +38,24 @@ int64_t parts(int64_t items, int64_t keys, int64_t least, int64_t wgs) {
 Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t prefix, int64_t most_keys, bool ragged, int cus) {
   const int64_t group = heads / kv_heads, rows = tokens * group;
   Plan n{};
-  n.prompts = ragged && rows > 32 * batch;
-  const int64_t tile = n.prompts ? 128 : 32;
+  n.many = ragged && rows > 32 * batch;
+  n.each = n.many || batch == 1;
+  const int64_t tile = n.many ? 128 : 32;
   // (every sequence has one tile that is not full at most)
   const int64_t at_most = ragged ? rows / tile + batch : batch * ((group + tile - 1) / tile);
-  if (n.prompts) {
+  if (n.each) {
     n.row_tiles = at_most;
-    n.own_slots = parts(rows / tile * kv_heads, prefix + most_keys, 256, 2 * cus);
+    const int64_t keys = prefix + most_keys;
+    // (four tiles of 128 keys one after the other take as long as one and the join)
+    n.own_slots = !n.many && keys <= 512 ? 1 : parts(rows / tile * kv_heads, keys, 256, 2 * cus);
   } else {
     // Two workgroups fit a CU.  The prefix takes one place on each, and the sequences' own keys, which memory bounds where the
     // prefix is bound by its matrix instructions, go on beside it.  us with 128 / 192 / 256 / 512 workgroups for the prefix: 64
     // sequences behind 8192 keys with 516 of their own on average 47.6 / 48.8 / 50.9 / 61.0, with one 35 / 29 / 28 / 33, behind
     // 32768 108 / 78 / 64 / 63, eight sequences 21.5 / 19.6 / 19.0 / 18.6.
+    n.many = rows > 32;
     n.own_tiles = at_most;
-    n.row_tiles = (rows + 127) / 128;
+    n.row_tiles = n.many ? (rows + 127) / 128 : 1;
     n.prefix_slots = prefix > 0 ? parts(n.row_tiles * kv_heads, prefix, 256, cus) : 0;
     n.own_slots = parts(at_most * kv_heads, most_keys, 256, 2 * cus);
   }
@@ -73,23 +77,21 @@ struct LdsOptIn {
 
 template <class T, int HD>
 hipError_t launch_attention(PrefixParams& p, const Plan& plan, int64_t wgs, hipStream_t stream) {
-  using S = typename Tiles<HD>::Shared;
-  using O = typename Tiles<HD>::Own;
-  using M = typename Tiles<HD>::Prompt;
-  constexpr int kDecodeLds = S::kLdsBytes > O::kLdsBytes ? S::kLdsBytes : O::kLdsBytes;
-  static LdsOptIn decode_opt_in, prompt_opt_in;
-  if (plan.prompts) {
-    auto kernel = prefix_prompt_kernel<T, M>;
-    const hipError_t e = prompt_opt_in(reinterpret_cast<const void*>(kernel), M::kLdsBytes);
+  using Many = typename Tiles<HD>::Many;
+  using Few = typename Tiles<HD>::Few;
+  auto go = [&](auto kernel, int threads, int lds, LdsOptIn& opt_in) {
+    const hipError_t e = opt_in(reinterpret_cast<const void*>(kernel), lds);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(M::NT), M::kLdsBytes, stream, p);
-  } else {
-    auto kernel = prefix_decode_kernel<T, S, O>;
-    const hipError_t e = decode_opt_in(reinterpret_cast<const void*>(kernel), kDecodeLds);
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(S::NT), kDecodeLds, stream, p);
-  }
-  return hipGetLastError();
+    hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(threads), lds, stream, p);
+    return hipGetLastError();
+  };
+  constexpr int kLds = Many::kLdsBytes > Few::kLdsBytes ? Many::kLdsBytes : Few::kLdsBytes;
+  static LdsOptIn opt_in[4];
+  if (plan.each)
+    return plan.many ? go(prefix_prompt_kernel<T, Many>, Many::NT, Many::kLdsBytes, opt_in[0])
+                     : go(prefix_prompt_kernel<T, Few>, Few::NT, Few::kLdsBytes, opt_in[1]);
+  return plan.many ? go(prefix_decode_kernel<T, Many, Few>, Many::NT, kLds, opt_in[2])
+                   : go(prefix_decode_kernel<T, Few, Few>, Few::NT, Few::kLdsBytes, opt_in[3]);
 }
 
 template <class T>
@@ -196,7 +198,7 @@ extern "C" int aitamd_prefix_attention(int dtype, const aitamd_paged_cache* cach
   p.by_own_slots = make_divisor(plan.own_slots);
   p.by_kv_heads = make_divisor(kv_heads);
   int64_t wgs;
-  if (plan.prompts) {
+  if (plan.each) {
     wgs = (plan.row_tiles * kv_heads * plan.own_slots + kNumXcd - 1) / kNumXcd * kNumXcd;
   } else {
     p.prefix_wgs = (int32_t)((plan.prefix_slots * kv_heads + kNumXcd - 1) / kNumXcd * kNumXcd * plan.row_tiles);
