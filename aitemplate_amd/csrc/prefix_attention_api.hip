@@ -35,7 +35,8 @@ int64_t parts(int64_t items, int64_t keys, int64_t least, int64_t wgs) {
   return n < 1 ? 1 : (n > kMostSlots / 2 ? kMostSlots / 2 : n);
 }
 
-Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t prefix, int64_t most_keys, bool ragged, int cus) {
+Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t prefix, int64_t most_keys, int64_t head_dim, bool ragged,
+               int cus) {
   const int64_t group = heads / kv_heads, rows = tokens * group;
   Plan n{};
   n.many = ragged && rows > 32 * batch;
@@ -49,14 +50,18 @@ Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, i
     // (four tiles of 128 keys one after the other take as long as one and the join)
     n.own_slots = !n.many && keys <= 512 ? 1 : parts(rows / tile * kv_heads, keys, 256, 2 * cus);
   } else {
-    // Two workgroups fit a CU.  The prefix takes one place on each, and the sequences' own keys, which memory bounds where the
-    // prefix is bound by its matrix instructions, go on beside it.  us with 128 / 192 / 256 / 512 workgroups for the prefix: 64
-    // sequences behind 8192 keys with 516 of their own on average 47.6 / 48.8 / 50.9 / 61.0, with one 35 / 29 / 28 / 33, behind
-    // 32768 108 / 78 / 64 / 63, eight sequences 21.5 / 19.6 / 19.0 / 18.6.
+    // Two workgroups fit a CU.  The prefix's workgroups, bound by their matrix instructions, come first and should last as long as
+    // what is beside them, the sequences' own keys, which memory bounds: of that only what the table has room for is known, and
+    // half of it taken.  One a CU at most (each leaves its rows' parts to the join), half as many at least.  us with 128 / 192 /
+    // 256 / 512 of them: 64 sequences behind 8192 keys with 516 of their own on average 46.6 / 47.7 / 49.5 / 61.0, with one 35 / 29 /
+    // 28 / 33, 32 sequences 32.6 / 32.5 / 34.0, 64 behind 32768 keys with one of their own 108 / 78 / 64 / 63.
     n.many = rows > 32;
     n.own_tiles = at_most;
     n.row_tiles = n.many ? (rows + 127) / 128 : 1;
-    n.prefix_slots = prefix > 0 ? parts(n.row_tiles * kv_heads, prefix, 256, cus) : 0;
+    const double tiles = (double)(n.row_tiles * kv_heads) * (double)prefix / 64.0, tile_us = 1.4 * (double)(64 + head_dim) / 192.0;
+    const double own_us = (double)(batch * kv_heads * head_dim) * (double)most_keys * 2.0 / 4.5e6;
+    const double wgs = own_us * cus > tiles * tile_us ? tiles * tile_us / own_us : cus;
+    n.prefix_slots = prefix > 0 ? parts(n.row_tiles * kv_heads, prefix, 256, wgs > cus / 2 ? (int64_t)wgs : cus / 2) : 0;
     n.own_slots = parts(at_most * kv_heads, most_keys, 256, 2 * cus);
   }
   return n;
@@ -137,8 +142,8 @@ extern "C" int64_t aitamd_prefix_attention_workspace_bytes(const aitamd_paged_ca
   PagedCache c{};
   if (check_sizes(who, cache, heads, prefix_length, &c)) return -1;
   if (cache->tokens == 0 || heads == 0 || cache->batch == 0 || cache->head_dim == 0) return 0;
-  const Plan plan = make_plan(cache->tokens, cache->batch, heads, cache->kv_heads, prefix_length, c.most_keys, cache->offsets != nullptr,
-                              current_device_cus());
+  const Plan plan = make_plan(cache->tokens, cache->batch, heads, cache->kv_heads, prefix_length, c.most_keys, cache->head_dim,
+                              cache->offsets != nullptr, current_device_cus());
   return workspace_of(plan, cache->tokens, heads, cache->head_dim);
 }
 
@@ -172,7 +177,8 @@ extern "C" int aitamd_prefix_attention(int dtype, const aitamd_paged_cache* cach
   for (int i = 1; i < 6; i += 3)
     if (strides[i] * cache->page_size * 2 > 0x7fffffffll) return fail("%s: pages of %lld tokens %lld elements apart are too large", who,
                                                                     (long long)cache->page_size, (long long)strides[i]);
-  const Plan plan = make_plan(tokens, batch, heads, kv_heads, prefix_length, p.cache.most_keys, cache->offsets != nullptr, current_device_cus());
+  const Plan plan = make_plan(tokens, batch, heads, kv_heads, prefix_length, p.cache.most_keys, head_dim, cache->offsets != nullptr,
+                              current_device_cus());
   const int64_t need = workspace_of(plan, tokens, heads, head_dim);
   if (need > 0) {
     if (!workspace || workspace_bytes < need)
