@@ -338,13 +338,14 @@ int64_t aitamd_gemm_int8_workspace_bytes(int dtype, int algo, int bias, int64_t 
   if (dtype != AITAMD_F16 && dtype != AITAMD_BF16) return 0;
   const int epilogue = bias ? kEpiBias : kEpiNone;
   if (algo >= 0) return aitamd_gemm_workspace_bytes(epilogue, dtype + kNumDTypes, algo, 1, M, N, K / 2);
+  if (M <= 0 || N <= 0 || K <= 0 || M > 0x7fffffffll || N > 0x7fffffffll || K > 131071) return 0;
+  if ((K & 3) != 0)  // (no instance shares tiles of such rows: they are laid out anew)
+    return int8_align_pays(K) ? kCounterBytes + (M + N) * ((K + 15) / 16 * 16) : 0;
   int64_t most = 0;
   for (int i = 0; i < gemm_table(epilogue, dtype + kNumDTypes).count; ++i) {
     const int64_t n = aitamd_gemm_workspace_bytes(epilogue, dtype + kNumDTypes, i, 1, M, N, K / 2);
     most = n > most ? n : most;
   }
-  if ((K & 3) != 0 && int8_align_pays(K) && M > 0 && N > 0 && K <= 131071 && M <= 0x7fffffffll && N <= 0x7fffffffll)
-    most = kCounterBytes + (M + N) * ((K + 15) / 16 * 16);  // (no instance shares tiles of such rows)
   return most;
 }
 

@@ -197,8 +197,8 @@ bool paged_cache(PyObject* const* args, Operands& ops, at::ScalarType type, int6
   return true;
 }
 
-// paged_kv_append(k, v, k_cache, v_cache, block_table, lengths, offsets, q, freqs, interleaved, scale, first_position, q_out): with
-// queries and frequencies only
+// paged_kv_append(k, v, k_cache, v_cache, block_table, lengths, offsets, q, freqs, interleaved, scale, first_position, q_out): without
+// frequencies the queries come back as they are
 PyObject* paged_kv_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
     int64_t first_position;
@@ -208,35 +208,37 @@ PyObject* paged_kv_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const int dt = first_operand(args[0], ops, &k);
     if (dt < 0 || k->dim() != 3 || k->numel() == 0) return not_ordinary();
     const at::ScalarType type = k->scalar_type();
-    const at::Tensor *v = ops.get(args[1], type), *q = ops.get(args[7], type), *freqs = ops.get(args[8], at::kFloat);
+    const at::Tensor *v = ops.get(args[1], type), *q = ops.optional(args[7], type), *freqs = ops.optional(args[8], at::kFloat),
+                     *out = ops.optional(args[12], type);
     const int64_t tokens = k->size(0), head_dim = k->size(2);
     aitamd_paged_cache cache;
     if (!ops.ok || !paged_cache(args + 2, ops, type, tokens, head_dim, &cache) || cache.kv_heads != k->size(1) || v->sizes() != k->sizes() ||
-        !dense(*k) || !dense(*v) || q->dim() != 3 || q->size(0) != tokens || q->size(2) != head_dim || q->numel() == 0 || !dense(*q) ||
-        freqs->dim() != 1 || !freqs->is_contiguous() || freqs->numel() == 0 || 2 * freqs->numel() > head_dim)
+        !dense(*k) || !dense(*v) ||
+        (q != nullptr ? q->dim() != 3 || q->size(0) != tokens || q->size(2) != head_dim || q->numel() == 0 || !dense(*q) : out != nullptr) ||
+        (freqs != nullptr ? freqs->dim() != 1 || !freqs->is_contiguous() || freqs->numel() == 0 || 2 * freqs->numel() > head_dim : out != nullptr))
       return not_ordinary();
+    const bool turns = q != nullptr && freqs != nullptr;
     at::Tensor made;
-    const at::Tensor* out = ops.optional(args[12], type);
-    if (!ops.ok) return not_ordinary();
-    if (out == nullptr) {
+    if (turns && out == nullptr) {
       if (!plain_allocation()) return not_ordinary();
       made = make(q->sizes(), type, *q);
       out = &made;
-    } else if (out->sizes() != q->sizes() || !dense(*out)) {
+    } else if (turns && (out->sizes() != q->sizes() || !dense(*out))) {
       return not_ordinary();
     }
-    const void *pk = k->data_ptr(), *pv = v->data_ptr(), *pq = q->data_ptr();
-    void *po = out->data_ptr(), *stream = current_stream();
-    const float* pf = static_cast<const float*>(freqs->data_ptr());
-    const int64_t kt = k->stride(0), kh = k->stride(1), vt = v->stride(0), vh = v->stride(1), qt = q->stride(0), qh = q->stride(1),
-                  ot = out->stride(0), oh = out->stride(1), heads = q->size(1), rotated = 2 * freqs->numel();
+    const void *pk = k->data_ptr(), *pv = v->data_ptr(), *pq = turns ? q->data_ptr() : nullptr;
+    void *po = turns ? out->data_ptr() : nullptr, *stream = current_stream();
+    const float* pf = freqs == nullptr ? nullptr : static_cast<const float*>(freqs->data_ptr());
+    const int64_t kt = k->stride(0), kh = k->stride(1), vt = v->stride(0), vh = v->stride(1), qt = turns ? q->stride(0) : 0,
+                  qh = turns ? q->stride(1) : 0, ot = turns ? out->stride(0) : 0, oh = turns ? out->stride(1) : 0, heads = turns ? q->size(1) : 0,
+                  rotated = freqs == nullptr ? 0 : 2 * freqs->numel();
     const float scale = (float)PyFloat_AS_DOUBLE(args[10]);
     const int interleaved = args[9] == Py_True;
     const int rc = unlocked([&] {
       return aitamd_paged_kv_append(dt, &cache, pk, kt, kh, pv, vt, vh, pq, qt, qh, po, ot, oh, heads, pf, rotated, first_position, scale,
                                     interleaved, stream);
     });
-    return finish(rc, "paged_kv_append", made.defined() ? &made : nullptr, args[12]);
+    return finish(rc, "paged_kv_append", made.defined() ? &made : nullptr, turns ? args[12] : args[7]);
   });
 }
 

@@ -37,6 +37,9 @@ def calls():
         "append": lambda: (eager.paged_kv_append(k, v, *cache, q=q, freqs=freqs), c.k.nan_to_num(0), c.v.nan_to_num(0)),
         "append_scaled": lambda: (eager.paged_kv_append(k, v, *cache, q=q, freqs=freqs, interleaved=True, scale=1.5, first_position=7,
                                                         q_out=torch.empty_like(q)), c.k.nan_to_num(0)),
+        "append_as_it_is": lambda: (eager.paged_kv_append(k, v, *cache, q=q), c.k.nan_to_num(0)),
+        "append_keys": lambda: (eager.paged_kv_append(k, v, *cache, freqs=freqs), c.k.nan_to_num(0), c.v.nan_to_num(0)),
+        "append_bare": lambda: (eager.paged_kv_append(k, v, *cache), c.k.nan_to_num(0), c.v.nan_to_num(0)),
         "attention": lambda: eager.prefix_attention(q, *cache),
         "attention_shared": lambda: eager.prefix_attention(q, *cache, **shared),
         "attention_scaled": lambda: eager.prefix_attention(q, *cache, scale=0.2, out=torch.empty_like(q), **shared),
@@ -48,7 +51,7 @@ def test_both_paths(name, monkeypatch):
     assert not isinstance(eager._native_decoder, _kernels._NoNative)
     call = calls()[name]
     leaves = lambda r: r if isinstance(r, tuple) else (r,)  # noqa: E731
-    native = [t.clone() for t in leaves(call())]
+    native = [t if t is None else t.clone() for t in leaves(call())]
 
     class Counted:  # the module takes each of these calls
         taken = 0
@@ -65,7 +68,7 @@ def test_both_paths(name, monkeypatch):
     assert Counted.taken >= 1
     monkeypatch.setattr(eager, "_native_decoder", _kernels._NoNative())
     for a, b in zip(native, leaves(call())):
-        assert a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b)
+        assert (a is None and b is None) or (a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b))
 
 
 @pytest.mark.parametrize("python_only", [False, True])
