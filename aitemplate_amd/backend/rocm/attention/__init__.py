@@ -1,1 +1,1 @@
-from . import mem_eff_attention  # noqa: F401  (registers the rocm.mem_eff_attention.* hooks)
+from . import mem_eff_attention, paged_attention  # noqa: F401  (registers the rocm.<op>.* hooks)

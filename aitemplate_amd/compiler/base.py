@@ -354,7 +354,7 @@ class ConstantTensorData:
         import torch
 
         name = {torch.float16: "float16", torch.bfloat16: "bfloat16", torch.float32: "float32",
-                torch.int32: "int32", torch.int64: "int64", torch.bool: "bool"}[t.dtype]
+                torch.int32: "int32", torch.int64: "int64", torch.bool: "bool", torch.int8: "int8"}[t.dtype]
         c = t.detach().contiguous().cpu()
         if c.dtype == torch.bfloat16:
             raw = c.view(torch.int16).numpy().tobytes()

@@ -49,7 +49,7 @@ class _CFormatAITData(ctypes.Structure):
     _fields_ = [("pointer", ctypes.c_void_p), ("shape", _AITemplateShape), ("dtype", ctypes.c_int)]
 
 
-_ENUM_TO_DTYPE = {1: "float16", 2: "float32", 3: "int32", 4: "int64", 5: "bool", 6: "bfloat16"}
+_ENUM_TO_DTYPE = {1: "float16", 2: "float32", 3: "int32", 4: "int64", 5: "bool", 6: "bfloat16", 7: "int8"}
 
 
 def _dlclose(dll: ctypes.CDLL) -> None:
@@ -81,7 +81,7 @@ def torch_dtype_to_string(dtype) -> str:
     import torch
 
     return {torch.float16: "float16", torch.bfloat16: "bfloat16", torch.float32: "float32",
-            torch.int32: "int32", torch.int64: "int64", torch.bool: "bool"}[dtype]
+            torch.int32: "int32", torch.int64: "int64", torch.bool: "bool", torch.int8: "int8"}[dtype]
 
 
 def torch_to_ait_data(tensor) -> AITData:

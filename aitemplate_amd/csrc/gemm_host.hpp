@@ -89,4 +89,8 @@ inline int split_k_rule(int64_t tiles, int64_t k_tiles, int bk, int64_t tile_ele
 // combination is not compiled in.
 GemmAlgoTable gemm_table(int epilogue, int dtype);
 
+// The checked launch behind every entry point (gemm_api.hip): instance `algo`, or the heuristic one for -1.  0, or 1 with the
+// message set.
+int run_gemm(int epilogue, int dtype, int algo, const GemmParams& p, hipStream_t stream);
+
 }  // namespace aitamd

@@ -281,6 +281,7 @@ bool model_dtype(at::ScalarType s, AITemplateDtype* out) {
     case at::kInt: *out = AITemplateDtype::kInt; return true;
     case at::kLong: *out = AITemplateDtype::kLong; return true;
     case at::kBool: *out = AITemplateDtype::kBool; return true;
+    case at::kChar: *out = AITemplateDtype::kInt8; return true;
     default: return false;
   }
 }

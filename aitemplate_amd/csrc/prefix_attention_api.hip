@@ -48,7 +48,7 @@ Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, i
     n.row_tiles = at_most;
     const int64_t keys = prefix + most_keys;
     // (four tiles of 128 keys one after the other take as long as one and the join)
-    n.own_slots = !n.many && keys <= 512 ? 1 : parts(rows / tile * kv_heads, keys, 256, 2 * cus);
+    n.own_slots = !n.many && keys <= 512 ? 1 : parts((rows > tile ? rows / tile : 1) * kv_heads, keys, 256, 2 * cus);
   } else {
     // Two workgroups fit a CU.  The prefix's workgroups, bound by their matrix instructions, come first and should last as long as
     // what is beside them, the sequences' own keys, which memory bounds: of that only what the table has room for is known, and

@@ -5,7 +5,7 @@ from typing import List
 import torch
 
 _TORCH_DTYPE = {"float16": torch.float16, "bfloat16": torch.bfloat16, "float32": torch.float32,
-                "float": torch.float32, "int32": torch.int32, "int64": torch.int64, "bool": torch.bool}
+                "float": torch.float32, "int32": torch.int32, "int64": torch.int64, "bool": torch.bool, "int8": torch.int8}
 
 
 def string_to_torch_dtype(dtype: str):

@@ -4,7 +4,7 @@ An "alignment" is the number of consecutive elements that one memory access may
 cover; the widest access is 128 bits."""
 from typing import List
 
-_ELEM_BYTES = {"float16": 2, "bfloat16": 2, "float32": 4, "float": 4, "int32": 4, "int64": 8, "bool": 1}
+_ELEM_BYTES = {"float16": 2, "bfloat16": 2, "float32": 4, "float": 4, "int32": 4, "int64": 8, "bool": 1, "int8": 1}
 
 
 def get_alignments(dtype: str) -> List[int]:

@@ -59,7 +59,7 @@ struct AITemplateParamShape {
   }
 };
 
-/* reference: model_interface.h:67-75 */
+/* reference: model_interface.h:67-75; kInt8 has no counterpart there */
 enum class AITemplateDtype {
   kUnset = 0,
   kHalf,
@@ -68,6 +68,7 @@ enum class AITemplateDtype {
   kLong,
   kBool,
   kBFloat16,
+  kInt8,
 };
 
 /* reference: model_interface.h:77-89 — one tensor handed across the boundary */
@@ -92,6 +93,7 @@ inline size_t AITemplateDtypeSizeBytes(AITemplateDtype dtype) {
     case AITemplateDtype::kLong:
       return 8;
     case AITemplateDtype::kBool:
+    case AITemplateDtype::kInt8:
       return 1;
     case AITemplateDtype::kUnset:
       throw std::runtime_error("Unset dtype has no size!");
