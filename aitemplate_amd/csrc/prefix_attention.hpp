@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) prefix_prompt_kernel(cons
 
 // The parts of a row joined.  A workgroup takes one row: LANES lanes of 4 dims each, and 256 / LANES groups of those that take
 // every so manieth part; the parts' weights are computed once, by as many lanes.  Bound: latency, of three trips to memory (offsets,
-// (m, l), parts) one after the other.  64 x 32 rows of 33 parts of 128 dims: 28 us with one lane going through a row's parts, <JOIN> so.
+// (m, l), parts) one after the other.  64 x 32 rows of 33 parts of 128 dims: 28 us with one lane going through a row's parts, 6 so (of 17).
 constexpr int kMostSlots = 128;
 template <class T, int LANES>
 __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p, int slots, Divisor by_heads) {

@@ -31,63 +31,76 @@ AITAMD_DEVICE void fill_rotary_table(float2* table, const float* freqs, int n, D
   }
 }
 
-// What a lane handles of a head at once: VEC = 8: eight pairs of halves 16 bytes each (HALVES), or four pairs of neighbours;
-// behind the rotated dims 8 elements.  VEC = 1: one pair, behind them one element.
+// What a lane handles of a head at once, a piece: VEC pairs of halves (VEC elements each), or VEC / 2 pairs of neighbours; behind
+// the rotated dims VEC elements.  VEC = 1: one pair, behind them one element.
 constexpr int rotary_pieces(int n, int head_dim, bool interleaved, int vec) {
-  return vec == 8 ? (interleaved ? n / 4 : n / 8) + (head_dim - 2 * n) / 8 : n + head_dim - 2 * n;
+  return vec > 1 ? (interleaved ? 2 * n / vec : n / vec) + (head_dim - 2 * n) / vec : n + head_dim - 2 * n;
+}
+// The widest pieces that heads of `head_dim` with n pairs divide into (at any alignment: see load_vec)
+inline int rotary_vec(int64_t n, int64_t head_dim, bool interleaved) {
+  for (int vec = 8; vec > 1; vec /= 2)
+    if (head_dim % vec == 0 && (interleaved ? (2 * n) % vec == 0 : n % vec == 0) && (head_dim - 2 * n) % vec == 0) return vec;
+  return 1;
 }
 
-// Piece `c` of the head at `x`, rotated by the token's table, to `y` (which may be `x`)
+template <class T, int N>
+struct RotaryVec {
+  typedef T type __attribute__((ext_vector_type(N)));
+};
+// One piece on its way: where it comes from and goes to, its elements, its pairs' sines (null: handed through)
 template <class T, int VEC, bool INTERLEAVED>
-AITAMD_DEVICE void rotate_piece(const T* x, T* y, int c, int n, const float2* table) {
+struct RotaryPiece {
   using Tr = ElemTraits<T>;
-  using vec8 = typename Tr::vec8;
-  if constexpr (VEC == 8) {
-    const int turned = INTERLEAVED ? n / 4 : n / 8;
+  using vec = typename RotaryVec<T, VEC>::type;
+  T *y1, *y2;
+  const float2* table;
+  vec v1, v2;
+  // piece `c` of the head at `x`, with the token's table, to `y` (which may be `x`)
+  AITAMD_DEVICE void load(const T* x, T* y, int c, int n, const float2* of_token) {
+    const int turned = VEC == 1 ? n : (INTERLEAVED ? 2 * n / VEC : n / VEC);
+    int i1, i2;
     if (c >= turned) {
-      const int at = 2 * n + (c - turned) * 8;
-      store_vec(y + at, load_vec<vec8>(x + at));
-    } else if constexpr (INTERLEAVED) {
-      const vec8 v = load_vec<vec8>(x + c * 8);
-      vec8 o;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 w = table[c * 4 + j];
-        const float a = Tr::to_float(v[2 * j]), b = Tr::to_float(v[2 * j + 1]);
-        o[2 * j] = Tr::from_float(a * w.x - b * w.y);
-        o[2 * j + 1] = Tr::from_float(b * w.x + a * w.y);
-      }
-      store_vec(y + c * 8, o);
+      i1 = 2 * n + (c - turned) * VEC;
+      i2 = i1;
+      table = nullptr;
     } else {
-      const vec8 v1 = load_vec<vec8>(x + c * 8), v2 = load_vec<vec8>(x + n + c * 8);
-      vec8 o1, o2;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float2 w = table[c * 8 + j];
-        const float a = Tr::to_float(v1[j]), b = Tr::to_float(v2[j]);
-        o1[j] = Tr::from_float(a * w.x - b * w.y);
-        o2[j] = Tr::from_float(b * w.x + a * w.y);
-      }
-      store_vec(y + c * 8, o1);
-      store_vec(y + n + c * 8, o2);
+      // (VEC = 1: neighbours are two elements of their own)
+      i1 = INTERLEAVED && VEC == 1 ? 2 * c : c * VEC;
+      i2 = INTERLEAVED ? i1 + 1 : n + i1;
+      table = of_token + (INTERLEAVED && VEC > 1 ? c * (VEC / 2) : c * VEC);
     }
-  } else {
-    if (c >= n) {
-      y[n + c] = x[n + c];
-    } else {
-      const int i1 = INTERLEAVED ? 2 * c : c, i2 = INTERLEAVED ? 2 * c + 1 : n + c;
-      const float2 w = table[c];
-      const float a = Tr::to_float(x[i1]), b = Tr::to_float(x[i2]);
-      y[i1] = Tr::from_float(a * w.x - b * w.y);
-      y[i2] = Tr::from_float(b * w.x + a * w.y);
-    }
+    y1 = y + i1;
+    y2 = y + i2;
+    v1 = load_vec<vec>(x + i1);
+    if constexpr (!INTERLEAVED || VEC == 1) v2 = load_vec<vec>(x + i2);
   }
-}
+  AITAMD_DEVICE void store() {
+    if (table != nullptr) {
+      if constexpr (INTERLEAVED && VEC > 1) {
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+          const float2 w = table[j];
+          const float a = Tr::to_float(v1[2 * j]), b = Tr::to_float(v1[2 * j + 1]);
+          v1[2 * j] = Tr::from_float(a * w.x - b * w.y);
+          v1[2 * j + 1] = Tr::from_float(b * w.x + a * w.y);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float2 w = table[j];
+          const float a = Tr::to_float(v1[j]), b = Tr::to_float(v2[j]);
+          v1[j] = Tr::from_float(a * w.x - b * w.y);
+          v2[j] = Tr::from_float(b * w.x + a * w.y);
+        }
+        store_vec(y2, v2);
+      }
+    }
+    store_vec(y1, v1);
+  }
+};
 
-// Whether heads of `head_dim` with n pairs go 8 elements at a time (at any alignment: see load_vec)
-inline bool rotary_wide(int64_t n, int64_t head_dim, bool interleaved) {
-  return head_dim % 8 == 0 && (interleaved ? (2 * n) % 8 == 0 : n % 8 == 0);
-}
+// Pieces of a lane on their way together (16384 x 32 x 128, 64 dims of neighbours: 46.9 us with one, 40.8 with two)
+constexpr int kRotaryAhead = 2;
 
 // Tokens of a workgroup: about four pieces for each lane where there are tokens enough for every CU, within the table
 inline int rotary_tokens(int64_t tokens, int64_t pieces_per_token, int64_t n, int cus) {

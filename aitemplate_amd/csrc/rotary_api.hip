@@ -33,23 +33,40 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
   });
   __syncthreads();
   const int items = tokens * p.heads * p.pieces;
-  for (int i = threadIdx.x; i < items; i += kRotaryThreads) {
-    const int th = quotient(i, p.by_pieces), piece = i - th * p.pieces;
-    const int t = quotient(th, p.by_heads), head = th - t * p.heads;
-    const int b = quotient(t0 + t, p.by_seq), s = t0 + t - b * p.seq;
-    rotate_piece<T, VEC, INTERLEAVED>(reinterpret_cast<const T*>(p.x) + b * p.x_batch + s * p.x_seq + head * p.x_head,
-                                      reinterpret_cast<T*>(p.out) + b * p.out_batch + s * p.out_seq + head * p.out_head, piece, p.n,
-                                      table + t * p.n);
+  for (int i0 = threadIdx.x; i0 < items; i0 += kRotaryAhead * kRotaryThreads) {
+    RotaryPiece<T, VEC, INTERLEAVED> piece[kRotaryAhead];
+#pragma unroll
+    for (int a = 0; a < kRotaryAhead; ++a) {
+      const int i = i0 + a * kRotaryThreads;
+      if (i >= items) continue;
+      const int th = quotient(i, p.by_pieces), c = i - th * p.pieces;
+      const int t = quotient(th, p.by_heads), head = th - t * p.heads;
+      const int b = quotient(t0 + t, p.by_seq), s = t0 + t - b * p.seq;
+      piece[a].load(reinterpret_cast<const T*>(p.x) + b * p.x_batch + s * p.x_seq + head * p.x_head,
+                    reinterpret_cast<T*>(p.out) + b * p.out_batch + s * p.out_seq + head * p.out_head, c, p.n, table + t * p.n);
+    }
+#pragma unroll
+    for (int a = 0; a < kRotaryAhead; ++a)
+      if (i0 + a * kRotaryThreads < items) piece[a].store();
   }
 }
 
-template <class T>
-hipError_t launch_rotary(const RotaryParams& p, bool wide, bool interleaved, hipStream_t stream) {
-  const auto kernel = wide ? (interleaved ? rotary_kernel<T, 8, true> : rotary_kernel<T, 8, false>)
-                           : (interleaved ? rotary_kernel<T, 1, true> : rotary_kernel<T, 1, false>);
+template <class T, int VEC>
+hipError_t launch_rotary(const RotaryParams& p, bool interleaved, hipStream_t stream) {
+  const auto kernel = interleaved ? rotary_kernel<T, VEC, true> : rotary_kernel<T, VEC, false>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)((p.tokens + p.per_wg - 1) / p.per_wg)), dim3(kRotaryThreads), 0, stream, p);
   return hipGetLastError();
 }
+template <class T>
+hipError_t launch_rotary(const RotaryParams& p, int vec, bool interleaved, hipStream_t stream) {
+  return vec == 8 ? launch_rotary<T, 8>(p, interleaved, stream)
+      : vec == 4  ? launch_rotary<T, 4>(p, interleaved, stream)
+      : vec == 2  ? launch_rotary<T, 2>(p, interleaved, stream)
+                  : launch_rotary<T, 1>(p, interleaved, stream);
+}
+
+// (two: 50.0 us for eight prompts of 517 to 2048 tokens, 32 + 2 x 8 heads of 128 dims; one: 48.8)
+constexpr int kAppendAhead = 1;
 
 struct AppendParams {
   PagedCache cache;
@@ -102,38 +119,53 @@ __global__ void __launch_bounds__(kRotaryThreads) append_kernel(const AppendPara
     fill_rotary_table(table, p.freqs, p.n, p.by_n, tokens, p.scale, 1.0f, [&](int t) { return p.first_position + slot[t]; });
     __syncthreads();
   }
-  const int q_items = p.heads * p.pieces, k_items = q_items + c.kv_heads * p.pieces;
-  for (int i = threadIdx.x; i < tokens * p.per_token; i += kRotaryThreads) {
-    const int t = quotient(i, p.by_token), item = i - t * p.per_token;
-    if (!live[t]) continue;
-    const int64_t row = t0 + t;
-    if (item < q_items) {
-      const int head = quotient(item, p.by_pieces), piece = item - head * p.pieces;
-      rotate_piece<T, VEC, INTERLEAVED>(reinterpret_cast<const T*>(p.q) + row * p.q_token + head * p.q_head,
-                                        reinterpret_cast<T*>(p.q_out) + row * p.q_out_token + head * p.q_out_head, piece, p.n,
-                                        table + t * p.n);
-    } else if (page[t] < 0) {
-      continue;
-    } else if (item < k_items) {
-      const int head = quotient(item - q_items, p.by_pieces), piece = item - q_items - head * p.pieces;
-      rotate_piece<T, VEC, INTERLEAVED>(
-          reinterpret_cast<const T*>(p.k) + row * p.k_token + head * p.k_head,
-          reinterpret_cast<T*>(c.k) + page[t] * c.k_page + in_page[t] * c.k_slot + head * c.k_head, piece, p.n, table + t * p.n);
-    } else {
-      const int head = quotient(item - k_items, p.by_pieces_v), piece = item - k_items - head * p.pieces_v;
-      rotate_piece<T, VEC, INTERLEAVED>(
-          reinterpret_cast<const T*>(p.v) + row * p.v_token + head * p.v_head,
-          reinterpret_cast<T*>(c.v) + page[t] * c.v_page + in_page[t] * c.v_slot + head * c.v_head, piece, 0, table);
+  const int q_items = p.heads * p.pieces, k_items = q_items + c.kv_heads * p.pieces, items = tokens * p.per_token;
+  for (int i0 = threadIdx.x; i0 < items; i0 += kAppendAhead * kRotaryThreads) {
+    RotaryPiece<T, VEC, INTERLEAVED> piece[kAppendAhead];
+    bool on[kAppendAhead];
+#pragma unroll
+    for (int a = 0; a < kAppendAhead; ++a) {
+      const int i = i0 + a * kRotaryThreads;
+      const int t = i < items ? quotient(i, p.by_token) : 0, item = i - t * p.per_token;
+      on[a] = i < items && live[t] && (item < q_items || page[t] >= 0);
+      if (!on[a]) continue;
+      const int64_t row = t0 + t;
+      // where the item's head lies and goes to, and which of its pieces it is
+      const bool is_v = item >= k_items;
+      const int of = item < q_items ? item : (is_v ? item - k_items : item - q_items);
+      const int head = quotient(of, is_v ? p.by_pieces_v : p.by_pieces), at = of - head * (is_v ? p.pieces_v : p.pieces);
+      const T* x;
+      T* y;
+      if (item < q_items) {
+        x = reinterpret_cast<const T*>(p.q) + row * p.q_token + head * p.q_head;
+        y = reinterpret_cast<T*>(p.q_out) + row * p.q_out_token + head * p.q_out_head;
+      } else if (!is_v) {
+        x = reinterpret_cast<const T*>(p.k) + row * p.k_token + head * p.k_head;
+        y = reinterpret_cast<T*>(c.k) + page[t] * c.k_page + in_page[t] * c.k_slot + head * c.k_head;
+      } else {
+        x = reinterpret_cast<const T*>(p.v) + row * p.v_token + head * p.v_head;
+        y = reinterpret_cast<T*>(c.v) + page[t] * c.v_page + in_page[t] * c.v_slot + head * c.v_head;
+      }
+      piece[a].load(x, y, at, is_v ? 0 : p.n, table + t * p.n);
     }
+#pragma unroll
+    for (int a = 0; a < kAppendAhead; ++a)
+      if (on[a]) piece[a].store();
   }
 }
 
-template <class T>
-hipError_t launch_append(const AppendParams& p, bool wide, bool interleaved, hipStream_t stream) {
-  const auto kernel = wide ? (interleaved ? append_kernel<T, 8, true> : append_kernel<T, 8, false>)
-                           : (interleaved ? append_kernel<T, 1, true> : append_kernel<T, 1, false>);
+template <class T, int VEC>
+hipError_t launch_append(const AppendParams& p, bool interleaved, hipStream_t stream) {
+  const auto kernel = interleaved ? append_kernel<T, VEC, true> : append_kernel<T, VEC, false>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)((p.cache.tokens + p.per_wg - 1) / p.per_wg)), dim3(kRotaryThreads), 0, stream, p);
   return hipGetLastError();
+}
+template <class T>
+hipError_t launch_append(const AppendParams& p, int vec, bool interleaved, hipStream_t stream) {
+  return vec == 8 ? launch_append<T, 8>(p, interleaved, stream)
+      : vec == 4  ? launch_append<T, 4>(p, interleaved, stream)
+      : vec == 2  ? launch_append<T, 2>(p, interleaved, stream)
+                  : launch_append<T, 1>(p, interleaved, stream);
 }
 
 int check_rotation(const char* who, int64_t head_dim, int64_t rotated, const float* freqs) {
@@ -160,8 +192,8 @@ extern "C" int aitamd_rotary_embedding(int dtype, const void* x, void* out, cons
   if (batch == 0 || seq == 0 || heads == 0 || head_dim == 0) return 0;
   if (!x || !out || (rotated > 0 && !positions)) return fail("%s: null pointer", who);
   const int64_t n = rotated / 2;
-  const bool wide = rotary_wide(n, head_dim, interleaved != 0);
-  const int64_t pieces = rotary_pieces((int)n, (int)head_dim, interleaved != 0, wide ? 8 : 1);
+  const int vec = rotary_vec(n, head_dim, interleaved != 0);
+  const int64_t pieces = rotary_pieces((int)n, (int)head_dim, interleaved != 0, vec);
   if (batch > 0x7fffffffll / seq || heads > 0x7fffffffll / kRotaryMaxTokens / pieces) return fail("%s: dimension too large", who);
   RotaryParams p{};
   p.x = x;
@@ -185,7 +217,7 @@ extern "C" int aitamd_rotary_embedding(int dtype, const void* x, void* out, cons
   p.by_pieces = make_divisor(pieces);
   p.by_heads = make_divisor(heads);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const hipError_t e = dtype == AITAMD_F16 ? launch_rotary<f16>(p, wide, interleaved != 0, s) : launch_rotary<bf16>(p, wide, interleaved != 0, s);
+  const hipError_t e = dtype == AITAMD_F16 ? launch_rotary<f16>(p, vec, interleaved != 0, s) : launch_rotary<bf16>(p, vec, interleaved != 0, s);
   if (e != hipSuccess) return fail("%s: launch failed: %s", who, hipGetErrorString(e));
   return 0;
 }
@@ -206,9 +238,9 @@ extern "C" int aitamd_paged_kv_append(int dtype, const aitamd_paged_cache* cache
   if (kv_heads > 0 && (!k || !v || !cache->k || !cache->v)) return fail("%s: null pointer", who);
   if (heads > 0 && !q_out) return fail("%s: null pointer (q_out)", who);
   const int64_t n = rotated / 2;
-  const bool wide = rotary_wide(n, head_dim, interleaved != 0);
-  const int64_t pieces = rotary_pieces((int)n, (int)head_dim, interleaved != 0, wide ? 8 : 1);
-  const int64_t pieces_v = wide ? head_dim / 8 : head_dim;
+  const int vec = rotary_vec(n, head_dim, interleaved != 0);
+  const int64_t pieces = rotary_pieces((int)n, (int)head_dim, interleaved != 0, vec);
+  const int64_t pieces_v = head_dim / vec;
   if (heads > 0x7fffff || kv_heads > 0x7fffff || (heads + kv_heads) * pieces + kv_heads * pieces_v > 0x7fffffffll / kRotaryMaxTokens)
     return fail("%s: dimension too large", who);
   p.q = q, p.k = k, p.v = v;
@@ -229,7 +261,7 @@ extern "C" int aitamd_paged_kv_append(int dtype, const aitamd_paged_cache* cache
   p.by_pieces = make_divisor(pieces);
   p.by_pieces_v = make_divisor(pieces_v);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const hipError_t e = dtype == AITAMD_F16 ? launch_append<f16>(p, wide, interleaved != 0, s) : launch_append<bf16>(p, wide, interleaved != 0, s);
+  const hipError_t e = dtype == AITAMD_F16 ? launch_append<f16>(p, vec, interleaved != 0, s) : launch_append<bf16>(p, vec, interleaved != 0, s);
   if (e != hipSuccess) return fail("%s: launch failed: %s", who, hipGetErrorString(e));
   return 0;
 }
