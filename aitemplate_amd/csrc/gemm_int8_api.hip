@@ -56,6 +56,13 @@ int aitamd_gemm_rcr_int8(int dtype, int algo, const int8_t* a, const int8_t* b, 
     if (odd_k) K = row;
     p.ws = nullptr, p.ws_bytes = 0;
   }
+  // (rows further apart than the instances' 32-bit offsets reach over a tile of them)
+  constexpr int64_t kFar = 1 << 22;
+  if (algo < 0 && ((M > 1 && lda > kFar) || (N > 1 && ldb > kFar))) {
+    p.lda = lda, p.ldb = ldb, p.K = (int32_t)K;
+    const hipError_t e = launch_gemm_int8_any(p, dtype == AITAMD_BF16, current_device_cus(), s);
+    return e == hipSuccess ? 0 : fail("%s: launch failed: %s", who, hipGetErrorString(e));
+  }
   p.K = (int32_t)(K / 2), p.lda = M > 1 ? lda / 2 : K / 2, p.ldb = N > 1 ? ldb / 2 : K / 2;
   return run_gemm(bias ? kEpiBias : kEpiNone, dtype + kNumDTypes, algo, p, s);
 }

@@ -48,6 +48,8 @@ inline int paged_cache(const char* who, const aitamd_paged_cache* a, int64_t pag
   if (!a->offsets && a->tokens != a->batch)
     return fail("%s: without offsets every sequence has one row: %lld rows, %lld sequences", who, (long long)a->tokens, (long long)a->batch);
   if (a->batch > 0 && a->tokens > 0 && (!a->lengths || (a->max_pages > 0 && !a->table))) return fail("%s: null pointer (table, lengths)", who);
+  if ((reinterpret_cast<uintptr_t>(a->table) | reinterpret_cast<uintptr_t>(a->lengths) | reinterpret_cast<uintptr_t>(a->offsets)) & 3)
+    return fail("%s: table, lengths and offsets have to be 4-byte aligned", who);
   c->k = a->k, c->v = a->v;
   c->k_page = a->k_page_stride, c->k_slot = a->k_slot_stride, c->k_head = a->k_head_stride;
   c->v_page = a->v_page_stride, c->v_slot = a->v_slot_stride, c->v_head = a->v_head_stride;

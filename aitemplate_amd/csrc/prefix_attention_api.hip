@@ -161,6 +161,7 @@ extern "C" int aitamd_prefix_attention(int dtype, const aitamd_paged_cache* cach
   if (prefix_pages < 0 || prefix_length > prefix_pages * cache->page_size)
     return fail("%s: a prefix of %lld keys does not lie in %lld pages of %lld", who, (long long)prefix_length, (long long)prefix_pages,
                 (long long)cache->page_size);
+  if (reinterpret_cast<uintptr_t>(prefix_table) & 3) return fail("%s: the prefix's table has to be 4-byte aligned", who);
   // 16-byte loads, and 16 keys of a page within 32-bit offsets, one after the other
   if ((reinterpret_cast<uintptr_t>(cache->k) | reinterpret_cast<uintptr_t>(cache->v)) & 15)
     return fail("%s: the cache has to be 16-byte aligned", who);
@@ -177,6 +178,8 @@ extern "C" int aitamd_prefix_attention(int dtype, const aitamd_paged_cache* cach
   for (int i = 1; i < 6; i += 3)
     if (strides[i] * cache->page_size * 2 > 0x7fffffffll) return fail("%s: pages of %lld tokens %lld elements apart are too large", who,
                                                                     (long long)cache->page_size, (long long)strides[i]);
+  p.scale_log2e = scale * 1.4426950408889634f;
+  if (!__builtin_isfinite(p.scale_log2e)) return fail("%s: a scale of %g", who, (double)scale);
   const Plan plan = make_plan(tokens, batch, heads, kv_heads, prefix_length, p.cache.most_keys, head_dim, cache->offsets != nullptr,
                               current_device_cus());
   const int64_t need = workspace_of(plan, tokens, heads, head_dim);
@@ -198,7 +201,6 @@ extern "C" int aitamd_prefix_attention(int dtype, const aitamd_paged_cache* cach
   p.row_tiles = (int32_t)plan.row_tiles;
   p.prefix_slots = (int32_t)plan.prefix_slots;
   p.own_slots = (int32_t)plan.own_slots;
-  p.scale_log2e = scale * 1.4426950408889634f;
   p.by_group = make_divisor(p.group);
   p.by_row_tiles = make_divisor(plan.row_tiles > 0 ? plan.row_tiles : 1);
   p.by_own_slots = make_divisor(plan.own_slots);

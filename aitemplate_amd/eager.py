@@ -776,7 +776,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     Every row sees the first `prefix_length` keys of the pages `prefix_table` [n] int32, which the whole batch shares and which
     are read once for all of its rows, and those of its own sequence's pages up to itself.  Query head h reads key head
     h // (heads / kv_heads).  `scale` is head_dim ** -0.5 unless given.  Rows that see no key are zeros; rows of `out` from
-    offsets[batch] on are left as they were.
+    offsets[batch] on are left as they were.  What lies in a page behind a sequence's last key may be anything; keys and values
+    of the step's later rows do not count for a row, as long as they are finite.
 
     page_size has to be a multiple of 16, head_dim one of 8 up to 256.  `workspace`: a buffer from `new_workspace` of
     `prefix_attention_workspace_bytes`, allocated for the call otherwise; calls that may overlap in time need one each."""

@@ -95,6 +95,8 @@ def test_paged_kv_append():
     refused(append(cache(table=None)), "null")
     refused(append(cache(k=None)), "null")
     refused(append(cache(max_pages=1 << 28)), "large")
+    refused(append(cache(table=66)), "aligned")
+    refused(append(cache(lengths=65)), "aligned")
     refused(append(cache(), k=None), "null")
     refused(append(cache(), q_out=None), "q_out")
     refused(append(cache(), freqs=None), "freqs")
@@ -103,8 +105,9 @@ def test_paged_kv_append():
     assert append(cache(tokens=0, batch=0)) == 0
 
 
-def attention(c=None, dtype=0, q=P, out=P, heads=4, table=P, pages=4, length=0, workspace=None, nbytes=0):
-    return _kernels.load().aitamd_prefix_attention(dtype, c, q, 256, 64, out, 256, 64, heads, table, pages, length, 0.125, workspace,
+def attention(c=None, dtype=0, q=P, out=P, heads=4, table=P, pages=4, length=0, workspace=None, nbytes=0,
+              scale=0.125):
+    return _kernels.load().aitamd_prefix_attention(dtype, c, q, 256, 64, out, 256, 64, heads, table, pages, length, scale, workspace,
                                                    nbytes, None)
 
 
@@ -126,6 +129,9 @@ def test_prefix_attention():
     refused(attention(cache(), length=65), "prefix", "pages")
     refused(attention(cache(), length=-1), "negative")
     refused(attention(cache(k=72)), "aligned")
+    refused(attention(cache(), table=ctypes.c_void_p(66), length=5), "aligned")
+    refused(attention(cache(k_page_stride=-8)), "stride")
+    refused(attention(cache(page_size=1 << 20, max_pages=1, v_slot_stride=1 << 12)), "large")
     refused(attention(cache(v_head_stride=65)), "strides")
     refused(attention(cache(k_slot_stride=56)), "stride")
     refused(attention(cache(k_slot_stride=1 << 25)), "stride")
@@ -133,6 +139,8 @@ def test_prefix_attention():
     refused(attention(cache(max_pages=1 << 27)), "large")
     refused(attention(cache(max_pages=1 << 26)), "keys")
     refused(attention(cache(tokens=1 << 29, offsets=64)), "large")
+    for scale in (float("nan"), float("inf"), 3e38):
+        refused(attention(cache(), scale=scale), "scale")
     refused(attention(cache(), length=50), "workspace")
     refused(attention(cache(), length=50, workspace=P, nbytes=workspace_bytes(cache(), length=50) - 1), "workspace")
     refused(attention(cache(), length=50, workspace=ctypes.c_void_p(72), nbytes=1 << 30), "workspace", "aligned")

@@ -100,6 +100,16 @@ def test_pitches_addresses_and_places(dtype):
     check(got.view(6, 40), *x)
 
 
+def test_rows_far_apart():
+    # 8 MiB from row to row: further than a tile's 32-bit offsets reach
+    M, N, K, pitch = 300, 70, 128, 1 << 23
+    a, b, a_scale, b_scale, bias = inputs(M, N, K, torch.float16)
+    hold = torch.zeros(M * pitch, dtype=torch.int8, device=DEV)
+    far = hold.as_strided((M, K), (pitch, 1))
+    far.copy_(a)
+    check(eager.gemm_rcr_int8(far, b, a_scale, b_scale, bias), a, b, a_scale, b_scale, bias)
+
+
 def test_nothing_to_sum_and_nothing_to_write():
     a, b, a_scale, b_scale, bias = inputs(5, 8, 0, torch.float16)
     assert torch.equal(eager.gemm_rcr_int8(a, b, a_scale, b_scale, bias), bias.expand(5, 8))
