@@ -1,5 +1,5 @@
 // One translation unit per (epilogue, dtype): compiled repeatedly by the
-// Makefile with -DAITAMD_EPI=<EpilogueId> -DAITAMD_DT=<0 fp16 | 1 bf16>.
+// Makefile with -DAITAMD_EPI=<EpilogueId> -DAITAMD_DT=<0 fp16 | 1 bf16 | 2, 3 8-bit integers to fp16, bf16>.
 // It instantiates every tile of gemm_tiles.inc for that pair and exports the
 // resulting launcher table under a C symbol the dispatcher looks up.
 #include <cstdlib>

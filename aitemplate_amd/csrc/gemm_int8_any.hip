@@ -2,7 +2,7 @@
 // of gemm_tiles.inc do not take:  C[m, n] = scale_a[m] scale_b[n] sum_k A[m, k] B[n, k] (+ bias[n]).
 //
 // The slabs go through registers: 16 bytes of a row a lane, read at any address, the next slab's while one is multiplied; the
-// last slab's pieces that K ends in are put together byte by byte, so that nothing past the end of a row is read.  Rows that
+// piece that K ends in is the row's last 16 bytes, shifted, so that nothing past the end of a row is read.  Rows that
 // are not there are the last one once more.  One barrier a slab, two LDS stages.
 // What bounds it: the reads at odd addresses, half a microsecond a slab where a CU has one workgroup.  From a few slabs on it is
 // faster to lay the rows out in scratch memory first (int8_align_kernel, one launch for both operands) and multiply those with the
