@@ -25,9 +25,9 @@ struct QuantizeParams {
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
 template <class T>
-AITAMD_DEVICE float to_whole(uint16_t bits, float most) {
+AITAMD_DEVICE float to_whole(uint16_t bits, float factor, float divisor) {
   // (the bits by value: a bit cast of a vector's element itself takes the vector's first)
-  return __builtin_rintf(ElemTraits<T>::to_float(__builtin_bit_cast(T, bits)) * 127.0f / most);
+  return __builtin_rintf(ElemTraits<T>::to_float(__builtin_bit_cast(T, bits)) * factor / divisor);
 }
 
 // the 8 elements at column c (those past the row as zeros)
@@ -91,11 +91,13 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeParams
   // (a row with an infinity or a NaN has no scale: NaN, which makes every product with it one; a row of zeros has scale 0)
   if (lane == 0) p.scale[row] = bits >= kInf ? __builtin_nanf("") : most / 127.0f;
   const bool zeros = bits == 0 || bits >= kInf;
+  // (127 times a bfloat16 may leave the range of 32 bits: both sides of the division 2^-32 times as large there)
+  const float shrink = most > 0x1p100f ? 0x1p-32f : 1.0f, factor = 127.0f * shrink, divisor = most * shrink;
   auto put = [&](u16x8 w, int c) {
     u32x2 o = {};
     if (!zeros) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j / 4] |= ((uint32_t)(int)to_whole<T>(w[j], most) & 0xffu) << (8 * (j % 4));
+      for (int j = 0; j < 8; ++j) o[j / 4] |= ((uint32_t)(int)to_whole<T>(w[j], factor, divisor) & 0xffu) << (8 * (j % 4));
     }
     if (c + 8 <= p.columns) {
       store_vec(q + c, o);

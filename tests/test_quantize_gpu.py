@@ -41,6 +41,19 @@ def test_every_value_against_every_maximum(dtype):
         check(x, *eager.quantize_rows(x))
 
 
+@pytest.mark.parametrize("columns", [40, 3000, 20000])
+def test_the_largest_and_smallest_numbers(columns):
+    # 127 times the largest bfloat16 is beyond 32-bit floats
+    g = torch.Generator(device=DEV).manual_seed(columns)
+    x = (torch.rand(8, columns, device=DEV, generator=g) * 2 - 1).bfloat16()
+    x *= torch.tensor([2.0 ** e for e in (127, 126, 121, 120, 101, 100, -100, -120)], device=DEV)[:, None].bfloat16()
+    x[0, 3], x[0, 5] = torch.finfo(torch.bfloat16).max, torch.finfo(torch.bfloat16).min
+    check(x, *eager.quantize_rows(x))
+    x = torch.full((2, columns), torch.finfo(torch.float16).max, device=DEV, dtype=torch.float16)
+    x[1, ::2] = 2.0 ** -24
+    check(x, *eager.quantize_rows(x))
+
+
 def test_shapes_pitch_and_places():
     x = torch.randn(3, 5, 96, device=DEV).half()
     q, s = eager.quantize_rows(x)
