@@ -303,39 +303,36 @@ AITAMD_DEVICE void attend(const PrefixParams& p, const PagedWork& w, unsigned ch
       const bool shared = t < w.prefix_tiles;
       if (t == w.prefix_tiles) first = 0;
       lds_T* const vb = (lds_T*)(sV + v_at);
-      if (first < (shared ? p.prefix : some_own)) {
-        f32x16 s[KB];
-        scores(sK + k_at, s);
-        const bool whole = first + 32 * KB <= (shared ? p.prefix : every);
-        bool full = !ref_ok || !whole;
-        if (!full) {
-          // The probabilities against the reference point the row has (exact whatever it is, as long as nothing leaves its range),
-          // between the matrix instructions of the tile before.
-          const float l_before = l_run, mc = -m_run * cs;
+      // (the last tiles may hold nothing that this wave's rows see: masked like any other.  us, eight ragged prompts, with a branch
+      // around all of this / so: head dim 64 63.7 / 62.9, 80 82.4 / 79.3, 128 94.4 / 95.3, 256 251 / 252)
+      f32x16 s[KB];
+      scores(sK + k_at, s);
+      const bool whole = first + 32 * KB <= (shared ? p.prefix : every);
+      bool full = !ref_ok || !whole;
+      if (!full) {
+        // The probabilities against the reference point the row has (exact whatever it is, as long as nothing leaves its range),
+        // between the matrix instructions of the tile before.
+        const float l_before = l_run, mc = -m_run * cs;
 #pragma unroll
-          for (int i = 0; i < 2 * KB; ++i) {
+        for (int i = 0; i < 2 * KB; ++i) {
 #pragma unroll
-            for (int ot = 0; ot < OT; ++ot) oacc[ot] = Tr::mfma32(read_v(vb, i, ot), pf[i], oacc[ot]);
+          for (int ot = 0; ot < OT; ++ot) oacc[ot] = Tr::mfma32(read_v(vb, i, ot), pf[i], oacc[ot]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              pf[i][j] = Tr::from_float(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][(i & 1) * 8 + j], cs, mc)));
-            l_run = add_elements(pf[i], l_run);
-          }
-          if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(l_run <= kMaxRowSum)) != 0, 0)) {
-            l_run = l_before;  // (NaN, or a maximum far above the reference point: again, in the full form)
-            full = true;
-            due = false;
-          }
+          for (int j = 0; j < 8; ++j)
+            pf[i][j] = Tr::from_float(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][(i & 1) * 8 + j], cs, mc)));
+          l_run = add_elements(pf[i], l_run);
         }
-        if (full) {
-          if (due) second_product(vb);
-          due = true;
-          full_form(s, first, shared ? p.prefix : seen, whole);
-          ref_ok = __builtin_amdgcn_ballot_w64(__builtin_isinf(m_run)) == 0;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(l_run <= kMaxRowSum)) != 0, 0)) {
+          l_run = l_before;  // (NaN, or a maximum far above the reference point: again, in the full form)
+          full = true;
+          due = false;
         }
-      } else if (due) {
-        second_product(vb);
-        due = false;
+      }
+      if (full) {
+        if (due) second_product(vb);
+        due = first < (shared ? p.prefix : some_own);
+        full_form(s, first, shared ? p.prefix : seen, whole);
+        ref_ok = __builtin_amdgcn_ballot_w64(__builtin_isinf(m_run)) == 0;
       }
       k_at = k_at == (Tile::NK - 1) * Tile::STAGE ? 0 : k_at + Tile::STAGE;
       if (t > w.t_lo) v_at = v_at == (Tile::NV - 1) * Tile::STAGE ? 0 : v_at + Tile::STAGE;  // (V(t): behind V(t - 1)'s, which for the first is none)
