@@ -86,6 +86,7 @@ ONE_TOKEN = [
     ([513, 100, 31], 4, 2, 256, 64, 2041),
     ([5000], 4, 1, 128, 16, 0),             # one sequence, its keys shared between workgroups
     ([3], 4, 1, 128, 16, 9000),
+    ([20000, 3], 4, 1, 64, 16, 20000),      # as many parts of a row as the join takes
 ]
 
 
