@@ -29,4 +29,8 @@ inline int current_device_cus() {
   return device_cus(dev);
 }
 
+// Workgroups of `threads` that one launch may have: the runtime counts a launch's threads in 32 bits, refuses 2^32 and
+// launches the rest of a division by it for more.
+constexpr int64_t most_workgroups(int threads) { return 0xffffffffll / threads; }
+
 }  // namespace aitamd

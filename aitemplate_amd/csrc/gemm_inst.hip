@@ -240,6 +240,7 @@ hipError_t launch_kernel(const GemmParams& p_in, hipStream_t stream) {
       p.split_k = 1;
     grid = dim3((unsigned)(total * p.split_k), 1, 1);
   }
+  if (grid.x > most_workgroups(Tile::NT)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(kernel, grid, dim3(Tile::NT), Tile::kLdsBytes, stream, p);
   return hipGetLastError();
 }

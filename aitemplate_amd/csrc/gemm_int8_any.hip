@@ -10,6 +10,7 @@
 #include "gemm_int8_any.hpp"
 
 #include "common.hpp"
+#include "device.hpp"
 #include "epilogue.hpp"
 
 namespace aitamd {
@@ -190,7 +191,7 @@ hipError_t launch(GemmParams p, hipStream_t stream) {
   static_assert(2 * Tile::STAGE <= 64 * 1024, "no opt-in to more LDS");
   set_tiles(p, Tile::BM, Tile::BN, 3, -1);
   const int64_t total = (int64_t)p.tiles_m * p.tiles_n;
-  if (total > 0x7fffffffll) return hipErrorInvalidValue;
+  if (total > most_workgroups(Tile::NT)) return hipErrorInvalidValue;
   const auto kernel = p.bias != nullptr ? gemm_int8_any_kernel<Out, Tile, true> : gemm_int8_any_kernel<Out, Tile, false>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)total), dim3(Tile::NT), 2 * Tile::STAGE, stream, p);
   return hipGetLastError();

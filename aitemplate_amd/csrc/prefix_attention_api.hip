@@ -212,7 +212,7 @@ extern "C" int aitamd_prefix_attention(int dtype, const aitamd_paged_cache* cach
     p.prefix_wgs = (int32_t)((plan.prefix_slots * kv_heads + kNumXcd - 1) / kNumXcd * kNumXcd * plan.row_tiles);
     wgs = p.prefix_wgs + plan.own_tiles * kv_heads * plan.own_slots;
   }
-  if (wgs > 0x7fffffffll || tokens * heads > 0x7fffffffll) return fail("%s: dimension too large", who);
+  if (wgs > most_workgroups(256) || (plan.slots() > 1 && tokens * heads > most_workgroups(256))) return fail("%s: dimension too large", who);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const hipError_t e = dtype == AITAMD_F16 ? launch_all<f16>(p, plan, wgs, s) : launch_all<bf16>(p, plan, wgs, s);
   if (e != hipSuccess) return fail("%s: launch failed: %s", who, hipGetErrorString(e));

@@ -128,8 +128,15 @@ hipError_t launch_quantize(const QuantizeParams& p, hipStream_t stream) {
       : p.columns <= 16384 ? quantize_rows_kernel<T, 256, 8>
                            : quantize_rows_kernel<T, 256, 0>;
   const int64_t rows_per_wg = p.columns <= 128 ? 16 : (p.columns <= 1024 ? 4 : 1);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)((p.rows + rows_per_wg - 1) / rows_per_wg)), dim3(256), 0, stream, p);
-  return hipGetLastError();
+  const int64_t most = most_workgroups(256) * rows_per_wg;
+  for (int64_t row = 0; row < p.rows; row += most) {
+    const QuantizeParams part{reinterpret_cast<const T*>(p.x) + row * p.ldx, p.q + row * p.ldq, p.scale + row,
+                              p.rows - row < most ? p.rows - row : most, p.ldx, p.ldq, p.columns};
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((part.rows + rows_per_wg - 1) / rows_per_wg)), dim3(256), 0, stream, part);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace

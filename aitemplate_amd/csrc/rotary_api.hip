@@ -14,7 +14,7 @@ struct RotaryParams {
   const void* positions;
   const float* freqs;
   int32_t tokens, heads, n, seq;
-  int32_t per_wg, pieces, positions_64;
+  int32_t first, per_wg, pieces, positions_64;  // first: the launch's first token
   int64_t x_batch, x_seq, x_head, out_batch, out_seq, out_head, pos_batch, pos_seq;
   float scale, sine_sign;
   Divisor by_n, by_seq, by_pieces, by_heads;
@@ -24,7 +24,7 @@ struct RotaryParams {
 template <class T, int VEC, bool INTERLEAVED>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryParams p) {
   __shared__ float2 table[kRotaryTable];
-  const int t0 = blockIdx.x * p.per_wg;
+  const int t0 = p.first + blockIdx.x * p.per_wg;
   const int tokens = p.tokens - t0 < p.per_wg ? p.tokens - t0 : p.per_wg;
   fill_rotary_table(table, p.freqs, p.n, p.by_n, tokens, p.scale, p.sine_sign, [&](int t) -> int64_t {
     const int b = quotient(t0 + t, p.by_seq);
@@ -51,11 +51,22 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
   }
 }
 
+// p.per_wg tokens a workgroup, in as many launches as it takes
+template <class P>
+hipError_t launch_tokens(void (*kernel)(P), P p, int64_t tokens, hipStream_t stream) {
+  const int64_t wgs = (tokens + p.per_wg - 1) / p.per_wg, most = most_workgroups(kRotaryThreads);
+  for (int64_t wg = 0; wg < wgs; wg += most) {
+    p.first = (int32_t)(wg * p.per_wg);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(wgs - wg < most ? wgs - wg : most)), dim3(kRotaryThreads), 0, stream, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 template <class T, int VEC>
 hipError_t launch_rotary(const RotaryParams& p, bool interleaved, hipStream_t stream) {
-  const auto kernel = interleaved ? rotary_kernel<T, VEC, true> : rotary_kernel<T, VEC, false>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)((p.tokens + p.per_wg - 1) / p.per_wg)), dim3(kRotaryThreads), 0, stream, p);
-  return hipGetLastError();
+  return launch_tokens(interleaved ? rotary_kernel<T, VEC, true> : rotary_kernel<T, VEC, false>, p, p.tokens, stream);
 }
 template <class T>
 hipError_t launch_rotary(const RotaryParams& p, int vec, bool interleaved, hipStream_t stream) {
@@ -73,7 +84,7 @@ struct AppendParams {
   const void *q, *k, *v;
   void* q_out;
   const float* freqs;
-  int32_t heads, n, per_wg, pieces, pieces_v, per_token;
+  int32_t heads, n, first, per_wg, pieces, pieces_v, per_token;
   int64_t q_token, q_head, q_out_token, q_out_head, k_token, k_head, v_token, v_head, first_position;
   float scale;
   Divisor by_n, by_token, by_pieces, by_pieces_v;
@@ -89,7 +100,7 @@ __global__ void __launch_bounds__(kRotaryThreads) append_kernel(const AppendPara
   __shared__ int32_t in_page[kRotaryMaxTokens];
   __shared__ bool live[kRotaryMaxTokens];
   const PagedCache& c = p.cache;
-  const int t0 = blockIdx.x * p.per_wg;
+  const int t0 = p.first + blockIdx.x * p.per_wg;
   const int tokens = c.tokens - t0 < p.per_wg ? c.tokens - t0 : p.per_wg;
   const int s0 = c.offsets != nullptr ? sequence_of_row(c, t0) : t0;  // (every wave for itself)
   if ((int)threadIdx.x < tokens) {
@@ -156,9 +167,7 @@ __global__ void __launch_bounds__(kRotaryThreads) append_kernel(const AppendPara
 
 template <class T, int VEC>
 hipError_t launch_append(const AppendParams& p, bool interleaved, hipStream_t stream) {
-  const auto kernel = interleaved ? append_kernel<T, VEC, true> : append_kernel<T, VEC, false>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)((p.cache.tokens + p.per_wg - 1) / p.per_wg)), dim3(kRotaryThreads), 0, stream, p);
-  return hipGetLastError();
+  return launch_tokens(interleaved ? append_kernel<T, VEC, true> : append_kernel<T, VEC, false>, p, p.cache.tokens, stream);
 }
 template <class T>
 hipError_t launch_append(const AppendParams& p, int vec, bool interleaved, hipStream_t stream) {

@@ -139,6 +139,8 @@ def test_prefix_attention():
     refused(attention(cache(max_pages=1 << 27)), "large")
     refused(attention(cache(max_pages=1 << 26)), "keys")
     refused(attention(cache(tokens=1 << 29, offsets=64)), "large")
+    # (2^24 workgroups of 256 threads are more than a launch takes)
+    refused(attention(cache(tokens=1 << 24, batch=1 << 24), workspace=P, nbytes=1 << 62), "large")
     for scale in (float("nan"), float("inf"), 3e38):
         refused(attention(cache(), scale=scale), "scale")
     refused(attention(cache(), length=50), "workspace")

@@ -137,6 +137,20 @@ def test_offsets_past_32_bits():
     assert torch.equal(k_all[at:at + D], k[0, 0]) and torch.equal(v_all[at:at + D], v[0, 0])
 
 
+def test_more_tokens_than_one_launch_takes():
+    # (2^24 workgroups of 64 tokens and two more)
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GiB of free memory")
+    tokens, page = (1 << 30) + 70, 1 << 20
+    k = torch.ones(tokens, 1, 2, dtype=torch.float16, device=DEV)
+    k_cache, v_cache = (torch.zeros(tokens // page + 1, page, 1, 2, dtype=torch.float16, device=DEV) for _ in range(2))
+    table = torch.arange(k_cache.shape[0], dtype=torch.int32, device=DEV)[None]
+    lengths, offsets = (torch.tensor(at, dtype=torch.int32, device=DEV) for at in ([0], [0, tokens]))
+    eager.paged_kv_append(k, k, k_cache, v_cache, table, lengths, offsets)
+    for cache in (k_cache, v_cache):
+        assert (cache.view(-1)[:2 * tokens] == 1).all() and not cache.view(-1)[2 * tokens:].any()
+
+
 def test_captured_and_replayed_while_lengths_grow():
     c = Paged(torch.float16, [3, 14], [1, 1], 2, 64, 16, spare=8)
     c.table = torch.cat((c.table, c.spare[:4].int().view(2, 2)), 1).contiguous()

@@ -84,6 +84,13 @@ def test_rows_of_zeros_infinities_and_nan(dtype, columns):
     assert s[1] == 0 and torch.isnan(s[2:5]).all() and not q[1:5].any()
 
 
+def test_more_rows_than_one_launch_takes():
+    # (2^24 workgroups of 16 rows and one more)
+    x = torch.ones((1 << 28) + 5, 1, dtype=torch.float16, device=DEV)
+    q, s = eager.quantize_rows(x)
+    assert (q == 127).all() and (s == 1 / torch.tensor(127.0, device=DEV)).all()
+
+
 def test_captured_and_replayed():
     x = torch.randn(64, 4096, device=DEV).half()
     q, s = eager.quantize_rows(x)

@@ -72,6 +72,16 @@ def test_far_positions(far):
     assert ((eager.rotary_embedding(x, positions, freqs).double() - want).abs() <= allowed).all()
 
 
+def test_more_tokens_than_one_launch_takes():
+    # (2^24 workgroups of 64 tokens and two more)
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GiB of free memory")
+    x = torch.ones((1 << 30) + 70, 1, 2, dtype=torch.float16, device=DEV)
+    positions = torch.zeros(x.shape[0], dtype=torch.int32, device=DEV)
+    assert eager.rotary_embedding(x, positions, freqs_of(2), scale=2.0, out=x) is x
+    assert (x == 2).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_strides_batches_and_places(dtype):
     B, S, H, D = 3, 17, 4, 64
