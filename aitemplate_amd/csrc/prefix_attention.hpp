@@ -26,12 +26,34 @@
 
 namespace aitamd {
 
+// The weights exp(c (s - m)) are rounded to the type's 16 bits for the second product, by half a step at most (2^-11 relative in fp16,
+// 2^-8 in bf16), and their sum is taken of the rounded ones: a result moves by as much of the weighted mean of |v|.  As sums of two
+// 16-bit numbers they would take the second product, half of the matrix instructions, twice.  Error of three timed cases against
+// 64 bits (norm, relative): 2.9e-4 in fp16 and 2.3e-3 in bf16, of which rounding the result alone is 2.1e-4 and 1.7e-3.
+//
+// fp16 also ends at 2^-25 below and at 2^16 above.  What is below is lost, however many keys it is of: with the reference point's
+// weight at 1, 2^17 keys of 2^-25.5 of the largest weight each, 0.3 % of the result, were none.  So weights in fp16 are held
+// 2^kRaiseLog2 times as large (the sum too: it cancels), and the full form leaves the reference point 2^kLazyLog2 below a row's
+// maximum at most, 2^15 together.  What is lost is below 2^-36 of the largest weight, n such keys n 2^-36.  bf16 has the range of 32
+// bits.
+template <class T>
+struct Weights {
+  static constexpr float kRaiseLog2 = 11.0f, kLazyLog2 = 4.0f;
+  // Row sums up to which the fast form stands: a weight out of range is an infinity and shows in any finite bound; 2^30 keys of up
+  // to 2^16 do not trip it, and their products with values stay far below the largest float.
+  static constexpr float kMaxSum = 0x1p47f;
+};
+template <>
+struct Weights<bf16> {
+  static constexpr float kRaiseLog2 = 0.0f, kLazyLog2 = 8.0f, kMaxSum = kMaxRowSum;
+};
+
 struct PrefixParams {
   PagedCache cache;
   const void* q;
   void* out;
   float* part_o;   // [slot, token, head, head_dim]
-  float2* part_ml; // [slot, token, head]: c * m and l
+  float2* part_ml; // [slot, token, head]: c * m and l (l, as part_o, 2^kRaiseLog2 times as large: see Weights)
   const int32_t* prefix_table;
   int64_t q_token, q_head, out_token, out_head;
   int32_t heads, group, head_dim, prefix;
@@ -90,6 +112,7 @@ AITAMD_DEVICE void load_to_lds(__amdgpu_buffer_rsrc_t r, void* dst, uint32_t off
 template <class T, class Tile>
 AITAMD_DEVICE void attend(const PrefixParams& p, const PagedWork& w, unsigned char* smem_raw) {
   using Tr = ElemTraits<T>;
+  using W = Weights<T>;
   using vec8 = typename Tr::vec8;
   using vec4 = typename Tr::vec4;
   typedef __attribute__((address_space(3))) const T lds_T;
@@ -255,15 +278,14 @@ AITAMD_DEVICE void attend(const PrefixParams& p, const PagedWork& w, unsigned ch
       for (int e = 0; e < 16; ++e) most = fmaxf(most, s[kb][e]);
     most = max_across_halves(most);
     // The reference point moves only when the row maximum has grown by more than kLazyLog2 binary orders since it was last
-    // taken: until then P may exceed 1 by at most 2^kLazyLog2, harmless in fp32 sums and in P.
-    constexpr float kLazyLog2 = 8.0f;
+    // taken: until then P is 2^kLazyLog2 times what it is at the reference point at most, harmless in fp32 sums and in P.
     const float m_cand = fmaxf(m_run, most);
     const float drift = (m_run - m_cand) * cs;  // <= 0; -inf (or NaN for inf - inf) on the first live tile
-    const bool move = !(drift >= -kLazyLog2);
+    const bool move = !(drift >= -W::kLazyLog2);
     const float m_new = move ? m_cand : m_run;
     const float m_safe = __builtin_isinf(m_new) ? 0.0f : m_new;  // every key so far masked
     const float alpha = !move ? 1.0f : (__builtin_isinf(m_run) ? 0.0f : __builtin_amdgcn_exp2f(drift));
-    const float mc = -m_safe * cs;
+    const float mc = W::kRaiseLog2 - m_safe * cs;
     l_run *= alpha;
 #pragma unroll
     for (int i = 0; i < 2 * KB; ++i) {
@@ -312,7 +334,7 @@ AITAMD_DEVICE void attend(const PrefixParams& p, const PagedWork& w, unsigned ch
       if (!full) {
         // The probabilities against the reference point the row has (exact whatever it is, as long as nothing leaves its range),
         // between the matrix instructions of the tile before.
-        const float l_before = l_run, mc = -m_run * cs;
+        const float l_before = l_run, mc = W::kRaiseLog2 - m_run * cs;
 #pragma unroll
         for (int i = 0; i < 2 * KB; ++i) {
 #pragma unroll
@@ -322,7 +344,7 @@ AITAMD_DEVICE void attend(const PrefixParams& p, const PagedWork& w, unsigned ch
             pf[i][j] = Tr::from_float(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][(i & 1) * 8 + j], cs, mc)));
           l_run = add_elements(pf[i], l_run);
         }
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(l_run <= kMaxRowSum)) != 0, 0)) {
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(l_run <= W::kMaxSum)) != 0, 0)) {
           l_run = l_before;  // (NaN, or a maximum far above the reference point: again, in the full form)
           full = true;
           due = false;

@@ -361,9 +361,10 @@ AITAMD_API int aitamd_paged_kv_append(int dtype, const aitamd_paged_cache* cache
  * sequence's own pages (the step's keys are in the cache already, lengths are those from before the step; none where
  * that is not positive, all that the table has room for where there are not as many):
  *   out[r, h, :] = sum_n softmax_n(scale * q[r, h, :] . k[n, h / (heads / kv_heads), :]) v[n, h / (heads / kv_heads), :]
- * Rows that see no key are written as zeros.  A table entry that a row's keys need and that is not in [0, pages) counts as
- * a page of zeros.  What lies behind a sequence's last key is not read.  Keys that only later rows of the step see do not
- * count for a row, as long as their values are finite.
+ * Sums and maxima are held in 32 bits, the weights of a tile's keys in the type's 16 bits (in fp16 those below 2^-36 of the
+ * row's largest count as none).  Rows that see no key are written as zeros.  A table entry that a row's keys need and that is
+ * not in [0, pages) counts as a page of zeros.  What lies behind a sequence's last key is not read.  Keys that only later rows
+ * of the step see do not count for a row, as long as their values are finite.
  * page_size a multiple of 16; head_dim a multiple of 8 up to 256; heads a multiple of kv_heads; cache 16-byte aligned, its
  * strides multiples of 8; q and out with contiguous head dims, their strides in elements.
  * workspace: device memory, 16-byte aligned, of aitamd_prefix_attention_workspace_bytes() bytes (may be null where that is
