@@ -56,20 +56,24 @@ def rotary_func_call(func_attrs: Dict[str, Any], indent: str = "  ") -> str:
 
 # ---- the paged cache ----
 
-_CACHE_PARAMS = ("void* k_cache, void* v_cache, const void* block_table, const void* lengths, const void* offsets, int64_t tokens, "
-                 "int64_t batch, int64_t pages, int64_t max_pages")
+_CACHE_PARAMS = ("void* k_cache, void* v_cache, const void* block_table, const void* lengths, const void* offsets, int64_t ends, "
+                 "int64_t tokens, int64_t batch, int64_t pages, int64_t max_pages")
 
 
-def _cache_code(k_cache) -> str:
+def _cache_code(func_name: str, k_cache) -> str:
+    """The cache's description; `ends`: the number of offsets, which the kernels follow to offsets[batch]."""
     page_size, kv_heads, head_dim = (_value(k_cache, i) for i in (1, 2, 3))
     strides = f"{page_size * kv_heads * head_dim}, {kv_heads * head_dim}, {head_dim}"
-    return (f"  const aitamd_paged_cache cache = {{k_cache, v_cache, pages, {page_size}, {kv_heads}, {head_dim}, {strides},\n"
+    return (f'  if (offsets != nullptr && ends != batch + 1)\n    throw std::runtime_error("{func_name}: " + std::to_string(ends) + '
+            '" offsets for " + std::to_string(batch) + " sequences (batch + 1 are wanted)");\n'
+            f"  const aitamd_paged_cache cache = {{k_cache, v_cache, pages, {page_size}, {kv_heads}, {head_dim}, {strides},\n"
             f"                                    {strides}, static_cast<const int32_t*>(block_table), max_pages, max_pages,\n"
             "                                    static_cast<const int32_t*>(lengths), static_cast<const int32_t*>(offsets), batch, tokens};")
 
 
 def _cache_args(q, k_cache, v_cache, block_table, lengths, offsets):
-    return [_name(k_cache), _name(v_cache), _name(block_table), _name(lengths), _name(offsets) if offsets is not None else "nullptr",
+    ends = [_name(offsets), _dim(offsets, 0)] if offsets is not None else ["nullptr", "0"]
+    return [_name(k_cache), _name(v_cache), _name(block_table), _name(lengths)] + ends + [
             _dim(q, 0), _dim(lengths, 0), _dim(k_cache, 0), _dim(block_table, 1)]
 
 
@@ -84,7 +88,7 @@ def append_gen_function(func_attrs: Dict[str, Any]) -> str:
     heads, head_dim, kv_heads = _value(q, 1), _value(q, 2), _value(k_cache, 2)
     return f"""{common.HEADER}
 {_append_signature(func_name)} {{
-{_cache_code(k_cache)}
+{_cache_code(func_name, k_cache)}
   check_rc(aitamd_paged_kv_append({common.DTYPE_ID[q._attrs["dtype"]]}, &cache, k, {kv_heads * head_dim}, {head_dim}, v,
                                   {kv_heads * head_dim}, {head_dim}, q, {heads * head_dim}, {head_dim}, out, {heads * head_dim},
                                   {head_dim}, {heads}, static_cast<const float*>(freqs), {2 * _value(freqs, 0)},
@@ -119,7 +123,7 @@ def attention_gen_function(func_attrs: Dict[str, Any]) -> str:
     # (behind the first 4096 bytes of the shared workspace, which other ops keep zero)
     return f"""{common.HEADER}
 {_attention_signature(func_name)} {{
-{_cache_code(k_cache)}
+{_cache_code(func_name, k_cache)}
   check_rc(aitamd_prefix_attention({common.DTYPE_ID[q._attrs["dtype"]]}, &cache, q, {heads * head_dim}, {head_dim}, out,
                                    {heads * head_dim}, {head_dim}, {heads}, static_cast<const int32_t*>(prefix_table), prefix_pages,
                                    {func_attrs["prefix_length"]}, {float_literal(scale)}, workspace + 4096, workspace_bytes - 4096,

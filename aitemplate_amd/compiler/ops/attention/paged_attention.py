@@ -28,6 +28,11 @@ def _check_cache(op: str, q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tab
         raise RuntimeError(f"{op}: the heads of q and of the cache do not match")
     if len(block_table._attrs["shape"]) != 2 or len(lengths._attrs["shape"]) != 1 or (offsets is not None and len(offsets._attrs["shape"]) != 1):
         raise RuntimeError(f"{op}: block_table must be [batch, pages of a sequence], lengths [batch], offsets [batch + 1]")
+    if offsets is not None:
+        # (numbers of their own in the graph: where they may fit, a run checks that they do)
+        ends, batch = offsets._attrs["shape"][0]._attrs["values"], lengths._attrs["shape"][0]._attrs["values"]
+        if max(ends) < min(batch) + 1 or min(ends) > max(batch) + 1:
+            raise RuntimeError(f"{op}: offsets must be [batch + 1], got {ends} for batch {batch}")
     if block_table._attrs["shape"][0] != lengths._attrs["shape"][0]:
         raise RuntimeError(f"{op}: block_table and lengths differ in the number of sequences")
     if offsets is None and q._attrs["shape"][0] != lengths._attrs["shape"][0]:
