@@ -72,7 +72,8 @@ class paged_kv_append(_paged):
             if list(t._attrs["shape"]) != [q._attrs["shape"][0]] + list(k_cache._attrs["shape"][2:]):
                 raise RuntimeError(f"paged_kv_append: {name} must be [tokens, kv_heads, head_dim]")
         for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-            if t.src_ops():
+            if not t._attrs["is_input"]:
+                # (neither another op's result nor a constant, which the runtimes of a container share)
                 raise RuntimeError(f"paged_kv_append: {name} is written in place and must be an input of the model")
         check_dtypes("paged_kv_append", freqs=(freqs, ("float32",)))
         if check_freqs("paged_kv_append", freqs, head_dim) == 0:
