@@ -85,7 +85,8 @@ def test_offsets_of_another_batch_at_a_run(make, tmp_path):
                       f"  try {{ ait::{call.strip()} }} catch (const std::exception& x) {{ snprintf(what, n, \"%s\", x.what()); return 1; }}",
                       "  return 0;", "}"])
     (tmp_path / "op.cpp").write_text(main)
-    subprocess.run(["g++", "-O0", "-std=c++17", "-fPIC", "-shared", "-w", "-D__HIP_PLATFORM_AMD__", f"-I{ROOT}/include", "-I/opt/rocm/include",
+    # (-Bsymbolic: its own entry points, also where the library of the same names is loaded)
+    subprocess.run(["g++", "-O0", "-std=c++17", "-fPIC", "-shared", "-Wl,-Bsymbolic", "-w", "-D__HIP_PLATFORM_AMD__", f"-I{ROOT}/include", "-I/opt/rocm/include",
                     str(tmp_path / "op.cpp"), "-o", str(tmp_path / "op.so")], check=True)
     lib = ctypes.CDLL(str(tmp_path / "op.so"))
     lib.run.argtypes = [ctypes.c_int64] * 3 + [ctypes.c_char_p, ctypes.c_int64]
