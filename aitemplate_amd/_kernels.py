@@ -94,6 +94,7 @@ EXPORTED_SYMBOLS = [
     "aitamd_quantize_rows",
     "aitamd_gemm_rcr_int8",
     "aitamd_gemm_int8_workspace_bytes",
+    "aitamd_gemm_int8_layout_bytes",
     "aitamd_rotary_embedding",
     "aitamd_paged_kv_append",
     "aitamd_prefix_attention_workspace_bytes",
@@ -103,7 +104,6 @@ EXPORTED_SYMBOLS = [
     "aitamd_gemm_rcr_noalloc",
     "aitamd_gemm_noalloc_scratch_bytes",
 ]
-
 
 
 class PagedCache(ctypes.Structure):
@@ -197,6 +197,8 @@ def load() -> ctypes.CDLL:
         lib.aitamd_gemm_rcr_int8.argtypes = [i32, i32, vp, vp, vp, vp, vp, vp] + [i64] * 6 + [vp, i64, vp]
         lib.aitamd_gemm_int8_workspace_bytes.restype = i64
         lib.aitamd_gemm_int8_workspace_bytes.argtypes = [i32, i32, i32, i64, i64, i64]
+        lib.aitamd_gemm_int8_layout_bytes.restype = i64
+        lib.aitamd_gemm_int8_layout_bytes.argtypes = [i64, i64, i64]
         lib.aitamd_rotary_embedding.restype = i32
         lib.aitamd_rotary_embedding.argtypes = [i32, vp, vp, vp, i32, vp] + [i64] * 13 + [ctypes.c_float, i32, i32, vp]
         cache = ctypes.POINTER(PagedCache)

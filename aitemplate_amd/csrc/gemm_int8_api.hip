@@ -11,6 +11,13 @@ namespace {
 // (of the scratch memory: what its users leave zero)
 constexpr int64_t kCounterBytes = 4096;
 
+// rows of K bytes of an operand laid out in scratch memory
+int64_t laid_out(int64_t rows, int64_t K) { return rows * ((K + 15) / 16 * 16); }
+// whether rows of K bytes, `pitch` apart, are no whole dwords
+bool off_dwords(const int8_t* x, int64_t rows, int64_t K, int64_t pitch) {
+  return ((K | (int64_t)reinterpret_cast<uintptr_t>(x) | (rows > 1 ? pitch : 0)) & 3) != 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -37,13 +44,11 @@ int aitamd_gemm_rcr_int8(int dtype, int algo, const int8_t* a, const int8_t* b, 
   p.ws = workspace, p.ws_bytes = workspace ? workspace_bytes : 0;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   // rows that are no whole dwords
-  const bool odd_k = (K & 3) != 0;
-  const bool odd_a = odd_k || ((reinterpret_cast<uintptr_t>(a) | (M > 1 ? (uintptr_t)lda : 0)) & 3) != 0;
-  const bool odd_b = odd_k || ((reinterpret_cast<uintptr_t>(b) | (N > 1 ? (uintptr_t)ldb : 0)) & 3) != 0;
+  const bool odd_k = (K & 3) != 0, odd_a = off_dwords(a, M, K, lda), odd_b = off_dwords(b, N, K, ldb);
   if (odd_a || odd_b) {
     if (algo >= 0) return fail("%s: instance %d takes rows of whole dwords only", who, algo);
     // to the scratch memory, behind the counters of the instances that share tiles, which are zero and stay zero
-    const int64_t row = (K + 15) / 16 * 16, bytes_a = odd_a ? M * row : 0, bytes_b = odd_b ? N * row : 0;
+    const int64_t row = laid_out(1, K), bytes_a = odd_a ? M * row : 0, bytes_b = odd_b ? N * row : 0;
     if (!int8_align_pays(K) || kCounterBytes + bytes_a + bytes_b > p.ws_bytes || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) {
       const hipError_t e = launch_gemm_int8_any(p, dtype == AITAMD_BF16, current_device_cus(), s);
       return e == hipSuccess ? 0 : fail("%s: launch failed: %s", who, hipGetErrorString(e));
@@ -67,13 +72,18 @@ int aitamd_gemm_rcr_int8(int dtype, int algo, const int8_t* a, const int8_t* b, 
   return run_gemm(bias ? kEpiBias : kEpiNone, dtype + kNumDTypes, algo, p, s);
 }
 
+int64_t aitamd_gemm_int8_layout_bytes(int64_t rows_a, int64_t rows_b, int64_t K) {
+  if (rows_a < 0 || rows_b < 0 || rows_a + rows_b == 0 || K <= 0 || rows_a > 0x7fffffffll || rows_b > 0x7fffffffll || K > 131071) return 0;
+  return int8_align_pays(K) ? kCounterBytes + laid_out(rows_a + rows_b, K) : 0;
+}
+
 int64_t aitamd_gemm_int8_workspace_bytes(int dtype, int algo, int bias, int64_t M, int64_t N, int64_t K) {
   if (dtype != AITAMD_F16 && dtype != AITAMD_BF16) return 0;
   const int epilogue = bias ? kEpiBias : kEpiNone;
   if (algo >= 0) return aitamd_gemm_workspace_bytes(epilogue, dtype + kNumDTypes, algo, 1, M, N, K / 2);
   if (M <= 0 || N <= 0 || K <= 0 || M > 0x7fffffffll || N > 0x7fffffffll || K > 131071) return 0;
   if ((K & 3) != 0)  // (no instance shares tiles of such rows: they are laid out anew)
-    return int8_align_pays(K) ? kCounterBytes + (M + N) * ((K + 15) / 16 * 16) : 0;
+    return aitamd_gemm_int8_layout_bytes(M, N, K);
   int64_t most = 0;
   for (int i = 0; i < gemm_table(epilogue, dtype + kNumDTypes).count; ++i) {
     const int64_t n = aitamd_gemm_workspace_bytes(epilogue, dtype + kNumDTypes, i, 1, M, N, K / 2);

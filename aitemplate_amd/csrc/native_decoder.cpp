@@ -97,6 +97,11 @@ PyObject* quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
+// whether rows of K bytes, `pitch` apart, are no whole dwords
+bool off_dwords(const int8_t* x, int64_t rows, int64_t K, int64_t pitch) {
+  return ((K | (int64_t)reinterpret_cast<uintptr_t>(x) | (rows > 1 ? pitch : 0)) & 3) != 0;
+}
+
 // gemm_rcr_int8(a, b, a_scale, b_scale, bias, bf16, out, algo, workspace): bf16 is the result's type
 PyObject* gemm_rcr_int8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
@@ -116,15 +121,16 @@ PyObject* gemm_rcr_int8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     c10::SmallVector<int64_t, 6> sizes(a->sizes().begin(), a->sizes().end());
     sizes.back() = N;
     at::Tensor out = make(sizes, type, *a);
-    at::Tensor scratch;  // (rows that are no whole dwords are laid out there first)
-    if (ws == nullptr && K % 4 != 0 && algo < 0) {
-      const int64_t need = aitamd_gemm_int8_workspace_bytes(dt, -1, bias != nullptr, M, N, K);
+    const int8_t *pa = static_cast<const int8_t*>(a->data_ptr()), *pb = static_cast<const int8_t*>(b->data_ptr());
+    at::Tensor scratch;  // (an operand whose rows are no whole dwords is laid out there first)
+    const bool odd_a = off_dwords(pa, M, K, lda), odd_b = off_dwords(pb, N, K, ldb);
+    if (ws == nullptr && algo < 0 && (odd_a || odd_b)) {
+      const int64_t need = aitamd_gemm_int8_layout_bytes(odd_a ? M : 0, odd_b ? N : 0, K);
       if (need > 0) {
         scratch = make({need}, at::kByte, *a);
         ws = &scratch;
       }
     }
-    const int8_t *pa = static_cast<const int8_t*>(a->data_ptr()), *pb = static_cast<const int8_t*>(b->data_ptr());
     const float *sa = static_cast<const float*>(a_scale->data_ptr()), *sb = static_cast<const float*>(b_scale->data_ptr());
     const void* pbias = pointer(bias);
     void *c = out.data_ptr(), *w = ws == nullptr ? nullptr : ws->data_ptr(), *stream = current_stream();

@@ -527,9 +527,19 @@ def quantize_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
     return out, scale
 
 
-def gemm_int8_workspace_bytes(M: int, N: int, K: int, bias: bool = False, dtype=torch.float16, algo: int = -1) -> int:
-    """Bytes of scratch memory with which `gemm_rcr_int8` may choose any of its instances for this problem (0: none takes any)."""
-    return int(_kernels.load().aitamd_gemm_int8_workspace_bytes(_TORCH_DTYPE_ID[dtype], algo, int(bool(bias)), M, N, K))
+def gemm_int8_workspace_bytes(M: int, N: int, K: int, bias: bool = False, dtype=torch.float16, algo: int = -1,
+                              any_byte: bool = False) -> int:
+    """Bytes of scratch memory with which `gemm_rcr_int8` may choose any of its instances for this problem (0: none takes any).
+    `any_byte`: operands that are views at any pitch and address, whose rows may be no whole dwords (they are laid out there first)."""
+    lib = _kernels.load()
+    need = int(lib.aitamd_gemm_int8_workspace_bytes(_TORCH_DTYPE_ID[dtype], algo, int(bool(bias)), M, N, K))
+    return max(need, int(lib.aitamd_gemm_int8_layout_bytes(M, N, K))) if any_byte else need
+
+
+def _off_dwords(t: torch.Tensor, name: str) -> bool:
+    """Whether the rows of an 8-bit operand are no whole dwords."""
+    rows, columns = t.shape
+    return (columns | t.data_ptr() | (_row_pitch(t, name) if rows > 1 else 0)) % 4 != 0
 
 
 def gemm_rcr_int8(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -538,7 +548,8 @@ def gemm_rcr_int8(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_sca
     """out = a_scale * b_scale * (a @ b.T) (+ bias) of 8-bit integers `a` [..., K] with a fp32 scale for each row ([...], see
     `quantize_rows`) and `b` [N, K] with one for each of its rows ([N]: a layer's output channels); `out` and `bias` [N] are of
     type `dtype`.  The sums are exact, K goes up to 131071, rows may lie at any byte.  `a` and `b` may have row pitch (2-D views);
-    `algo` and `workspace` as of `gemm` (sizes from `gemm_int8_workspace_bytes`)."""
+    `algo` and `workspace` as of `gemm` (sizes from `gemm_int8_workspace_bytes`); without one, rows that are no whole dwords have
+    theirs for the call."""
     if dtype not in _TORCH_DTYPE_ID:
         raise ValueError(f"unsupported dtype {dtype}")
     result = _native_decoder.gemm_rcr_int8(a, b, a_scale, b_scale, bias, dtype is torch.bfloat16, out, algo, workspace)
@@ -570,9 +581,10 @@ def gemm_rcr_int8(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_sca
     if workspace is not None and not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous uint8 GPU tensor (see new_workspace)")
     with torch.cuda.device(device):
-        if workspace is None and K % 4 != 0 and algo < 0:
-            # (rows that are no whole dwords are laid out there first; nothing in it has to be zero for that)
-            need = gemm_int8_workspace_bytes(M, N, K, bias is not None, dtype)
+        odd_a, odd_b = _off_dwords(a2, "a"), _off_dwords(b, "b")
+        if workspace is None and algo < 0 and (odd_a or odd_b):
+            # (an operand whose rows are no whole dwords is laid out there first; nothing in it has to be zero for that)
+            need = int(_kernels.load().aitamd_gemm_int8_layout_bytes(M if odd_a else 0, N if odd_b else 0, K))
             workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         rc = _kernels.load().aitamd_gemm_rcr_int8(
             _TORCH_DTYPE_ID[dtype], algo, _p(a2), _p(b), _p(a_scale), _p(b_scale), _p(bias), _p(out2), M, N, K, _row_pitch(a2, "a"),

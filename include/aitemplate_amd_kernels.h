@@ -307,14 +307,16 @@ AITAMD_API int aitamd_quantize_rows(int dtype, const void* x, int8_t* q, float* 
  * Any K, pitch and address; rows of whole dwords, and more so of whole 16-byte pieces, are faster.  algo = -1: the
  * heuristic instance; otherwise an instance of aitamd_gemm_num_algos(bias ? AITAMD_EPI_BIAS : AITAMD_EPI_NONE, 2 + dtype),
  * for rows of whole dwords (queries about them count K, lda and ldb in pairs of bytes).  workspace: as of
- * aitamd_gemm_rcr_ws, aitamd_gemm_int8_workspace_bytes() bytes (algo = -1: enough for any instance) or null; where K % 4
- * is not 0 it takes the operands in whole 16-byte pieces instead, and its first 4096 bytes, which are not touched then,
- * need not be zero. */
+ * aitamd_gemm_rcr_ws, aitamd_gemm_int8_workspace_bytes() bytes (algo = -1: enough for any instance) or null.  An operand whose
+ * rows are no whole dwords (K % 4, or its pitch or address) is laid out in it first, in whole 16-byte pieces, where it has
+ * aitamd_gemm_int8_layout_bytes() bytes for the rows of such operands (0: that would not be faster; for K % 4 the same as
+ * aitamd_gemm_int8_workspace_bytes()); its first 4096 bytes are not touched then and need not be zero. */
 AITAMD_API int aitamd_gemm_rcr_int8(int dtype, int algo, const int8_t* a, const int8_t* b, const float* scale_a,
                                     const float* scale_b, const void* bias, void* c, int64_t M, int64_t N, int64_t K,
                                     int64_t lda, int64_t ldb, int64_t ldc, void* workspace, int64_t workspace_bytes,
                                     void* stream);
 AITAMD_API int64_t aitamd_gemm_int8_workspace_bytes(int dtype, int algo, int bias, int64_t M, int64_t N, int64_t K);
+AITAMD_API int64_t aitamd_gemm_int8_layout_bytes(int64_t rows_a, int64_t rows_b, int64_t K);
 
 /* out[b, s, h, :] = x[b, s, h, :] with its first `rotated` dims turned by the position: with n = rotated / 2 and
  * angle = position(b, s) * freqs[i], the pair (x[i], x[n + i]), or (x[2 i], x[2 i + 1]) with `interleaved`, becomes
