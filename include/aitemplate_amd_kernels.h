@@ -363,7 +363,7 @@ AITAMD_API int aitamd_paged_kv_append(int dtype, const aitamd_paged_cache* cache
  * sequence's own pages (the step's keys are in the cache already, lengths are those from before the step; none where
  * that is not positive, all that the table has room for where there are not as many):
  *   out[r, h, :] = sum_n softmax_n(scale * q[r, h, :] . k[n, h / (heads / kv_heads), :]) v[n, h / (heads / kv_heads), :]
- * Sums and maxima are held in 32 bits, the weights of a tile's keys in the type's 16 bits (in fp16 those below 2^-36 of the
+ * Sums and maxima are held in 32 bits, the weights of a tile's keys in the type's 16 bits (in fp16 those below 2^-33 of the
  * row's largest count as none).  Rows that see no key are written as zeros.  A table entry that a row's keys need and that is
  * not in [0, pages) counts as a page of zeros.  What lies behind a sequence's last key is not read.  Keys that only later rows
  * of the step see do not count for a row, as long as their values are finite.
