@@ -10,11 +10,12 @@
 // the probabilities never leave the registers.  WR waves stand side by side over rows and share every tile of keys; WK waves
 // take 32 keys of a tile each, for themselves, and join at the end.
 //
-// Bound, 128 rows: a tile of 64 keys takes 1.1 us of a CU with two workgroups on it and 1.3 us of one with one (head dim 96),
-// 0.3 of that matrix instructions and 0.4 vector instructions, which two waves a SIMD cover only in part: 890 TFLOP/s with
-// head dim 96 and 975 with 128 for 32 heads of 2048 rows over some 10 000 keys.  It is neither the reads of K from LDS (the next
-// tile's K read into registers between the second product's steps: 902 and 950) nor the latency of the loads (a third
-// stage for K: no faster).
+// Bound, 128 rows of 96 dims: a tile of 64 keys is 768 cycles of each SIMD's matrix unit, 0.32 us, and as many of vector
+// instructions.  A workgroup alone on its CU takes 1.4 us for it, one after the other with the reads of LDS and the scalars between
+// them; of two workgroups on a CU the one's matrix instructions run beside the other's vector instructions in part, 0.83 us a tile
+// (128 dims: 1.6 and 1.1): 960 TFLOP/s for 32 heads of 2048 rows over a prefix of 9984 keys, 1040 with 128 dims.  It is neither the
+// reads of K from LDS nor the latency of the loads: some 10 000 keys, the rows' own among them, at 890 and 975 TFLOP/s, with the next
+// tile's K read into registers between the second product's steps at 902 and 950, no faster with a third stage for K.
 //
 // Keys and values go from their pages straight to LDS: 16 consecutive keys lie in one page (page sizes are multiples of
 // 16), so the page is one scalar per 16 keys and the bounds of its buffer descriptor cut off what is past the last key:

@@ -785,11 +785,15 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     """Attention of one step's queries `q` [tokens, heads, head_dim] over a paged cache, after `paged_kv_append` of the same step
     (`k_cache`, `v_cache`, `block_table`, `lengths`, `offsets` as there, `lengths` still those from before the step).
 
-    Every row sees the first `prefix_length` keys of the pages `prefix_table` [n] int32, which the whole batch shares and which
-    are read once for all of its rows, and those of its own sequence's pages up to itself.  Query head h reads key head
-    h // (heads / kv_heads).  `scale` is head_dim ** -0.5 unless given.  Rows that see no key are zeros; rows of `out` from
-    offsets[batch] on are left as they were.  What lies in a page behind a sequence's last key may be anything; keys and values
-    of the step's later rows do not count for a row, as long as they are finite.
+    Every row sees the first `prefix_length` keys of the pages `prefix_table` [n] int32, which the whole batch shares, and those of
+    its own sequence's pages up to itself.  Query head h reads key head h // (heads / kv_heads).  `scale` is head_dim ** -0.5
+    unless given.  In fp16, keys of less than 2^-33 of the weight of a row's largest count as none.  Rows that see no key are zeros;
+    rows of `out` from offsets[batch] on are left as they were.  What lies in a page behind a sequence's last key may be anything;
+    keys and values of the step's later rows do not count for a row, as long as they are finite.
+
+    Without `offsets`, or with up to 32 rows a sequence on average (a token has heads / kv_heads of them for each key head), the prefix
+    is read once for every 128 rows of the whole batch; otherwise, and for one sequence alone, once for every tile of a sequence's
+    own rows, where a sequence of one token beside prompts has a tile for itself.
 
     page_size has to be a multiple of 16, head_dim one of 8 up to 256.  `workspace`: a buffer from `new_workspace` of
     `prefix_attention_workspace_bytes`, allocated for the call otherwise; calls that may overlap in time need one each."""
