@@ -170,6 +170,19 @@ void ModelBase::SetInput(const void* src, const AITemplateParamShape& shape, siz
   SetParam(src, idx);
 }
 
+void ModelBase::CheckInputShape(const AITemplateParamShape& shape, size_t idx) const {
+  const ParamInfo& p = params_[idx];
+  for (size_t i = 0; i < shape.size; ++i) {
+    const int64_t now = *p.shape_ptrs[i].value;
+    if (shape.shape_data[i] != now) {
+      std::ostringstream os;
+      os << "Shape of input " << p.name << " is invalid: dim " << i << " = " << shape.shape_data[i] << ", but another input has " << now
+         << " for the same dimension";
+      throw std::runtime_error(os.str());
+    }
+  }
+}
+
 void ModelBase::SetOutput(void* src, size_t idx) {
   if (idx >= num_outputs_) throw std::out_of_range("output index out of range");
   SetParam(src, idx + num_inputs_);

@@ -144,6 +144,7 @@ void ModelContainer::PrepareForRun(ModelBase* m, const AITData* inputs, size_t n
       throw std::runtime_error("Input " + meta_->inputs[i].name + " has a null data pointer");
     m->SetInput(in.ptr, in.shape, i);
   }
+  for (size_t i = 0; i < num_inputs; ++i) m->CheckInputShape(inputs[i].shape, i);
   for (size_t i = 0; i < num_outputs; ++i) {
     if (outputs[i].dtype != meta_->outputs[i].dtype)
       throw std::runtime_error("Got wrong dtype for output " + meta_->outputs[i].name);

@@ -97,6 +97,9 @@ class ModelBase {
   size_t NumOutputs() const { return num_outputs_; }
 
   void SetInput(const void* src, const AITemplateParamShape& shape, size_t idx);
+  // After all inputs are set: a dimension that inputs share has one value (the op launchers read it for all of them, and would
+  // follow the shorter tensor past its end)
+  void CheckInputShape(const AITemplateParamShape& shape, size_t idx) const;
   void SetOutput(void* src, size_t idx);
   // writes the current shape of output idx; output must have max-rank entries
   void GetOutputShape(size_t idx, int64_t* output_shape_out);
