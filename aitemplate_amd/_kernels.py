@@ -99,6 +99,12 @@ EXPORTED_SYMBOLS = [
     "aitamd_paged_kv_append",
     "aitamd_prefix_attention_workspace_bytes",
     "aitamd_prefix_attention",
+    "aitamd_gemm_rcr_lora",
+    "aitamd_gemm_lora_workspace_bytes",
+    "aitamd_qk_norm_rotary",
+    "aitamd_paged_kv_append_norm",
+    "aitamd_token_logprobs",
+    "aitamd_token_logprobs_workspace_bytes",
     "aitamd_gemm_workspace_bytes",
     "aitamd_gemm_rcr_ws",
     "aitamd_gemm_rcr_noalloc",
@@ -114,6 +120,15 @@ class PagedCache(ctypes.Structure):
                                                  "k_head_stride", "v_page_stride", "v_slot_stride", "v_head_stride")]
                 + [("table", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ("table_pitch", "max_pages")]
                 + [(n, ctypes.c_void_p) for n in ("lengths", "offsets")] + [(n, ctypes.c_int64) for n in ("batch", "tokens")])
+
+
+class Heads(ctypes.Structure):
+    """aitamd_heads of the C ABI."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "out")]
+                + [(n, ctypes.c_int64) for n in ("heads", "batch_stride", "seq_stride", "head_stride", "out_batch_stride", "out_seq_stride",
+                                                 "out_head_stride")]
+                + [("weight", ctypes.c_void_p), ("weight_head_stride", ctypes.c_int64)])
 
 
 _lock = threading.Lock()
@@ -209,6 +224,21 @@ def load() -> ctypes.CDLL:
         lib.aitamd_prefix_attention_workspace_bytes.argtypes = [cache, i64, i64]
         lib.aitamd_prefix_attention.restype = i32
         lib.aitamd_prefix_attention.argtypes = [i32, cache, vp, i64, i64, vp, i64, i64, i64, vp, i64, i64, ctypes.c_float, vp, i64, vp]
+        f32 = ctypes.c_float
+        lib.aitamd_gemm_rcr_lora.restype = i32
+        lib.aitamd_gemm_rcr_lora.argtypes = [i32, i32] + [vp] * 8 + [i64] * 8 + [vp, i64, vp]
+        lib.aitamd_gemm_lora_workspace_bytes.restype = i64
+        lib.aitamd_gemm_lora_workspace_bytes.argtypes = [i32, i32, i32, i64, i64, i64, i64]
+        heads = ctypes.POINTER(Heads)
+        lib.aitamd_qk_norm_rotary.restype = i32
+        lib.aitamd_qk_norm_rotary.argtypes = [i32, heads, heads, vp, i32, vp] + [i64] * 6 + [f32, f32, i32, vp]
+        lib.aitamd_paged_kv_append_norm.restype = i32
+        lib.aitamd_paged_kv_append_norm.argtypes = [i32, cache, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, i64, vp, i64, vp, i64,
+                                                    f32, vp, i64, i64, f32, i32, vp]
+        lib.aitamd_token_logprobs.restype = i32
+        lib.aitamd_token_logprobs.argtypes = [i32, vp, vp, i32] + [vp] * 5 + [i64] * 4 + [f32, vp, i64, vp]
+        lib.aitamd_token_logprobs_workspace_bytes.restype = i64
+        lib.aitamd_token_logprobs_workspace_bytes.argtypes = [i64, i64, i64]
         _lib = lib
         return lib
 

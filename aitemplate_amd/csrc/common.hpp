@@ -88,6 +88,23 @@ struct ElemTraits<i8x2> {
   }
 };
 
+template <class T, int MT>
+struct MfmaOp;
+template <class T>
+struct MfmaOp<T, 32> {
+  using acc_t = f32x16;
+  static AITAMD_DEVICE acc_t run(typename ElemTraits<T>::vec8 a, typename ElemTraits<T>::vec8 b, acc_t c) {
+    return ElemTraits<T>::mfma32(a, b, c);
+  }
+};
+template <class T>
+struct MfmaOp<T, 16> {
+  using acc_t = f32x4;
+  static AITAMD_DEVICE acc_t run(typename ElemTraits<T>::vec8 a, typename ElemTraits<T>::vec8 b, acc_t c) {
+    return ElemTraits<T>::mfma16(a, b, c);
+  }
+};
+
 // LDS transpose read: 4 x 16-bit per lane, gathered across the 16 lanes of a block.
 // __restrict__ is for the compiler's wait insertion: without alias information on the read it assumes that any
 // direct-to-LDS load on its way may be the data and drains them all (s_waitcnt vmcnt(0)) in front of every read, which

@@ -113,6 +113,10 @@ AITAMD_DEF_EPI(kEpiAdd, false, 1, 1, acc + d0)
 template <int ID, class OUT>
 struct ScaledEpilogue : Epilogue<ID> {};
 
+// The expression is of the accumulator with the row's low-rank adapter added to it (lora.hpp)
+template <int ID, class T>
+struct LoraEpilogue : Epilogue<ID> {};
+
 // the type of results, bias and residuals, and whether the accumulators are integers that are scaled first
 template <class T, class Epi>
 struct OutElem {
@@ -123,6 +127,14 @@ template <class T, int ID, class OUT>
 struct OutElem<T, ScaledEpilogue<ID, OUT>> {
   using type = OUT;
   static constexpr bool scaled = true;
+};
+template <class Epi>
+struct IsLora {
+  static constexpr bool value = false;
+};
+template <int ID, class T>
+struct IsLora<LoraEpilogue<ID, T>> {
+  static constexpr bool value = true;
 };
 // an integer accumulator that stands in a float's place, scaled (the one rounding to 32 bits that it does not have in 24)
 AITAMD_DEVICE float scaled_sum(float acc, float scale) { return (float)__float_as_int(acc) * scale; }

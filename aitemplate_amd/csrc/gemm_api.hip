@@ -177,7 +177,8 @@ int remembered_heuristic(const GemmAlgoTable& t, int64_t batch, int64_t M, int64
 
 int run_gemm(int epilogue, int dtype, int algo, const GemmParams& p, hipStream_t stream) {
   // (the tables of 8-bit integers take scales: aitamd_gemm_rcr_int8)
-  if (dtype >= kNumDTypes && !p.scale_a) return fail("aitamd_gemm: bad dtype %d", dtype);
+  // ... and those of adapters take them: aitamd_gemm_rcr_lora
+  if (dtype >= kNumDTypes && !(dtype < 2 * kNumDTypes ? (const void*)p.scale_a : p.lora_t)) return fail("aitamd_gemm: bad dtype %d", dtype);
   const GemmAlgoTable t = gemm_table(epilogue, dtype);
   if (t.count == 0) return fail("aitamd_gemm: no kernels compiled for epilogue %d dtype %d", epilogue, dtype);
   if (p.M < 0 || p.N < 0 || p.K < 0 || p.batch < 0) return fail("aitamd_gemm: negative dimension");

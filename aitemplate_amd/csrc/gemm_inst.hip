@@ -1,5 +1,6 @@
 // One translation unit per (epilogue, dtype): compiled repeatedly by the
-// Makefile with -DAITAMD_EPI=<EpilogueId> -DAITAMD_DT=<0 fp16 | 1 bf16 | 2, 3 8-bit integers to fp16, bf16>.
+// Makefile with -DAITAMD_EPI=<EpilogueId> -DAITAMD_DT=<0 fp16 | 1 bf16 | 2, 3 8-bit integers to fp16, bf16 |
+// 4, 5 fp16, bf16 with low-rank adapters>.
 // It instantiates every tile of gemm_tiles.inc for that pair and exports the
 // resulting launcher table under a C symbol the dispatcher looks up.
 #include <cstdlib>
@@ -16,7 +17,7 @@
 #error "compile with -DAITAMD_EPI=<id>"
 #endif
 #ifndef AITAMD_DT
-#error "compile with -DAITAMD_DT=<0|1|2|3>"
+#error "compile with -DAITAMD_DT=<0|1|2|3|4|5>"
 #endif
 
 namespace aitamd {
@@ -28,6 +29,12 @@ using Elem = f16;
 #elif AITAMD_DT == 1
 using Elem = bf16;
 #define AITAMD_DT_NAME "bf16"
+#elif AITAMD_DT == 4
+using Elem = f16;
+#define AITAMD_DT_NAME "f16_lora"
+#elif AITAMD_DT == 5
+using Elem = bf16;
+#define AITAMD_DT_NAME "bf16_lora"
 #else
 // 8-bit integers, results in fp16 or bf16
 using Elem = i8x2;
@@ -44,6 +51,8 @@ constexpr int kMaxDevices = 64;
 
 #if AITAMD_DT < 2
 using Epi = Epilogue<AITAMD_EPI>;
+#elif AITAMD_DT >= 4
+using Epi = LoraEpilogue<AITAMD_EPI, Elem>;
 #else
 using Epi = ScaledEpilogue<AITAMD_EPI, Scaled>;
 #endif
@@ -337,15 +346,18 @@ const GemmAlgo kAlgos[] = {
   entry<GemmTileDma<BM, BN, BK, WM, WN, NS, OCC, PIPE, MT, AUX>, 1, OCC>(                                            \
       AITAMD_NAME #BM "x" #BN "x" #BK "_w" #WM "x" #WN "_dma" #NS "_o" #OCC "_p" #PIPE "_m" #MT "_c" #AUX, {__VA_ARGS__}),
 #if AITAMD_DT >= 2
-// (the persistent kernel on eight waves rounds its accumulators to the operands' type ahead of the epilogue; rows at any
-// byte have a kernel of their own)
+// (the persistent kernel on eight waves rounds its accumulators to the operands' type ahead of the epilogue)
 #define AITAMD_GEMM_TILE_PERSIST(...)
-#define AITAMD_GEMM_TILE_STAGED(...)
-#define AITAMD_GEMM_ROWS_ELEM(...)
 #else
 #define AITAMD_GEMM_TILE_PERSIST(BM, BN, BK, WM, WN, NS, MT, LBM, ...)                                               \
   entry<GemmTilePersist<BM, BN, BK, WM, WN, NS, MT, LBM>, 2, 1>(                                                     \
       AITAMD_NAME #BM "x" #BN "x" #BK "_w" #WM "x" #WN "_persist" #NS "_m" #MT, {__VA_ARGS__}),
+#endif
+#if AITAMD_DT == 2 || AITAMD_DT == 3
+// (rows at any byte have a kernel of their own)
+#define AITAMD_GEMM_TILE_STAGED(...)
+#define AITAMD_GEMM_ROWS_ELEM(...)
+#else
 #define AITAMD_GEMM_TILE_STAGED(BM, BN, BK, WM, WN, NS, OCC, MT, ...)                                                \
   entry<GemmTileDma<BM, BN, BK, WM, WN, NS, OCC, 0, MT, 0, 4>, 0, OCC>(                                              \
       AITAMD_NAME #BM "x" #BN "x" #BK "_w" #WM "x" #WN "_reg" #NS "_o" #OCC "_v1", {__VA_ARGS__}),

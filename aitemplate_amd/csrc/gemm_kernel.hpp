@@ -62,6 +62,11 @@ struct GemmParams {
   int32_t split_k;  // number of workgroups that share a tile along K (set by the launcher of a split-K instance)
   // Operands of 8-bit integers (i8x2: K, lda, ldb, sa and sb count pairs): fp32 scales of the M rows of A and of the N rows of B
   const float *scale_a, *scale_b;
+  // Low-rank adapters (LoraEpilogue; see lora.hpp): lora_n of them, lora_rank wide; t of every row, the adapters' [lora_n, N,
+  // lora_rank], each row's adapter (outside [0, lora_n): none)
+  const void *lora_t, *lora_b;
+  const int32_t* lora_of;
+  int32_t lora_n, lora_rank;
 };
 
 // The launcher's part of the walk over tiles of bm x bn.  xcd_shift: see GemmParams; -1 for the grouped walk.

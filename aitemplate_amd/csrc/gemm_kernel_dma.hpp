@@ -24,6 +24,7 @@
 #include "common.hpp"
 #include "epilogue.hpp"
 #include "gemm_kernel.hpp"
+#include "lora.hpp"
 
 namespace aitamd {
 
@@ -116,23 +117,6 @@ AITAMD_DEVICE void wait_vmcnt() {
   constexpr int imm = (N & 0xf) | ((N >> 4) << 14) | (0x7 << 4) | (0xf << 8);
   __builtin_amdgcn_s_waitcnt(imm);
 }
-
-template <class T, int MT>
-struct MfmaOp;
-template <class T>
-struct MfmaOp<T, 32> {
-  using acc_t = f32x16;
-  static AITAMD_DEVICE acc_t run(typename ElemTraits<T>::vec8 a, typename ElemTraits<T>::vec8 b, acc_t c) {
-    return ElemTraits<T>::mfma32(a, b, c);
-  }
-};
-template <class T>
-struct MfmaOp<T, 16> {
-  using acc_t = f32x4;
-  static AITAMD_DEVICE acc_t run(typename ElemTraits<T>::vec8 a, typename ElemTraits<T>::vec8 b, acc_t c) {
-    return ElemTraits<T>::mfma16(a, b, c);
-  }
-};
 
 // Scheduling hints for one MFMA step of MFMAS matrix instructions that also
 // issues READS LDS fragment reads (for the next step) and VM direct-to-LDS
@@ -628,6 +612,16 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
         mfmas(ta, tb);
       }
     }
+    // low-rank adapters: behind K, by the last of the workgroups that share a tile; of waves with many, in the epilogue
+    constexpr bool kLora = IsLora<Epi>::value;
+    LoraTile<std::conditional_t<kLora, T, bf16>, MT, MI, NI> lora;
+    if constexpr (kLora) {
+      lora.read(p, m0 + wm * Tile::WTM, lane);
+      lora.count();
+      if (!lora.many && (Tile::SPLITK == 0 || split == splits - 1))
+        lora.add(p, m0 + wm * Tile::WTM, n0 + wn * Tile::WTN, lane,
+                 [&](bf16x8 b, bf16x8 a, auto mi, auto ni) __attribute__((always_inline)) { acc[mi][ni] = MfmaOp<bf16, MT>::run(b, a, acc[mi][ni]); });
+    }
 
     if constexpr (Tile::SPLITK != 0) {
       // ---------------- split-K: partial tile to the scratch memory; the last workgroup of the tile sums ----
@@ -752,6 +746,9 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
           const f32x4 v0 = *reinterpret_cast<const f32x4*>(strip + row * PITCH + rd_col);
           const f32x4 v1 = *reinterpret_cast<const f32x4*>(strip + row * PITCH + rd_col + 4);
           float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+          if constexpr (kLora) {
+            if (lora.many) lora_add<T, 8>(v, p, m, n);
+          }
           const int64_t c_idx = out_index<PERM>(p, m, n);
           const int64_t d_idx = (int64_t)m * p.ldd + n;
           float scale = 1.0f;  // (of the row)

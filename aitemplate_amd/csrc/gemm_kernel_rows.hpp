@@ -31,6 +31,7 @@
 #include "common.hpp"
 #include "epilogue.hpp"
 #include "gemm_kernel.hpp"
+#include "lora.hpp"
 
 namespace aitamd {
 
@@ -244,6 +245,11 @@ __global__ void __launch_bounds__(Tile::NT) gemm_rcr_rows_kernel(const GemmParam
         v = kScaled ? __int_as_float(__float_as_int(v) + __float_as_int(more)) : v + more;
       }
       if constexpr (kScaled) v = scaled_sum(v, scale_v[o]);
+      if constexpr (IsLora<Epi>::value) {
+        float sum[1] = {v};
+        lora_add<T, 1>(sum, p, m0 + m, n0 + out_n);
+        v = sum[0];
+      }
       Cb[out_index<PERM>(p, m0 + m, n0 + out_n)] = epilogue1<Epi, Out>(v, bias_v[o], d0_v[o], d1_v[o], one);
     }
   }

@@ -1,0 +1,235 @@
+// The low-rank part of a projection that many requests share: rows of one launch belong to different adapters,
+//     y[m, n] = sum_k x[m, k] w[n, k] (+ bias[n]) + sum_j t[m, j] b[i(m)][n, j],   t[m, j] = scale[i(m)] sum_k x[m, k] a[i(m)][j, k].
+// A launch ahead of the product's makes t (lora_api.hip); the product's tiles add t b to their accumulators behind the K loop, as
+// if K went on, and round once.
+//
+// t lies in scratch memory in two bfloat16 numbers that add up to it (off by 2^-17 at most, and of the range of 32 bits, which
+// one half of the other type or both do not have), the first of eight ranks and then the second of them.  bfloat16 adapters are
+// multiplied with both; a half is the sum of two bfloat16 numbers too (8 of its 11 bits and the 3 behind them), so that halves are
+// four products: exact, all of them.
+//
+// Per wave: the adapters of its rows one after the other, each with the rows of the others set to zero, on matrix instructions; with
+// more than kLoraFew of them every output by itself, from its row's own adapter.
+#pragma once
+
+#include <type_traits>
+
+#include "common.hpp"
+#include "epilogue.hpp"
+#include "gemm_kernel.hpp"
+
+namespace aitamd {
+
+constexpr int kLoraFew = 4;
+
+// a row's elements in scratch memory: chunks of eight ranks, two parts each
+constexpr int lora_chunks(int rank) { return (rank + 7) / 8; }
+AITAMD_DEVICE const bf16* lora_row(const GemmParams& p, int m) {
+  return reinterpret_cast<const bf16*>(p.lora_t) + (int64_t)m * (lora_chunks(p.lora_rank) * 16);
+}
+// the adapter of row m, or -1
+AITAMD_DEVICE int lora_adapter(const GemmParams& p, int m) {
+  if (m >= p.M) return -1;
+  const int id = p.lora_of[m];
+  return (uint32_t)id < (uint32_t)p.lora_n ? id : -1;
+}
+// the adapter's row of column n
+template <class T>
+AITAMD_DEVICE const T* lora_column(const GemmParams& p, int id, int n) {
+  return reinterpret_cast<const T*>(p.lora_b) + ((int64_t)id * p.N + n) * p.lora_rank;
+}
+// eight numbers as the sums of two (an infinity or a NaN as itself and zero)
+template <class T>
+AITAMD_DEVICE void lora_parts(typename ElemTraits<T>::vec8 v, bf16x8& one, bf16x8& two) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float f = ElemTraits<T>::to_float(v[j]);
+    one[j] = (bf16)f;
+    two[j] = __builtin_isfinite(f) ? (bf16)(f - (float)one[j]) : (bf16)0.0f;
+  }
+}
+// eight bfloat16 numbers: whether they all are; those that are, or (pass 1) the largest number for those that are not; the largest
+// number with the sign of each
+AITAMD_DEVICE bool lora_numbers(u32x4 v) {
+  bool all = true;
+#pragma unroll
+  for (int d = 0; d < 4; ++d) all = all && (v[d] & 0x7f80u) != 0x7f80u && (v[d] & 0x7f800000u) != 0x7f800000u;
+  return all;
+}
+AITAMD_DEVICE u32x4 lora_split(u32x4 v, int pass) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const uint32_t none = ((v[d] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((v[d] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+    v[d] = pass == 0 ? v[d] & ~none : ((v[d] & 0x80008000u) | 0x7f7f7f7fu) & none;
+  }
+  return v;
+}
+AITAMD_DEVICE u32x4 lora_largest(u32x4 v) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d) v[d] = (v[d] & 0x80008000u) | 0x7f7f7f7fu;
+  return v;
+}
+
+// The part of a wave whose rows row0 + mi * MT + (lane % MT) meet columns col0 + ni * MT + (lane % MT)
+template <class T, int MT, int MI, int NI>
+struct LoraTile {
+  static constexpr int QN = 64 / MT;
+  int of[MI];
+  bool many;
+
+  AITAMD_DEVICE void read(const GemmParams& p, int row0, int lane) {
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) of[mi] = lora_adapter(p, row0 + mi * MT + lane % MT);
+  }
+  // the first adapter of those left, or -1 (the same for all lanes)
+  static AITAMD_DEVICE int first_of(const int (&left)[MI]) {
+    int id = -1;
+    static_for<0, MI>([&](auto i) __attribute__((always_inline)) {
+      constexpr int mi = MI - 1 - decltype(i)::value;
+      const uint64_t some = __builtin_amdgcn_ballot_w64(left[mi] >= 0);
+      if (some != 0) id = __builtin_amdgcn_readlane(left[mi], __builtin_ctzll(some));
+    });
+    return id;
+  }
+  AITAMD_DEVICE void count() {
+    int left[MI], n = 0;
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) left[mi] = of[mi];
+    for (;;) {
+      const int id = first_of(left);
+      if (id < 0 || ++n > kLoraFew) break;
+#pragma unroll
+      for (int mi = 0; mi < MI; ++mi) left[mi] = left[mi] == id ? -1 : left[mi];
+    }
+    many = n > kLoraFew;
+  }
+  // multiply(b, a, mi, ni): accumulator (mi, ni) plus the product of the weight rows b and the rows a, both bf16x8.  Through
+  // buffers that end with the rows and the columns: 32-bit offsets, and no branch around what is not there.
+  template <class M>
+  AITAMD_DEVICE void add(const GemmParams& p, int row0, int col0, int lane, M&& multiply) const {
+    const int fr = lane % MT, fq = lane / MT;
+    const int rank = p.lora_rank, chunks = lora_chunks(rank);
+    const int rows = p.M - row0 < MI * MT ? p.M - row0 : MI * MT, columns = p.N - col0 < NI * MT ? p.N - col0 : NI * MT;
+    if (rows <= 0 || columns <= 0) return;
+    const uint32_t t_pitch = (uint32_t)chunks * 32u, b_pitch = (uint32_t)rank * 2u;
+    const __amdgpu_buffer_rsrc_t rt = make_rsrc(lora_row(p, row0), (uint32_t)rows * t_pitch);
+    // 16 x 16: a step's four quarters are both parts of t of two chunks (halves: both by both of one); 32 x 32: its two
+    // halves are both parts of t of one chunk (halves: once with each of the adapter's)
+    constexpr bool kHalves = !std::is_same_v<T, bf16>;
+    constexpr int PER = MT == 16 && !kHalves ? 2 : 1;
+    const int half = PER == 2 ? fq & 1 : 0;
+    const int part = MT == 32 ? fq : (PER == 2 ? fq >> 1 : fq & 1);
+    uint32_t t_at = (uint32_t)fr * t_pitch + (uint32_t)(half * 32 + part * 16), b_at = (uint32_t)fr * b_pitch + (uint32_t)(half * 16);
+    // (opaque: what hangs on the tile alone would be computed ahead of the K loop, held over it and spilled)
+    asm volatile("" : "+v"(t_at), "+v"(b_at));
+    int left[MI];
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) left[mi] = of[mi];
+    for (;;) {
+      const int id = first_of(left);
+      if (id < 0) break;
+      const __amdgpu_buffer_rsrc_t rb = make_rsrc(lora_column<T>(p, id, col0), (uint32_t)columns * b_pitch);
+      for (int c0 = 0; c0 < chunks; c0 += PER) {
+        const bool on = c0 + half < chunks;
+        const uint32_t tc = t_at + (uint32_t)c0 * 32u, bc = b_at + (uint32_t)c0 * 16u;
+        // Numbers that are none, times the zeros of other requests' rows, would reach them: where a wave meets some, the product is
+        // taken without them first, then again with the largest number in their places and zeros in the others', times the
+        // largest: an infinity where it belongs and zero elsewhere.
+        bool again = false;
+        for (int pass = 0; pass < 2; ++pass) {
+          u32x4 w[NI], t[MI];
+          if ((rank & 7) == 0) {
+            static_for<0, NI>([&](auto ni) __attribute__((always_inline)) {
+              w[ni] = buffer_load_16B(rb, on ? bc + (uint32_t)(decltype(ni)::value * MT) * b_pitch : kOobOffset);
+            });
+          } else {
+            static_for<0, NI>([&](auto ni) __attribute__((always_inline)) {
+#pragma unroll
+              for (int d = 0; d < 4; ++d) {
+                uint32_t e[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                  e[j] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(
+                      rb, 8 * (c0 + half) + 2 * d + j < rank ? bc + (uint32_t)(decltype(ni)::value * MT) * b_pitch + (2 * d + j) * 2u : kOobOffset, 0, 0);
+                w[ni][d] = e[0] | e[1] << 16;
+              }
+            });
+          }
+          static_for<0, MI>([&](auto mi) __attribute__((always_inline)) {
+            t[mi] = buffer_load_16B(rt, on && left[mi] == id ? tc + (uint32_t)(decltype(mi)::value * MT) * t_pitch : kOobOffset);
+          });
+          bf16x8 two[NI];
+          static_for<0, NI>([&](auto ni) __attribute__((always_inline)) {
+            if constexpr (kHalves) {
+              bf16x8 one;
+              lora_parts<T>(__builtin_bit_cast(typename ElemTraits<T>::vec8, w[ni]), one, two[ni]);
+              w[ni] = __builtin_bit_cast(u32x4, MT == 16 && (fq >> 1) ? two[ni] : one);
+            }
+          });
+          if (pass == 0) {
+            bool numbers = true;
+            static_for<0, NI>([&](auto ni) __attribute__((always_inline)) { numbers = numbers && lora_numbers(w[ni]); });
+            again = __builtin_amdgcn_ballot_w64(!numbers) != 0;
+          }
+          if (again) {
+            static_for<0, NI>([&](auto ni) __attribute__((always_inline)) { w[ni] = lora_split(w[ni], pass); });
+            if (pass == 1)
+              static_for<0, MI>([&](auto mi) __attribute__((always_inline)) { t[mi] = on && left[mi] == id ? lora_largest(t[mi]) : u32x4{}; });
+          }
+          static_for<0, MI>([&](auto mi) __attribute__((always_inline)) {
+            if (__builtin_amdgcn_ballot_w64(left[mi] == id) == 0) return;
+            const bf16x8 a = __builtin_bit_cast(bf16x8, t[mi]);
+            static_for<0, NI>([&](auto ni) __attribute__((always_inline)) { multiply(__builtin_bit_cast(bf16x8, w[ni]), a, mi, ni); });
+            if constexpr (kHalves && MT == 32) {
+              if (pass == 0)
+                static_for<0, NI>([&](auto ni) __attribute__((always_inline)) { multiply(two[ni], a, mi, ni); });
+            }
+          });
+          if (!again) break;
+        }
+      }
+#pragma unroll
+      for (int mi = 0; mi < MI; ++mi) left[mi] = left[mi] == id ? -1 : left[mi];
+    }
+  }
+};
+
+// t of eight ranks
+AITAMD_DEVICE void lora_sum(const bf16* t, int c, float (&f)[8]) {
+  const bf16x8 one = load_vec<bf16x8>(t + c * 16), two = load_vec<bf16x8>(t + c * 16 + 8);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = (float)one[j] + (float)two[j];
+}
+// Columns n .. n + COLS - 1 of row m by themselves (those from N on may be anything)
+template <class T, int COLS>
+AITAMD_DEVICE void lora_add(float (&v)[COLS], const GemmParams& p, int m, int n) {
+  using Tr = ElemTraits<T>;
+  const int id = lora_adapter(p, m);
+  if (id < 0) return;
+  const int rank = p.lora_rank, chunks = lora_chunks(rank);
+  const bf16* t = lora_row(p, m);
+  const T* row[COLS];
+#pragma unroll
+  for (int j = 0; j < COLS; ++j) row[j] = lora_column<T>(p, id, n + j < p.N ? n + j : n);
+  const int whole = rank / 8;
+#pragma unroll 1
+  for (int c = 0; c < whole; ++c) {
+    float f[8];
+    lora_sum(t, c, f);
+    typename Tr::vec8 w[COLS];
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) w[j] = load_vec<typename Tr::vec8>(row[j] + c * 8);
+#pragma unroll
+    for (int j = 0; j < COLS; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[j] = __builtin_fmaf(f[e], Tr::to_float(w[j][e]), v[j]);
+  }
+#pragma unroll 1
+  for (int e = whole * 8; e < rank; ++e) {
+    const float f = (float)t[whole * 16 + e % 8] + (float)t[whole * 16 + 8 + e % 8];
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) v[j] = __builtin_fmaf(f, Tr::to_float(row[j][e]), v[j]);
+  }
+}
+
+}  // namespace aitamd

@@ -1,5 +1,5 @@
 // The common case of the eager calls of the decoder operators (quantize_rows, gemm_rcr_int8, rotary_embedding,
-// paged_kv_append, prefix_attention), without the interpreter: see native_calls.cpp, whose rules these follow.  One token's
+// paged_kv_append, prefix_attention, gemm_rcr_lora, qk_norm_rotary, token_logprobs), without the interpreter: see native_calls.cpp, whose rules these follow.  One token's
 // rotation takes 3 us on the GPU and took 16 through Python's attribute reads, checks and ctypes.
 //
 // Beside what native_calls.cpp asks for, every tensor has to be on the current device: the Python path changes it where it is
@@ -203,12 +203,68 @@ bool paged_cache(PyObject* const* args, Operands& ops, at::ScalarType type, int6
   return true;
 }
 
+// the weights of `heads` heads' norms, of one or of each: false where they are no [head_dim] or [heads, head_dim]
+bool norm_weight(const at::Tensor* w, int64_t heads, int64_t head_dim, const void** at, int64_t* stride) {
+  *at = w == nullptr ? nullptr : w->data_ptr();
+  *stride = 0;
+  if (w == nullptr) return true;
+  if (!dense(*w)) return false;
+  if (w->dim() == 1) return w->size(0) == head_dim;
+  if (w->dim() != 2 || w->size(0) != heads || w->size(1) != head_dim) return false;
+  *stride = w->stride(0);
+  return true;
+}
+
+// qk_norm_rotary(q, k, q_weight, k_weight, positions, freqs, eps, interleaved, scale, q_out, k_out): keys, frequencies and new results
+PyObject* qk_norm_rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  return guarded([&]() -> PyObject* {
+    if (nargs != 11 || !PyFloat_CheckExact(args[6]) || !PyBool_Check(args[7]) || !PyFloat_CheckExact(args[8]) || args[9] != Py_None ||
+        args[10] != Py_None || !plain_allocation())
+      return not_ordinary();
+    Operands ops;
+    const at::Tensor* q;
+    const int dt = first_operand(args[0], ops, &q);
+    if (dt < 0 || q->numel() == 0 || !dense(*q)) return not_ordinary();
+    const at::ScalarType type = q->scalar_type();
+    const at::Tensor *k = ops.get(args[1], type), *q_weight = ops.optional(args[2], type), *k_weight = ops.optional(args[3], type),
+                     *positions = gpu_tensor(args[4]), *freqs = ops.get(args[5], at::kFloat);
+    if (!ops.ok || positions == nullptr || positions->device() != q->device()) return not_ordinary();
+    const bool wide = positions->scalar_type() == at::kLong;
+    const int64_t dims = q->dim();
+    if ((!wide && positions->scalar_type() != at::kInt) || (dims != 3 && dims != 4) || freqs->dim() != 1 || !freqs->is_contiguous() ||
+        2 * freqs->numel() > q->size(-1) || positions->dim() < 1 || positions->dim() > dims - 2 || positions->size(-1) != q->size(-3) ||
+        (positions->dim() == 2 && positions->size(0) != q->size(0)) || k->dim() != dims || k->numel() == 0 || !dense(*k) ||
+        k->size(-1) != q->size(-1) || k->size(-3) != q->size(-3) || (dims == 4 && k->size(0) != q->size(0)))
+      return not_ordinary();
+    const bool flat = dims == 3;
+    const int64_t batch = flat ? 1 : q->size(0), seq = q->size(-3), head_dim = q->size(-1), rotated = 2 * freqs->numel();
+    at::Tensor out[2] = {make(q->sizes(), type, *q), make(k->sizes(), type, *q)};
+    aitamd_heads h[2];
+    for (int i = 0; i < 2; ++i) {
+      const at::Tensor &x = i ? *k : *q, &o = out[i];
+      h[i] = {x.data_ptr(), o.data_ptr(), x.size(-2), flat ? 0 : x.stride(0), x.stride(-3), x.stride(-2), flat ? 0 : o.stride(0), o.stride(-3),
+              o.stride(-2), nullptr, 0};
+      if (!norm_weight(i ? k_weight : q_weight, x.size(-2), head_dim, &h[i].weight, &h[i].weight_head_stride)) return not_ordinary();
+    }
+    const int64_t pb = positions->dim() == 2 ? positions->stride(0) : 0, ps = positions->stride(-1);
+    const void* pp = positions->data_ptr();
+    const float *pf = static_cast<const float*>(freqs->data_ptr()), eps = (float)PyFloat_AS_DOUBLE(args[6]), scale = (float)PyFloat_AS_DOUBLE(args[8]);
+    void* stream = current_stream();
+    const int interleaved = args[7] == Py_True;
+    const int rc = unlocked([&] {
+      return aitamd_qk_norm_rotary(dt, &h[0], &h[1], pp, wide, pf, batch, seq, head_dim, rotated, pb, ps, eps, scale, interleaved, stream);
+    });
+    return pair_of(rc, "qk_norm_rotary", out[0], out[1]);
+  });
+}
+
 // paged_kv_append(k, v, k_cache, v_cache, block_table, lengths, offsets, q, freqs, interleaved, scale, first_position, q_out): without
-// frequencies the queries come back as they are
-PyObject* paged_kv_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+// frequencies the queries come back as they are.  With norms, (..., q_weight, k_weight, eps) behind that: of queries and keys that are
+// turned
+PyObject* append_rows(PyObject* const* args, bool normed) {
   return guarded([&]() -> PyObject* {
     int64_t first_position;
-    if (nargs != 13 || !PyBool_Check(args[9]) || !PyFloat_CheckExact(args[10]) || !number(args[11], &first_position)) return not_ordinary();
+    if (!PyBool_Check(args[9]) || !PyFloat_CheckExact(args[10]) || !number(args[11], &first_position)) return not_ordinary();
     Operands ops;
     const at::Tensor* k;
     const int dt = first_operand(args[0], ops, &k);
@@ -224,6 +280,17 @@ PyObject* paged_kv_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         (freqs != nullptr ? freqs->dim() != 1 || !freqs->is_contiguous() || freqs->numel() == 0 || 2 * freqs->numel() > head_dim : out != nullptr))
       return not_ordinary();
     const bool turns = q != nullptr && freqs != nullptr;
+    const void *q_weight = nullptr, *k_weight = nullptr;
+    int64_t q_weight_head = 0, k_weight_head = 0;
+    float eps = 0.0f;
+    if (normed) {
+      if (!turns || !PyFloat_CheckExact(args[15])) return not_ordinary();
+      const at::Tensor *qw = ops.optional(args[13], type), *kw = ops.optional(args[14], type);
+      if (!ops.ok || !norm_weight(qw, q->size(1), head_dim, &q_weight, &q_weight_head) ||
+          !norm_weight(kw, k->size(1), head_dim, &k_weight, &k_weight_head))
+        return not_ordinary();
+      eps = (float)PyFloat_AS_DOUBLE(args[15]);
+    }
     at::Tensor made;
     if (turns && out == nullptr) {
       if (!plain_allocation()) return not_ordinary();
@@ -241,12 +308,16 @@ PyObject* paged_kv_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const float scale = (float)PyFloat_AS_DOUBLE(args[10]);
     const int interleaved = args[9] == Py_True;
     const int rc = unlocked([&] {
-      return aitamd_paged_kv_append(dt, &cache, pk, kt, kh, pv, vt, vh, pq, qt, qh, po, ot, oh, heads, pf, rotated, first_position, scale,
-                                    interleaved, stream);
+      return normed ? aitamd_paged_kv_append_norm(dt, &cache, pk, kt, kh, pv, vt, vh, pq, qt, qh, po, ot, oh, heads, q_weight, q_weight_head,
+                                                  k_weight, k_weight_head, eps, pf, rotated, first_position, scale, interleaved, stream)
+                    : aitamd_paged_kv_append(dt, &cache, pk, kt, kh, pv, vt, vh, pq, qt, qh, po, ot, oh, heads, pf, rotated, first_position,
+                                             scale, interleaved, stream);
     });
     return finish(rc, "paged_kv_append", made.defined() ? &made : nullptr, turns ? args[12] : args[7]);
   });
 }
+PyObject* paged_kv_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return nargs == 13 ? append_rows(args, false) : not_ordinary(); }
+PyObject* paged_kv_append_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return nargs == 16 ? append_rows(args, true) : not_ordinary(); }
 
 // prefix_attention(q, k_cache, v_cache, block_table, lengths, offsets, prefix_table, prefix_length, scale, out, workspace): a new
 // result, a workspace of its own
@@ -291,6 +362,96 @@ PyObject* prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
+// gemm_rcr_lora(x, w, lora_a, lora_b, adapters, scales, bias, out, algo, workspace): a new result
+PyObject* gemm_rcr_lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  return guarded([&]() -> PyObject* {
+    int64_t algo;
+    if (nargs != 10 || args[7] != Py_None || !number(args[8], &algo) || !plain_allocation()) return not_ordinary();
+    Operands ops;
+    const at::Tensor* x;
+    const int dt = first_operand(args[0], ops, &x);
+    if (dt < 0 || x->dim() < 1 || x->numel() == 0) return not_ordinary();
+    const at::ScalarType type = x->scalar_type();
+    const at::Tensor *w = ops.get(args[1], type), *a = ops.get(args[2], type), *b = ops.get(args[3], type), *of = ops.get(args[4], at::kInt),
+                     *scales = ops.optional(args[5], at::kFloat), *bias = ops.optional(args[6], type), *ws = ops.optional(args[9], at::kByte);
+    const int64_t K = x->size(-1), M = x->numel() / K;
+    if (!ops.ok || w->dim() != 2 || w->numel() == 0 || w->size(1) != K || a->dim() != 3 || a->numel() == 0 || a->size(2) != K ||
+        !a->is_contiguous() || b->dim() != 3 || !b->is_contiguous() || of->numel() != M || !of->is_contiguous())
+      return not_ordinary();
+    const int64_t N = w->size(0), n = a->size(0), rank = a->size(1);
+    int64_t ldx, ldw;
+    if (b->size(0) != n || b->size(1) != N || b->size(2) != rank || !flat_row_pitch(*x, M, K, &ldx) || !row_pitch(*w, &ldw) ||
+        (scales != nullptr && (scales->numel() != n || !scales->is_contiguous())) ||
+        (bias != nullptr && (bias->numel() != N || !bias->is_contiguous())) || (ws != nullptr && !ws->is_contiguous()))
+      return not_ordinary();
+    c10::SmallVector<int64_t, 6> sizes(x->sizes().begin(), x->sizes().end());
+    sizes.back() = N;
+    at::Tensor out = make(sizes, type, *x), scratch;
+    if (ws == nullptr) {
+      const int64_t need = aitamd_gemm_lora_workspace_bytes(dt, (int)algo, bias != nullptr, M, N, K, rank);
+      scratch = make({std::max<int64_t>(need, 16)}, at::kByte, *x);
+      ws = &scratch;
+    }
+    const void *px = x->data_ptr(), *pw = w->data_ptr(), *pa = a->data_ptr(), *pb = b->data_ptr(), *pbias = pointer(bias);
+    const int32_t* po = static_cast<const int32_t*>(of->data_ptr());
+    const float* ps = scales == nullptr ? nullptr : static_cast<const float*>(scales->data_ptr());
+    void *c = out.data_ptr(), *scratch_at = ws->data_ptr(), *stream = current_stream();
+    const int64_t ws_bytes = ws->numel();
+    const int rc = unlocked([&] {
+      return aitamd_gemm_rcr_lora(dt, (int)algo, px, pw, pbias, pa, pb, po, ps, c, M, N, K, rank, n, ldx, ldw, N, scratch_at, ws_bytes, stream);
+    });
+    return finish(rc, "gemm_rcr_lora", &out, nullptr);
+  });
+}
+
+// token_logprobs(logits, tokens, top, scale, workspace)
+PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  return guarded([&]() -> PyObject* {
+    int64_t top;
+    if (nargs != 5 || !number(args[2], &top) || !PyFloat_CheckExact(args[3]) || top < 0 || !plain_allocation()) return not_ordinary();
+    const at::Tensor *x = gpu_tensor(args[0]), *tokens = gpu_tensor(args[1]);
+    if (x == nullptr || tokens == nullptr) return not_ordinary();
+    Operands ops;
+    const int dt = x->scalar_type() == at::kFloat ? (int)AITAMD_F32 : dtype_id(*x);
+    const bool wide = tokens->scalar_type() == at::kLong;
+    const at::Tensor* ws = ops.optional(args[4], at::kByte);
+    if (dt < 0 || !ops.ok || !ops.here(*x) || !ops.here(*tokens) || (!wide && tokens->scalar_type() != at::kInt) || x->dim() < 1 || x->numel() == 0 ||
+        !tokens->is_contiguous() || tokens->sizes() != x->sizes().slice(0, x->dim() - 1) || (ws != nullptr && !ws->is_contiguous()))
+      return not_ordinary();
+    const int64_t V = x->size(-1), rows = x->numel() / V;
+    int64_t ld;
+    if (!flat_row_pitch(*x, rows, V, &ld)) return not_ordinary();
+    c10::SmallVector<int64_t, 6> sizes(x->sizes().begin(), x->sizes().end());
+    sizes.back() = top;
+    const at::IntArrayRef lead = x->sizes().slice(0, x->dim() - 1);
+    at::Tensor made[5] = {make(lead, at::kFloat, *x), make(lead, at::kFloat, *x), make(lead, at::kInt, *x), make(sizes, at::kFloat, *x),
+                          make(sizes, at::kInt, *x)};
+    at::Tensor scratch;
+    if (ws == nullptr) {
+      const int64_t need = aitamd_token_logprobs_workspace_bytes(rows, V, top);
+      if (need > 0) {
+        scratch = make({need}, at::kByte, *x);
+        ws = &scratch;
+      }
+    }
+    const void *px = x->data_ptr(), *pt = tokens->data_ptr();
+    float *lp = static_cast<float*>(made[0].data_ptr()), *en = static_cast<float*>(made[1].data_ptr()), *tl = static_cast<float*>(made[3].data_ptr());
+    int32_t *rank = static_cast<int32_t*>(made[2].data_ptr()), *tt = static_cast<int32_t*>(made[4].data_ptr());
+    void *w = ws == nullptr ? nullptr : ws->data_ptr(), *stream = current_stream();
+    const int64_t ws_bytes = ws == nullptr ? 0 : ws->numel();
+    const float scale = (float)PyFloat_AS_DOUBLE(args[3]);
+    const int rc = unlocked([&] { return aitamd_token_logprobs(dt, px, pt, wide, lp, en, rank, tl, tt, rows, V, ld, top, scale, w, ws_bytes, stream); });
+    if (rc != 0) return PyErr_Format(PyExc_RuntimeError, "token_logprobs failed: %s", aitamd_last_error());
+    THPObjectPtr tuple(PyTuple_New(5));
+    for (int i = 0; tuple && i < 5; ++i) {
+      PyObject* o = THPVariable_Wrap(made[i]);
+      if (o == nullptr) return nullptr;
+      PyTuple_SET_ITEM(tuple.get(), i, o);
+    }
+    return tuple.release();
+  });
+}
+
 PyMethodDef kMethods[] = {
 #define AITAMD_METHOD(f, doc) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)), METH_FASTCALL, doc}
     AITAMD_METHOD(quantize_rows, "quantize_rows(x)"),
@@ -298,6 +459,12 @@ PyMethodDef kMethods[] = {
     AITAMD_METHOD(rotary_embedding, "rotary_embedding(x, positions, freqs, interleaved, scale, inverse, out)"),
     AITAMD_METHOD(paged_kv_append,
                   "paged_kv_append(k, v, k_cache, v_cache, block_table, lengths, offsets, q, freqs, interleaved, scale, first_position, q_out)"),
+    AITAMD_METHOD(paged_kv_append_norm,
+                  "paged_kv_append_norm(k, v, k_cache, v_cache, block_table, lengths, offsets, q, freqs, interleaved, scale, first_position, "
+                  "q_out, q_weight, k_weight, eps)"),
+    AITAMD_METHOD(qk_norm_rotary, "qk_norm_rotary(q, k, q_weight, k_weight, positions, freqs, eps, interleaved, scale, q_out, k_out)"),
+    AITAMD_METHOD(gemm_rcr_lora, "gemm_rcr_lora(x, w, lora_a, lora_b, adapters, scales, bias, out, algo, workspace)"),
+    AITAMD_METHOD(token_logprobs, "token_logprobs(logits, tokens, top, scale, workspace)"),
     AITAMD_METHOD(prefix_attention,
                   "prefix_attention(q, k_cache, v_cache, block_table, lengths, offsets, prefix_table, prefix_length, scale, out, workspace)"),
 #undef AITAMD_METHOD

@@ -1,0 +1,483 @@
+// C ABI launchers of aitamd_qk_norm_rotary and aitamd_paged_kv_append_norm.
+//
+// A head x of D numbers becomes x r w with r = 1 / sqrt(sum x^2 / D + eps), then its pairs turn by the token's position
+// (rotary.hpp): all in 32 bits, rounded once.  A head's pieces lie on neighbouring lanes of a wave, one each (a power of two of
+// lanes for a head, up to the wave; of longer heads several each), which sum their squares among themselves and go on with
+// what they have in registers.
+// Bound: memory, 4 bytes an element, as the rotation alone.
+#include "../../include/aitemplate_amd_kernels.h"
+#include "device.hpp"
+#include "errors.hpp"
+#include "paged.hpp"
+#include "rotary.hpp"
+
+namespace aitamd {
+namespace {
+
+// One piece of a head (see RotaryPiece): elements i1 .. and, of pairs of halves, i2 ..
+template <class T, int VEC, bool INTERLEAVED>
+struct NormPiece {
+  using Tr = ElemTraits<T>;
+  using vec = typename RotaryVec<T, VEC>::type;
+  static constexpr bool kTwo = !INTERLEAVED || VEC == 1;  // (VEC = 1: neighbours are two elements of their own)
+  int i1, i2, pair;                                       // pair: the first of the piece's, -1 behind the rotated dims
+  vec v1, v2;
+
+  AITAMD_DEVICE void load(const T* x, int c, int n) {
+    const int turned = VEC == 1 ? n : (INTERLEAVED ? 2 * n / VEC : n / VEC);
+    if (c >= turned) {
+      i1 = i2 = 2 * n + (c - turned) * VEC;
+      pair = -1;
+    } else {
+      i1 = INTERLEAVED && VEC == 1 ? 2 * c : c * VEC;
+      i2 = INTERLEAVED ? i1 + 1 : n + i1;
+      pair = INTERLEAVED && VEC > 1 ? c * (VEC / 2) : c * VEC;
+    }
+    v1 = load_vec<vec>(x + i1);
+    v2 = vec{};
+    if constexpr (kTwo) {
+      if (pair >= 0) v2 = load_vec<vec>(x + i2);
+    }
+  }
+  // the sum of squares, in 32 or 64 bits
+  template <class S>
+  AITAMD_DEVICE S squares() const {
+    S s = 0;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const S a = (S)Tr::to_float(v1[j]);
+      s += a * a;
+      if constexpr (kTwo) {
+        const S b = (S)Tr::to_float(v2[j]);
+        s += b * b;
+      }
+    }
+    return s;
+  }
+  // as it is
+  AITAMD_DEVICE void copy(T* y) const {
+    store_vec(y + i1, v1);
+    if constexpr (kTwo) {
+      if (pair >= 0) store_vec(y + i2, v2);
+    }
+  }
+  // times ra, times rb and the weights (of one without: weight null), turned
+  AITAMD_DEVICE void store(T* y, const T* weight, float ra, float rb, const float2* table) const {
+    float a[VEC], b[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      a[j] = Tr::to_float(v1[j]);
+      b[j] = Tr::to_float(v2[j]);
+    }
+    if (weight != nullptr) {
+      const vec w1 = load_vec<vec>(weight + i1);
+      vec w2 = w1;
+      if constexpr (kTwo) {
+        if (pair >= 0) w2 = load_vec<vec>(weight + i2);
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        a[j] = a[j] * ra * (rb * Tr::to_float(w1[j]));
+        if constexpr (kTwo) b[j] = b[j] * ra * (rb * Tr::to_float(w2[j]));
+      }
+    }
+    vec o1, o2;
+    if (pair >= 0) {
+      if constexpr (kTwo) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float2 t = table[pair + j];
+          o1[j] = Tr::from_float(a[j] * t.x - b[j] * t.y);
+          o2[j] = Tr::from_float(b[j] * t.x + a[j] * t.y);
+        }
+        store_vec(y + i2, o2);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+          const float2 t = table[pair + j];
+          o1[2 * j] = Tr::from_float(a[2 * j] * t.x - a[2 * j + 1] * t.y);
+          o1[2 * j + 1] = Tr::from_float(a[2 * j + 1] * t.x + a[2 * j] * t.y);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) o1[j] = Tr::from_float(a[j]);
+    }
+    store_vec(y + i1, o1);
+  }
+};
+
+template <class S>
+AITAMD_DEVICE S lanes_sum(S v, int lanes) {
+  for (int d = lanes >> 1; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+// 1 / sqrt(sum / dim + eps) as ra * rb.  Where the sum leaves the range of 32 bits (numbers above 2^57 or so; below 2^-50 without an
+// eps), `again` gives it in 64.
+template <class F>
+AITAMD_DEVICE void inverse_length(float sum, float by_dim, float eps, float& ra, float& rb, F&& again) {
+  const float mean = __builtin_fmaf(sum, by_dim, eps);
+  const bool fits = mean > 1e-30f && mean < 1e30f;
+  ra = rsqrtf(mean);
+  rb = 1.0f;
+  if (__builtin_amdgcn_ballot_w64(!fits) != 0) {
+    const double exact = again() * (double)by_dim + (double)eps;
+    if (!fits) {
+      // (a NaN is neither; an infinity makes zeros, and NaN of itself)
+      const double r = exact == 0.0 ? 0.0 : 1.0 / sqrt(exact);
+      const double half = sqrt(r);
+      ra = (float)half;
+      rb = (float)half;
+    }
+  }
+}
+
+enum HeadKind : int { kNothing = 0, kNorm = 1, kTurnOnly = 2, kCopy = 3 };
+template <class T>
+struct Head {
+  int kind;
+  const T* x;
+  T* y;
+  const T* weight;
+  const float2* table;
+};
+
+struct Lanes {
+  int32_t per_head, shift, pieces, n;  // lanes of a head (1 << shift), its pieces, its pairs
+  float by_dim, eps;
+};
+
+// Heads 0 .. count - 1 of a workgroup, kAhead of a lane's on their way together.  head(i) is the same for all lanes of a head.
+template <class T, int VEC, bool INTERLEAVED, int AHEAD, class F>
+AITAMD_DEVICE void heads_of_workgroup(const Lanes& l, int count, F&& head) {
+  const int lane = threadIdx.x & (l.per_head - 1), at_once = kRotaryThreads >> l.shift;
+  const bool one_each = l.pieces <= l.per_head;
+  // (whole waves stay together: their lanes exchange sums)
+  for (int i0 = threadIdx.x >> l.shift; i0 - (int)(threadIdx.x >> l.shift) < count; i0 += AHEAD * at_once) {
+    Head<T> h[AHEAD];
+    NormPiece<T, VEC, INTERLEAVED> piece[AHEAD];
+    float sum[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int i = i0 + a * at_once;
+      h[a].kind = kNothing;
+      sum[a] = 0.0f;
+      if (i >= count) continue;
+      h[a] = head(i);
+      if (h[a].kind == kNothing || lane >= l.pieces) continue;
+      piece[a].load(h[a].x, lane, l.n);
+    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const bool on = h[a].kind != kNothing && lane < l.pieces;
+      if (on && h[a].kind == kNorm) {
+        sum[a] = piece[a].template squares<float>();
+        if (!one_each) {
+          for (int c = lane + l.per_head; c < l.pieces; c += l.per_head) {
+            NormPiece<T, VEC, INTERLEAVED> more;
+            more.load(h[a].x, c, l.n);
+            sum[a] += more.template squares<float>();
+          }
+        }
+      }
+      float ra = 1.0f, rb = 1.0f;
+      if (__builtin_amdgcn_ballot_w64(h[a].kind == kNorm) != 0) {
+        sum[a] = lanes_sum(sum[a], l.per_head);
+        // (of lanes without a head: of a sum that fits)
+        inverse_length(h[a].kind == kNorm ? sum[a] : 1.0f / l.by_dim, l.by_dim, l.eps, ra, rb, [&]() {
+          double s = 0.0;
+          if (on && h[a].kind == kNorm) {
+            s = piece[a].template squares<double>();
+            for (int c = lane + l.per_head; c < l.pieces; c += l.per_head) {
+              NormPiece<T, VEC, INTERLEAVED> more;
+              more.load(h[a].x, c, l.n);
+              s += more.template squares<double>();
+            }
+          }
+          return lanes_sum(s, l.per_head);
+        });
+      }
+      if (!on) continue;
+      auto put = [&](const NormPiece<T, VEC, INTERLEAVED>& q) __attribute__((always_inline)) {
+        if (h[a].kind == kCopy)
+          q.copy(h[a].y);
+        else
+          q.store(h[a].y, h[a].kind == kNorm ? h[a].weight : nullptr, ra, rb, h[a].table);
+      };
+      put(piece[a]);
+      if (!one_each) {
+        for (int c = lane + l.per_head; c < l.pieces; c += l.per_head) {
+          NormPiece<T, VEC, INTERLEAVED> more;
+          more.load(h[a].x, c, l.n);
+          put(more);
+        }
+      }
+    }
+  }
+}
+
+struct HeadsParams {
+  const void* x;
+  void* out;
+  const void* weight;
+  int64_t x_batch, x_seq, x_head, out_batch, out_seq, out_head, weight_head;
+};
+struct NormParams {
+  HeadsParams q, k;
+  const void* positions;
+  const float* freqs;
+  int64_t pos_batch, pos_seq;
+  int32_t tokens, heads, all_heads, seq, first, per_wg, positions_64;
+  float scale;
+  Lanes lanes;
+  Divisor by_n, by_seq, by_heads;
+};
+
+constexpr int kNormAhead = 2;
+
+template <class T, int VEC, bool INTERLEAVED>
+__global__ void __launch_bounds__(kRotaryThreads) norm_rotary_kernel(const NormParams p) {
+  __shared__ float2 table[kRotaryTable];
+  const int t0 = p.first + blockIdx.x * p.per_wg;
+  const int tokens = p.tokens - t0 < p.per_wg ? p.tokens - t0 : p.per_wg;
+  fill_rotary_table(table, p.freqs, p.lanes.n, p.by_n, tokens, p.scale, 1.0f, [&](int t) -> int64_t {
+    const int b = quotient(t0 + t, p.by_seq);
+    const int64_t at = b * p.pos_batch + (t0 + t - b * p.seq) * p.pos_seq;
+    return p.positions_64 ? reinterpret_cast<const int64_t*>(p.positions)[at] : reinterpret_cast<const int32_t*>(p.positions)[at];
+  });
+  __syncthreads();
+  heads_of_workgroup<T, VEC, INTERLEAVED, kNormAhead>(p.lanes, tokens * p.all_heads, [&](int i) __attribute__((always_inline)) {
+    const int t = quotient(i, p.by_heads);
+    int head = i - t * p.all_heads;
+    const int b = quotient(t0 + t, p.by_seq), s = t0 + t - b * p.seq;
+    const bool is_k = head >= p.heads;
+    if (is_k) head -= p.heads;
+    const HeadsParams& h = is_k ? p.k : p.q;
+    Head<T> r;
+    r.kind = h.weight != nullptr ? kNorm : kTurnOnly;
+    r.x = reinterpret_cast<const T*>(h.x) + b * h.x_batch + s * h.x_seq + head * h.x_head;
+    r.y = reinterpret_cast<T*>(h.out) + b * h.out_batch + s * h.out_seq + head * h.out_head;
+    r.weight = reinterpret_cast<const T*>(h.weight) + head * h.weight_head;
+    r.table = table + t * p.lanes.n;
+    return r;
+  });
+}
+
+struct AppendNormParams {
+  PagedCache cache;
+  const void *q, *k, *v, *q_weight, *k_weight;
+  void* q_out;
+  const float* freqs;
+  int64_t q_token, q_head, q_out_token, q_out_head, k_token, k_head, v_token, v_head, q_weight_head, k_weight_head, first_position;
+  int32_t heads, all_heads, first, per_wg;
+  float scale;
+  Lanes lanes;
+  Divisor by_n, by_heads;
+};
+
+constexpr int kAppendNormAhead = 2;
+
+// One launch for a layer's new tokens, as append_kernel (rotary_api.hip)
+template <class T, int VEC, bool INTERLEAVED>
+__global__ void __launch_bounds__(kRotaryThreads) append_norm_kernel(const AppendNormParams p) {
+  __shared__ float2 table[kRotaryTable];
+  __shared__ int64_t slot[kRotaryMaxTokens];  // among the sequence's own tokens
+  __shared__ int32_t page[kRotaryMaxTokens];  // -1: nowhere to go
+  __shared__ int32_t in_page[kRotaryMaxTokens];
+  __shared__ bool live[kRotaryMaxTokens];
+  const PagedCache& c = p.cache;
+  const int t0 = p.first + blockIdx.x * p.per_wg;
+  const int tokens = c.tokens - t0 < p.per_wg ? c.tokens - t0 : p.per_wg;
+  const int s0 = c.offsets != nullptr ? sequence_of_row(c, t0) : t0;  // (every wave for itself)
+  if ((int)threadIdx.x < tokens) {
+    const int t = threadIdx.x, row = t0 + t;
+    int s = c.offsets != nullptr ? s0 : row;
+    int first = row;
+    if (c.offsets != nullptr) {
+      while (s < c.batch && c.offsets[s + 1] <= row) ++s;
+      first = s < c.batch ? c.offsets[s] : 0;
+    }
+    const bool in = s < c.batch && row >= first;
+    live[t] = in;
+    const int64_t at = in ? (int64_t)c.lengths[s] + (row - first) : -1;
+    slot[t] = at;
+    int pg = -1, within = 0;
+    if (at >= 0 && at < c.most_keys) {
+      const int which = quotient((int)at, c.by_page);
+      within = (int)at - which * c.page_size;
+      pg = c.table[s * c.table_pitch + which];
+      if (pg >= c.pages) pg = -1;
+    }
+    page[t] = pg;
+    in_page[t] = within;
+  }
+  __syncthreads();
+  if (p.lanes.n > 0) {
+    fill_rotary_table(table, p.freqs, p.lanes.n, p.by_n, tokens, p.scale, 1.0f, [&](int t) { return p.first_position + slot[t]; });
+    __syncthreads();
+  }
+  heads_of_workgroup<T, VEC, INTERLEAVED, kAppendNormAhead>(p.lanes, tokens * p.all_heads, [&](int i) __attribute__((always_inline)) {
+    const int t = quotient(i, p.by_heads);
+    int head = i - t * p.all_heads;
+    const int64_t row = t0 + t;
+    Head<T> r;
+    r.kind = kNothing;
+    r.table = table + t * p.lanes.n;
+    r.weight = nullptr;
+    if (head < p.heads) {
+      if (live[t]) r.kind = p.q_weight != nullptr ? kNorm : kTurnOnly;
+      r.x = reinterpret_cast<const T*>(p.q) + row * p.q_token + head * p.q_head;
+      r.y = reinterpret_cast<T*>(p.q_out) + row * p.q_out_token + head * p.q_out_head;
+      r.weight = reinterpret_cast<const T*>(p.q_weight) + head * p.q_weight_head;
+      return r;
+    }
+    head -= p.heads;
+    const bool is_v = head >= c.kv_heads;
+    if (is_v) head -= c.kv_heads;
+    const int64_t pg = page[t], within = in_page[t];
+    if (live[t] && pg >= 0) r.kind = is_v ? kCopy : (p.k_weight != nullptr ? kNorm : kTurnOnly);
+    r.x = is_v ? reinterpret_cast<const T*>(p.v) + row * p.v_token + head * p.v_head : reinterpret_cast<const T*>(p.k) + row * p.k_token + head * p.k_head;
+    r.y = is_v ? reinterpret_cast<T*>(c.v) + pg * c.v_page + within * c.v_slot + head * c.v_head
+               : reinterpret_cast<T*>(c.k) + pg * c.k_page + within * c.k_slot + head * c.k_head;
+    r.weight = reinterpret_cast<const T*>(p.k_weight) + head * p.k_weight_head;
+    return r;
+  });
+}
+
+template <class P>
+hipError_t launch_wgs(void (*kernel)(P), P p, int64_t tokens, hipStream_t stream) {
+  const int64_t wgs = (tokens + p.per_wg - 1) / p.per_wg, most = most_workgroups(kRotaryThreads);
+  for (int64_t wg = 0; wg < wgs; wg += most) {
+    p.first = (int32_t)(wg * p.per_wg);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(wgs - wg < most ? wgs - wg : most)), dim3(kRotaryThreads), 0, stream, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+#define AITAMD_BY_VEC(KERNEL)                                                         \
+  (interleaved ? (vec == 8     ? KERNEL<T, 8, true>                                   \
+                      : vec == 4 ? KERNEL<T, 4, true>                                 \
+                      : vec == 2 ? KERNEL<T, 2, true>                                 \
+                                 : KERNEL<T, 1, true>)                                \
+               : (vec == 8     ? KERNEL<T, 8, false>                                  \
+                      : vec == 4 ? KERNEL<T, 4, false>                                \
+                      : vec == 2 ? KERNEL<T, 2, false>                                \
+                                 : KERNEL<T, 1, false>))
+template <class T>
+hipError_t launch_norm(const NormParams& p, int vec, bool interleaved, hipStream_t stream) {
+  return launch_wgs(AITAMD_BY_VEC(norm_rotary_kernel), p, p.tokens, stream);
+}
+template <class T>
+hipError_t launch_append(const AppendNormParams& p, int vec, bool interleaved, hipStream_t stream) {
+  return launch_wgs(AITAMD_BY_VEC(append_norm_kernel), p, p.cache.tokens, stream);
+}
+#undef AITAMD_BY_VEC
+
+int check_norm(const char* who, int64_t head_dim, int64_t rotated, const float* freqs, float eps) {
+  if (head_dim > kRotaryMaxDim) return fail("%s: head_dim %lld is beyond %lld", who, (long long)head_dim, (long long)kRotaryMaxDim);
+  if (rotated < 0 || rotated % 2 != 0 || rotated > head_dim)
+    return fail("%s: %lld rotated dims: an even number up to head_dim %lld is wanted", who, (long long)rotated, (long long)head_dim);
+  if (rotated > 0 && !freqs) return fail("%s: null pointer (freqs)", who);
+  if (!(eps >= 0.0f) || !__builtin_isfinite(eps)) return fail("%s: eps %g is no number of at least 0", who, (double)eps);
+  return 0;
+}
+// Lanes of a head: as many as it has pieces, rounded up to a power of two, up to a wave
+Lanes head_lanes(int64_t n, int64_t head_dim, bool interleaved, int vec, float eps) {
+  Lanes l{};
+  l.n = (int32_t)n;
+  l.pieces = rotary_pieces((int)n, (int)head_dim, interleaved, vec);
+  while ((1 << l.shift) < l.pieces && l.shift < 6) ++l.shift;
+  l.per_head = 1 << l.shift;
+  l.by_dim = 1.0f / (float)head_dim;
+  l.eps = eps;
+  return l;
+}
+
+}  // namespace
+}  // namespace aitamd
+
+using namespace aitamd;
+
+extern "C" int aitamd_qk_norm_rotary(int dtype, const aitamd_heads* q, const aitamd_heads* k, const void* positions, int positions_64,
+                                     const float* freqs, int64_t batch, int64_t seq, int64_t head_dim, int64_t rotated, int64_t pos_batch,
+                                     int64_t pos_seq, float eps, float scale, int interleaved, void* stream) {
+  const char* who = "aitamd_qk_norm_rotary";
+  if (dtype != AITAMD_F16 && dtype != AITAMD_BF16) return fail("%s: bad dtype %d", who, dtype);
+  if (batch < 0 || seq < 0 || head_dim < 0 || (q && q->heads < 0) || (k && k->heads < 0)) return fail("%s: negative dimension", who);
+  if (check_norm(who, head_dim, rotated, freqs, eps)) return 1;
+  const int64_t heads = q ? q->heads : 0, kv_heads = k ? k->heads : 0;
+  if (batch == 0 || seq == 0 || heads + kv_heads == 0 || head_dim == 0) return 0;
+  if ((heads > 0 && (!q->x || !q->out)) || (kv_heads > 0 && (!k->x || !k->out)) || (rotated > 0 && !positions)) return fail("%s: null pointer", who);
+  const int64_t n = rotated / 2;
+  const int vec = rotary_vec(n, head_dim, interleaved != 0);
+  NormParams p{};
+  p.lanes = head_lanes(n, head_dim, interleaved != 0, vec, eps);
+  if (batch > 0x7fffffffll / seq || heads > 0x7fffffffll || kv_heads > 0x7fffffffll ||
+      heads + kv_heads > 0x3fffffffll / kRotaryMaxTokens / p.lanes.per_head)
+    return fail("%s: dimension too large", who);
+  auto fill = [](const aitamd_heads* a) {
+    HeadsParams h{};
+    if (a) h = {a->x, a->out, a->weight, a->batch_stride, a->seq_stride, a->head_stride, a->out_batch_stride, a->out_seq_stride, a->out_head_stride,
+                a->weight_head_stride};
+    return h;
+  };
+  p.q = fill(q), p.k = fill(k);
+  p.positions = positions, p.positions_64 = positions_64;
+  p.freqs = freqs;
+  p.pos_batch = pos_batch, p.pos_seq = pos_seq;
+  p.tokens = (int32_t)(batch * seq), p.heads = (int32_t)heads, p.all_heads = (int32_t)(heads + kv_heads), p.seq = (int32_t)seq;
+  p.per_wg = rotary_tokens(batch * seq, (heads + kv_heads) * p.lanes.per_head, n, current_device_cus());
+  p.scale = scale;
+  p.by_n = make_divisor(n > 0 ? n : 1);
+  p.by_seq = make_divisor(seq);
+  p.by_heads = make_divisor(heads + kv_heads);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const hipError_t e = dtype == AITAMD_F16 ? launch_norm<f16>(p, vec, interleaved != 0, s) : launch_norm<bf16>(p, vec, interleaved != 0, s);
+  if (e != hipSuccess) return fail("%s: launch failed: %s", who, hipGetErrorString(e));
+  return 0;
+}
+
+extern "C" int aitamd_paged_kv_append_norm(int dtype, const aitamd_paged_cache* cache, const void* k, int64_t k_token, int64_t k_head,
+                                           const void* v, int64_t v_token, int64_t v_head, const void* q, int64_t q_token, int64_t q_head,
+                                           void* q_out, int64_t q_out_token, int64_t q_out_head, int64_t heads, const void* q_weight,
+                                           int64_t q_weight_head, const void* k_weight, int64_t k_weight_head, float eps, const float* freqs,
+                                           int64_t rotated, int64_t first_position, float scale, int interleaved, void* stream) {
+  if (!q_weight && !k_weight)
+    return aitamd_paged_kv_append(dtype, cache, k, k_token, k_head, v, v_token, v_head, q, q_token, q_head, q_out, q_out_token, q_out_head, heads,
+                                  freqs, rotated, first_position, scale, interleaved, stream);
+  const char* who = "aitamd_paged_kv_append_norm";
+  AppendNormParams p{};
+  if (dtype != AITAMD_F16 && dtype != AITAMD_BF16) return fail("%s: bad dtype %d", who, dtype);
+  if (paged_cache(who, cache, 1, &p.cache)) return 1;
+  const int64_t head_dim = cache->head_dim, kv_heads = cache->kv_heads, tokens = cache->tokens;
+  if (check_norm(who, head_dim, rotated, freqs, eps)) return 1;
+  if (heads < 0) return fail("%s: negative dimension", who);
+  if (!q) heads = 0;
+  if (tokens == 0 || (kv_heads == 0 && heads == 0) || cache->batch == 0 || head_dim == 0) return 0;
+  if (kv_heads > 0 && (!k || !v || !cache->k || !cache->v)) return fail("%s: null pointer", who);
+  if (heads > 0 && !q_out) return fail("%s: null pointer (q_out)", who);
+  const int64_t n = rotated / 2;
+  const int vec = rotary_vec(n, head_dim, interleaved != 0);
+  p.lanes = head_lanes(n, head_dim, interleaved != 0, vec, eps);
+  if (heads > 0x7fffff || kv_heads > 0x7fffff || heads + 2 * kv_heads > 0x3fffffffll / kRotaryMaxTokens / p.lanes.per_head)
+    return fail("%s: dimension too large", who);
+  p.q = q, p.k = k, p.v = v;
+  p.q_weight = q_weight, p.k_weight = k_weight;
+  p.q_weight_head = q_weight_head, p.k_weight_head = k_weight_head;
+  p.q_out = q_out;
+  p.freqs = freqs;
+  p.heads = (int32_t)heads, p.all_heads = (int32_t)(heads + 2 * kv_heads);
+  p.per_wg = rotary_tokens(tokens, p.all_heads * p.lanes.per_head, n, current_device_cus());
+  p.q_token = q_token, p.q_head = q_head, p.q_out_token = q_out_token, p.q_out_head = q_out_head;
+  p.k_token = k_token, p.k_head = k_head, p.v_token = v_token, p.v_head = v_head;
+  p.first_position = first_position;
+  p.scale = scale;
+  p.by_n = make_divisor(n > 0 ? n : 1);
+  p.by_heads = make_divisor(p.all_heads);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const hipError_t e = dtype == AITAMD_F16 ? launch_append<f16>(p, vec, interleaved != 0, s) : launch_append<bf16>(p, vec, interleaved != 0, s);
+  if (e != hipSuccess) return fail("%s: launch failed: %s", who, hipGetErrorString(e));
+  return 0;
+}

@@ -686,6 +686,69 @@ def rotary_embedding(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tens
     return out
 
 
+def _norm_weight(weight: Optional[torch.Tensor], name: str, heads: int, head_dim: int) -> Tuple[Optional[ctypes.c_void_p], int]:
+    """(pointer, elements from one head's weights to the next's) of [head_dim] or [heads, head_dim]."""
+    if weight is None:
+        return None, 0
+    if tuple(weight.shape) not in ((head_dim,), (heads, head_dim)):
+        raise ValueError(f"{name} must be [{head_dim}] or [{heads}, {head_dim}], got {tuple(weight.shape)}")
+    _dense_heads(weight, name)
+    return _p(weight), weight.stride(0) if weight.dim() == 2 else 0
+
+
+def qk_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                   positions: torch.Tensor, freqs: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+                   scale: float = 1.0, q_out: Optional[torch.Tensor] = None,
+                   k_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Heads of the queries `q` and the keys `k` [tokens, heads, head_dim] or [batch, seq, heads, head_dim] (any strides, contiguous
+    head dims; `k` may be None and have another number of heads), normalized and rotated in one launch: every head x becomes
+    x / sqrt(mean(x ** 2) + eps) * weight, with `q_weight` or `k_weight` [head_dim] or [heads, head_dim], and is then turned as by
+    `rotary_embedding` (`positions`, `freqs`, `interleaved`, `scale` as there; without `freqs` it is not), in fp32, rounded once.
+    An operand whose weight is None is rotated only.  A head of zeros stays one, also with eps = 0.
+
+    `q_out` and `k_out` may be `q` and `k` themselves and must not overlap operands otherwise.  Returns (q_out, k_out)."""
+    result = _native_decoder.qk_norm_rotary(q, k, q_weight, k_weight, positions, freqs, eps, interleaved, scale, q_out, k_out)
+    if result is not NotImplemented:
+        return result
+    device = _operands(("q", q, tuple(_TORCH_DTYPE_ID)), ("k", k, (q.dtype,)), ("q_weight", q_weight, (q.dtype,)),
+                       ("k_weight", k_weight, (q.dtype,)), ("positions", positions, (torch.int32, torch.int64)),
+                       ("freqs", freqs, (torch.float32,)), ("q_out", q_out, (q.dtype,)), ("k_out", k_out, (q.dtype,)))
+    if q.dim() not in (3, 4):
+        raise ValueError("q must be [tokens, heads, head_dim] or [batch, seq, heads, head_dim]")
+    if k is None and (k_weight is not None or k_out is not None):
+        raise ValueError("k_weight or k_out without k")
+    if k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]):
+        raise ValueError(f"k of shape {tuple(k.shape)} does not fit q of shape {tuple(q.shape)}")
+    head_dim = q.shape[-1]
+    rotated = 0 if freqs is None else _check_freqs(freqs, head_dim)
+    if tuple(positions.shape) not in (tuple(q.shape[:-2]), tuple(q.shape[-3:-2])):
+        raise ValueError(f"positions of shape {tuple(positions.shape)} do not fit q of shape {tuple(q.shape)}")
+    flat = q.dim() == 3
+    operands, outs = [], []
+    for x, weight, out, name in ((q, q_weight, q_out, "q"), (k, k_weight, k_out, "k")):
+        if x is None:
+            operands.append(None)
+            outs.append(None)
+            continue
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=device)
+        elif out.shape != x.shape:
+            raise ValueError(f"{name}_out must be {tuple(x.shape)}, got {tuple(out.shape)}")
+        _dense_heads(x, name), _dense_heads(out, name + "_out")
+        at, head_stride = _norm_weight(weight, name + "_weight", x.shape[-2], head_dim)
+        xs, os = ((0,) + t.stride() if flat else t.stride() for t in (x, out))
+        operands.append(_kernels.Heads(_p(x), _p(out), x.shape[-2], *xs[:3], *os[:3], at, head_stride))
+        outs.append(out)
+    batch, seq = (1, q.shape[0]) if flat else (q.shape[0], q.shape[1])
+    ps = (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()
+    with torch.cuda.device(device):
+        rc = _kernels.load().aitamd_qk_norm_rotary(
+            _TORCH_DTYPE_ID[q.dtype], *operands, _p(positions), int(positions.dtype == torch.int64), _p(freqs) if rotated else None, batch, seq,
+            head_dim, rotated, *ps, float(eps), float(scale), int(bool(interleaved)), _stream_ptr())
+    _kernels.check(rc, "qk_norm_rotary")
+    return outs[0], outs[1]
+
+
 def _paged_cache(k_cache, v_cache, block_table, lengths, offsets, tokens, head_dim) -> "_kernels.PagedCache":
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
         raise ValueError(f"k_cache and v_cache must be [pages, page_size, kv_heads, head_dim], got {tuple(k_cache.shape)} and "
@@ -711,7 +774,8 @@ def _paged_cache(k_cache, v_cache, block_table, lengths, offsets, tokens, head_d
 def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                     lengths: torch.Tensor, offsets: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
                     freqs: Optional[torch.Tensor] = None, interleaved: bool = False, scale: float = 1.0, first_position: int = 0,
-                    q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+                    q_out: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
+                    k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> Optional[torch.Tensor]:
     """One step's keys and values `k`, `v` [tokens, kv_heads, head_dim] into the pages of their sequences, in one launch with the
     rotation of the keys and of the queries `q` [tokens, heads, head_dim]; returns the rotated queries (None without `q`).
 
@@ -721,18 +785,22 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     int32: sequence i has the rows offsets[i] to offsets[i + 1]; without it, row i.  Row j of a sequence goes to its place
     lengths[i] + j, rotated (with `freqs`, as by `rotary_embedding`) for position first_position + lengths[i] + j.
 
+    With `q_weight` the heads of the queries, with `k_weight` those of the keys are normalized ahead of the rotation, as by
+    `qk_norm_rotary` (the same launch).
+
     Rows from offsets[batch] on are left as they were, in `q_out` too; keys and values that no page is there for are dropped.
     Pages that are written must not be shared between sequences.  `lengths` stay as they are: the attention of the same step
     takes them as they are too.  `q_out` may be `q`."""
-    result = _native_decoder.paged_kv_append(k, v, k_cache, v_cache, block_table, lengths, offsets, q, freqs, interleaved, scale,
-                                             first_position, q_out)
+    normed = q_weight is not None or k_weight is not None
+    args = (k, v, k_cache, v_cache, block_table, lengths, offsets, q, freqs, interleaved, scale, first_position, q_out)
+    result = _native_decoder.paged_kv_append_norm(*args, q_weight, k_weight, eps) if normed else _native_decoder.paged_kv_append(*args)
     if result is not NotImplemented:
         return result
     types = tuple(_TORCH_DTYPE_ID)
     device = _operands(("k", k, types), ("v", v, (k.dtype,)), ("k_cache", k_cache, (k.dtype,)), ("v_cache", v_cache, (k.dtype,)),
                        ("block_table", block_table, (torch.int32,)), ("lengths", lengths, (torch.int32,)),
                        ("offsets", offsets, (torch.int32,)), ("q", q, (k.dtype,)), ("freqs", freqs, (torch.float32,)),
-                       ("q_out", q_out, (k.dtype,)))
+                       ("q_out", q_out, (k.dtype,)), ("q_weight", q_weight, (k.dtype,)), ("k_weight", k_weight, (k.dtype,)))
     if k.dim() != 3 or k.shape != v.shape:
         raise ValueError(f"k and v must be [tokens, kv_heads, head_dim], got {tuple(k.shape)} and {tuple(v.shape)}")
     tokens, kv_heads, head_dim = k.shape
@@ -743,25 +811,28 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     rotated = 0 if freqs is None else _check_freqs(freqs, head_dim)
     q_in, heads, qs, os = None, 0, (0, 0), (0, 0)
     if q is None:
-        if q_out is not None:
-            raise ValueError("q_out without q")
+        if q_out is not None or q_weight is not None:
+            raise ValueError("q_out or q_weight without q")
     else:
         if q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != head_dim:
             raise ValueError(f"q must be [{tokens}, heads, {head_dim}], got {tuple(q.shape)}")
         _dense_heads(q, "q")
-        if q_out is None and rotated == 0:
+        if q_out is None and rotated == 0 and q_weight is None:
             q_out = q  # (nothing is done to it)
         elif q_out is None:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
         elif q_out.shape != q.shape:
             raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
         _dense_heads(q_out, "q_out")
-        if q_out is not q or rotated:
+        if q_out is not q or rotated or q_weight is not None:
             q_in, heads, qs, os = q, q.shape[1], q.stride(), q_out.stride()
+    norms = (_norm_weight(q_weight, "q_weight", heads, head_dim) + _norm_weight(k_weight, "k_weight", kv_heads, head_dim) + (float(eps),)
+             if normed else ())
+    lib = _kernels.load()
     with torch.cuda.device(device):
-        rc = _kernels.load().aitamd_paged_kv_append(
+        rc = (lib.aitamd_paged_kv_append_norm if normed else lib.aitamd_paged_kv_append)(
             _TORCH_DTYPE_ID[k.dtype], cache, _p(k), *k.stride()[:2], _p(v), *v.stride()[:2], _p(q_in), *qs[:2],
-            _p(q_out) if q_in is not None else None, *os[:2], heads, _p(freqs) if rotated else None, rotated, int(first_position),
+            _p(q_out) if q_in is not None else None, *os[:2], heads, *norms, _p(freqs) if rotated else None, rotated, int(first_position),
             float(scale), int(bool(interleaved)), _stream_ptr())
     _kernels.check(rc, "paged_kv_append")
     return q_out
@@ -832,3 +903,125 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
             float(head_dim ** -0.5 if scale is None else scale), _p(workspace), 0 if workspace is None else workspace.numel(), _stream_ptr())
     _kernels.check(rc, "prefix_attention")
     return out
+
+
+# ---- what a served decoder computes around its attention ----------------------------------------------------------
+
+def gemm_lora_workspace_bytes(M: int, N: int, K: int, rank: int, bias: bool = False, dtype=torch.float16, algo: int = -1) -> int:
+    """Bytes of scratch memory with which `gemm_rcr_lora` may choose any of its instances for this problem."""
+    return int(_kernels.load().aitamd_gemm_lora_workspace_bytes(_TORCH_DTYPE_ID[dtype], algo, int(bool(bias)), M, N, K, rank))
+
+
+def gemm_rcr_lora(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapters: torch.Tensor,
+                  scales: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                  algo: int = -1, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A projection that many requests share with the low-rank adapter of each row's request beside it:
+    out[m] = x[m] @ w.T (+ bias) + scales[i] * (x[m] @ lora_a[i].T) @ lora_b[i].T with i = adapters[m], rounded once.
+
+    `x` [..., K] and `w` [N, K] (2-D views may have row pitch), `lora_a` [n, rank, K] and `lora_b` [n, N, rank] (rank 1 to 1024;
+    adapters of a lower rank have zeros in the rest) and `bias` [N] of one type; `scales` fp32 [n] (1 without); `adapters` int32
+    [...], one for each row of `x`: rows whose number is not in [0, n), for instance -1, have none.  The rows may be in any order;
+    neighbours with the same adapter are faster.
+
+    `algo` as of `gemm`.  `workspace`: `gemm_lora_workspace_bytes` bytes, which need not be zero, allocated for the call otherwise;
+    calls that may overlap in time need one each."""
+    result = _native_decoder.gemm_rcr_lora(x, w, lora_a, lora_b, adapters, scales, bias, out, algo, workspace)
+    if result is not NotImplemented:
+        return result
+    dtype = x.dtype
+    device = _operands(("x", x, tuple(_TORCH_DTYPE_ID)), ("w", w, (dtype,)), ("lora_a", lora_a, (dtype,)), ("lora_b", lora_b, (dtype,)),
+                       ("adapters", adapters, (torch.int32,)), ("scales", scales, (torch.float32,)), ("bias", bias, (dtype,)),
+                       ("out", out, (dtype,)), ("workspace", workspace, (torch.uint8,)))
+    if x.dim() < 1:
+        raise ValueError("x must have at least one dimension")
+    lead, K = x.shape[:-1], x.shape[-1]
+    M = 1
+    for d in lead:
+        M *= d
+    if w.dim() != 2 or w.shape[1] != K:
+        raise ValueError(f"w must be [N, K={K}], got {tuple(w.shape)}")
+    N = w.shape[0]
+    if lora_a.dim() != 3 or lora_a.shape[2] != K or not lora_a.is_contiguous():
+        raise ValueError(f"lora_a must be contiguous [adapters, rank, K={K}], got {tuple(lora_a.shape)}")
+    n, rank = lora_a.shape[:2]
+    if tuple(lora_b.shape) != (n, N, rank) or not lora_b.is_contiguous():
+        raise ValueError(f"lora_b must be contiguous {(n, N, rank)}, got {tuple(lora_b.shape)}")
+    for t, count, name in ((adapters, M, "adapters"), (scales, n, "scales"), (bias, N, "bias")):
+        if t is not None and (t.numel() != count or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous with {count} elements, got shape {tuple(t.shape)}")
+    x2 = x if x.dim() == 2 else x.reshape(M, K)
+    if out is None:
+        out = torch.empty(*lead, N, dtype=dtype, device=device)
+    if out.dim() == 2 and out.shape == (M, N) and (out.stride(1) == 1 or N == 1) and out.stride(0) >= N:
+        out2 = out  # (rows of a wider buffer: written in place)
+    else:
+        _check_out(out, M * N, "M*N")
+        out2 = out.view(M, N)
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous uint8 GPU tensor (see new_workspace)")
+    lib = _kernels.load()
+    with torch.cuda.device(device):
+        if workspace is None:
+            need = int(lib.aitamd_gemm_lora_workspace_bytes(_TORCH_DTYPE_ID[dtype], algo, int(bias is not None), M, N, K, rank))
+            workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+        rc = lib.aitamd_gemm_rcr_lora(
+            _TORCH_DTYPE_ID[dtype], algo, _p(x2), _p(w), _p(bias), _p(lora_a), _p(lora_b), _p(adapters), _p(scales), _p(out2), M, N, K, rank, n,
+            _row_pitch(x2, "x"), _row_pitch(w, "w"), _row_pitch(out2, "out"), _p(workspace), workspace.numel(), _stream_ptr())
+    _kernels.check(rc, "gemm_rcr_lora")
+    return out
+
+
+_LOGITS_DTYPE_ID = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 8}
+
+
+def token_logprobs_workspace_bytes(rows: int, vocabulary: int, top: int = 0) -> int:
+    """Bytes of scratch memory that `token_logprobs` of these sizes needs on the current device."""
+    return int(_kernels.load().aitamd_token_logprobs_workspace_bytes(rows, vocabulary, top))
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, scale: float = 1.0, workspace: Optional[torch.Tensor] = None
+                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """How probable given tokens are, in one pass over the logits: with p = softmax(scale * logits) over the last dimension
+
+    * logprob [...] fp32: log p of `tokens` [...] (int32 or int64); 0 where that is no token, for instance -1;
+    * entropy [...] fp32: - sum p log p;
+    * rank [...] int32: how many tokens stand before it in the order of their logits (equal ones: of their indexes); -1 for none;
+    * top_logprob, top_token [..., top] fp32, int32: the first `top` (up to 64) tokens of that order with their log p.
+
+    `logits` [..., vocabulary], fp16, bf16 or fp32: contiguous, or a 2-D view with row pitch.  `scale` is the reciprocal of a
+    temperature.  Logits of -inf are tokens of probability 0, a row of nothing else has log probabilities of -inf and entropy 0; a row
+    with a NaN or +inf has NaN for both (NaN are no alternatives: where there are not `top` others, top_token is -1).
+
+    `workspace`: `token_logprobs_workspace_bytes` bytes, allocated for the call otherwise; calls that may overlap in time need one
+    each."""
+    result = _native_decoder.token_logprobs(logits, tokens, top, scale, workspace)
+    if result is not NotImplemented:
+        return result
+    device = _operands(("logits", logits, tuple(_LOGITS_DTYPE_ID)), ("tokens", tokens, (torch.int32, torch.int64)),
+                       ("workspace", workspace, (torch.uint8,)))
+    if logits.dim() < 1:
+        raise ValueError("logits must have at least one dimension")
+    lead, vocabulary = logits.shape[:-1], logits.shape[-1]
+    rows = 1
+    for d in lead:
+        rows *= d
+    if logits.dim() != 2 and not logits.is_contiguous():
+        raise ValueError("logits must be contiguous, or 2-D with a contiguous last dimension")
+    ld = _row_pitch(logits, "logits") if logits.dim() == 2 else vocabulary
+    if tokens.shape != lead or not tokens.is_contiguous():
+        raise ValueError(f"tokens must be contiguous {tuple(lead)}, got shape {tuple(tokens.shape)}")
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous uint8 GPU tensor (see new_workspace)")
+    top = int(top)
+    lib = _kernels.load()
+    with torch.cuda.device(device):
+        made = [torch.empty(lead, dtype=d, device=device) for d in (torch.float32, torch.float32, torch.int32)]
+        made += [torch.empty(*lead, max(top, 0), dtype=d, device=device) for d in (torch.float32, torch.int32)]
+        if workspace is None:
+            need = int(lib.aitamd_token_logprobs_workspace_bytes(rows, vocabulary, top))
+            workspace = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+        rc = lib.aitamd_token_logprobs(
+            _LOGITS_DTYPE_ID[logits.dtype], _p(logits), _p(tokens), int(tokens.dtype == torch.int64), *(_p(t) for t in made), rows, vocabulary, ld,
+            top, float(scale), _p(workspace), 0 if workspace is None else workspace.numel(), _stream_ptr())
+    _kernels.check(rc, "token_logprobs")
+    return tuple(made)

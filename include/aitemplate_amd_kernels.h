@@ -59,7 +59,7 @@ enum {
   AITAMD_NUM_EPILOGUES = 18
 };
 
-enum { AITAMD_F16 = 0, AITAMD_BF16 = 1 };
+enum { AITAMD_F16 = 0, AITAMD_BF16 = 1, AITAMD_F32 = 8 /* logits only */ };
 
 /* Library version string, e.g. "aitemplate_amd 0.1 gfx950". */
 AITAMD_API const char* aitamd_version(void);
@@ -378,6 +378,69 @@ AITAMD_API int aitamd_prefix_attention(int dtype, const aitamd_paged_cache* cach
                                        int64_t q_head, void* out, int64_t out_token, int64_t out_head, int64_t heads,
                                        const int32_t* prefix_table, int64_t prefix_pages, int64_t prefix_length, float scale,
                                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- what a served decoder computes around its attention: adapters beside a projection, heads that are normalized, log
+ * probabilities of tokens.  No counterpart in the reference. ---- */
+
+/* y[m, n] = sum_k x[m, k] w[n, k] (+ bias[n]) + scales[i] sum_j (sum_k x[m, k] lora_a[i, j, k]) lora_b[i, n, j] with
+ * i = adapters[m]; where that is not in [0, num_adapters) the last term is none.  x [M, K], w [N, K], y [M, N] with row pitches
+ * ldx, ldw, ldy, lora_a [num_adapters, rank, K] and lora_b [num_adapters, N, rank] contiguous, bias (may be null), all of type
+ * `dtype`; adapters int32 [M], scales fp32 [num_adapters] (null: 1), on the device.  rank 1 to 1024.  Two launches: the sums over K
+ * of the adapters, held in two bfloat16 numbers each that add up to them within 2^-17, and the product, whose tiles add the
+ * second sums to their accumulators of 32 bits and round once.  algo = -1: the heuristic instance; otherwise one of
+ * aitamd_gemm_num_algos(bias ? AITAMD_EPI_BIAS : AITAMD_EPI_NONE, 4 + dtype).  workspace: device memory, 16-byte aligned, of
+ * aitamd_gemm_lora_workspace_bytes() bytes (algo = -1: enough for any instance); nothing in it has to be set, its first 4096
+ * bytes are zero afterwards.  Launches that overlap in time need one each. */
+AITAMD_API int aitamd_gemm_rcr_lora(int dtype, int algo, const void* x, const void* w, const void* bias, const void* lora_a,
+                                    const void* lora_b, const int32_t* adapters, const float* scales, void* y, int64_t M,
+                                    int64_t N, int64_t K, int64_t rank, int64_t num_adapters, int64_t ldx, int64_t ldw,
+                                    int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream);
+AITAMD_API int64_t aitamd_gemm_lora_workspace_bytes(int dtype, int algo, int bias, int64_t M, int64_t N, int64_t K,
+                                                    int64_t rank);
+
+/* Heads of queries and keys, one launch: of each x = a head's head_dim numbers, x / sqrt(mean(x^2) + eps) * weight, rotated as by
+ * aitamd_rotary_embedding, rounded once.  A head of zeros stays one, also with eps = 0.  An operand whose weight is null is
+ * rotated only.  q [batch, seq, heads, head_dim] and k [batch, seq, kv_heads, head_dim] (null: none) with their outputs, strides in
+ * elements and head dims contiguous; q_weight, k_weight [heads (kv_heads), head_dim] of type `dtype`, heads *_weight_head apart (0: one
+ * for all).  Outputs may be their inputs with the same strides and must not overlap them otherwise. */
+typedef struct {
+  const void* x;
+  void* out;
+  int64_t heads, batch_stride, seq_stride, head_stride, out_batch_stride, out_seq_stride, out_head_stride;
+  const void* weight;
+  int64_t weight_head_stride;
+} aitamd_heads;
+AITAMD_API int aitamd_qk_norm_rotary(int dtype, const aitamd_heads* q, const aitamd_heads* k, const void* positions,
+                                     int positions_64, const float* freqs, int64_t batch, int64_t seq, int64_t head_dim,
+                                     int64_t rotated, int64_t pos_batch, int64_t pos_seq, float eps, float scale,
+                                     int interleaved, void* stream);
+
+/* aitamd_paged_kv_append with heads that are normalized ahead of their rotation, as by aitamd_qk_norm_rotary: those of the queries
+ * with q_weight, those of the keys with k_weight (null: as they are; without both the same as aitamd_paged_kv_append). */
+AITAMD_API int aitamd_paged_kv_append_norm(int dtype, const aitamd_paged_cache* cache, const void* k, int64_t k_token,
+                                           int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const void* q,
+                                           int64_t q_token, int64_t q_head, void* q_out, int64_t q_out_token,
+                                           int64_t q_out_head, int64_t heads, const void* q_weight, int64_t q_weight_head,
+                                           const void* k_weight, int64_t k_weight_head, float eps, const float* freqs,
+                                           int64_t rotated, int64_t first_position, float scale, int interleaved, void* stream);
+
+/* Of each row of logits [rows, vocabulary] (AITAMD_F16, AITAMD_BF16 or AITAMD_F32, row pitch ld), with
+ * p = softmax(scale * logits):
+ *   logprob[r] = log p[tokens[r]] (0 where tokens[r] is not in [0, vocabulary)),
+ *   entropy[r] = - sum p log p,
+ *   rank[r] = how many tokens stand before tokens[r] in the order of their logits, equal ones in that of their indexes (-1 where
+ *     there is no token),
+ *   top_token[r, :], top_logprob[r, :] = the first `top` tokens of that order, and their log p.
+ * tokens: int32, or int64 with tokens_64.  All sums in 32 bits.  Logits of -inf are tokens of probability 0; a row of nothing else
+ * has log probabilities of -inf and entropy 0.  A row with a NaN or +inf has NaN for both; NaN are behind all others in the order,
+ * and where there are not `top` others the rest of top_token is -1, with NaN.  top up to 64.
+ * workspace: device memory, 16-byte aligned, of aitamd_token_logprobs_workspace_bytes() bytes (may be null where that is 0);
+ * nothing in it has to be set and nothing is kept in it.  Launches that overlap in time need one each. */
+AITAMD_API int aitamd_token_logprobs(int dtype, const void* logits, const void* tokens, int tokens_64, float* logprob,
+                                     float* entropy, int32_t* rank, float* top_logprob, int32_t* top_token, int64_t rows,
+                                     int64_t vocabulary, int64_t ld, int64_t top, float scale, void* workspace,
+                                     int64_t workspace_bytes, void* stream);
+AITAMD_API int64_t aitamd_token_logprobs_workspace_bytes(int64_t rows, int64_t vocabulary, int64_t top);
 
 #ifdef __cplusplus
 } /* extern "C" */
