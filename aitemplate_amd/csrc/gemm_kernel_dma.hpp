@@ -614,7 +614,7 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
     }
     // low-rank adapters: behind K, by the last of the workgroups that share a tile; of waves with many, in the epilogue
     constexpr bool kLora = IsLora<Epi>::value;
-    LoraTile<std::conditional_t<kLora, T, bf16>, MT, MI, NI> lora;
+    LoraTile<std::conditional_t<kLora, T, bf16>, MT, MI, NI, true> lora;
     if constexpr (kLora) {
       lora.read(p, m0 + wm * Tile::WTM, lane);
       lora.count();

@@ -1,16 +1,20 @@
 // C ABI launcher of aitamd_token_logprobs: of rows of logits the log probabilities and ranks of given tokens, the entropies and the
 // most probable tokens, in one pass over the logits.
 //
-// With z = scale * x and m the largest x seen so far, a thread keeps s = sum 2^d and u = sum 2^d d of its elements, d = (x - m) scale
-// log2(e), both in 32 bits; a larger m multiplies s by f = 2^(m - m') and makes u f (u + s (m - m')).  Joined over a row,
-//     log p(t) = scale (x_t - m) - ln s,     entropy = ln s - ln 2 u / s.
-// Bound: memory, where the vector instructions (14 an element, the exponential as four of them) leave off: 2-byte logits are at
-// both.  Few rows: several workgroups a row, joined by a second launch.
+// With c = scale log2(e) and m the largest x seen so far, a thread keeps s = sum 2^d and u = sum 2^d d of its elements, d = c x - R with
+// R = c m rounded (any number next to it would do: it comes off again), both in 32 bits; a larger m multiplies s by f = 2^(R - R') and
+// makes u f (u + s (R - R')).  Joined over a row,
+//     log p(t) = scale (x_t - m) + ln 2 (c m - R) - ln s,     entropy = ln s - ln 2 u / s.
+// Bound: memory; the vector instructions, ten an element (the exponential as four of them), are next to it for 2-byte logits.  Few rows:
+// several workgroups a row, joined by a second launch.
 //
 // The most probable: 64-bit keys (value, then the lower token), all different.  A workgroup keeps those that may be among them in
-// LDS.  The first round's bound is one that enough elements are known to reach, from the largest of every lane; what reaches it is
-// put behind the others with one atomic addition each, so their order varies from run to run, and the outcome does not.  Where they do not
-// fit (ascending rows, many equal ones), the round is done again with the exact bound that at most `top` threads reach.
+// LDS: what reaches a bound is put behind the others with one atomic addition each, so their order varies from run to run, and the
+// outcome does not.  The first round's bound is next to the `top`-th largest of its lanes' largest (with the least of the waves'
+// shares of them for one, some five times as many reach it: 4096 x 32768 in fp16 with 20 alternatives 157 us with that bound to the
+// end, 104 with a selection behind every round); whenever as many again have come, the best `top` are picked and the last of them is
+// the bound from there on.  Where they do not fit (ascending rows, many equal ones), the round is done again with the exact
+// bound that at most `top` threads reach.
 #include "../../include/aitemplate_amd_kernels.h"
 #include "common.hpp"
 #include "device.hpp"
@@ -24,6 +28,7 @@ constexpr int kEach = 16;                       // elements of a thread in a rou
 constexpr int kRound = kThreads * kEach;
 constexpr int kMostTop = 64;
 constexpr int kKeys = 2048;                     // candidates in LDS
+static_assert(kWaves * (kMostTop / kWaves + 2) <= 128, "two of a lane");
 constexpr int kMostSplits = kKeys / kMostTop;
 static_assert(kMostTop + kMostTop * kEach <= kKeys, "a round done again fits behind those kept");
 
@@ -60,31 +65,79 @@ AITAMD_DEVICE uint32_t ordered(float x) {
 AITAMD_DEVICE float unordered(uint32_t o) { return __uint_as_float((int32_t)o < 0 ? o & 0x7fffffffu : ~o); }
 AITAMD_DEVICE uint64_t key_of(float x, int token) { return (uint64_t)ordered(x) << 32 | (uint32_t)~token; }
 
-AITAMD_DEVICE float wave_max(float v) {
+// the largest number of a piece (-inf where there is none)
+template <class T>
+AITAMD_DEVICE float largest_of(typename Logits<T>::vec v) {
+  if constexpr (std::is_same_v<T, f16>) {
+    // (two at a time)
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(f16x2{v[0], v[1]}, f16x2{v[2], v[3]}),
+                                              __builtin_elementwise_max(f16x2{v[4], v[5]}, f16x2{v[6], v[7]}));
+    return fmaxf(fmaxf((float)m[0], (float)m[1]), -__builtin_inff());
+  } else {
+    float m = (float)v[0];
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-  return v;
+    for (int e = 1; e < Logits<T>::VEC; ++e) m = fmaxf(m, (float)v[e]);
+    return fmaxf(m, -__builtin_inff());
+  }
+}
+// v joined with that of the lane which a step of a reduction along the wave gives (none: `none`)
+template <int CTRL>
+AITAMD_DEVICE float lane_step(float v, float none) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+// over the 64 lanes, for all of them: neighbours in rows of 16 (row_shr 1, 2, 4, 8), then rows (row_bcast 15, 31)
+template <class F>
+AITAMD_DEVICE float wave_reduce(float v, float none, F&& f) {
+  v = f(v, lane_step<0x111>(v, none));
+  v = f(v, lane_step<0x112>(v, none));
+  v = f(v, lane_step<0x114>(v, none));
+  v = f(v, lane_step<0x118>(v, none));
+  v = f(v, lane_step<0x142>(v, none));
+  v = f(v, lane_step<0x143>(v, none));
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+AITAMD_DEVICE float wave_max(float v) {
+  return wave_reduce(v, -__builtin_inff(), [](float a, float b) { return fmaxf(a, b); });
+}
+AITAMD_DEVICE float wave_sum(float v) {
+  return wave_reduce(v, 0.0f, [](float a, float b) { return a + b; });
 }
 
 // The `keep` largest of n keys, in order, zeros behind the last: every key counts those above it (they are all different, but for
-// zeros, which are none).  All threads; `out` must not overlap the keys.
+// zeros, which are none), several neighbouring lanes the keys of one where there are fewer than threads.  All threads; there is room
+// for 8 keys more (or for THREADS + 8 in all), which are overwritten, and `out` does not overlap them.
 template <int THREADS>
-AITAMD_DEVICE void largest(const uint64_t* keys, int n, uint64_t* out, int keep) {
+AITAMD_DEVICE void largest(uint64_t* keys, int n, uint64_t* out, int keep) {
+  int shift = 0;
+  while (shift < 6 && n << (shift + 1) <= THREADS) ++shift;
+  const int parts = 1 << shift, part = threadIdx.x & (parts - 1);
   for (int i = threadIdx.x; i < keep; i += THREADS) out[i] = 0;
+  for (int i = threadIdx.x; i < 8 * parts; i += THREADS) keys[n + i] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += THREADS) {
-    const uint64_t mine = keys[i];
+  for (int i0 = 0; i0 < n; i0 += THREADS >> shift) {
+    const int i = i0 + (threadIdx.x >> shift);
+    const uint64_t mine = i < n ? keys[i] : ~0ull;
     int above = 0;
-    int j = 0;
-    for (; j + 4 <= n; j += 4) above += (keys[j] > mine ? 1 : 0) + (keys[j + 1] > mine ? 1 : 0) + (keys[j + 2] > mine ? 1 : 0) + (keys[j + 3] > mine ? 1 : 0);
-    for (; j < n; ++j) above += keys[j] > mine ? 1 : 0;
-    if (mine != 0 && above < keep) out[above] = mine;
+    // (eight at a time: one by one, every read is waited for)
+    for (int j = part; j < n; j += 8 * parts) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) above += keys[j + e * parts] > mine ? 1 : 0;
+    }
+    for (int d = 1; d < parts; d <<= 1) above += __shfl_xor(above, d);
+    if (i < n && mine != 0 && part == 0 && above < keep) out[above] = mine;
   }
 }
 
+// Numbers next to the lowest of the type (a mask's) times c may leave the range: they go by their differences.
+AITAMD_DEVICE bool in_range(float m, float c) { return fabsf(m * c) < 1e38f; }
+// From one R to another, at least -1000 (2^-1000 is 0)
+AITAMD_DEVICE float step_down(float m, float to, float c) {
+  return fmaxf(in_range(m, c) && in_range(to, c) ? m * c - to * c : (m - to) * c, -1000.0f);
+}
 AITAMD_DEVICE void join(float& m, float& s, float& u, float m2, float s2, float u2, float c) {
   const float to = fmaxf(m, m2);
-  const float d1 = fmaxf((m - to) * c, -1000.0f), d2 = fmaxf((m2 - to) * c, -1000.0f);
+  const float d1 = step_down(m, to, c), d2 = step_down(m2, to, c);
   const float f1 = exp2_fast(d1), f2 = exp2_fast(d2);
   u = f1 * (u + s * d1) + f2 * (u2 + s2 * d2);
   s = s * f1 + s2 * f2;
@@ -100,7 +153,8 @@ AITAMD_DEVICE int token_of(const LogprobParams& p, int row) {
 template <class T>
 AITAMD_DEVICE void finish(const LogprobParams& p, int row, float m, float s, float u, int ahead, const uint64_t* best) {
   const int lane = threadIdx.x & 63;
-  const float log_s = logf(s);
+  // (the sum is of 2^(c x - R), and R not quite c m)
+  const float c = p.scale * kLog2e, log_s = logf(s) - (in_range(m, c) ? kLn2 * __builtin_fmaf(m, c, -(m * c)) : 0.0f);
   if (lane == 0) {
     const int token = token_of(p, row);
     float lp = 0.0f;
@@ -109,7 +163,7 @@ AITAMD_DEVICE void finish(const LogprobParams& p, int row, float m, float s, flo
       lp = s == 0.0f ? -__builtin_inff() : (x - m) * p.scale - log_s;
     }
     p.logprob[row] = lp;
-    p.entropy[row] = s == 0.0f ? 0.0f : log_s - kLn2 * (u / s);
+    p.entropy[row] = s == 0.0f ? 0.0f : logf(s) - kLn2 * (u / s);
     p.rank[row] = token >= 0 ? ahead : -1;
   }
   if (lane < p.top) {
@@ -124,11 +178,11 @@ AITAMD_DEVICE void finish(const LogprobParams& p, int row, float m, float s, flo
 AITAMD_DEVICE void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <class T, bool TOP>
-__global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParams p) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 8 : 6) logprob_kernel(const LogprobParams p) {
   constexpr int VEC = Logits<T>::VEC, PIECES = kEach / VEC;
   using vec = typename Logits<T>::vec;
-  __shared__ uint64_t keys[TOP ? kKeys : 1], best[TOP ? kThreads : 1];
-  __shared__ float wave_bound[kWaves];
+  __shared__ uint64_t keys[TOP ? kKeys + 8 : 1], best[TOP ? kThreads : 1];
+  __shared__ float lane_best[kWaves * (kMostTop / kWaves + 2)];
   __shared__ PartHead heads[kWaves];
   __shared__ int added[3];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -136,6 +190,31 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
   const int v0 = split * p.per_split, v1 = p.V - v0 < p.per_split ? p.V : v0 + p.per_split;
   const T* x = reinterpret_cast<const T*>(p.logits) + row * p.ld;
   const float c = p.scale * kLog2e;
+  vec next[PIECES];
+  const int rounds = (v1 - v0 + kRound - 1) / kRound;
+  auto piece_at = [&](int round, int i) { return v0 + round * kRound + (i * kThreads + tid) * VEC; };
+  // (a branch for the whole workgroup: one for each piece would be waited at)
+  auto load = [&](int round, vec (&v)[PIECES]) __attribute__((always_inline)) {
+    if (v0 + (round + 1) * kRound <= v1) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) v[i] = load_vec<vec>(x + piece_at(round, i));
+    } else {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int at = piece_at(round, i);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[i][e] = (T)-__builtin_inff();
+        if (at + VEC <= v1) {
+          v[i] = load_vec<vec>(x + at);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (at + e < v1) v[i][e] = x[at + e];
+        }
+      }
+    }
+  };
+  load(0, next);
   const int token = token_of(p, row);
   const float given = token >= 0 ? (float)x[token] : __builtin_inff();
   // (what of the elements in front of the token is not at most the number below its logit is at least as large)
@@ -154,104 +233,103 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
   if (TOP && tid < 3) added[tid] = 0;
   if constexpr (TOP) barrier();
 
-  auto piece_at = [&](int round, int i) { return v0 + round * kRound + (i * kThreads + tid) * VEC; };
-  auto load = [&](int round, vec (&v)[PIECES]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const int at = piece_at(round, i);
-      if (at + VEC <= v1) {
-        v[i] = load_vec<vec>(x + at);
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[i][e] = at + e < v1 ? x[at + e] : (T)-__builtin_inff();
-      }
-    }
-  };
-  const int rounds = (v1 - v0 + kRound - 1) / kRound;
-  vec next[PIECES];
-  load(0, next);
   for (int r = 0; r < rounds; ++r) {
     vec v[PIECES];
     float most[PIECES], here = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       v[i] = next[i];
-      most[i] = (float)v[i][0];
-#pragma unroll
-      for (int e = 1; e < VEC; ++e) most[i] = fmaxf(most[i], (float)v[i][e]);
+      most[i] = largest_of<T>(v[i]);
       here = fmaxf(here, most[i]);
     }
     if (r + 1 < rounds) load(r + 1, next);
     if (here > m) {
-      const float d = fmaxf((m - here) * c, -1000.0f), f = exp2_fast(d);
+      const float d = step_down(m, here, c), f = exp2_fast(d);
       u = f * (u + s * d);
       s *= f;
       m = here;
     }
+    auto sum = [&](auto by_product) __attribute__((always_inline)) {
+      const float R = m * c;
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const float than = piece_at(r, i) + VEC <= token ? below : given;
+      for (int i = 0; i < PIECES; ++i) {
+        const float than = piece_at(r, i) + VEC <= token ? below : given;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float xe = (float)v[i][e];
-        const float d = (xe - m) * c, w = exp2_fast(d);
-        s += w;
-        u = __builtin_fmaf(w, fmaxf(d, -1000.0f), u);
-        ahead += __builtin_popcountll(__builtin_amdgcn_ballot_w64(!(xe <= than)));
+        for (int e = 0; e < VEC; ++e) {
+          const float xe = (float)v[i][e];
+          const float d = decltype(by_product)::value ? __builtin_fmaf(xe, c, -R) : (xe - m) * c;
+          const float w = exp2_fast(d);
+          s += w;
+          u = __builtin_fmaf(w, fmaxf(d, -1000.0f), u);
+          ahead += __builtin_popcountll(__builtin_amdgcn_ballot_w64(!(xe <= than)));
+        }
       }
-    }
+    };
+    if (__builtin_amdgcn_ballot_w64(!in_range(m, c)) == 0)
+      sum(std::true_type{});
+    else
+      sum(std::false_type{});
     if constexpr (TOP) {
       if (r == 0) {
-        // every wave's g-th largest of its lanes' largest, g so that all waves with elements together have `top`: the least of them
-        const int pieces = (v1 - v0 + VEC - 1) / VEC, waves = pieces >= kThreads ? kWaves : (pieces + 63) / 64;
-        const int g = (p.top + waves - 1) / waves;
-        float left = here, at_least = -__builtin_inff();
+        // The largest of every wave's lanes, a few more each than make `top` together: the `top`-th of them all, found by halving to
+        // 20 bits, is a bound that `top` elements reach and not many more.
+        const int g = (p.top + kWaves - 1) / kWaves + 2;
+        float left = here;
         for (int i = 0; i < g; ++i) {
-          at_least = wave_max(left);
-          const uint64_t who = __builtin_amdgcn_ballot_w64(left == at_least);
-          if (who == 0) break;
-          if (lane == __builtin_ctzll(who)) left = -__builtin_inff();
+          const float top_one = wave_max(left);
+          const uint64_t who = __builtin_amdgcn_ballot_w64(left == top_one);
+          if (who != 0 && lane == __builtin_ctzll(who)) left = -__builtin_inff();
+          if (lane == 0) lane_best[wave * g + i] = top_one;
         }
-        if (lane == 0) wave_bound[wave] = wave < waves ? at_least : __builtin_inff();
         barrier();
-        bound = wave_bound[0];
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) bound = fminf(bound, wave_bound[w]);
+        const uint32_t one = lane < kWaves * g ? ordered(lane_best[lane]) : 0u;
+        const uint32_t two = lane + 64 < kWaves * g ? ordered(lane_best[lane + 64]) : 0u;
+        uint32_t at_least = 0;
+        for (int bit = 31; bit >= 12; --bit) {
+          const uint32_t more = at_least | 1u << bit;
+          const int reach = __builtin_popcountll(__builtin_amdgcn_ballot_w64(one >= more)) + __builtin_popcountll(__builtin_amdgcn_ballot_w64(two >= more));
+          if (reach >= p.top) at_least = more;
+        }
+        if (at_least > ordered(-__builtin_inff())) bound = unordered(at_least);
       }
       int* const count = &added[r % 3];
       if (tid == 0) added[(r + 1) % 3] = 0;
-      auto put = [&](uint64_t least) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-          if (most[i] >= bound) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              const float xe = (float)v[i][e];
-              const int t = piece_at(r, i) + e;
-              if (xe >= bound && t < v1) {
-                const uint64_t key = key_of(xe, t);
-                if (key >= least) {
-                  const int place = kept + atomicAdd(count, 1);
-                  if (place < kKeys) keys[place] = key;
-                }
-              }
-            }
-          }
+      auto put = [&](float xe, int t, uint64_t least) __attribute__((always_inline)) {
+        const uint64_t key = key_of(xe, t);
+        if (t < v1 && key >= least) {
+          const int place = kept + atomicAdd(count, 1);
+          if (place < kKeys) keys[place] = key;
         }
       };
-      put(bound_key);
-      barrier();
-      if (kept + *count > kKeys) {
-        // the largest of those from the rounds before (at their places still), then of every thread its largest
-        uint64_t mine = 0;
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i)
+      for (int i = 0; i < PIECES; ++i) {
+        if (most[i] >= bound) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            const int t = piece_at(r, i) + e;
-            const uint64_t key = t < v1 ? key_of((float)v[i][e], t) : 0;
-            mine = key > mine ? key : mine;
+            const float xe = (float)v[i][e];
+            if (xe >= bound) put(xe, piece_at(r, i) + e, bound_key);
           }
+        }
+      }
+      barrier();
+      const int found = kept + *count;
+      if (found > kKeys) {
+        // (the elements from memory once more: rarely needed, not to be held in registers for it)
+        auto each = [&](auto&& f) __attribute__((always_inline)) {
+#pragma unroll 1
+          for (int i = 0; i < PIECES; ++i)
+#pragma unroll 1
+            for (int e = 0; e < VEC; ++e) {
+              const int t = piece_at(r, i) + e;
+              if (t < v1) f((float)x[t], t);
+            }
+        };
+        // the largest of those from the rounds before (at their places still), then of every thread its largest
+        uint64_t mine = 0;
+        each([&](float xe, int t) {
+          const uint64_t key = key_of(xe, t);
+          mine = key > mine ? key : mine;
+        });
         barrier();
         if (tid == 0) *count = 0;
         largest<kThreads>(keys, kept, best, p.top);
@@ -263,23 +341,22 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
         largest<kThreads>(keys + kMostTop, kThreads, best, p.top);
         barrier();
         const uint64_t least = best[p.top - 1] > bound_key ? best[p.top - 1] : bound_key;
-        bound = -__builtin_inff();
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) most[i] = __builtin_inff();
-        put(least);
+        each([&](float xe, int t) {
+          if (xe == xe) put(xe, t, least);
+        });
         barrier();
-        // ... and of all of them: a bound for the rounds to come
         kept += *count;
+      } else {
+        kept = found;
+      }
+      if (kept > p.top && (found > kKeys || (kept >= 2 * p.top + 32 && r + 1 < rounds))) {
+        // the best of them, and a bound for the rounds to come (paid for by as many that have come)
         largest<kThreads>(keys, kept, best, p.top);
         barrier();
-        if (kept >= p.top) {
-          kept = p.top;
-          bound_key = best[p.top - 1];
-          bound = unordered((uint32_t)(bound_key >> 32));
-        }
+        kept = p.top;
+        bound_key = best[p.top - 1];
+        bound = unordered((uint32_t)(bound_key >> 32));
         if (tid < kept) keys[tid] = best[tid];
-      } else {
-        kept += *count;
       }
     }
   }
@@ -294,14 +371,9 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
   // the workgroup's sums
   float to = wave_max(m);
   {
-    const float d = fmaxf((m - to) * c, -1000.0f), f = exp2_fast(d);
-    u = f * (u + s * d);
-    s *= f;
-#pragma unroll
-    for (int d2 = 32; d2 > 0; d2 >>= 1) {
-      s += __shfl_xor(s, d2);
-      u += __shfl_xor(u, d2);
-    }
+    const float d = step_down(m, to, c), f = exp2_fast(d);
+    u = wave_sum(f * (u + s * d));
+    s = wave_sum(s * f);
   }
   if (lane == 0) heads[wave] = {to, s, u, ahead};
   barrier();
@@ -326,10 +398,11 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
   }
 }
 
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 512;
 template <class T>
 __global__ void __launch_bounds__(kJoinThreads) logprob_join_kernel(const LogprobParams p) {
-  __shared__ uint64_t keys[kKeys], best[kMostTop];
+  __shared__ uint64_t keys[kKeys], some[kKeys + 8], best[kMostTop];
+  __shared__ int count;
   const int tid = threadIdx.x, row = p.first + blockIdx.x;
   const unsigned char* const part = p.parts + (int64_t)row * p.splits * p.part_bytes;
   const float c = p.scale * kLog2e;
@@ -337,6 +410,7 @@ __global__ void __launch_bounds__(kJoinThreads) logprob_join_kernel(const Logpro
     const int w = i / p.top;
     keys[i] = reinterpret_cast<const uint64_t*>(part + (int64_t)w * p.part_bytes + sizeof(PartHead))[i - w * p.top];
   }
+  if (tid == 0) count = 0;
   PartHead all{-3.402823466e38f, 0.0f, 0.0f, 0};
   if (tid < 64) {
     if (tid < p.splits) all = *reinterpret_cast<const PartHead*>(part + (int64_t)tid * p.part_bytes);
@@ -349,7 +423,14 @@ __global__ void __launch_bounds__(kJoinThreads) logprob_join_kernel(const Logpro
   }
   __syncthreads();
   if (p.top > 0) {
-    largest<kJoinThreads>(keys, p.splits * p.top, best, p.top);
+    // every part's keys are in order: `top` of all of them reach the least of the parts' g-th ones
+    const int n = p.splits * p.top, g = (p.top + p.splits - 1) / p.splits;
+    uint64_t bound = keys[g - 1];
+    for (int w = 1; w < p.splits; ++w) bound = keys[w * p.top + g - 1] < bound ? keys[w * p.top + g - 1] : bound;
+    for (int i = tid; i < n; i += kJoinThreads)
+      if (keys[i] >= bound) some[atomicAdd(&count, 1)] = keys[i];
+    __syncthreads();
+    largest<kJoinThreads>(some, count, best, p.top);
     __syncthreads();
   }
   if (tid < 64) finish<T>(p, row, all.m, all.s, all.u, all.ahead, best);

@@ -70,8 +70,9 @@ AITAMD_DEVICE u32x4 lora_largest(u32x4 v) {
   return v;
 }
 
-// The part of a wave whose rows row0 + mi * MT + (lane % MT) meet columns col0 + ni * MT + (lane % MT)
-template <class T, int MT, int MI, int NI>
+// The part of a wave whose rows row0 + mi * MT + (lane % MT) meet columns col0 + ni * MT + (lane % MT).  ODD: any rank, else even
+// ones.
+template <class T, int MT, int MI, int NI, bool ODD>
 struct LoraTile {
   static constexpr int QN = 64 / MT;
   int of[MI];
@@ -138,11 +139,20 @@ struct LoraTile {
         bool again = false;
         for (int pass = 0; pass < 2; ++pass) {
           u32x4 w[NI], t[MI];
-          if ((rank & 7) == 0) {
+          if (!ODD || (rank & 1) == 0) {
             static_for<0, NI>([&](auto ni) __attribute__((always_inline)) {
               w[ni] = buffer_load_16B(rb, on ? bc + (uint32_t)(decltype(ni)::value * MT) * b_pitch : kOobOffset);
             });
+            // (behind the last rank is the next column's first; the buffer ends with a dword)
+            if (8 * (c0 + PER) > rank) {
+              const int dwords = rank / 2 - 4 * (c0 + half);
+              static_for<0, NI>([&](auto ni) __attribute__((always_inline)) {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) w[ni][d] = d < dwords ? w[ni][d] : 0u;
+              });
+            }
           } else {
+            // (one column's loads at a time: all together need more registers than there are)
             static_for<0, NI>([&](auto ni) __attribute__((always_inline)) {
 #pragma unroll
               for (int d = 0; d < 4; ++d) {
@@ -153,6 +163,7 @@ struct LoraTile {
                       rb, 8 * (c0 + half) + 2 * d + j < rank ? bc + (uint32_t)(decltype(ni)::value * MT) * b_pitch + (2 * d + j) * 2u : kOobOffset, 0, 0);
                 w[ni][d] = e[0] | e[1] << 16;
               }
+              asm volatile("" : "+v"(w[ni]));
             });
           }
           static_for<0, MI>([&](auto mi) __attribute__((always_inline)) {
