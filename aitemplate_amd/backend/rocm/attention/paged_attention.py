@@ -1,4 +1,4 @@
-"""Registry hooks of rotary_embedding, paged_kv_append and prefix_attention: one generated function each, heads, head dims and the
+"""Registry hooks of rotary_embedding, qk_norm_rotary, paged_kv_append and prefix_attention: one generated function each, heads, head dims and the
 page size as literals, the numbers of tokens, sequences and pages (which may be dynamic) as its arguments."""
 from typing import Any, Dict
 
@@ -54,6 +54,47 @@ def rotary_func_call(func_attrs: Dict[str, Any], indent: str = "  ") -> str:
     return f"{indent}{func_attrs['name']}({', '.join(args)});"
 
 
+# ---- qk_norm_rotary ----
+
+def _norm_signature(func_name: str) -> str:
+    return (f"void {func_name}(void* q_out, void* k_out, const void* q, const void* k, const void* q_weight, const void* k_weight, "
+            "const void* positions, const void* freqs, int64_t batch, int64_t seq, hipStream_t stream)")
+
+
+def norm_gen_function(func_attrs: Dict[str, Any]) -> str:
+    func_name = func_attrs["name"]
+    q, k, q_weight, k_weight, positions, freqs = func_attrs["inputs"]
+    head_dim = _value(q, -1)
+
+    def heads(name, x, weight):
+        strides = f"seq * {_value(x, -2) * head_dim}, {_value(x, -2) * head_dim}, {head_dim}"
+        return (f"  const aitamd_heads {name}_heads = {{{name}, {name}_out, {_value(x, -2)}, {strides}, {strides}, {name}_weight, "
+                f"{_weight_stride(weight)}}};")
+
+    return f"""{common.HEADER}
+{_norm_signature(func_name)} {{
+{heads("q", q, q_weight)}
+{heads("k", k, k_weight)}
+  check_rc(aitamd_qk_norm_rotary({common.DTYPE_ID[q._attrs["dtype"]]}, &q_heads, &k_heads, positions,
+                                 {int(positions._attrs["dtype"] == "int64")}, static_cast<const float*>(freqs), batch, seq, {head_dim},
+                                 {2 * _value(freqs, 0)}, {"seq" if len(positions._attrs["shape"]) == 2 else "0"}, 1,
+                                 {float_literal(func_attrs["eps"])}, {float_literal(func_attrs["scale"])},
+                                 {int(func_attrs["interleaved"])}, stream), "{func_name}");
+}}
+{common.FOOTER}"""
+
+
+def norm_func_decl(func_attrs: Dict[str, Any]) -> str:
+    return _norm_signature(func_attrs["name"]) + ";"
+
+
+def norm_func_call(func_attrs: Dict[str, Any], indent: str = "  ") -> str:
+    q = func_attrs["inputs"][0]
+    batch = _dim(q, 0) if len(q._attrs["shape"]) == 4 else "1"
+    args = [_name(t) for t in func_attrs["outputs"] + func_attrs["inputs"]] + [batch, _dim(q, -3), "stream"]
+    return f"{indent}{func_attrs['name']}({', '.join(args)});"
+
+
 # ---- the paged cache ----
 
 _CACHE_PARAMS = ("void* k_cache, void* v_cache, const void* block_table, const void* lengths, const void* offsets, int64_t ends, "
@@ -79,19 +120,35 @@ def _cache_args(q, k_cache, v_cache, block_table, lengths, offsets):
 
 def _append_signature(func_name: str) -> str:
     return (f"void {func_name}(void* out, const void* q, const void* k, const void* v, const void* freqs, {_CACHE_PARAMS}, "
-            "hipStream_t stream)")
+            "const void* q_weight, const void* k_weight, hipStream_t stream)")
+
+
+def _append_options(func_attrs: Dict[str, Any]) -> Dict[str, Any]:
+    """The optional inputs that there are, by name."""
+    return dict(zip(func_attrs["optional_inputs"], func_attrs["inputs"][8:]))
+
+
+def _weight_stride(weight) -> int:
+    """From one head's weights to the next's."""
+    return _value(weight, 1) if weight is not None and len(weight._attrs["shape"]) == 2 else 0
 
 
 def append_gen_function(func_attrs: Dict[str, Any]) -> str:
     func_name = func_attrs["name"]
     q, _, _, k_cache, _, _, _, freqs = func_attrs["inputs"][:8]
     heads, head_dim, kv_heads = _value(q, 1), _value(q, 2), _value(k_cache, 2)
+    options = _append_options(func_attrs)
+    q_weight, k_weight = options.get("q_weight"), options.get("k_weight")
+    entry, norms = "aitamd_paged_kv_append", ""
+    if q_weight is not None or k_weight is not None:
+        entry += "_norm"
+        norms = f"q_weight, {_weight_stride(q_weight)}, k_weight, {_weight_stride(k_weight)}, {float_literal(func_attrs['eps'])}, "
     return f"""{common.HEADER}
 {_append_signature(func_name)} {{
 {_cache_code(func_name, k_cache)}
-  check_rc(aitamd_paged_kv_append({common.DTYPE_ID[q._attrs["dtype"]]}, &cache, k, {kv_heads * head_dim}, {head_dim}, v,
+  check_rc({entry}({common.DTYPE_ID[q._attrs["dtype"]]}, &cache, k, {kv_heads * head_dim}, {head_dim}, v,
                                   {kv_heads * head_dim}, {head_dim}, q, {heads * head_dim}, {head_dim}, out, {heads * head_dim},
-                                  {head_dim}, {heads}, static_cast<const float*>(freqs), {2 * _value(freqs, 0)},
+                                  {head_dim}, {heads}, {norms}static_cast<const float*>(freqs), {2 * _value(freqs, 0)},
                                   {func_attrs["first_position"]}, {float_literal(func_attrs["scale"])},
                                   {int(func_attrs["interleaved"])}, stream), "{func_name}");
 }}
@@ -104,9 +161,10 @@ def append_func_decl(func_attrs: Dict[str, Any]) -> str:
 
 def append_func_call(func_attrs: Dict[str, Any], indent: str = "  ") -> str:
     q, k, v, k_cache, v_cache, block_table, lengths, freqs = func_attrs["inputs"][:8]
-    offsets = (func_attrs["inputs"][8:] or [None])[0]
+    options = _append_options(func_attrs)
     args = [_name(func_attrs["outputs"][0])] + [_name(t) for t in (q, k, v, freqs)]
-    args += _cache_args(q, k_cache, v_cache, block_table, lengths, offsets) + ["stream"]
+    args += _cache_args(q, k_cache, v_cache, block_table, lengths, options.get("offsets"))
+    args += [_name(options[w]) if w in options else "nullptr" for w in ("q_weight", "k_weight")] + ["stream"]
     return f"{indent}{func_attrs['name']}({', '.join(args)});"
 
 
@@ -149,6 +207,9 @@ def attention_func_call(func_attrs: Dict[str, Any], indent: str = "  ") -> str:
 registry.reg("rocm.rotary_embedding.gen_function", rotary_gen_function)
 registry.reg("rocm.rotary_embedding.func_decl", rotary_func_decl)
 registry.reg("rocm.rotary_embedding.func_call", rotary_func_call)
+registry.reg("rocm.qk_norm_rotary.gen_function", norm_gen_function)
+registry.reg("rocm.qk_norm_rotary.func_decl", norm_func_decl)
+registry.reg("rocm.qk_norm_rotary.func_call", norm_func_call)
 registry.reg("rocm.paged_kv_append.gen_function", append_gen_function)
 registry.reg("rocm.paged_kv_append.func_decl", append_func_decl)
 registry.reg("rocm.paged_kv_append.func_call", append_func_call)

@@ -10,6 +10,7 @@ from typing import Optional
 from ....backend import registry
 from ....backend.target import Target
 from ...base import Operator, Tensor
+from .qk_norm_rotary import check_eps, check_weight
 from .rotary_embedding import check_dtypes, check_freqs, static_dim
 
 
@@ -54,18 +55,22 @@ class _paged(Operator):
 
 class paged_kv_append(_paged):
     """Keys and values [tokens, kv_heads, head_dim] into the cache, keys and queries rotated on the way (as by `rotary_embedding`, for
-    position first_position + the token's place in its sequence); returns the rotated queries."""
+    position first_position + the token's place in its sequence); returns the rotated queries.  With `q_weight` the heads of the
+    queries, with `k_weight` those of the keys ([head_dim] or [heads, head_dim]) are normalized ahead of that, as by `qk_norm_rotary`
+    with `eps`."""
 
-    def __init__(self, interleaved: bool = False, scale: float = 1.0, first_position: int = 0) -> None:
+    def __init__(self, interleaved: bool = False, scale: float = 1.0, first_position: int = 0, eps: float = 1e-6) -> None:
         super().__init__()
         self._attrs["op"] = "paged_kv_append"
         self._attrs["has_profiler"] = False
         self._attrs["interleaved"] = bool(interleaved)
         self._attrs["scale"] = float(scale)
         self._attrs["first_position"] = int(first_position)
+        self._attrs["eps"] = check_eps("paged_kv_append", eps)
 
     def __call__(self, q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, lengths: Tensor,
-                 freqs: Tensor, offsets: Optional[Tensor] = None) -> Tensor:
+                 freqs: Tensor, offsets: Optional[Tensor] = None, q_weight: Optional[Tensor] = None,
+                 k_weight: Optional[Tensor] = None) -> Tensor:
         _, head_dim = _check_cache("paged_kv_append", q, k_cache, v_cache, block_table, lengths, offsets)
         for t, name in ((k, "k"), (v, "v")):
             check_dtypes("paged_kv_append", **{name: (t, (q._attrs["dtype"],))})
@@ -78,10 +83,15 @@ class paged_kv_append(_paged):
         check_dtypes("paged_kv_append", freqs=(freqs, ("float32",)))
         if check_freqs("paged_kv_append", freqs, head_dim) == 0:
             raise RuntimeError("paged_kv_append: freqs is empty")
-        return self._finish(q, [q, k, v, k_cache, v_cache, block_table, lengths, freqs] + ([] if offsets is None else [offsets]))
+        for name, weight, x in (("q_weight", q_weight, q), ("k_weight", k_weight, k)):
+            if weight is not None:
+                check_weight("paged_kv_append", name, weight, x)
+        rest = {"offsets": offsets, "q_weight": q_weight, "k_weight": k_weight}
+        self._attrs["optional_inputs"] = [name for name, t in rest.items() if t is not None]
+        return self._finish(q, [q, k, v, k_cache, v_cache, block_table, lengths, freqs] + [t for t in rest.values() if t is not None])
 
     def _get_op_attributes(self):
-        return {name: self._attrs[name] for name in ("interleaved", "scale", "first_position")}
+        return {name: self._attrs[name] for name in ("interleaved", "scale", "first_position", "eps")}
 
 
 class prefix_attention(_paged):

@@ -38,4 +38,5 @@ from .gemm_rcr_bias_broadcast import (  # noqa: F401
     gemm_rcr_bias_sigmoid_mul_tanh,
 )
 from .gemm_rcr_int8 import gemm_rcr_int8, quantize_rows  # noqa: F401
+from .gemm_rcr_lora import gemm_rcr_lora  # noqa: F401
 from .gemm_rcr_permute import gemm_rcr_bias_permute, gemm_rcr_permute  # noqa: F401

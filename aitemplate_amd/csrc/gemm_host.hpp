@@ -41,7 +41,6 @@ inline bool four_waves_store(const GemmParams& p) {
   auto dwords = [](const void* v) { return (reinterpret_cast<uintptr_t>(v) & 3) == 0; };
   bool ok = p.perm_on == 0 && p.layout == 0 && (p.N & 7) == 0 && (p.ldc & 1) == 0 && (p.sc & 1) == 0 && (p.sc_outer & 1) == 0 &&
       dwords(p.c) && 256 * p.ldc * 2 < 0x7fffffffll;
-  if (p.lora_t != nullptr) ok = ok && (p.lora_rank & 1) == 0;
   if (p.d0 != nullptr) ok = ok && (p.ldd & 1) == 0 && (p.sd & 1) == 0 && dwords(p.d0) && dwords(p.d1) && 256 * p.ldd * 2 < 0x7fffffffll;
   return ok;
 }

@@ -153,6 +153,9 @@ struct IsRows<GemmTileRows<NW, NS, ELEM>> {
   static constexpr bool value = true;
 };
 
+// Workgroups of a shared tile that have no part of K, but the adapters
+constexpr int kLoraParts = IsLora<Epi>::value ? 1 : 0;
+
 // Workgroups per tile of a split-K launch (split_k_rule)
 template <class Tile>
 int split_k_factor(const GemmParams& p, int cus) {
@@ -167,7 +170,7 @@ int64_t workspace_of(const GemmParams& p) {
     if (hipGetDevice(&dev) != hipSuccess) dev = 0;
     const int64_t tiles = (int64_t)((p.M + Tile::BM - 1) / Tile::BM) * ((p.N + Tile::BN - 1) / Tile::BN) * p.batch;
     const int s = split_k_factor<Tile>(p, device_cus(dev));
-    return s > 1 ? Tile::ws_bytes(tiles, s) : 0;
+    return s > 1 ? Tile::ws_bytes(tiles, s + kLoraParts) : 0;
   }
   return 0;
 }
@@ -245,9 +248,9 @@ hipError_t launch_kernel(const GemmParams& p_in, hipStream_t stream) {
     // tiles are shared along K only with enough scratch memory to hold the partial tiles; without it the
     // instance runs as its plain counterpart (one workgroup per tile, nothing written to the scratch memory)
     p.split_k = split_k_factor<Tile>(p, device_cus(dev));
-    if (p.ws == nullptr || p.ws_bytes < Tile::ws_bytes(total, p.split_k) || total * p.split_k > 0x7fffffffll)
+    if (p.ws == nullptr || p.ws_bytes < Tile::ws_bytes(total, p.split_k + kLoraParts) || total * (p.split_k + kLoraParts) > 0x7fffffffll)
       p.split_k = 1;
-    grid = dim3((unsigned)(total * p.split_k), 1, 1);
+    grid = dim3((unsigned)(total * (p.split_k > 1 ? p.split_k + kLoraParts : 1)), 1, 1);
   }
   if (grid.x > most_workgroups(Tile::NT)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(kernel, grid, dim3(Tile::NT), Tile::kLdsBytes, stream, p);

@@ -272,8 +272,12 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
   const int k_tiles_all = (k_main + BK - 1) / BK;
   // this workgroup's K-slabs [k_lo, k_lo + k_tiles)
   const int splits = Tile::SPLITK ? p.split_k : 1;
+  // (adapters: of tiles that are shared, one more workgroup has them and none of K)
+  constexpr bool kLora = IsLora<Epi>::value;
+  const int parts = splits + (kLora && splits > 1 ? 1 : 0);
+  const bool lora_alone = kLora && Tile::SPLITK && split == splits;
   const int k_lo = Tile::SPLITK ? (int)((int64_t)split * k_tiles_all / splits) : 0;
-  const int k_tiles = Tile::SPLITK ? (int)((int64_t)(split + 1) * k_tiles_all / splits) - k_lo : k_tiles_all;
+  const int k_tiles = lora_alone ? 0 : Tile::SPLITK ? (int)((int64_t)(split + 1) * k_tiles_all / splits) - k_lo : k_tiles_all;
 
   {
     // a transposed operand starts at its first column of the tile and ends with the tile's columns of row K-1
@@ -377,6 +381,10 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
         }
       }
     }
+
+    // the adapters of the wave's rows, likewise (tiles whose registers are all taken read one step's operands at a time)
+    LoraTile<std::conditional_t<kLora, T, bf16>, MT, MI, NI, (MI + NI) * MT <= 128 && (Tile::OCC < 4 || MI * NI * ACC_N < 64) ? 2 : 1> lora;
+    if constexpr (kLora) lora.read(p, m0 + wm * Tile::WTM, lane);
 
     // dword K tail: the up to three dwords behind the last whole 16-byte piece of each of the lane's operand rows,
     // requested before the slab loads (so every wait of the loop covers them) and used after the loop
@@ -612,25 +620,62 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
         mfmas(ta, tb);
       }
     }
-    // low-rank adapters: behind K, by the last of the workgroups that share a tile; of waves with many, in the epilogue
-    constexpr bool kLora = IsLora<Epi>::value;
-    LoraTile<std::conditional_t<kLora, T, bf16>, MT, MI, NI, true> lora;
+    // low-rank adapters: behind K; of waves with many, in the epilogue, or here through the wave's strip where they are all there is
+    constexpr int PITCH = Tile::EPI_PITCH;
+    constexpr int NG = ACC_N / 4;  // groups of 4 consecutive columns per lane per MFMA tile
+    float* strip = reinterpret_cast<float*>(smem_raw) + wave * MT * PITCH;
     if constexpr (kLora) {
-      lora.read(p, m0 + wm * Tile::WTM, lane);
       lora.count();
-      if (!lora.many && (Tile::SPLITK == 0 || split == splits - 1))
+      if (!lora.many && (splits == 1 || lora_alone))
         lora.add(p, m0 + wm * Tile::WTM, n0 + wn * Tile::WTN, lane,
                  [&](bf16x8 b, bf16x8 a, auto mi, auto ni) __attribute__((always_inline)) { acc[mi][ni] = MfmaOp<bf16, MT>::run(b, a, acc[mi][ni]); });
+    }
+    // the wave's rows of block mi in its strip, plus their adapters' (in a loop: of the epilogue there are as many copies as passes)
+    auto add_many = [&](int mi, bool from_zero) {
+#pragma unroll 1
+      for (int ps = 0; ps < PASSES; ++ps) {
+        const int row = ps * ROWS_PER_PASS + rd_row, m = epi_row(mi, ps);
+        if ((ACTIVE != 64 && lane >= ACTIVE) || row >= MT) continue;
+        float v[8];
+        float* const at = strip + row * PITCH + rd_col;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = from_zero ? 0.0f : at[j];
+        if constexpr (kLora) {
+          if (m < p.M && n_epi < p.N) lora_add<T, 8>(v, p, m, n_epi);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) at[j] = v[j];
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    if constexpr (kLora && Tile::SPLITK != 0) {
+      if (lora_alone && lora.many) {
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi) {
+          add_many(mi, true);
+#pragma unroll
+          for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              const f32x4 v = *reinterpret_cast<const f32x4*>(strip + fr * PITCH + ni * MT + g * (QN * 4) + fq * 4);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[mi][ni][g * 4 + j] = v[j];
+            }
+        }
+        __syncthreads();  // (the strips share LDS with the exchange's broadcast word)
+      }
     }
 
     if constexpr (Tile::SPLITK != 0) {
       // ---------------- split-K: partial tile to the scratch memory; the last workgroup of the tile sums ----
-      // ws: int32 counter per (batch, tile) pair, padded to 4 KiB, then slot (pair * splits + split) of BM * BN
+      // ws: int32 counter per (batch, tile) pair, padded to 4 KiB, then slot (pair * parts + split) of BM * BN
       // floats.  A lane's 16-byte pieces lie as ((wave * PIECES + q) * 64 + lane) * 16 bytes: every wave-store and
       // wave-load is one contiguous KiB.  The slots may be read on another XCD than they were written on, whose L2
       // does not see this one's lines: they are written through to memory and read from there (sc1), and a store
       // is complete when vmcnt says so - no cache write-back or invalidate.
-      if (splits > 1) {
+      if (parts > 1) {
         constexpr int PIECES = MI * NI * (ACC_N / 4);
         constexpr int kCoherent = 16;
         const int pair = batch * (p.tiles_m * p.tiles_n) + tm * p.tiles_n + tn;
@@ -638,7 +683,7 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
         const int64_t counter_bytes = ((int64_t)grid_tiles * 4 + Tile::kCounterAlign - 1) / Tile::kCounterAlign * Tile::kCounterAlign;
         unsigned char* const slots = reinterpret_cast<unsigned char*>(p.ws) + counter_bytes;
         auto slot_rsrc = [&](int s_idx, uint32_t bytes) {
-          const uint64_t a = reinterpret_cast<uint64_t>(slots + ((int64_t)pair * splits + s_idx) * Tile::kSlotBytes);
+          const uint64_t a = reinterpret_cast<uint64_t>(slots + ((int64_t)pair * parts + s_idx) * Tile::kSlotBytes);
           const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a), hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
           return make_rsrc(reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), bytes);
         };
@@ -663,7 +708,7 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
         int* const word = reinterpret_cast<int*>(smem_raw);
         if (tid == 0) *word = __hip_atomic_fetch_add(&counters[pair], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
         __syncthreads();
-        const bool last = *word == splits - 1;
+        const bool last = *word == parts - 1;
         __syncthreads();
         if (!last) return;
 #pragma unroll
@@ -676,11 +721,11 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
         // 11.5 us, 8.9 so; 384 x 768 x 3072 in three 10.2 and 9.9; eight at a time cost three splits more than they give
         // eight).  Those past the last give zeros, which leave the sum as it is.
         constexpr int AT_ONCE = MI * NI * ACC_N <= 32 ? 4 : 2;
-        for (int s0 = 0; s0 < splits; s0 += AT_ONCE) {
+        for (int s0 = 0; s0 < parts; s0 += AT_ONCE) {
           u32x4 part[AT_ONCE][PIECES];
 #pragma unroll
           for (int s = 0; s < AT_ONCE; ++s) {
-            const __amdgpu_buffer_rsrc_t rs = slot_rsrc(s0 + s < splits ? s0 + s : 0, s0 + s < splits ? (uint32_t)Tile::kSlotBytes : 0u);
+            const __amdgpu_buffer_rsrc_t rs = slot_rsrc(s0 + s < parts ? s0 + s : 0, s0 + s < parts ? (uint32_t)Tile::kSlotBytes : 0u);
 #pragma unroll
             for (int q = 0; q < PIECES; ++q) part[s][q] = __builtin_amdgcn_raw_buffer_load_b128(rs, lane_off, q * 1024, kCoherent);
           }
@@ -716,10 +761,6 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
 
     float one = 1.0f;
     asm volatile("" : "+s"(one));  // (opaque to the optimizer: see to_float_plus)
-    constexpr int PITCH = Tile::EPI_PITCH;
-    float* strip = reinterpret_cast<float*>(smem_raw) + wave * MT * PITCH;
-    constexpr int NG = ACC_N / 4;  // groups of 4 consecutive columns per lane per MFMA tile
-
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) {
       // this wave's MT x WTN strip, row-major fp32
@@ -736,6 +777,9 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      if constexpr (kLora) {
+        if (lora.many && splits == 1) add_many(mi, false);
+      }
 #pragma unroll
       for (int ps = 0; ps < PASSES; ++ps) {
         const int row = ps * ROWS_PER_PASS + rd_row;
@@ -746,9 +790,6 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
           const f32x4 v0 = *reinterpret_cast<const f32x4*>(strip + row * PITCH + rd_col);
           const f32x4 v1 = *reinterpret_cast<const f32x4*>(strip + row * PITCH + rd_col + 4);
           float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-          if constexpr (kLora) {
-            if (lora.many) lora_add<T, 8>(v, p, m, n);
-          }
           const int64_t c_idx = out_index<PERM>(p, m, n);
           const int64_t d_idx = (int64_t)m * p.ldd + n;
           float scale = 1.0f;  // (of the row)

@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(Tile::NT, 1) gemm_rcr_wide_kernel(const GemmPa
       const GemmParams& q = arguments_anew<GemmParams>();
       int row0 = cur.m0 + wm * Tile::WTM, col0 = cur.n0 + wn * Tile::WTN, at_lane = lane;
       asm volatile("" : "+s"(row0), "+s"(col0), "+v"(at_lane));
-      LoraTile<std::conditional_t<IsLora<Epi>::value, T, bf16>, 16, MI, NI, false> lora;
+      LoraTile<std::conditional_t<IsLora<Epi>::value, T, bf16>, 16, MI, NI, 1> lora;
       lora.read(q, row0, at_lane);
       lora.add(q, row0, col0, at_lane, [&](bf16x8 b, bf16x8 a, auto mi, auto ni) __attribute__((always_inline)) {
         f32x4& c = acc[mi][ni];

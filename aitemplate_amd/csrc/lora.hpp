@@ -27,9 +27,9 @@ constexpr int lora_chunks(int rank) { return (rank + 7) / 8; }
 AITAMD_DEVICE const bf16* lora_row(const GemmParams& p, int m) {
   return reinterpret_cast<const bf16*>(p.lora_t) + (int64_t)m * (lora_chunks(p.lora_rank) * 16);
 }
-// the adapter of row m, or -1
+// the adapter of row m, or -1 (-2: there is no such row)
 AITAMD_DEVICE int lora_adapter(const GemmParams& p, int m) {
-  if (m >= p.M) return -1;
+  if (m >= p.M) return -2;
   const int id = p.lora_of[m];
   return (uint32_t)id < (uint32_t)p.lora_n ? id : -1;
 }
@@ -70,9 +70,8 @@ AITAMD_DEVICE u32x4 lora_largest(u32x4 v) {
   return v;
 }
 
-// The part of a wave whose rows row0 + mi * MT + (lane % MT) meet columns col0 + ni * MT + (lane % MT).  ODD: any rank, else even
-// ones.
-template <class T, int MT, int MI, int NI, bool ODD>
+// The part of a wave whose rows row0 + mi * MT + (lane % MT) meet columns col0 + ni * MT + (lane % MT).  STEPS: matrix instructions' worth of ranks whose operands are on their way together.
+template <class T, int MT, int MI, int NI, int STEPS>
 struct LoraTile {
   static constexpr int QN = 64 / MT;
   int of[MI];
@@ -130,71 +129,81 @@ struct LoraTile {
       const int id = first_of(left);
       if (id < 0) break;
       const __amdgpu_buffer_rsrc_t rb = make_rsrc(lora_column<T>(p, id, col0), (uint32_t)columns * b_pitch);
-      for (int c0 = 0; c0 < chunks; c0 += PER) {
-        const bool on = c0 + half < chunks;
-        const uint32_t tc = t_at + (uint32_t)c0 * 32u, bc = b_at + (uint32_t)c0 * 16u;
+      // rows of others among the wave's
+      bool mixed = false;
+      static_for<0, MI>([&](auto mi) __attribute__((always_inline)) {
+        mixed = mixed || __builtin_amdgcn_ballot_w64(of[mi] != id && of[mi] != -2) != 0;
+      });
+      for (int c0 = 0; c0 < chunks; c0 += STEPS * PER) {
         // Numbers that are none, times the zeros of other requests' rows, would reach them: where a wave meets some, the product is
         // taken without them first, then again with the largest number in their places and zeros in the others', times the
         // largest: an infinity where it belongs and zero elsewhere.
         bool again = false;
         for (int pass = 0; pass < 2; ++pass) {
-          u32x4 w[NI], t[MI];
-          if (!ODD || (rank & 1) == 0) {
+          u32x4 w[STEPS][NI], t[STEPS][MI];
+          static_for<0, STEPS>([&](auto s_c) __attribute__((always_inline)) {
+            constexpr int s = decltype(s_c)::value;
+            const bool on = c0 + s * PER + half < chunks;
+            const uint32_t tc = t_at + (uint32_t)(c0 + s * PER) * 32u, bc = b_at + (uint32_t)(c0 + s * PER) * 16u;
             static_for<0, NI>([&](auto ni) __attribute__((always_inline)) {
-              w[ni] = buffer_load_16B(rb, on ? bc + (uint32_t)(decltype(ni)::value * MT) * b_pitch : kOobOffset);
+              w[s][ni] = buffer_load_16B(rb, on ? bc + (uint32_t)(decltype(ni)::value * MT) * b_pitch : kOobOffset);
             });
-            // (behind the last rank is the next column's first; the buffer ends with a dword)
-            if (8 * (c0 + PER) > rank) {
-              const int dwords = rank / 2 - 4 * (c0 + half);
+            static_for<0, MI>([&](auto mi) __attribute__((always_inline)) {
+              t[s][mi] = buffer_load_16B(rt, on && left[mi] == id ? tc + (uint32_t)(decltype(mi)::value * MT) * t_pitch : kOobOffset);
+            });
+          });
+          if (8 * (c0 + STEPS * PER) > rank) {
+            // behind the last rank is the next column's first; an odd one shares its dword with that (with the buffer's end, which
+            // takes whole dwords), and is read again by itself
+            static_for<0, STEPS>([&](auto s_c) __attribute__((always_inline)) {
+              const int c = c0 + decltype(s_c)::value * PER + half, dwords = rank / 2 - 4 * c;
               static_for<0, NI>([&](auto ni) __attribute__((always_inline)) {
+                const uint32_t at = b_at + (uint32_t)(decltype(ni)::value * MT) * b_pitch + (uint32_t)((rank - 1) * 2 - half * 16);
+                const uint32_t last =
+                    (rank & 1) != 0 && c < chunks ? (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rb, at, 0, 0) : 0u;
 #pragma unroll
-                for (int d = 0; d < 4; ++d) w[ni][d] = d < dwords ? w[ni][d] : 0u;
+                for (int d = 0; d < 4; ++d) w[decltype(s_c)::value][ni][d] = d < dwords ? w[decltype(s_c)::value][ni][d] : (d == dwords ? last : 0u);
+              });
+            });
+          }
+          bf16x8 two[STEPS][NI];
+          if constexpr (kHalves) {
+            static_for<0, STEPS>([&](auto s) __attribute__((always_inline)) {
+              static_for<0, NI>([&](auto ni) __attribute__((always_inline)) {
+                bf16x8 one;
+                lora_parts<T>(__builtin_bit_cast(typename ElemTraits<T>::vec8, w[s][ni]), one, two[s][ni]);
+                w[s][ni] = __builtin_bit_cast(u32x4, MT == 16 && (fq >> 1) ? two[s][ni] : one);
+              });
+            });
+          }
+          if (mixed) {
+            if (pass == 0) {
+              bool numbers = true;
+              static_for<0, STEPS>([&](auto s) __attribute__((always_inline)) {
+                static_for<0, NI>([&](auto ni) __attribute__((always_inline)) { numbers = numbers && lora_numbers(w[s][ni]); });
+              });
+              again = __builtin_amdgcn_ballot_w64(!numbers) != 0;
+            }
+            if (again) {
+              static_for<0, STEPS>([&](auto s) __attribute__((always_inline)) {
+                static_for<0, NI>([&](auto ni) __attribute__((always_inline)) { w[s][ni] = lora_split(w[s][ni], pass); });
+                if (pass == 1) {
+                  const bool on = c0 + decltype(s)::value * PER + half < chunks;
+                  static_for<0, MI>([&](auto mi) __attribute__((always_inline)) { t[s][mi] = on && left[mi] == id ? lora_largest(t[s][mi]) : u32x4{}; });
+                }
               });
             }
-          } else {
-            // (one column's loads at a time: all together need more registers than there are)
-            static_for<0, NI>([&](auto ni) __attribute__((always_inline)) {
-#pragma unroll
-              for (int d = 0; d < 4; ++d) {
-                uint32_t e[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                  e[j] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(
-                      rb, 8 * (c0 + half) + 2 * d + j < rank ? bc + (uint32_t)(decltype(ni)::value * MT) * b_pitch + (2 * d + j) * 2u : kOobOffset, 0, 0);
-                w[ni][d] = e[0] | e[1] << 16;
-              }
-              asm volatile("" : "+v"(w[ni]));
-            });
-          }
-          static_for<0, MI>([&](auto mi) __attribute__((always_inline)) {
-            t[mi] = buffer_load_16B(rt, on && left[mi] == id ? tc + (uint32_t)(decltype(mi)::value * MT) * t_pitch : kOobOffset);
-          });
-          bf16x8 two[NI];
-          static_for<0, NI>([&](auto ni) __attribute__((always_inline)) {
-            if constexpr (kHalves) {
-              bf16x8 one;
-              lora_parts<T>(__builtin_bit_cast(typename ElemTraits<T>::vec8, w[ni]), one, two[ni]);
-              w[ni] = __builtin_bit_cast(u32x4, MT == 16 && (fq >> 1) ? two[ni] : one);
-            }
-          });
-          if (pass == 0) {
-            bool numbers = true;
-            static_for<0, NI>([&](auto ni) __attribute__((always_inline)) { numbers = numbers && lora_numbers(w[ni]); });
-            again = __builtin_amdgcn_ballot_w64(!numbers) != 0;
-          }
-          if (again) {
-            static_for<0, NI>([&](auto ni) __attribute__((always_inline)) { w[ni] = lora_split(w[ni], pass); });
-            if (pass == 1)
-              static_for<0, MI>([&](auto mi) __attribute__((always_inline)) { t[mi] = on && left[mi] == id ? lora_largest(t[mi]) : u32x4{}; });
           }
           static_for<0, MI>([&](auto mi) __attribute__((always_inline)) {
             if (__builtin_amdgcn_ballot_w64(left[mi] == id) == 0) return;
-            const bf16x8 a = __builtin_bit_cast(bf16x8, t[mi]);
-            static_for<0, NI>([&](auto ni) __attribute__((always_inline)) { multiply(__builtin_bit_cast(bf16x8, w[ni]), a, mi, ni); });
-            if constexpr (kHalves && MT == 32) {
-              if (pass == 0)
-                static_for<0, NI>([&](auto ni) __attribute__((always_inline)) { multiply(two[ni], a, mi, ni); });
-            }
+            static_for<0, STEPS>([&](auto s) __attribute__((always_inline)) {
+              const bf16x8 a = __builtin_bit_cast(bf16x8, t[s][mi]);
+              static_for<0, NI>([&](auto ni) __attribute__((always_inline)) { multiply(__builtin_bit_cast(bf16x8, w[s][ni]), a, mi, ni); });
+              if constexpr (kHalves && MT == 32) {
+                if (pass == 0)
+                  static_for<0, NI>([&](auto ni) __attribute__((always_inline)) { multiply(two[s][ni], a, mi, ni); });
+              }
+            });
           });
           if (!again) break;
         }

@@ -1,9 +1,12 @@
 // C ABI launchers of aitamd_gemm_rcr_lora: the adapters' first halves here, the product with their second halves in the tiles of
 // the GEMM (lora.hpp, gemm_inst.hip with AITAMD_DT 4 and 5).
+#include <mutex>
+
 #include "../../include/aitemplate_amd_kernels.h"
 #include "device.hpp"
 #include "errors.hpp"
 #include "gemm_host.hpp"
+#include "gemm_kernel_dma.hpp"
 #include "lora.hpp"
 
 namespace aitamd {
@@ -71,87 +74,261 @@ AITAMD_DEVICE float wave_dot(const T* x, const T* a, int K, int lane) {
 
 constexpr int kRowThreads = 256;
 // Few rows, which may all have adapters of their own: a wave for a rank of a row.  Bound: the latency of two trips to memory
-// (adapter, then the rows of x and a together).
+// (the row and its adapter's number, then the adapter; up to 4096 of K at once).
 template <class T>
 __global__ void __launch_bounds__(kRowThreads) low_rows_kernel(const LowParams p) {
-  clear_counters(p, kRowThreads);
+  using vec8 = typename ElemTraits<T>::vec8;
+  constexpr int AHEAD = 8;
   const int lane = threadIdx.x & 63, m = p.first + blockIdx.x;
   const int padded = lora_chunks(p.rank) * 8;
   const int j = blockIdx.y * (kRowThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (j >= padded) return;
+  const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)m * p.ldx;
+  // whole pieces of the first trip; what there is no whole piece for is left to wave_dot
+  vec8 xv[AHEAD], av[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) {
+    xv[i] = vec8{};
+    if (i * 512 + lane * 8 + 8 <= p.K) xv[i] = load_vec<vec8>(x + i * 512 + lane * 8);
+  }
   const int id = __builtin_amdgcn_readfirstlane(adapter_of(p, m));
+  clear_counters(p, kRowThreads);
+  if (j >= padded) return;
   float v = 0.0f;
   if (id >= 0 && j < p.rank) {
-    v = wave_dot(reinterpret_cast<const T*>(p.x) + (int64_t)m * p.ldx, reinterpret_cast<const T*>(p.a) + ((int64_t)id * p.rank + j) * p.K, p.K, lane);
-    v *= p.scales != nullptr ? p.scales[id] : 1.0f;
+    const T* a = reinterpret_cast<const T*>(p.a) + ((int64_t)id * p.rank + j) * p.K;
+    const float scale = p.scales != nullptr ? p.scales[id] : 1.0f;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      av[i] = vec8{};
+      if (i * 512 + lane * 8 + 8 <= p.K) av[i] = load_vec<vec8>(a + i * 512 + lane * 8);
+    }
+    float s[2] = {};
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) s[i & 1] = dot8<T>(xv[i], av[i], s[i & 1]);
+    // behind them: the rest of a piece, more pieces
+    const int k = p.K < AHEAD * 512 ? p.K & ~7 : AHEAD * 512;
+    v = wave_sum(s[0] + s[1]);
+    if (k < p.K) v += wave_dot(x + k, a + k, p.K - k, lane);
+    v *= scale;
   }
   if (lane == 0) put_low(p.t + (int64_t)m * padded * 2, j, v);
 }
 
-// Rows of prompts, neighbours of one adapter mostly: ROWS of them and up to 64 ranks a workgroup, on matrix instructions, every
-// wave with a part of K; a step is 64 deep, each lane with 32 neighbouring bytes of a row for two matrix instructions (which k is
-// which does not matter where both operands have it alike), so that a row's share of a step is a line.  Bound: memory, x once.
-// Several adapters among the rows: one after the other; more than kLoraFew: row by row.
-constexpr int kTileWaves = 8, kTileRows = 32, kTileRanks = 64;
+// Rows of prompts, neighbours of one adapter mostly: ROWS of them and NR x 16 ranks a workgroup.  Several adapters among the rows: one
+// after the other; more than kLoraFew: row by row.
+struct LowTile {
+  int mine, left, distinct;  // the lane's row's adapter, that or -1, how many there are among the rows
+  AITAMD_DEVICE int first() const {
+    const uint64_t some = __builtin_amdgcn_ballot_w64(left >= 0);
+    return some == 0 ? -1 : __builtin_amdgcn_readlane(left, __builtin_ctzll(some));
+  }
+  AITAMD_DEVICE void drop(int id) { left = left == id ? -1 : left; }
+};
+// Zeros where there is no adapter, and all rows where there are many adapters; false if that was all.  of: the rows' adapters, in LDS.
+template <class T, int THREADS>
+AITAMD_DEVICE bool low_begin(const LowParams& p, LowTile& l, int* of, int m0, int rows, int j0, int ranks, int padded) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  l.mine = l.left = lane < rows ? adapter_of(p, m0 + lane) : -1;
+  clear_counters(p, THREADS);
+  if (tid < rows) of[tid] = l.mine;
+  l.distinct = 0;
+  for (int id = l.first(); id >= 0 && l.distinct <= kLoraFew; id = l.first(), ++l.distinct) l.drop(id);
+  l.left = l.mine;
+  bf16* const t = p.t + ((int64_t)m0 * padded + j0) * 2;
+  if (__builtin_amdgcn_ballot_w64(lane < rows && l.mine < 0) != 0) {
+    __syncthreads();
+    const int chunks = ranks / 8;
+    for (int i = tid; i < rows * chunks; i += THREADS) {
+      const int r = i / chunks, c = i - r * chunks;
+      if (of[r] < 0) {
+        bf16* const at = t + ((int64_t)r * padded + c * 8) * 2;
+        store_vec(at, bf16x8{});
+        store_vec(at + 8, bf16x8{});
+      }
+    }
+  }
+  if (l.distinct <= kLoraFew) return l.distinct > 0;
+  for (int i = wave; i < rows * ranks; i += THREADS / 64) {
+    const int r = i / ranks, j = j0 + i - r * ranks;
+    const int id = __builtin_amdgcn_readlane(l.mine, r);
+    if (id < 0) continue;
+    float v = 0.0f;
+    if (j < p.rank)
+      v = wave_dot(reinterpret_cast<const T*>(p.x) + (int64_t)(m0 + r) * p.ldx, reinterpret_cast<const T*>(p.a) + ((int64_t)id * p.rank + j) * p.K, p.K, lane) *
+          (p.scales != nullptr ? p.scales[id] : 1.0f);
+    if (lane == 0) put_low(p.t + (int64_t)(m0 + r) * padded * 2, j, v);
+  }
+  return false;
+}
+// The waves' sums part[wave][row][rank], PITCH floats a row, of the rows that belong to `id`: a chunk of a row for a thread
+template <int WAVES, int PITCH>
+AITAMD_DEVICE void low_end(const LowParams& p, const float* part, const int* of, int id, int m0, int rows, int j0, int ranks, int padded, int tile_rows) {
+  const float scale = p.scales != nullptr ? p.scales[id] : 1.0f;
+  const int chunks = ranks / 8;
+  for (int i = threadIdx.x; i < rows * chunks; i += WAVES * 64) {
+    const int r = i / chunks, c = i - r * chunks;
+    if (of[r] != id) continue;
+    float v[8] = {};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float* at = part + (w * tile_rows + r) * PITCH + c * 8;
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(at), hi = *reinterpret_cast<const f32x4*>(at + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += lo[e], v[4 + e] += hi[e];
+    }
+    bf16x8 one, two;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float f = j0 + c * 8 + e < p.rank ? v[e] * scale : 0.0f;
+      one[e] = (bf16)f;
+      two[e] = (bf16)(__builtin_isfinite((float)one[e]) ? f - (float)one[e] : 0.0f);
+    }
+    bf16* const at = p.t + ((int64_t)(m0 + r) * padded + j0 + c * 8) * 2;
+    store_vec(at, one);
+    store_vec(at + 8, two);
+  }
+}
+
+// Rows of whole dwords.  Bound: memory, x once.  Slabs of 128 of K of the rows and of the adapter go straight to a ring in LDS, 16
+// lanes for 256 bytes of a row (to registers, in the layout of the operands, every lane fetches from a line of its own: 8192 x 4096,
+// rank 64, 52 us), each of the four waves multiplies a quarter of a slab.
+template <class T, int NR_, int MB_>
+struct LowRing {
+  static constexpr int NR = NR_, MB = MB_;
+  static constexpr int ROWS = 16 * MB, RANKS = 16 * NR, WAVES = 4, NS = 6, BK = 128;
+  static constexpr int LOADS = (ROWS + RANKS) / 4 / WAVES;  // of a wave for a slab, four rows each
+  static constexpr int STAGE = (ROWS + RANKS) * BK;         // elements
+  static constexpr int PITCH = RANKS + 4;
+  static constexpr int kLdsBytes = NS * STAGE * 2;
+  static_assert((ROWS + RANKS) % (4 * WAVES) == 0 && WAVES * ROWS * PITCH * 4 <= kLdsBytes && kLdsBytes + ROWS * 4 <= 160 * 1024);
+};
+template <class T, class R>
+__global__ void __launch_bounds__(R::WAVES * 64) low_ring_kernel(const LowParams p) {
+  using Tr = ElemTraits<T>;
+  using vec8 = typename Tr::vec8;
+  constexpr int NR = R::NR, MB = R::MB, NS = R::NS;
+  typedef __attribute__((address_space(3))) void lds_void;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
+  T* const smem = reinterpret_cast<T*>(smem_raw);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int fr = lane & 15, fq = lane >> 4;
+  const int m0 = p.first + blockIdx.x * R::ROWS, j0 = blockIdx.y * R::RANKS;
+  const int padded = lora_chunks(p.rank) * 8;
+  const int rows = p.M - m0 < R::ROWS ? p.M - m0 : R::ROWS, ranks = padded - j0 < R::RANKS ? padded - j0 : R::RANKS;
+  LowTile l;
+  __shared__ int of[R::ROWS];
+  if (!low_begin<T, R::WAVES * 64>(p, l, of, m0, rows, j0, ranks, padded)) return;
+  const int slabs = (p.K + R::BK - 1) / R::BK;
+  const __amdgpu_buffer_rsrc_t rx = make_rsrc(reinterpret_cast<const T*>(p.x) + (int64_t)m0 * p.ldx, (uint32_t)(((rows - 1) * (uint32_t)p.ldx + (uint32_t)p.K) * 2u));
+  // row r's piece c of a slab lies at place c ^ r of the row's 256 bytes: the 16 rows of a fragment are on different banks
+  uint32_t off[R::LOADS];
+  int at_k[R::LOADS];
+#pragma unroll
+  for (int i = 0; i < R::LOADS; ++i) {
+    const int row = (wave + i * R::WAVES) * 4 + (lane >> 4);
+    const bool of_x = row < R::ROWS;
+    at_k[i] = ((lane & 15) ^ (row & 15)) * 8;
+    off[i] = (uint32_t)(of_x ? row * (int)p.ldx : (row - R::ROWS) * p.K) * 2u + (uint32_t)at_k[i] * 2u;
+  }
+  for (;;) {
+    const int id = l.first();
+    if (id < 0) break;
+    const int there = p.rank - j0 < R::RANKS ? p.rank - j0 : R::RANKS;
+    const __amdgpu_buffer_rsrc_t ra = make_rsrc(reinterpret_cast<const T*>(p.a) + ((int64_t)id * p.rank + j0) * p.K, (uint32_t)(there > 0 ? there : 0) * (uint32_t)p.K * 2u);
+    auto issue = [&](int kt) __attribute__((always_inline)) {
+      T* const stage = smem + kt % NS * R::STAGE;
+#pragma unroll
+      for (int i = 0; i < R::LOADS; ++i) {
+        const int j = wave + i * R::WAVES;
+        const uint32_t o = at_k[i] + kt * R::BK < p.K ? off[i] + (uint32_t)(kt * R::BK * 2) : kOobOffset;
+        if (j * 4 < R::ROWS)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_void*)(stage + j * 512), 16, o, 0, 0, 0);
+        else
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void*)(stage + j * 512), 16, o, 0, 0, 0);
+      }
+    };
+    f32x4 acc[MB][NR] = {};
+    // LEFT: slabs behind this one that are on their way or to come, NS - 1 standing for any number from there on
+    auto slab = [&](int kt, auto left_c) __attribute__((always_inline)) {
+      constexpr int LEFT = decltype(left_c)::value;
+      wait_vmcnt<(LEFT >= NS - 1 ? NS - 2 : LEFT) * R::LOADS>();
+      __builtin_amdgcn_s_barrier();
+      const T* const stage = smem + kt % NS * R::STAGE;
+      const int c = wave * 4 + fq;
+      u32x4 f[MB + NR];
+#pragma unroll
+      for (int b = 0; b < MB + NR; ++b) f[b] = *reinterpret_cast<const u32x4*>(stage + (b * 16 + fr) * R::BK + ((c ^ fr) << 3));
+      if constexpr (LEFT >= NS - 1) issue(kt + NS - 1);
+      if (LEFT == 0 && (p.K & 7) != 0) {
+        // (the last piece of a row goes on in the next one)
+        const int dwords = (p.K - kt * R::BK - c * 8) / 2;
+#pragma unroll
+        for (int b = 0; b < MB + NR; ++b)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) f[b][d] = d < dwords ? f[b][d] : 0u;
+      }
+#pragma unroll
+      for (int b = 0; b < MB; ++b)
+#pragma unroll
+        for (int r = 0; r < NR; ++r) acc[b][r] = Tr::mfma16(__builtin_bit_cast(vec8, f[MB + r]), __builtin_bit_cast(vec8, f[b]), acc[b][r]);
+    };
+#pragma unroll
+    for (int s = 0; s < NS - 1; ++s)
+      if (s < slabs) issue(s);
+    int kt = 0;
+    for (; kt + NS - 1 < slabs; ++kt) slab(kt, std::integral_constant<int, NS - 1>{});
+    static_for<0, NS - 1>([&](auto i) __attribute__((always_inline)) {
+      constexpr int left = NS - 2 - decltype(i)::value;
+      if (left < slabs) slab(slabs - 1 - left, std::integral_constant<int, left>{});
+    });
+    __syncthreads();
+    // (the operands swapped: a lane has four neighbouring ranks of one row)
+    float* const part = reinterpret_cast<float*>(smem_raw);
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+        *reinterpret_cast<f32x4*>(part + (wave * R::ROWS + b * 16 + fr) * R::PITCH + r * 16 + fq * 4) = acc[b][r];
+    __syncthreads();
+    low_end<R::WAVES, R::PITCH>(p, part, of, id, m0, rows, j0, ranks, padded, R::ROWS);
+    __syncthreads();
+    l.drop(id);
+  }
+}
+
+// Rows at any element, through registers: a step is 64 deep, each lane with 32 neighbouring bytes of a row for two matrix instructions
+// (which k is which does not matter where both operands have it alike).
+constexpr int kTileWaves = 8, kTileRows = 32;
 template <class T, int NR>
 __global__ void __launch_bounds__(kTileWaves * 64) low_tile_kernel(const LowParams p) {
   using Tr = ElemTraits<T>;
   using vec8 = typename Tr::vec8;
-  constexpr int MB = kTileRows / 16;
-  __shared__ float part[kTileWaves][kTileRows][NR * 16 + 1];
-  clear_counters(p, kTileWaves * 64);
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int MB = kTileRows / 16, PITCH = NR * 16 + 4;
+  __shared__ __attribute__((aligned(16))) float part[kTileWaves * kTileRows * PITCH];
+  __shared__ int of[kTileRows];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int fr = lane & 15, fq = lane >> 4;
   const int m0 = p.first + blockIdx.x * kTileRows, j0 = blockIdx.y * (NR * 16);
   const int padded = lora_chunks(p.rank) * 8;
-  // (rows past the last: of the last one, with no adapter)
-  int left[1];
-  left[0] = lane < kTileRows && m0 + lane < p.M ? adapter_of(p, m0 + lane) : -1;
-  const int mine = left[0];
-  auto first_of = [&]() __attribute__((always_inline)) {
-    const uint64_t some = __builtin_amdgcn_ballot_w64(left[0] >= 0);
-    return some == 0 ? -1 : __builtin_amdgcn_readlane(left[0], __builtin_ctzll(some));
-  };
-  int distinct = 0;
-  for (int id = first_of(); id >= 0 && distinct <= kLoraFew; id = first_of(), ++distinct)
-    if (left[0] == id) left[0] = -1;
-  left[0] = mine;
-  const T* x = reinterpret_cast<const T*>(p.x);
-  const T* a = reinterpret_cast<const T*>(p.a);
-  bf16* const t = p.t + (int64_t)m0 * padded * 2;
-  const int rows = p.M - m0 < kTileRows ? p.M - m0 : kTileRows;
-  const int ranks = padded - j0 < NR * 16 ? padded - j0 : NR * 16;
-  // zeros: rows without an adapter, ranks from p.rank on
-  for (int i = tid; i < rows * ranks; i += kTileWaves * 64) {
-    const int r = i / ranks, j = j0 + i - r * ranks;
-    if (j >= p.rank || adapter_of(p, m0 + r) < 0) put_low(t + (int64_t)r * padded * 2, j, 0.0f);
-  }
-  if (distinct > kLoraFew) {
-    for (int i = wave; i < rows * ranks; i += kTileWaves) {
-      const int r = i / ranks, j = j0 + i - r * ranks;
-      const int id = __builtin_amdgcn_readlane(mine, r);
-      if (id < 0 || j >= p.rank) continue;
-      const float v = wave_dot(x + (int64_t)(m0 + r) * p.ldx, a + ((int64_t)id * p.rank + j) * p.K, p.K, lane);
-      if (lane == 0) put_low(t + (int64_t)r * padded * 2, j, v * (p.scales != nullptr ? p.scales[id] : 1.0f));
-    }
-    return;
-  }
+  const int rows = p.M - m0 < kTileRows ? p.M - m0 : kTileRows, ranks = padded - j0 < NR * 16 ? padded - j0 : NR * 16;
+  LowTile l;
+  if (!low_begin<T, kTileWaves * 64>(p, l, of, m0, rows, j0, ranks, padded)) return;
   const T* xr[MB];
 #pragma unroll
   for (int b = 0; b < MB; ++b) {
     const int m = m0 + b * 16 + fr;
-    xr[b] = x + (int64_t)(m < p.M ? m : p.M - 1) * p.ldx + fq * 16;
+    xr[b] = reinterpret_cast<const T*>(p.x) + (int64_t)(m < p.M ? m : p.M - 1) * p.ldx + fq * 16;
   }
   const int steps = p.K / 64, per = (steps + kTileWaves - 1) / kTileWaves;
   const int s0 = wave * per < steps ? wave * per : steps, s1 = s0 + per < steps ? s0 + per : steps;
   for (;;) {
-    const int id = first_of();
+    const int id = l.first();
     if (id < 0) break;
     const T* ar[NR];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       const int j = j0 + r * 16 + fr;
-      ar[r] = a + ((int64_t)id * p.rank + (j < p.rank ? j : p.rank - 1)) * p.K + fq * 16;
+      ar[r] = reinterpret_cast<const T*>(p.a) + ((int64_t)id * p.rank + (j < p.rank ? j : p.rank - 1)) * p.K + fq * 16;
     }
     f32x4 acc[MB][NR] = {};
     auto step = [&](int k, auto whole) __attribute__((always_inline)) {
@@ -180,26 +357,50 @@ __global__ void __launch_bounds__(kTileWaves * 64) low_tile_kernel(const LowPara
     };
     for (int s = s0; s < s1; ++s) step(s * 64, std::true_type{});
     if (wave == kTileWaves - 1 && steps * 64 < p.K) step(steps * 64, std::false_type{});
-    // (the operands swapped: a lane has four neighbouring ranks of one row)
 #pragma unroll
     for (int b = 0; b < MB; ++b)
 #pragma unroll
       for (int r = 0; r < NR; ++r)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) part[wave][b * 16 + fr][r * 16 + fq * 4 + e] = acc[b][r][e];
+        *reinterpret_cast<f32x4*>(part + (wave * kTileRows + b * 16 + fr) * PITCH + r * 16 + fq * 4) = acc[b][r];
     __syncthreads();
-    const float scale = p.scales != nullptr ? p.scales[id] : 1.0f;
-    for (int i = tid; i < rows * ranks; i += kTileWaves * 64) {
-      const int r = i / ranks, j = i - r * ranks;
-      if (adapter_of(p, m0 + r) != id || j0 + j >= p.rank) continue;
-      float v = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kTileWaves; ++w) v += part[w][r][j];
-      put_low(t + (int64_t)r * padded * 2, j0 + j, v * scale);
-    }
+    low_end<kTileWaves, PITCH>(p, part, of, id, m0, rows, j0, ranks, padded, kTileRows);
     __syncthreads();
-    if (left[0] == id) left[0] = -1;
+    l.drop(id);
   }
+}
+
+// tiles of `tile_rows` rows by `groups` groups of ranks, in as many launches as it takes
+hipError_t launch_tiles(void (*kernel)(const LowParams), LowParams p, int tile_rows, int64_t groups, int threads, int lds, hipStream_t stream) {
+  const int64_t tiles = ((int64_t)p.M + tile_rows - 1) / tile_rows, most = most_workgroups(threads) / groups;
+  for (int64_t at = 0; at < tiles; at += most) {
+    p.first = (int32_t)(at * tile_rows);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles - at < most ? tiles - at : most), (unsigned)groups), dim3(threads), lds, stream, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+template <class T, int NR, int MB>
+hipError_t launch_ring(const LowParams& p, int64_t groups, hipStream_t stream) {
+  using R = LowRing<T, NR, MB>;
+  auto kernel = low_ring_kernel<T, R>;
+  // LDS above 64 KiB has to be opted into once per device
+  constexpr int kMaxDevices = 64;
+  static std::once_flag once[kMaxDevices];
+  static hipError_t errors[kMaxDevices];
+  int dev = 0;
+  const hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  std::call_once(once[dev % kMaxDevices], [&] {
+    errors[dev % kMaxDevices] = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, R::kLdsBytes);
+  });
+  if (errors[dev % kMaxDevices] != hipSuccess) return errors[dev % kMaxDevices];
+  return launch_tiles(kernel, p, R::ROWS, groups, R::WAVES * 64, R::kLdsBytes, stream);
+}
+template <class T, int NR>
+hipError_t launch_ring(const LowParams& p, int64_t groups, int cus, hipStream_t stream) {
+  // 32 rows share an adapter's lines where that leaves a tile for every CU
+  return (int64_t)p.M >= 32ll * cus ? launch_ring<T, NR, 2>(p, groups, stream) : launch_ring<T, NR, 1>(p, groups, stream);
 }
 
 template <class T>
@@ -213,16 +414,15 @@ hipError_t launch_low(LowParams p, hipStream_t stream) {
     return hipGetLastError();
   }
   const int nr = padded > 32 ? 4 : (padded > 16 ? 2 : 1);
-  auto kernel = nr == 4 ? low_tile_kernel<T, 4> : (nr == 2 ? low_tile_kernel<T, 2> : low_tile_kernel<T, 1>);
-  const int64_t tiles = ((int64_t)p.M + kTileRows - 1) / kTileRows, groups = (padded + nr * 16 - 1) / (nr * 16);
-  const int64_t most = most_workgroups(kTileWaves * 64) / groups;
-  for (int64_t at = 0; at < tiles; at += most) {
-    p.first = (int32_t)(at * kTileRows);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles - at < most ? tiles - at : most), (unsigned)groups), dim3(kTileWaves * 64), 0, stream, p);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+  const int64_t groups = (padded + nr * 16 - 1) / (nr * 16);
+  const bool dwords = ((p.K | p.ldx) & 1) == 0 && ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.a)) & 3) == 0 &&
+      p.ldx <= (1 << 24) && p.K <= (1 << 23);
+  if (dwords) {
+    const int cus = current_device_cus();
+    return nr == 4 ? launch_ring<T, 4>(p, groups, cus, stream) : (nr == 2 ? launch_ring<T, 2>(p, groups, cus, stream) : launch_ring<T, 1>(p, groups, cus, stream));
   }
-  return hipSuccess;
+  auto kernel = nr == 4 ? low_tile_kernel<T, 4> : (nr == 2 ? low_tile_kernel<T, 2> : low_tile_kernel<T, 1>);
+  return launch_tiles(kernel, p, kTileRows, groups, kTileWaves * 64, 0, stream);
 }
 
 constexpr int64_t kMostRank = 1024;

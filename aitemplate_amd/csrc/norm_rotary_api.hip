@@ -3,8 +3,9 @@
 // A head x of D numbers becomes x r w with r = 1 / sqrt(sum x^2 / D + eps), then its pairs turn by the token's position
 // (rotary.hpp): all in 32 bits, rounded once.  A head's pieces lie on neighbouring lanes of a wave, one each (a power of two of
 // lanes for a head, up to the wave; of longer heads several each), which sum their squares among themselves and go on with
-// what they have in registers.
-// Bound: memory, 4 bytes an element, as the rotation alone.
+// what they have in registers.  A workgroup goes through its tokens' queries, then their keys (and values), so that a lane's weights
+// are read once for all heads.
+// Bound: memory, 4 bytes an element, as the rotation alone; registers for eight waves a SIMD.
 #include "../../include/aitemplate_amd_kernels.h"
 #include "device.hpp"
 #include "errors.hpp"
@@ -23,7 +24,7 @@ struct NormPiece {
   int i1, i2, pair;                                       // pair: the first of the piece's, -1 behind the rotated dims
   vec v1, v2;
 
-  AITAMD_DEVICE void load(const T* x, int c, int n) {
+  AITAMD_DEVICE void place(int c, int n) {
     const int turned = VEC == 1 ? n : (INTERLEAVED ? 2 * n / VEC : n / VEC);
     if (c >= turned) {
       i1 = i2 = 2 * n + (c - turned) * VEC;
@@ -33,6 +34,8 @@ struct NormPiece {
       i2 = INTERLEAVED ? i1 + 1 : n + i1;
       pair = INTERLEAVED && VEC > 1 ? c * (VEC / 2) : c * VEC;
     }
+  }
+  AITAMD_DEVICE void load(const T* x) {
     v1 = load_vec<vec>(x + i1);
     v2 = vec{};
     if constexpr (kTwo) {
@@ -61,22 +64,22 @@ struct NormPiece {
       if (pair >= 0) store_vec(y + i2, v2);
     }
   }
-  // times ra, times rb and the weights (of one without: weight null), turned
-  AITAMD_DEVICE void store(T* y, const T* weight, float ra, float rb, const float2* table) const {
+  // the weights of the same elements
+  AITAMD_DEVICE void weigh(const T* weight, vec& w1, vec& w2) const {
+    w1 = w2 = load_vec<vec>(weight + i1);
+    if constexpr (kTwo) {
+      if (pair >= 0) w2 = load_vec<vec>(weight + i2);
+    }
+  }
+  // times ra, times rb and the weights (NORM), turned
+  template <bool NORM>
+  AITAMD_DEVICE void store(T* y, vec w1, vec w2, float ra, float rb, const float2* table) const {
     float a[VEC], b[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       a[j] = Tr::to_float(v1[j]);
       b[j] = Tr::to_float(v2[j]);
-    }
-    if (weight != nullptr) {
-      const vec w1 = load_vec<vec>(weight + i1);
-      vec w2 = w1;
-      if constexpr (kTwo) {
-        if (pair >= 0) w2 = load_vec<vec>(weight + i2);
-      }
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
+      if constexpr (NORM) {
         a[j] = a[j] * ra * (rb * Tr::to_float(w1[j]));
         if constexpr (kTwo) b[j] = b[j] * ra * (rb * Tr::to_float(w2[j]));
       }
@@ -107,9 +110,29 @@ struct NormPiece {
   }
 };
 
-template <class S>
-AITAMD_DEVICE S lanes_sum(S v, int lanes) {
-  for (int d = lanes >> 1; d > 0; d >>= 1) v += __shfl_xor(v, d);
+// The sum over 1 << shift neighbouring lanes, in all of them: quads and rows of 16 by moves along the row (mirrored once their halves
+// are even), then rows and halves of the wave exchanged.  (Through LDS, a trip for each step: 16384 x 20 x 256 100 us.)
+template <int CTRL>
+AITAMD_DEVICE float lane_move(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+AITAMD_DEVICE float lanes_sum(float v, int shift) {
+  if (shift > 0) v += lane_move<0xb1>(v);   // quad_perm 1 0 3 2
+  if (shift > 1) v += lane_move<0x4e>(v);   // quad_perm 2 3 0 1
+  if (shift > 2) v += lane_move<0x141>(v);  // row_half_mirror
+  if (shift > 3) v += lane_move<0x140>(v);  // row_mirror
+  if (shift > 4) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if (shift > 5) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return v;
+}
+AITAMD_DEVICE double lanes_sum(double v, int shift) {
+  for (int d = 1; d < 1 << shift; d <<= 1) v += __shfl_xor(v, d);
   return v;
 }
 
@@ -133,13 +156,11 @@ AITAMD_DEVICE void inverse_length(float sum, float by_dim, float eps, float& ra,
   }
 }
 
-enum HeadKind : int { kNothing = 0, kNorm = 1, kTurnOnly = 2, kCopy = 3 };
+enum HeadKind : int { kNorm = 0, kTurnOnly = 1, kCopy = 2 };
 template <class T>
 struct Head {
-  int kind;
-  const T* x;
+  const T* x;  // null: nothing to do
   T* y;
-  const T* weight;
   const float2* table;
 };
 
@@ -148,68 +169,74 @@ struct Lanes {
   float by_dim, eps;
 };
 
-// Heads 0 .. count - 1 of a workgroup, kAhead of a lane's on their way together.  head(i) is the same for all lanes of a head.
-template <class T, int VEC, bool INTERLEAVED, int AHEAD, class F>
-AITAMD_DEVICE void heads_of_workgroup(const Lanes& l, int count, F&& head) {
-  const int lane = threadIdx.x & (l.per_head - 1), at_once = kRotaryThreads >> l.shift;
+// Heads 0 .. count - 1 of one kind, AHEAD of a lane's on their way together.  head(i, h) is the same for all lanes of a head;
+// weight(i): its weights (the same for all with weight_head = 0).
+template <class T, int VEC, bool INTERLEAVED, int KIND, int AHEAD, class F, class W>
+AITAMD_DEVICE void heads_of_workgroup(const Lanes& l, int count, bool one_weight, F&& head, W&& weight) {
+  using Piece = NormPiece<T, VEC, INTERLEAVED>;
+  const int lane = threadIdx.x & (l.per_head - 1), mine = threadIdx.x >> l.shift, at_once = kRotaryThreads >> l.shift;
   const bool one_each = l.pieces <= l.per_head;
+  typename Piece::vec w1 = {}, w2 = {};
+  if (KIND == kNorm && one_weight && count > 0 && lane < l.pieces) {
+    Piece at;
+    at.place(lane, l.n);
+    at.weigh(weight(0), w1, w2);
+  }
   // (whole waves stay together: their lanes exchange sums)
-  for (int i0 = threadIdx.x >> l.shift; i0 - (int)(threadIdx.x >> l.shift) < count; i0 += AHEAD * at_once) {
+  for (int first = 0; first < count; first += AHEAD * at_once) {
     Head<T> h[AHEAD];
-    NormPiece<T, VEC, INTERLEAVED> piece[AHEAD];
-    float sum[AHEAD];
+    Piece piece[AHEAD];
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      const int i = i0 + a * at_once;
-      h[a].kind = kNothing;
-      sum[a] = 0.0f;
-      if (i >= count) continue;
-      h[a] = head(i);
-      if (h[a].kind == kNothing || lane >= l.pieces) continue;
-      piece[a].load(h[a].x, lane, l.n);
+      const int i = first + mine + a * at_once;
+      h[a].x = nullptr;
+      if (i < count && lane < l.pieces) head(i, h[a]);
+      piece[a].place(lane, l.n);
+      if (h[a].x != nullptr) piece[a].load(h[a].x);
     }
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      const bool on = h[a].kind != kNothing && lane < l.pieces;
-      if (on && h[a].kind == kNorm) {
-        sum[a] = piece[a].template squares<float>();
-        if (!one_each) {
+      const bool on = h[a].x != nullptr;
+      float ra = 1.0f, rb = 1.0f;
+      if constexpr (KIND == kNorm) {
+        float sum = on ? piece[a].template squares<float>() : 0.0f;
+        if (!one_each && on) {
           for (int c = lane + l.per_head; c < l.pieces; c += l.per_head) {
-            NormPiece<T, VEC, INTERLEAVED> more;
-            more.load(h[a].x, c, l.n);
-            sum[a] += more.template squares<float>();
+            Piece more;
+            more.place(c, l.n);
+            more.load(h[a].x);
+            sum += more.template squares<float>();
           }
         }
-      }
-      float ra = 1.0f, rb = 1.0f;
-      if (__builtin_amdgcn_ballot_w64(h[a].kind == kNorm) != 0) {
-        sum[a] = lanes_sum(sum[a], l.per_head);
+        sum = lanes_sum(sum, l.shift);
         // (of lanes without a head: of a sum that fits)
-        inverse_length(h[a].kind == kNorm ? sum[a] : 1.0f / l.by_dim, l.by_dim, l.eps, ra, rb, [&]() {
+        inverse_length(on ? sum : 1.0f / l.by_dim, l.by_dim, l.eps, ra, rb, [&]() {
           double s = 0.0;
-          if (on && h[a].kind == kNorm) {
-            s = piece[a].template squares<double>();
-            for (int c = lane + l.per_head; c < l.pieces; c += l.per_head) {
-              NormPiece<T, VEC, INTERLEAVED> more;
-              more.load(h[a].x, c, l.n);
-              s += more.template squares<double>();
-            }
+          for (int c = lane; on && c < l.pieces; c += l.per_head) {
+            Piece again;
+            again.place(c, l.n);
+            again.load(h[a].x);
+            s += again.template squares<double>();
           }
-          return lanes_sum(s, l.per_head);
+          return lanes_sum(s, l.shift);
         });
       }
       if (!on) continue;
-      auto put = [&](const NormPiece<T, VEC, INTERLEAVED>& q) __attribute__((always_inline)) {
-        if (h[a].kind == kCopy)
+      const T* w = KIND == kNorm && !(one_weight && one_each) ? weight(first + mine + a * at_once) : nullptr;
+      auto put = [&](const Piece& q) __attribute__((always_inline)) {
+        if constexpr (KIND == kCopy) {
           q.copy(h[a].y);
-        else
-          q.store(h[a].y, h[a].kind == kNorm ? h[a].weight : nullptr, ra, rb, h[a].table);
+        } else {
+          if (w != nullptr) q.weigh(w, w1, w2);
+          q.template store<KIND == kNorm>(h[a].y, w1, w2, ra, rb, h[a].table);
+        }
       };
       put(piece[a]);
       if (!one_each) {
         for (int c = lane + l.per_head; c < l.pieces; c += l.per_head) {
-          NormPiece<T, VEC, INTERLEAVED> more;
-          more.load(h[a].x, c, l.n);
+          Piece more;
+          more.place(c, l.n);
+          more.load(h[a].x);
           put(more);
         }
       }
@@ -228,16 +255,18 @@ struct NormParams {
   const void* positions;
   const float* freqs;
   int64_t pos_batch, pos_seq;
-  int32_t tokens, heads, all_heads, seq, first, per_wg, positions_64;
+  int32_t tokens, heads, kv_heads, seq, first, per_wg, positions_64;
   float scale;
   Lanes lanes;
-  Divisor by_n, by_seq, by_heads;
+  Divisor by_n, by_seq, by_heads, by_kv_heads;
 };
 
 constexpr int kNormAhead = 2;
+// waves of a SIMD (the widest pieces, of pairs of halves above all, have more to hold)
+constexpr int norm_waves(int vec, bool interleaved) { return vec < 8 ? 8 : (interleaved ? 6 : 5); }
 
 template <class T, int VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRotaryThreads) norm_rotary_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kRotaryThreads, norm_waves(VEC, INTERLEAVED)) norm_rotary_kernel(const NormParams p) {
   __shared__ float2 table[kRotaryTable];
   const int t0 = p.first + blockIdx.x * p.per_wg;
   const int tokens = p.tokens - t0 < p.per_wg ? p.tokens - t0 : p.per_wg;
@@ -247,21 +276,25 @@ __global__ void __launch_bounds__(kRotaryThreads) norm_rotary_kernel(const NormP
     return p.positions_64 ? reinterpret_cast<const int64_t*>(p.positions)[at] : reinterpret_cast<const int32_t*>(p.positions)[at];
   });
   __syncthreads();
-  heads_of_workgroup<T, VEC, INTERLEAVED, kNormAhead>(p.lanes, tokens * p.all_heads, [&](int i) __attribute__((always_inline)) {
-    const int t = quotient(i, p.by_heads);
-    int head = i - t * p.all_heads;
-    const int b = quotient(t0 + t, p.by_seq), s = t0 + t - b * p.seq;
-    const bool is_k = head >= p.heads;
-    if (is_k) head -= p.heads;
-    const HeadsParams& h = is_k ? p.k : p.q;
-    Head<T> r;
-    r.kind = h.weight != nullptr ? kNorm : kTurnOnly;
-    r.x = reinterpret_cast<const T*>(h.x) + b * h.x_batch + s * h.x_seq + head * h.x_head;
-    r.y = reinterpret_cast<T*>(h.out) + b * h.out_batch + s * h.out_seq + head * h.out_head;
-    r.weight = reinterpret_cast<const T*>(h.weight) + head * h.weight_head;
-    r.table = table + t * p.lanes.n;
-    return r;
-  });
+  auto all = [&](const HeadsParams& h, int heads, Divisor by) __attribute__((always_inline)) {
+    if (heads == 0) return;
+    auto head = [&](int i, Head<T>& r) __attribute__((always_inline)) {
+      const int t = quotient(i, by), head = i - t * heads;
+      const int b = quotient(t0 + t, p.by_seq), s = t0 + t - b * p.seq;
+      r.x = reinterpret_cast<const T*>(h.x) + b * h.x_batch + s * h.x_seq + head * h.x_head;
+      r.y = reinterpret_cast<T*>(h.out) + b * h.out_batch + s * h.out_seq + head * h.out_head;
+      r.table = table + t * p.lanes.n;
+    };
+    auto weight = [&](int i) { return reinterpret_cast<const T*>(h.weight) + (i - quotient(i, by) * heads) * h.weight_head; };
+    if (h.weight != nullptr)
+      heads_of_workgroup<T, VEC, INTERLEAVED, kNorm, kNormAhead>(p.lanes, tokens * heads, h.weight_head == 0, head, weight);
+    else
+      heads_of_workgroup<T, VEC, INTERLEAVED, kTurnOnly, kNormAhead>(p.lanes, tokens * heads, true, head, weight);
+  };
+  // (the arguments of the one operand and then of the other: of both at once there are more than scalar registers)
+  all(p.q, p.heads, p.by_heads);
+  const NormParams& q = arguments_anew<NormParams>();
+  all(q.k, q.kv_heads, q.by_kv_heads);
 }
 
 struct AppendNormParams {
@@ -270,17 +303,17 @@ struct AppendNormParams {
   void* q_out;
   const float* freqs;
   int64_t q_token, q_head, q_out_token, q_out_head, k_token, k_head, v_token, v_head, q_weight_head, k_weight_head, first_position;
-  int32_t heads, all_heads, first, per_wg;
+  int32_t heads, first, per_wg;
   float scale;
   Lanes lanes;
-  Divisor by_n, by_heads;
+  Divisor by_n, by_heads, by_kv_heads;
 };
 
 constexpr int kAppendNormAhead = 2;
 
 // One launch for a layer's new tokens, as append_kernel (rotary_api.hip)
 template <class T, int VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRotaryThreads) append_norm_kernel(const AppendNormParams p) {
+__global__ void __launch_bounds__(kRotaryThreads, norm_waves(VEC, INTERLEAVED)) append_norm_kernel(const AppendNormParams p) {
   __shared__ float2 table[kRotaryTable];
   __shared__ int64_t slot[kRotaryMaxTokens];  // among the sequence's own tokens
   __shared__ int32_t page[kRotaryMaxTokens];  // -1: nowhere to go
@@ -317,32 +350,39 @@ __global__ void __launch_bounds__(kRotaryThreads) append_norm_kernel(const Appen
     fill_rotary_table(table, p.freqs, p.lanes.n, p.by_n, tokens, p.scale, 1.0f, [&](int t) { return p.first_position + slot[t]; });
     __syncthreads();
   }
-  heads_of_workgroup<T, VEC, INTERLEAVED, kAppendNormAhead>(p.lanes, tokens * p.all_heads, [&](int i) __attribute__((always_inline)) {
-    const int t = quotient(i, p.by_heads);
-    int head = i - t * p.all_heads;
-    const int64_t row = t0 + t;
-    Head<T> r;
-    r.kind = kNothing;
+  auto all = [&](const T* weights, int64_t weight_head, int heads, Divisor by, auto&& head) __attribute__((always_inline)) {
+    if (heads == 0) return;
+    auto weight = [&](int i) { return weights + (i - quotient(i, by) * heads) * weight_head; };
+    if (weights != nullptr)
+      heads_of_workgroup<T, VEC, INTERLEAVED, kNorm, kAppendNormAhead>(p.lanes, tokens * heads, weight_head == 0, head, weight);
+    else
+      heads_of_workgroup<T, VEC, INTERLEAVED, kTurnOnly, kAppendNormAhead>(p.lanes, tokens * heads, true, head, weight);
+  };
+  all(reinterpret_cast<const T*>(p.q_weight), p.q_weight_head, p.heads, p.by_heads, [&](int i, Head<T>& r) __attribute__((always_inline)) {
+    const int t = quotient(i, p.by_heads), head = i - t * p.heads;
+    if (!live[t]) return;
+    r.x = reinterpret_cast<const T*>(p.q) + (int64_t)(t0 + t) * p.q_token + head * p.q_head;
+    r.y = reinterpret_cast<T*>(p.q_out) + (int64_t)(t0 + t) * p.q_out_token + head * p.q_out_head;
     r.table = table + t * p.lanes.n;
-    r.weight = nullptr;
-    if (head < p.heads) {
-      if (live[t]) r.kind = p.q_weight != nullptr ? kNorm : kTurnOnly;
-      r.x = reinterpret_cast<const T*>(p.q) + row * p.q_token + head * p.q_head;
-      r.y = reinterpret_cast<T*>(p.q_out) + row * p.q_out_token + head * p.q_out_head;
-      r.weight = reinterpret_cast<const T*>(p.q_weight) + head * p.q_weight_head;
-      return r;
-    }
-    head -= p.heads;
-    const bool is_v = head >= c.kv_heads;
-    if (is_v) head -= c.kv_heads;
-    const int64_t pg = page[t], within = in_page[t];
-    if (live[t] && pg >= 0) r.kind = is_v ? kCopy : (p.k_weight != nullptr ? kNorm : kTurnOnly);
-    r.x = is_v ? reinterpret_cast<const T*>(p.v) + row * p.v_token + head * p.v_head : reinterpret_cast<const T*>(p.k) + row * p.k_token + head * p.k_head;
-    r.y = is_v ? reinterpret_cast<T*>(c.v) + pg * c.v_page + within * c.v_slot + head * c.v_head
-               : reinterpret_cast<T*>(c.k) + pg * c.k_page + within * c.k_slot + head * c.k_head;
-    r.weight = reinterpret_cast<const T*>(p.k_weight) + head * p.k_weight_head;
-    return r;
   });
+  // (the arguments of the one operand and then of the other: of both at once there are more than scalar registers)
+  const AppendNormParams& p2 = arguments_anew<AppendNormParams>();
+  all(reinterpret_cast<const T*>(p2.k_weight), p2.k_weight_head, p2.cache.kv_heads, p2.by_kv_heads, [&](int i, Head<T>& r) __attribute__((always_inline)) {
+    const int t = quotient(i, p2.by_kv_heads), head = i - t * p2.cache.kv_heads;
+    if (!live[t] || page[t] < 0) return;
+    r.x = reinterpret_cast<const T*>(p2.k) + (int64_t)(t0 + t) * p2.k_token + head * p2.k_head;
+    r.y = reinterpret_cast<T*>(p2.cache.k) + page[t] * p2.cache.k_page + in_page[t] * p2.cache.k_slot + head * p2.cache.k_head;
+    r.table = table + t * p2.lanes.n;
+  });
+  const AppendNormParams& p3 = arguments_anew<AppendNormParams>();
+  auto value = [&](int i, Head<T>& r) __attribute__((always_inline)) {
+    const int t = quotient(i, p3.by_kv_heads), head = i - t * p3.cache.kv_heads;
+    if (!live[t] || page[t] < 0) return;
+    r.x = reinterpret_cast<const T*>(p3.v) + (int64_t)(t0 + t) * p3.v_token + head * p3.v_head;
+    r.y = reinterpret_cast<T*>(p3.cache.v) + page[t] * p3.cache.v_page + in_page[t] * p3.cache.v_slot + head * p3.cache.v_head;
+    r.table = table;
+  };
+  heads_of_workgroup<T, VEC, INTERLEAVED, kCopy, kAppendNormAhead>(p3.lanes, tokens * p3.cache.kv_heads, true, value, [](int) -> const T* { return nullptr; });
 }
 
 template <class P>
@@ -427,12 +467,13 @@ extern "C" int aitamd_qk_norm_rotary(int dtype, const aitamd_heads* q, const ait
   p.positions = positions, p.positions_64 = positions_64;
   p.freqs = freqs;
   p.pos_batch = pos_batch, p.pos_seq = pos_seq;
-  p.tokens = (int32_t)(batch * seq), p.heads = (int32_t)heads, p.all_heads = (int32_t)(heads + kv_heads), p.seq = (int32_t)seq;
+  p.tokens = (int32_t)(batch * seq), p.heads = (int32_t)heads, p.kv_heads = (int32_t)kv_heads, p.seq = (int32_t)seq;
   p.per_wg = rotary_tokens(batch * seq, (heads + kv_heads) * p.lanes.per_head, n, current_device_cus());
   p.scale = scale;
   p.by_n = make_divisor(n > 0 ? n : 1);
   p.by_seq = make_divisor(seq);
-  p.by_heads = make_divisor(heads + kv_heads);
+  p.by_heads = make_divisor(heads > 0 ? heads : 1);
+  p.by_kv_heads = make_divisor(kv_heads > 0 ? kv_heads : 1);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const hipError_t e = dtype == AITAMD_F16 ? launch_norm<f16>(p, vec, interleaved != 0, s) : launch_norm<bf16>(p, vec, interleaved != 0, s);
   if (e != hipSuccess) return fail("%s: launch failed: %s", who, hipGetErrorString(e));
@@ -468,14 +509,15 @@ extern "C" int aitamd_paged_kv_append_norm(int dtype, const aitamd_paged_cache* 
   p.q_weight_head = q_weight_head, p.k_weight_head = k_weight_head;
   p.q_out = q_out;
   p.freqs = freqs;
-  p.heads = (int32_t)heads, p.all_heads = (int32_t)(heads + 2 * kv_heads);
-  p.per_wg = rotary_tokens(tokens, p.all_heads * p.lanes.per_head, n, current_device_cus());
+  p.heads = (int32_t)heads;
+  p.per_wg = rotary_tokens(tokens, (heads + 2 * kv_heads) * p.lanes.per_head, n, current_device_cus());
   p.q_token = q_token, p.q_head = q_head, p.q_out_token = q_out_token, p.q_out_head = q_out_head;
   p.k_token = k_token, p.k_head = k_head, p.v_token = v_token, p.v_head = v_head;
   p.first_position = first_position;
   p.scale = scale;
   p.by_n = make_divisor(n > 0 ? n : 1);
-  p.by_heads = make_divisor(p.all_heads);
+  p.by_heads = make_divisor(heads > 0 ? heads : 1);
+  p.by_kv_heads = make_divisor(kv_heads > 0 ? kv_heads : 1);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const hipError_t e = dtype == AITAMD_F16 ? launch_append<f16>(p, vec, interleaved != 0, s) : launch_append<bf16>(p, vec, interleaved != 0, s);
   if (e != hipSuccess) return fail("%s: launch failed: %s", who, hipGetErrorString(e));
