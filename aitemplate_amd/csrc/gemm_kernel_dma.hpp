@@ -383,7 +383,11 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
     }
 
     // the adapters of the wave's rows, likewise (tiles whose registers are all taken read one step's operands at a time)
-    LoraTile<std::conditional_t<kLora, T, bf16>, MT, MI, NI, (MI + NI) * MT <= 128 && (Tile::OCC < 4 || MI * NI * ACC_N < 64) ? 2 : 1> lora;
+    constexpr int kLoraSteps = (MI + NI) * MT <= 128 && (Tile::OCC < 4 || MI * NI * ACC_N < 64) ? 2 : 1;
+    // adapters whose operands fit into the registers that the sums and the rows leave
+    constexpr int kLoraFree = 512 / Tile::OCC - MI * NI * ACC_N - kLoraSteps * MI * 4 - NI * ACC_N - 56;
+    constexpr int kLoraFit = kLoraFree / (kLoraSteps * NI * 4), kLoraAhead = kLoraFit < 1 ? 1 : (kLoraFit < 8 ? kLoraFit : 8);
+    LoraTile<std::conditional_t<kLora, T, bf16>, MT, MI, NI, kLoraSteps> lora;
     if constexpr (kLora) lora.read(p, m0 + wm * Tile::WTM, lane);
 
     // dword K tail: the up to three dwords behind the last whole 16-byte piece of each of the lane's operand rows,
@@ -620,52 +624,9 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
         mfmas(ta, tb);
       }
     }
-    // low-rank adapters: behind K; of waves with many, in the epilogue, or here through the wave's strip where they are all there is
-    constexpr int PITCH = Tile::EPI_PITCH;
-    constexpr int NG = ACC_N / 4;  // groups of 4 consecutive columns per lane per MFMA tile
-    float* strip = reinterpret_cast<float*>(smem_raw) + wave * MT * PITCH;
+    // low-rank adapters: behind K
     if constexpr (kLora) {
-      lora.count();
-      if (!lora.many && (splits == 1 || lora_alone))
-        lora.add(p, m0 + wm * Tile::WTM, n0 + wn * Tile::WTN, lane,
-                 [&](bf16x8 b, bf16x8 a, auto mi, auto ni) __attribute__((always_inline)) { acc[mi][ni] = MfmaOp<bf16, MT>::run(b, a, acc[mi][ni]); });
-    }
-    // the wave's rows of block mi in its strip, plus their adapters' (in a loop: of the epilogue there are as many copies as passes)
-    auto add_many = [&](int mi, bool from_zero) {
-#pragma unroll 1
-      for (int ps = 0; ps < PASSES; ++ps) {
-        const int row = ps * ROWS_PER_PASS + rd_row, m = epi_row(mi, ps);
-        if ((ACTIVE != 64 && lane >= ACTIVE) || row >= MT) continue;
-        float v[8];
-        float* const at = strip + row * PITCH + rd_col;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = from_zero ? 0.0f : at[j];
-        if constexpr (kLora) {
-          if (m < p.M && n_epi < p.N) lora_add<T, 8>(v, p, m, n_epi);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) at[j] = v[j];
-      }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    };
-    if constexpr (kLora && Tile::SPLITK != 0) {
-      if (lora_alone && lora.many) {
-#pragma unroll
-        for (int mi = 0; mi < MI; ++mi) {
-          add_many(mi, true);
-#pragma unroll
-          for (int ni = 0; ni < NI; ++ni)
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-              const f32x4 v = *reinterpret_cast<const f32x4*>(strip + fr * PITCH + ni * MT + g * (QN * 4) + fq * 4);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[mi][ni][g * 4 + j] = v[j];
-            }
-        }
-        __syncthreads();  // (the strips share LDS with the exchange's broadcast word)
-      }
+      if (splits == 1 || lora_alone) lora.template add_own<kLoraAhead>(p, m0 + wm * Tile::WTM, n0 + wn * Tile::WTN, lane, acc);
     }
 
     if constexpr (Tile::SPLITK != 0) {
@@ -761,6 +722,10 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
 
     float one = 1.0f;
     asm volatile("" : "+s"(one));  // (opaque to the optimizer: see to_float_plus)
+    constexpr int PITCH = Tile::EPI_PITCH;
+    float* strip = reinterpret_cast<float*>(smem_raw) + wave * MT * PITCH;
+    constexpr int NG = ACC_N / 4;  // groups of 4 consecutive columns per lane per MFMA tile
+
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) {
       // this wave's MT x WTN strip, row-major fp32
@@ -777,9 +742,6 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-      if constexpr (kLora) {
-        if (lora.many && splits == 1) add_many(mi, false);
-      }
 #pragma unroll
       for (int ps = 0; ps < PASSES; ++ps) {
         const int row = ps * ROWS_PER_PASS + rd_row;

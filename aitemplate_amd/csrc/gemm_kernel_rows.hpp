@@ -246,9 +246,7 @@ __global__ void __launch_bounds__(Tile::NT) gemm_rcr_rows_kernel(const GemmParam
       }
       if constexpr (kScaled) v = scaled_sum(v, scale_v[o]);
       if constexpr (IsLora<Epi>::value) {
-        float sum[1] = {v};
-        lora_add<T, 1>(sum, p, m0 + m, n0 + out_n);
-        v = sum[0];
+        v = lora_add<T>(v, p, m0 + m, n0 + out_n);
       }
       Cb[out_index<PERM>(p, m0 + m, n0 + out_n)] = epilogue1<Epi, Out>(v, bias_v[o], d0_v[o], d1_v[o], one);
     }

@@ -8,8 +8,8 @@
 // multiplied with both; a half is the sum of two bfloat16 numbers too (8 of its 11 bits and the 3 behind them), so that halves are
 // four products: exact, all of them.
 //
-// Per wave: the adapters of its rows one after the other, each with the rows of the others set to zero, on matrix instructions; with
-// more than kLoraFew of them every output by itself, from its row's own adapter.
+// Per wave: the adapters of its rows one after the other, on matrix instructions, for all its rows at once; each row takes the
+// products with its own.
 #pragma once
 
 #include <type_traits>
@@ -19,8 +19,6 @@
 #include "gemm_kernel.hpp"
 
 namespace aitamd {
-
-constexpr int kLoraFew = 4;
 
 // a row's elements in scratch memory: chunks of eight ranks, two parts each
 constexpr int lora_chunks(int rank) { return (rank + 7) / 8; }
@@ -73,9 +71,11 @@ AITAMD_DEVICE u32x4 lora_largest(u32x4 v) {
 // The part of a wave whose rows row0 + mi * MT + (lane % MT) meet columns col0 + ni * MT + (lane % MT).  STEPS: matrix instructions' worth of ranks whose operands are on their way together.
 template <class T, int MT, int MI, int NI, int STEPS>
 struct LoraTile {
-  static constexpr int QN = 64 / MT;
+  // 16 x 16: a step's four quarters are both parts of t of two chunks (halves: both by both of one); 32 x 32: its two
+  // halves are both parts of t of one chunk (halves: once with each of the adapter's)
+  static constexpr bool kHalves = !std::is_same_v<T, bf16>;
+  static constexpr int PER = MT == 16 && !kHalves ? 2 : 1;
   int of[MI];
-  bool many;
 
   AITAMD_DEVICE void read(const GemmParams& p, int row0, int lane) {
 #pragma unroll
@@ -91,18 +91,101 @@ struct LoraTile {
     });
     return id;
   }
-  AITAMD_DEVICE void count() {
-    int left[MI], n = 0;
+  // the operands w of chunks c0 on, without what lies behind the last rank: the next column's first.  An odd rank shares its dword
+  // with that (with the buffer's end, which takes whole dwords), and is read again by itself.
+  static AITAMD_DEVICE void last_ranks(int rank, int c0, int half, __amdgpu_buffer_rsrc_t rb, uint32_t b_at, u32x4 (&w)[STEPS][NI]) {
+    if (8 * (c0 + STEPS * PER) <= rank) return;
+    const uint32_t b_pitch = (uint32_t)rank * 2u;
+    static_for<0, STEPS>([&](auto s_c) __attribute__((always_inline)) {
+      const int c = c0 + decltype(s_c)::value * PER + half, dwords = rank / 2 - 4 * c;
+      static_for<0, NI>([&](auto ni) __attribute__((always_inline)) {
+        const uint32_t at = b_at + (uint32_t)(decltype(ni)::value * MT) * b_pitch + (uint32_t)((rank - 1) * 2 - half * 16);
+        const uint32_t last =
+            (rank & 1) != 0 && 8 * c < rank ? (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rb, at, 0, 0) : 0u;
 #pragma unroll
-    for (int mi = 0; mi < MI; ++mi) left[mi] = of[mi];
-    for (;;) {
-      const int id = first_of(left);
-      if (id < 0 || ++n > kLoraFew) break;
-#pragma unroll
-      for (int mi = 0; mi < MI; ++mi) left[mi] = left[mi] == id ? -1 : left[mi];
-    }
-    many = n > kLoraFew;
+        for (int d = 0; d < 4; ++d) w[decltype(s_c)::value][ni][d] = d < dwords ? w[decltype(s_c)::value][ni][d] : (d == dwords ? last : 0u);
+      });
+    });
   }
+  // The products of every row with each adapter, of which a row takes those with its own: acc[mi][ni], whose elements are all of row
+  // lane % MT of block mi.  AHEAD adapters' operands are on their way together: where each row has its own, the time is that of the
+  // trips to memory.
+  template <int AHEAD, class Acc>
+  AITAMD_DEVICE void add_own(const GemmParams& p, int row0, int col0, int lane, Acc (&acc)[MI][NI]) const {
+    using Op = MfmaOp<bf16, MT>;
+    const int fr = lane % MT, fq = lane / MT;
+    const int rank = p.lora_rank, chunks = lora_chunks(rank);
+    const int rows = p.M - row0 < MI * MT ? p.M - row0 : MI * MT, columns = p.N - col0 < NI * MT ? p.N - col0 : NI * MT;
+    if (rows <= 0 || columns <= 0) return;
+    const uint32_t t_pitch = (uint32_t)chunks * 32u, b_pitch = (uint32_t)rank * 2u;
+    const __amdgpu_buffer_rsrc_t rt = make_rsrc(lora_row(p, row0), (uint32_t)rows * t_pitch);
+    const int half = PER == 2 ? fq & 1 : 0;
+    const int part = MT == 32 ? fq : (PER == 2 ? fq >> 1 : fq & 1);
+    uint32_t t_at = (uint32_t)fr * t_pitch + (uint32_t)(half * 32 + part * 16), b_at = (uint32_t)fr * b_pitch + (uint32_t)(half * 16);
+    // (opaque: what hangs on the tile alone would be computed ahead of the K loop, held over it and spilled)
+    asm volatile("" : "+v"(t_at), "+v"(b_at));
+    int left[MI];
+#pragma unroll 1
+    for (int c0 = 0; c0 < chunks; c0 += STEPS * PER) {
+      u32x4 t[STEPS][MI];
+      static_for<0, MI>([&](auto mi) __attribute__((always_inline)) {
+        left[mi] = of[mi];
+        static_for<0, STEPS>([&](auto s) __attribute__((always_inline)) {
+          const uint32_t tc = t_at + (uint32_t)(c0 + s * PER) * 32u + (uint32_t)(decltype(mi)::value * MT) * t_pitch;
+          t[s][mi] = buffer_load_16B(rt, c0 + s * PER + half < chunks ? tc : kOobOffset);
+        });
+      });
+      for (;;) {
+        int id[AHEAD];
+        u32x4 w[AHEAD][STEPS][NI];
+        static_for<0, AHEAD>([&](auto i) __attribute__((always_inline)) {
+          id[i] = first_of(left);
+          if (id[i] < 0) return;
+          static_for<0, MI>([&](auto mi) __attribute__((always_inline)) { left[mi] = left[mi] == id[i] ? -1 : left[mi]; });
+          const __amdgpu_buffer_rsrc_t rb = make_rsrc(lora_column<T>(p, id[i], col0), (uint32_t)columns * b_pitch);
+          static_for<0, STEPS>([&](auto s) __attribute__((always_inline)) {
+            const uint32_t bc = b_at + (uint32_t)(c0 + s * PER) * 16u;
+            static_for<0, NI>([&](auto ni) __attribute__((always_inline)) {
+              w[i][s][ni] = buffer_load_16B(rb, c0 + s * PER + half < chunks ? bc + (uint32_t)(decltype(ni)::value * MT) * b_pitch : kOobOffset);
+            });
+          });
+        });
+        static_for<0, AHEAD>([&](auto i) __attribute__((always_inline)) {
+          if (id[i] < 0) return;
+          if (8 * (c0 + STEPS * PER) > rank) {
+            const __amdgpu_buffer_rsrc_t rb = make_rsrc(lora_column<T>(p, id[i], col0), (uint32_t)columns * b_pitch);
+            last_ranks(rank, c0, half, rb, b_at, w[i]);
+          }
+          bf16x8 two[STEPS][NI];
+          if constexpr (kHalves) {
+            static_for<0, STEPS>([&](auto s) __attribute__((always_inline)) {
+              static_for<0, NI>([&](auto ni) __attribute__((always_inline)) {
+                bf16x8 one;
+                lora_parts<T>(__builtin_bit_cast(typename ElemTraits<T>::vec8, w[i][s][ni]), one, two[s][ni]);
+                w[i][s][ni] = __builtin_bit_cast(u32x4, MT == 16 && (fq >> 1) ? two[s][ni] : one);
+              });
+            });
+          }
+          static_for<0, MI>([&](auto mi) __attribute__((always_inline)) {
+            const bool own = of[mi] == id[i];
+            if (__builtin_amdgcn_ballot_w64(own) == 0) return;
+            static_for<0, NI>([&](auto ni) __attribute__((always_inline)) {
+              Acc sum{};
+              static_for<0, STEPS>([&](auto s) __attribute__((always_inline)) {
+                const bf16x8 a = __builtin_bit_cast(bf16x8, t[s][mi]);
+                sum = Op::run(__builtin_bit_cast(bf16x8, w[i][s][ni]), a, sum);
+                if constexpr (kHalves && MT == 32) sum = Op::run(two[s][ni], a, sum);
+              });
+#pragma unroll
+              for (int e = 0; e < (int)(sizeof(Acc) / 4); ++e) acc[mi][ni][e] += own ? sum[e] : 0.0f;
+            });
+          });
+        });
+        if (id[AHEAD - 1] < 0) break;
+      }
+    }
+  }
+  // ... for accumulators that matrix instructions alone may touch: each adapter with the rows of the others set to zero.
   // multiply(b, a, mi, ni): accumulator (mi, ni) plus the product of the weight rows b and the rows a, both bf16x8.  Through
   // buffers that end with the rows and the columns: 32-bit offsets, and no branch around what is not there.
   template <class M>
@@ -113,10 +196,6 @@ struct LoraTile {
     if (rows <= 0 || columns <= 0) return;
     const uint32_t t_pitch = (uint32_t)chunks * 32u, b_pitch = (uint32_t)rank * 2u;
     const __amdgpu_buffer_rsrc_t rt = make_rsrc(lora_row(p, row0), (uint32_t)rows * t_pitch);
-    // 16 x 16: a step's four quarters are both parts of t of two chunks (halves: both by both of one); 32 x 32: its two
-    // halves are both parts of t of one chunk (halves: once with each of the adapter's)
-    constexpr bool kHalves = !std::is_same_v<T, bf16>;
-    constexpr int PER = MT == 16 && !kHalves ? 2 : 1;
     const int half = PER == 2 ? fq & 1 : 0;
     const int part = MT == 32 ? fq : (PER == 2 ? fq >> 1 : fq & 1);
     uint32_t t_at = (uint32_t)fr * t_pitch + (uint32_t)(half * 32 + part * 16), b_at = (uint32_t)fr * b_pitch + (uint32_t)(half * 16);
@@ -152,20 +231,7 @@ struct LoraTile {
               t[s][mi] = buffer_load_16B(rt, on && left[mi] == id ? tc + (uint32_t)(decltype(mi)::value * MT) * t_pitch : kOobOffset);
             });
           });
-          if (8 * (c0 + STEPS * PER) > rank) {
-            // behind the last rank is the next column's first; an odd one shares its dword with that (with the buffer's end, which
-            // takes whole dwords), and is read again by itself
-            static_for<0, STEPS>([&](auto s_c) __attribute__((always_inline)) {
-              const int c = c0 + decltype(s_c)::value * PER + half, dwords = rank / 2 - 4 * c;
-              static_for<0, NI>([&](auto ni) __attribute__((always_inline)) {
-                const uint32_t at = b_at + (uint32_t)(decltype(ni)::value * MT) * b_pitch + (uint32_t)((rank - 1) * 2 - half * 16);
-                const uint32_t last =
-                    (rank & 1) != 0 && c < chunks ? (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rb, at, 0, 0) : 0u;
-#pragma unroll
-                for (int d = 0; d < 4; ++d) w[decltype(s_c)::value][ni][d] = d < dwords ? w[decltype(s_c)::value][ni][d] : (d == dwords ? last : 0u);
-              });
-            });
-          }
+          last_ranks(rank, c0, half, rb, b_at, w);
           bf16x8 two[STEPS][NI];
           if constexpr (kHalves) {
             static_for<0, STEPS>([&](auto s) __attribute__((always_inline)) {
@@ -220,36 +286,26 @@ AITAMD_DEVICE void lora_sum(const bf16* t, int c, float (&f)[8]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) f[j] = (float)one[j] + (float)two[j];
 }
-// Columns n .. n + COLS - 1 of row m by themselves (those from N on may be anything)
-template <class T, int COLS>
-AITAMD_DEVICE void lora_add(float (&v)[COLS], const GemmParams& p, int m, int n) {
+// column n of row m by itself: the sum v and its adapter's
+template <class T>
+AITAMD_DEVICE float lora_add(float v, const GemmParams& p, int m, int n) {
   using Tr = ElemTraits<T>;
   const int id = lora_adapter(p, m);
-  if (id < 0) return;
-  const int rank = p.lora_rank, chunks = lora_chunks(rank);
-  const bf16* t = lora_row(p, m);
-  const T* row[COLS];
-#pragma unroll
-  for (int j = 0; j < COLS; ++j) row[j] = lora_column<T>(p, id, n + j < p.N ? n + j : n);
-  const int whole = rank / 8;
-#pragma unroll 1
+  if (id < 0) return v;
+  const int rank = p.lora_rank, whole = rank / 8;
+  const bf16* const t = lora_row(p, m);
+  const T* const row = lora_column<T>(p, id, n);
+  float f[8];
   for (int c = 0; c < whole; ++c) {
-    float f[8];
+    const auto w = load_vec<typename Tr::vec8>(row + c * 8);
     lora_sum(t, c, f);
-    typename Tr::vec8 w[COLS];
 #pragma unroll
-    for (int j = 0; j < COLS; ++j) w[j] = load_vec<typename Tr::vec8>(row[j] + c * 8);
-#pragma unroll
-    for (int j = 0; j < COLS; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[j] = __builtin_fmaf(f[e], Tr::to_float(w[j][e]), v[j]);
+    for (int e = 0; e < 8; ++e) v = __builtin_fmaf(f[e], Tr::to_float(w[e]), v);
   }
 #pragma unroll 1
-  for (int e = whole * 8; e < rank; ++e) {
-    const float f = (float)t[whole * 16 + e % 8] + (float)t[whole * 16 + 8 + e % 8];
-#pragma unroll
-    for (int j = 0; j < COLS; ++j) v[j] = __builtin_fmaf(f, Tr::to_float(row[j][e]), v[j]);
-  }
+  for (int e = whole * 8; e < rank; ++e)
+    v = __builtin_fmaf((float)t[whole * 16 + e % 8] + (float)t[whole * 16 + 8 + e % 8], Tr::to_float(row[e]), v);
+  return v;
 }
 
 }  // namespace aitamd

@@ -53,69 +53,99 @@ AITAMD_DEVICE float wave_sum(float v) {
   for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
   return v;
 }
-// x . a over K, by a wave
+// x . a[e] over K, by a wave
 template <class T>
-AITAMD_DEVICE float wave_dot(const T* x, const T* a, int K, int lane) {
+AITAMD_DEVICE void wave_dots(const T* x, const T* const (&a)[4], int K, int lane, float (&v)[4]) {
   using vec8 = typename ElemTraits<T>::vec8;
-  constexpr int AHEAD = 4;
-  float s[AHEAD] = {};
+  constexpr int AHEAD = 2;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = 0.0f;
   int k = lane * 8;
   for (; k + (AHEAD - 1) * 512 + 8 <= K; k += AHEAD * 512) {
-    vec8 xv[AHEAD], av[AHEAD];
+    vec8 xv[AHEAD], av[AHEAD][4];
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) xv[i] = load_vec<vec8>(x + k + i * 512), av[i] = load_vec<vec8>(a + k + i * 512);
+    for (int i = 0; i < AHEAD; ++i) {
+      xv[i] = load_vec<vec8>(x + k + i * 512);
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) s[i] = dot8<T>(xv[i], av[i], s[i]);
+      for (int e = 0; e < 4; ++e) av[i][e] = load_vec<vec8>(a[e] + k + i * 512);
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = dot8<T>(xv[i], av[i][e], v[e]);
   }
-  for (; k + 8 <= K; k += 512) s[0] = dot8<T>(load_vec<vec8>(x + k), load_vec<vec8>(a + k), s[0]);
-  for (int e = k; e < K && e < k + 8; ++e) s[1] = __builtin_fmaf(ElemTraits<T>::to_float(x[e]), ElemTraits<T>::to_float(a[e]), s[1]);
-  return wave_sum((s[0] + s[1]) + (s[2] + s[3]));
+  for (; k < K; k += 512) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (k + 8 <= K) {
+        v[e] = dot8<T>(load_vec<vec8>(x + k), load_vec<vec8>(a[e] + k), v[e]);
+      } else {
+        for (int i = k; i < K; ++i) v[e] = __builtin_fmaf(ElemTraits<T>::to_float(x[i]), ElemTraits<T>::to_float(a[e][i]), v[e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = wave_sum(v[e]);
 }
 
 constexpr int kRowThreads = 256;
-// Few rows, which may all have adapters of their own: a wave for a rank of a row.  Bound: the latency of two trips to memory
-// (the row and its adapter's number, then the adapter; up to 4096 of K at once).
-template <class T>
+// Few rows, which may all have adapters of their own: a wave for RANKS ranks of a row.  Bound: the latency of two trips to memory
+// (the row and its adapter's number, then the adapter; AHEAD x 512 of K at once).
+template <class T, int RANKS>
 __global__ void __launch_bounds__(kRowThreads) low_rows_kernel(const LowParams p) {
   using vec8 = typename ElemTraits<T>::vec8;
   constexpr int AHEAD = 8;
   const int lane = threadIdx.x & 63, m = p.first + blockIdx.x;
   const int padded = lora_chunks(p.rank) * 8;
-  const int j = blockIdx.y * (kRowThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int j0 = (blockIdx.y * (kRowThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * RANKS;
   const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)m * p.ldx;
-  // whole pieces of the first trip; what there is no whole piece for is left to wave_dot
-  vec8 xv[AHEAD], av[AHEAD];
-#pragma unroll
-  for (int i = 0; i < AHEAD; ++i) {
-    xv[i] = vec8{};
-    if (i * 512 + lane * 8 + 8 <= p.K) xv[i] = load_vec<vec8>(x + i * 512 + lane * 8);
-  }
-  const int id = __builtin_amdgcn_readfirstlane(adapter_of(p, m));
-  clear_counters(p, kRowThreads);
-  if (j >= padded) return;
-  float v = 0.0f;
-  if (id >= 0 && j < p.rank) {
-    const T* a = reinterpret_cast<const T*>(p.a) + ((int64_t)id * p.rank + j) * p.K;
-    const float scale = p.scales != nullptr ? p.scales[id] : 1.0f;
+  // whole pieces from k on
+  auto load = [&](vec8 (&v)[AHEAD], const T* row, int k) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      av[i] = vec8{};
-      if (i * 512 + lane * 8 + 8 <= p.K) av[i] = load_vec<vec8>(a + i * 512 + lane * 8);
+      v[i] = vec8{};
+      if (k + i * 512 + lane * 8 + 8 <= p.K) v[i] = load_vec<vec8>(row + k + i * 512 + lane * 8);
     }
-    float s[2] = {};
+  };
+  vec8 xv[AHEAD], av[RANKS][AHEAD];
+  load(xv, x, 0);
+  const int id = __builtin_amdgcn_readfirstlane(adapter_of(p, m));
+  clear_counters(p, kRowThreads);
+  if (j0 >= padded) return;
+  float v[RANKS] = {};
+  if (id >= 0) {
+    const T* a[RANKS];
+    const float scale = p.scales != nullptr ? p.scales[id] : 1.0f;
+    // (ranks from p.rank on: of the last one, and zeros)
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) s[i & 1] = dot8<T>(xv[i], av[i], s[i & 1]);
-    // behind them: the rest of a piece, more pieces
-    const int k = p.K < AHEAD * 512 ? p.K & ~7 : AHEAD * 512;
-    v = wave_sum(s[0] + s[1]);
-    if (k < p.K) v += wave_dot(x + k, a + k, p.K - k, lane);
-    v *= scale;
+    for (int r = 0; r < RANKS; ++r) a[r] = reinterpret_cast<const T*>(p.a) + ((int64_t)id * p.rank + (j0 + r < p.rank ? j0 + r : p.rank - 1)) * p.K;
+    for (int k = 0;;) {
+#pragma unroll
+      for (int r = 0; r < RANKS; ++r) load(av[r], a[r], k);
+#pragma unroll
+      for (int r = 0; r < RANKS; ++r)
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+          if (RANKS == 1 || k + i * 512 < p.K) v[r] = dot8<T>(xv[i], av[r][i], v[r]);
+      k += AHEAD * 512;
+      if (k >= p.K) break;
+      load(xv, x, k);
+    }
+    const int whole = p.K & ~7;
+#pragma unroll
+    for (int r = 0; r < RANKS; ++r) {
+      if (whole + lane < p.K) v[r] = __builtin_fmaf(ElemTraits<T>::to_float(x[whole + lane]), ElemTraits<T>::to_float(a[r][whole + lane]), v[r]);
+      v[r] = j0 + r < p.rank ? wave_sum(v[r]) * scale : 0.0f;
+    }
   }
-  if (lane == 0) put_low(p.t + (int64_t)m * padded * 2, j, v);
+#pragma unroll
+  for (int r = 0; r < RANKS; ++r)
+    if (lane == r) put_low(p.t + (int64_t)m * padded * 2, j0 + r, v[r]);
 }
 
 // Rows of prompts, neighbours of one adapter mostly: ROWS of them and NR x 16 ranks a workgroup.  Several adapters among the rows: one
 // after the other; more than kLoraFew: row by row.
+constexpr int kLoraFew = 4;
 struct LowTile {
   int mine, left, distinct;  // the lane's row's adapter, that or -1, how many there are among the rows
   AITAMD_DEVICE int first() const {
@@ -148,15 +178,21 @@ AITAMD_DEVICE bool low_begin(const LowParams& p, LowTile& l, int* of, int m0, in
     }
   }
   if (l.distinct <= kLoraFew) return l.distinct > 0;
-  for (int i = wave; i < rows * ranks; i += THREADS / 64) {
-    const int r = i / ranks, j = j0 + i - r * ranks;
+  // four ranks of a row at a time (those from p.rank on: of the last one, and zeros)
+  for (int i = wave; i < rows * (ranks / 4); i += THREADS / 64) {
+    const int r = i / (ranks / 4), j = j0 + (i - r * (ranks / 4)) * 4;
     const int id = __builtin_amdgcn_readlane(l.mine, r);
     if (id < 0) continue;
-    float v = 0.0f;
-    if (j < p.rank)
-      v = wave_dot(reinterpret_cast<const T*>(p.x) + (int64_t)(m0 + r) * p.ldx, reinterpret_cast<const T*>(p.a) + ((int64_t)id * p.rank + j) * p.K, p.K, lane) *
-          (p.scales != nullptr ? p.scales[id] : 1.0f);
-    if (lane == 0) put_low(p.t + (int64_t)(m0 + r) * padded * 2, j, v);
+    const T* a = reinterpret_cast<const T*>(p.a) + (int64_t)id * p.rank * p.K;
+    const T* row[4];
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) row[e] = a + (int64_t)(j + e < p.rank ? j + e : p.rank - 1) * p.K;
+    wave_dots(reinterpret_cast<const T*>(p.x) + (int64_t)(m0 + r) * p.ldx, row, p.K, lane, v);
+    const float scale = p.scales != nullptr ? p.scales[id] : 1.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (lane == e) put_low(p.t + (int64_t)(m0 + r) * padded * 2, j + e, j + e < p.rank ? v[e] * scale : 0.0f);
   }
   return false;
 }
@@ -406,11 +442,15 @@ hipError_t launch_ring(const LowParams& p, int64_t groups, int cus, hipStream_t 
 template <class T>
 hipError_t launch_low(LowParams p, hipStream_t stream) {
   const int padded = lora_chunks(p.rank) * 8;
-  // A row by itself reads its adapter alone, from the caches where others have read it; a tile reads x once and an adapter once
-  // for 32 rows.
-  constexpr int kFewRows = 256;
-  if (p.M <= kFewRows) {
-    hipLaunchKernelGGL(low_rows_kernel<T>, dim3(p.M, (padded + kRowThreads / 64 - 1) / (kRowThreads / 64)), dim3(kRowThreads), 0, stream, p);
+  // A row by itself reads its whole adapter, from L2 mostly; a tile reads x once and an adapter once for its rows, and takes them one
+  // by one where they have many adapters.  By themselves up to twice the waves that the chip holds at once, two ranks each then.  Of
+  // rank 16, K = 4096, with one adapter / sixteen requests' rows in turn / 48 adapters at random: 1024 rows 15, 16 and 16 us by
+  // themselves, 9, 15 and 170 in tiles; 2048 rows 25, 25 and 24 by themselves, a tile's 9 to 16 with the first two.
+  const int64_t waves = (int64_t)p.M * padded;
+  constexpr int64_t kAtOnce = 8192;
+  if (waves <= 2 * kAtOnce) {
+    const int ranks = waves <= kAtOnce ? 1 : 2, per = kRowThreads / 64 * ranks;
+    hipLaunchKernelGGL((ranks == 1 ? low_rows_kernel<T, 1> : low_rows_kernel<T, 2>), dim3(p.M, (padded + per - 1) / per), dim3(kRowThreads), 0, stream, p);
     return hipGetLastError();
   }
   const int nr = padded > 32 ? 4 : (padded > 16 ? 2 : 1);
