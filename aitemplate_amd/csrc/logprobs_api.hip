@@ -436,10 +436,11 @@ __global__ void __launch_bounds__(kJoinThreads) logprob_join_kernel(const Logpro
   if (tid < 64) finish<T>(p, row, all.m, all.s, all.u, all.ahead, best);
 }
 
-// Workgroups of a row: as many as fill the chip with two each, of a round at least
+// Workgroups of a row: as many as fill the chip with two each, of a round at least; one where its rounds cost no more than the second
+// launch (1 x 32000 fp32, four rounds: 11.3 us by one, 7.6 and 4.4 by four and the join; another round is one more)
 int logprob_splits(int64_t rows, int64_t V, int cus) {
   const int64_t rounds = (V + kRound - 1) / kRound;
-  int64_t s = rows > 0 ? 2ll * cus / rows : 1;
+  int64_t s = rows > 0 && rounds > 4 ? 2ll * cus / rows : 1;
   if (s > rounds) s = rounds;
   if (s > kMostSplits) s = kMostSplits;
   return (int)(s < 1 ? 1 : s);
