@@ -5,7 +5,8 @@
 // lanes for a head, up to the wave; of longer heads several each), which sum their squares among themselves and go on with
 // what they have in registers.  A workgroup goes through its tokens' queries, then their keys (and values), so that a lane's weights
 // are read once for all heads.
-// Bound: memory, 4 bytes an element, as the rotation alone; registers for eight waves a SIMD.
+// Bound: memory, 4 bytes an element, as the rotation alone.  16384 x 20 x 256 in fp16, 335 MB: 69 us with half of each head turned
+// (neighbours; 72 halves), 4.9 TB/s, a copy's rate; with all of it turned 82, of which the sines are some 10.  16384 x 40 x 128 in bf16 71.
 #include "../../include/aitemplate_amd_kernels.h"
 #include "device.hpp"
 #include "errors.hpp"
@@ -15,32 +16,37 @@
 namespace aitamd {
 namespace {
 
-// One piece of a head (see RotaryPiece): elements i1 .. and, of pairs of halves, i2 ..
+// What a lane handles of a head at once: two vectors of VEC elements, whichever of them are turned and with whichever partners, so that
+// a lane's work is the same (with one vector where neighbours are paired or none are, 16384 x 20 x 256 in fp16, half of it turned: 85 us,
+// halves paired 120).  Pairs of halves: i1 .. and its partners i2 ..; pairs of neighbours, and what is not turned: neighbouring vectors,
+// of which a head's last may be without a second.  VEC = 1: a pair, or two elements.
 template <class T, int VEC, bool INTERLEAVED>
 struct NormPiece {
   using Tr = ElemTraits<T>;
   using vec = typename RotaryVec<T, VEC>::type;
-  static constexpr bool kTwo = !INTERLEAVED || VEC == 1;  // (VEC = 1: neighbours are two elements of their own)
-  int i1, i2, pair;                                       // pair: the first of the piece's, -1 behind the rotated dims
+  static constexpr bool kPartners = !INTERLEAVED || VEC == 1;  // the second vector's are the first one's partners
+  int i1, i2;       // i2 < 0: none
+  int pair, pair2;  // the first pair of each (kPartners: of both), -1 behind the rotated dims
   vec v1, v2;
 
-  AITAMD_DEVICE void place(int c, int n) {
-    const int turned = VEC == 1 ? n : (INTERLEAVED ? 2 * n / VEC : n / VEC);
-    if (c >= turned) {
-      i1 = i2 = 2 * n + (c - turned) * VEC;
-      pair = -1;
+  AITAMD_DEVICE void place(int c, int n, int dim) {
+    if constexpr (kPartners) {
+      const int turned = n / VEC;
+      pair = pair2 = c < turned ? c * VEC : -1;
+      i1 = c < turned ? (INTERLEAVED ? 2 * c : c * VEC) : 2 * n + (c - turned) * 2 * VEC;
+      i2 = c < turned && !INTERLEAVED ? n + i1 : i1 + VEC;
     } else {
-      i1 = INTERLEAVED && VEC == 1 ? 2 * c : c * VEC;
-      i2 = INTERLEAVED ? i1 + 1 : n + i1;
-      pair = INTERLEAVED && VEC > 1 ? c * (VEC / 2) : c * VEC;
+      i1 = c * 2 * VEC;
+      i2 = i1 + VEC;
+      pair = i1 < 2 * n ? i1 / 2 : -1;
+      pair2 = i2 < 2 * n ? i2 / 2 : -1;
     }
+    if (i2 >= dim) i2 = -1;
   }
   AITAMD_DEVICE void load(const T* x) {
     v1 = load_vec<vec>(x + i1);
     v2 = vec{};
-    if constexpr (kTwo) {
-      if (pair >= 0) v2 = load_vec<vec>(x + i2);
-    }
+    if (i2 >= 0) v2 = load_vec<vec>(x + i2);
   }
   // the sum of squares, in 32 or 64 bits
   template <class S>
@@ -48,67 +54,80 @@ struct NormPiece {
     S s = 0;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      const S a = (S)Tr::to_float(v1[j]);
+      const S a = (S)Tr::to_float(v1[j]), b = (S)Tr::to_float(v2[j]);
       s += a * a;
-      if constexpr (kTwo) {
-        const S b = (S)Tr::to_float(v2[j]);
-        s += b * b;
-      }
+      s += b * b;
     }
     return s;
   }
   // as it is
   AITAMD_DEVICE void copy(T* y) const {
     store_vec(y + i1, v1);
-    if constexpr (kTwo) {
-      if (pair >= 0) store_vec(y + i2, v2);
-    }
+    if (i2 >= 0) store_vec(y + i2, v2);
   }
   // the weights of the same elements
   AITAMD_DEVICE void weigh(const T* weight, vec& w1, vec& w2) const {
     w1 = w2 = load_vec<vec>(weight + i1);
-    if constexpr (kTwo) {
-      if (pair >= 0) w2 = load_vec<vec>(weight + i2);
-    }
+    if (i2 >= 0) w2 = load_vec<vec>(weight + i2);
   }
   // times ra, times rb and the weights (NORM), turned
   template <bool NORM>
   AITAMD_DEVICE void store(T* y, vec w1, vec w2, float ra, float rb, const float2* table) const {
-    float a[VEC], b[VEC];
+    auto times = [&](vec v, vec w, float (&f)[VEC]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      a[j] = Tr::to_float(v1[j]);
-      b[j] = Tr::to_float(v2[j]);
-      if constexpr (NORM) {
-        a[j] = a[j] * ra * (rb * Tr::to_float(w1[j]));
-        if constexpr (kTwo) b[j] = b[j] * ra * (rb * Tr::to_float(w2[j]));
+      for (int j = 0; j < VEC; ++j) {
+        f[j] = Tr::to_float(v[j]);
+        if constexpr (NORM) f[j] = f[j] * ra * (rb * Tr::to_float(w[j]));
       }
-    }
-    vec o1, o2;
-    if (pair >= 0) {
-      if constexpr (kTwo) {
+    };
+    if constexpr (kPartners) {
+      float a[VEC], b[VEC];
+      vec o1, o2;
+      times(v1, w1, a);
+      times(v2, w2, b);
+      if (pair >= 0) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const float2 t = table[pair + j];
-          o1[j] = Tr::from_float(a[j] * t.x - b[j] * t.y);
-          o2[j] = Tr::from_float(b[j] * t.x + a[j] * t.y);
-        }
-        store_vec(y + i2, o2);
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC / 2; ++j) {
-          const float2 t = table[pair + j];
-          o1[2 * j] = Tr::from_float(a[2 * j] * t.x - a[2 * j + 1] * t.y);
-          o1[2 * j + 1] = Tr::from_float(a[2 * j + 1] * t.x + a[2 * j] * t.y);
+          const float turned = a[j] * t.x - b[j] * t.y;
+          b[j] = b[j] * t.x + a[j] * t.y;
+          a[j] = turned;
         }
       }
-    } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) o1[j] = Tr::from_float(a[j]);
+      for (int j = 0; j < VEC; ++j) {
+        o1[j] = Tr::from_float(a[j]);
+        o2[j] = Tr::from_float(b[j]);
+      }
+      store_vec(y + i1, o1);
+      if (i2 >= 0) store_vec(y + i2, o2);
+    } else {
+      auto put = [&](vec v, vec w, int at, int of) __attribute__((always_inline)) {
+        float a[VEC];
+        vec o;
+        times(v, w, a);
+        if (of >= 0) {
+#pragma unroll
+          for (int j = 0; j < VEC; j += 2) {
+            const float2 t = table[of + j / 2];
+            const float turned = a[j] * t.x - a[j + 1] * t.y;
+            a[j + 1] = a[j + 1] * t.x + a[j] * t.y;
+            a[j] = turned;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = Tr::from_float(a[j]);
+        store_vec(y + at, o);
+      };
+      put(v1, w1, i1, pair);
+      if (i2 >= 0) put(v2, w2, i2, pair2);
     }
-    store_vec(y + i1, o1);
   }
 };
+// the pieces of a head
+constexpr int norm_pieces(int n, int head_dim, bool interleaved, int vec) {
+  return interleaved && vec > 1 ? (head_dim + 2 * vec - 1) / (2 * vec) : n / vec + (head_dim - 2 * n + 2 * vec - 1) / (2 * vec);
+}
 
 // The sum over 1 << shift neighbouring lanes, in all of them: quads and rows of 16 by moves along the row (mirrored once their halves
 // are even), then rows and halves of the wave exchanged.  (Through LDS, a trip for each step: 16384 x 20 x 256 100 us.)
@@ -165,7 +184,7 @@ struct Head {
 };
 
 struct Lanes {
-  int32_t per_head, shift, pieces, n;  // lanes of a head (1 << shift), its pieces, its pairs
+  int32_t per_head, shift, pieces, n, dim;  // lanes of a head (1 << shift), its pieces, its pairs, its elements
   float by_dim, eps;
 };
 
@@ -179,7 +198,7 @@ AITAMD_DEVICE void heads_of_workgroup(const Lanes& l, int count, bool one_weight
   typename Piece::vec w1 = {}, w2 = {};
   if (KIND == kNorm && one_weight && count > 0 && lane < l.pieces) {
     Piece at;
-    at.place(lane, l.n);
+    at.place(lane, l.n, l.dim);
     at.weigh(weight(0), w1, w2);
   }
   // (whole waves stay together: their lanes exchange sums)
@@ -191,7 +210,7 @@ AITAMD_DEVICE void heads_of_workgroup(const Lanes& l, int count, bool one_weight
       const int i = first + mine + a * at_once;
       h[a].x = nullptr;
       if (i < count && lane < l.pieces) head(i, h[a]);
-      piece[a].place(lane, l.n);
+      piece[a].place(lane, l.n, l.dim);
       if (h[a].x != nullptr) piece[a].load(h[a].x);
     }
 #pragma unroll
@@ -203,7 +222,7 @@ AITAMD_DEVICE void heads_of_workgroup(const Lanes& l, int count, bool one_weight
         if (!one_each && on) {
           for (int c = lane + l.per_head; c < l.pieces; c += l.per_head) {
             Piece more;
-            more.place(c, l.n);
+            more.place(c, l.n, l.dim);
             more.load(h[a].x);
             sum += more.template squares<float>();
           }
@@ -214,7 +233,7 @@ AITAMD_DEVICE void heads_of_workgroup(const Lanes& l, int count, bool one_weight
           double s = 0.0;
           for (int c = lane; on && c < l.pieces; c += l.per_head) {
             Piece again;
-            again.place(c, l.n);
+            again.place(c, l.n, l.dim);
             again.load(h[a].x);
             s += again.template squares<double>();
           }
@@ -235,7 +254,7 @@ AITAMD_DEVICE void heads_of_workgroup(const Lanes& l, int count, bool one_weight
       if (!one_each) {
         for (int c = lane + l.per_head; c < l.pieces; c += l.per_head) {
           Piece more;
-          more.place(c, l.n);
+          more.place(c, l.n, l.dim);
           more.load(h[a].x);
           put(more);
         }
@@ -262,11 +281,12 @@ struct NormParams {
 };
 
 constexpr int kNormAhead = 2;
-// waves of a SIMD (the widest pieces, of pairs of halves above all, have more to hold)
-constexpr int norm_waves(int vec, bool interleaved) { return vec < 8 ? 8 : (interleaved ? 6 : 5); }
+// Waves of a SIMD that the registers are shared out to, hardly any of them spilled (the widest pieces with four instead of five: a step
+// of eight prompts into the cache 54.8 us for 50.0)
+constexpr int norm_waves(int vec) { return vec < 8 ? 6 : 5; }
 
 template <class T, int VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRotaryThreads, norm_waves(VEC, INTERLEAVED)) norm_rotary_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kRotaryThreads, norm_waves(VEC)) norm_rotary_kernel(const NormParams p) {
   __shared__ float2 table[kRotaryTable];
   const int t0 = p.first + blockIdx.x * p.per_wg;
   const int tokens = p.tokens - t0 < p.per_wg ? p.tokens - t0 : p.per_wg;
@@ -313,7 +333,7 @@ constexpr int kAppendNormAhead = 2;
 
 // One launch for a layer's new tokens, as append_kernel (rotary_api.hip)
 template <class T, int VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRotaryThreads, norm_waves(VEC, INTERLEAVED)) append_norm_kernel(const AppendNormParams p) {
+__global__ void __launch_bounds__(kRotaryThreads, norm_waves(VEC)) append_norm_kernel(const AppendNormParams p) {
   __shared__ float2 table[kRotaryTable];
   __shared__ int64_t slot[kRotaryMaxTokens];  // among the sequence's own tokens
   __shared__ int32_t page[kRotaryMaxTokens];  // -1: nowhere to go
@@ -427,7 +447,8 @@ int check_norm(const char* who, int64_t head_dim, int64_t rotated, const float* 
 Lanes head_lanes(int64_t n, int64_t head_dim, bool interleaved, int vec, float eps) {
   Lanes l{};
   l.n = (int32_t)n;
-  l.pieces = rotary_pieces((int)n, (int)head_dim, interleaved, vec);
+  l.dim = (int32_t)head_dim;
+  l.pieces = norm_pieces((int)n, (int)head_dim, interleaved, vec);
   while ((1 << l.shift) < l.pieces && l.shift < 6) ++l.shift;
   l.per_head = 1 << l.shift;
   l.by_dim = 1.0f / (float)head_dim;
