@@ -153,8 +153,8 @@ struct IsRows<GemmTileRows<NW, NS, ELEM>> {
   static constexpr bool value = true;
 };
 
-// Workgroups of a shared tile that have no part of K, but the adapters
-constexpr int kLoraParts = IsLora<Epi>::value ? 1 : 0;
+// The most workgroups of a shared tile that have no part of K, but the adapters
+constexpr int kLoraParts = IsLora<Epi>::value ? kLoraMostParts : 0;
 
 // Workgroups per tile of a split-K launch (split_k_rule)
 template <class Tile>
@@ -248,9 +248,10 @@ hipError_t launch_kernel(const GemmParams& p_in, hipStream_t stream) {
     // tiles are shared along K only with enough scratch memory to hold the partial tiles; without it the
     // instance runs as its plain counterpart (one workgroup per tile, nothing written to the scratch memory)
     p.split_k = split_k_factor<Tile>(p, device_cus(dev));
-    if (p.ws == nullptr || p.ws_bytes < Tile::ws_bytes(total, p.split_k + kLoraParts) || total * (p.split_k + kLoraParts) > 0x7fffffffll)
+    const int lora_parts = kLoraParts > 0 ? lora_parts_of_tile(p.lora_rank) : 0;
+    if (p.ws == nullptr || p.ws_bytes < Tile::ws_bytes(total, p.split_k + lora_parts) || total * (p.split_k + lora_parts) > 0x7fffffffll)
       p.split_k = 1;
-    grid = dim3((unsigned)(total * (p.split_k > 1 ? p.split_k + kLoraParts : 1)), 1, 1);
+    grid = dim3((unsigned)(total * (p.split_k > 1 ? p.split_k + lora_parts : 1)), 1, 1);
   }
   if (grid.x > most_workgroups(Tile::NT)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(kernel, grid, dim3(Tile::NT), Tile::kLdsBytes, stream, p);

@@ -272,10 +272,10 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
   const int k_tiles_all = (k_main + BK - 1) / BK;
   // this workgroup's K-slabs [k_lo, k_lo + k_tiles)
   const int splits = Tile::SPLITK ? p.split_k : 1;
-  // (adapters: of tiles that are shared, one more workgroup has them and none of K)
+  // (adapters: of tiles that are shared, further workgroups have them and none of K)
   constexpr bool kLora = IsLora<Epi>::value;
-  const int parts = splits + (kLora && splits > 1 ? 1 : 0);
-  const bool lora_alone = kLora && Tile::SPLITK && split == splits;
+  const int parts = splits + (kLora && splits > 1 ? lora_parts_of_tile(p.lora_rank) : 0);
+  const bool lora_alone = kLora && Tile::SPLITK && split >= splits;
   const int k_lo = Tile::SPLITK ? (int)((int64_t)split * k_tiles_all / splits) : 0;
   const int k_tiles = lora_alone ? 0 : Tile::SPLITK ? (int)((int64_t)(split + 1) * k_tiles_all / splits) - k_lo : k_tiles_all;
 
@@ -382,12 +382,9 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
       }
     }
 
-    // the adapters of the wave's rows, likewise (tiles whose registers are all taken read one step's operands at a time)
-    constexpr int kLoraSteps = (MI + NI) * MT <= 128 && (Tile::OCC < 4 || MI * NI * ACC_N < 64) ? 2 : 1;
-    // adapters whose operands fit into the registers that the sums and the rows leave
-    constexpr int kLoraFree = 512 / Tile::OCC - MI * NI * ACC_N - kLoraSteps * MI * 4 - NI * ACC_N - 56;
-    constexpr int kLoraFit = kLoraFree / (kLoraSteps * NI * 4), kLoraAhead = kLoraFit < 1 ? 1 : (kLoraFit < 8 ? kLoraFit : 8);
-    LoraTile<std::conditional_t<kLora, T, bf16>, MT, MI, NI, kLoraSteps> lora;
+    // the adapters of the wave's rows, likewise
+    using Lora = LoraTile<std::conditional_t<kLora, T, bf16>, MT, MI, NI>;
+    Lora lora;
     if constexpr (kLora) lora.read(p, m0 + wm * Tile::WTM, lane);
 
     // dword K tail: the up to three dwords behind the last whole 16-byte piece of each of the lane's operand rows,
@@ -624,11 +621,24 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
         mfmas(ta, tb);
       }
     }
-    // low-rank adapters: behind K
+    // Low-rank adapters: behind K.  The adapters whose operands fit into the registers that the sums and the rows leave, of few ranks or of
+    // more: a column's ranks lie in one line, which is read once if they are read together (64 x 6144 x 4096, rank 64, 48 adapters at
+    // random: 57 us with two steps at a time).
     if constexpr (kLora) {
-      if (splits == 1 || lora_alone) lora.template add_own<kLoraAhead>(p, m0 + wm * Tile::WTM, n0 + wn * Tile::WTN, lane, acc);
+      constexpr auto fit = [](int steps) {
+        const int n = (512 / Tile::OCC - MI * NI * ACC_N - steps * (MI + (Lora::kHalves ? 2 * NI : 0)) * 4 - NI * ACC_N - 64) / (steps * NI * 4);
+        return n < 8 ? n : 8;
+      };
+      constexpr int kFew = (MI + NI) * MT <= 128 && fit(2) > 1 ? 2 : 1, kMore = MI * NI * ACC_N <= 32 && fit(4) > 0 ? 4 : kFew;
+      if (splits == 1 || lora_alone) {
+        const int row0 = m0 + wm * Tile::WTM, col0 = n0 + wn * Tile::WTN;
+        const int part_of = lora_alone ? split - splits : 0, others = lora_alone ? parts - splits - 1 : 0;
+        if (kMore == kFew || lora_chunks(p.lora_rank) <= kFew * Lora::PER)
+          lora.template add_own<kFew, (fit(kFew) > 1 ? fit(kFew) : 1)>(p, row0, col0, lane, part_of, others, acc);
+        else
+          lora.template add_own<kMore, (fit(kMore) > 1 ? fit(kMore) : 1)>(p, row0, col0, lane, part_of, others, acc);
+      }
     }
-
     if constexpr (Tile::SPLITK != 0) {
       // ---------------- split-K: partial tile to the scratch memory; the last workgroup of the tile sums ----
       // ws: int32 counter per (batch, tile) pair, padded to 4 KiB, then slot (pair * parts + split) of BM * BN

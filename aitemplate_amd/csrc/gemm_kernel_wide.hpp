@@ -490,9 +490,9 @@ __global__ void __launch_bounds__(Tile::NT, 1) gemm_rcr_wide_kernel(const GemmPa
       const GemmParams& q = arguments_anew<GemmParams>();
       int row0 = cur.m0 + wm * Tile::WTM, col0 = cur.n0 + wn * Tile::WTN, at_lane = lane;
       asm volatile("" : "+s"(row0), "+s"(col0), "+v"(at_lane));
-      LoraTile<std::conditional_t<IsLora<Epi>::value, T, bf16>, 16, MI, NI, 1> lora;
+      LoraTile<std::conditional_t<IsLora<Epi>::value, T, bf16>, 16, MI, NI> lora;
       lora.read(q, row0, at_lane);
-      lora.add(q, row0, col0, at_lane, [&](bf16x8 b, bf16x8 a, auto mi, auto ni) __attribute__((always_inline)) {
+      lora.template add<1>(q, row0, col0, at_lane, [&](bf16x8 b, bf16x8 a, auto mi, auto ni) __attribute__((always_inline)) {
         f32x4& c = acc[mi][ni];
         // (the operands may just have been written, by instructions that the compiler does not know to keep away from this one)
         asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(b), "v"(a));

@@ -20,6 +20,12 @@
 
 namespace aitamd {
 
+// The workgroups of a shared tile that have its adapters and none of K, a power of two of them: one alone takes longer than K where every
+// row has its own (64 x 6144 x 4096, 48 adapters at random, rank 16 / 64: 21.8 / 46 us with one workgroup, 18.6 / 36.8 so; with one
+// adapter for all rows 18.2 / 18.9 and 18.1 / 20.1).
+constexpr int kLoraMostParts = 4;
+constexpr int lora_parts_of_tile(int rank) { return rank > 32 ? kLoraMostParts : 2; }
+
 // a row's elements in scratch memory: chunks of eight ranks, two parts each
 constexpr int lora_chunks(int rank) { return (rank + 7) / 8; }
 AITAMD_DEVICE const bf16* lora_row(const GemmParams& p, int m) {
@@ -68,8 +74,8 @@ AITAMD_DEVICE u32x4 lora_largest(u32x4 v) {
   return v;
 }
 
-// The part of a wave whose rows row0 + mi * MT + (lane % MT) meet columns col0 + ni * MT + (lane % MT).  STEPS: matrix instructions' worth of ranks whose operands are on their way together.
-template <class T, int MT, int MI, int NI, int STEPS>
+// The part of a wave whose rows row0 + mi * MT + (lane % MT) meet columns col0 + ni * MT + (lane % MT).
+template <class T, int MT, int MI, int NI>
 struct LoraTile {
   // 16 x 16: a step's four quarters are both parts of t of two chunks (halves: both by both of one); 32 x 32: its two
   // halves are both parts of t of one chunk (halves: once with each of the adapter's)
@@ -93,6 +99,7 @@ struct LoraTile {
   }
   // the operands w of chunks c0 on, without what lies behind the last rank: the next column's first.  An odd rank shares its dword
   // with that (with the buffer's end, which takes whole dwords), and is read again by itself.
+  template <int STEPS>
   static AITAMD_DEVICE void last_ranks(int rank, int c0, int half, __amdgpu_buffer_rsrc_t rb, uint32_t b_at, u32x4 (&w)[STEPS][NI]) {
     if (8 * (c0 + STEPS * PER) <= rank) return;
     const uint32_t b_pitch = (uint32_t)rank * 2u;
@@ -108,10 +115,11 @@ struct LoraTile {
     });
   }
   // The products of every row with each adapter, of which a row takes those with its own: acc[mi][ni], whose elements are all of row
-  // lane % MT of block mi.  AHEAD adapters' operands are on their way together: where each row has its own, the time is that of the
-  // trips to memory.
-  template <int AHEAD, class Acc>
-  AITAMD_DEVICE void add_own(const GemmParams& p, int row0, int col0, int lane, Acc (&acc)[MI][NI]) const {
+  // lane % MT of block mi.  STEPS matrix instructions' worth of AHEAD adapters are on their way together: where each row has its own, the
+  // time is that of the trips to memory.
+  // Of the adapters in the order of their first rows, those whose numbers' bits `others` are `part_of`.
+  template <int STEPS, int AHEAD, class Acc>
+  AITAMD_DEVICE void add_own(const GemmParams& p, int row0, int col0, int lane, int part_of, int others, Acc (&acc)[MI][NI]) const {
     using Op = MfmaOp<bf16, MT>;
     const int fr = lane % MT, fq = lane / MT;
     const int rank = p.lora_rank, chunks = lora_chunks(rank);
@@ -135,13 +143,15 @@ struct LoraTile {
           t[s][mi] = buffer_load_16B(rt, c0 + s * PER + half < chunks ? tc : kOobOffset);
         });
       });
-      for (;;) {
+      for (int number = 0;;) {
         int id[AHEAD];
         u32x4 w[AHEAD][STEPS][NI];
         static_for<0, AHEAD>([&](auto i) __attribute__((always_inline)) {
-          id[i] = first_of(left);
+          do {
+            id[i] = first_of(left);
+            static_for<0, MI>([&](auto mi) __attribute__((always_inline)) { left[mi] = left[mi] == id[i] ? -1 : left[mi]; });
+          } while (id[i] >= 0 && (number++ & others) != part_of);
           if (id[i] < 0) return;
-          static_for<0, MI>([&](auto mi) __attribute__((always_inline)) { left[mi] = left[mi] == id[i] ? -1 : left[mi]; });
           const __amdgpu_buffer_rsrc_t rb = make_rsrc(lora_column<T>(p, id[i], col0), (uint32_t)columns * b_pitch);
           static_for<0, STEPS>([&](auto s) __attribute__((always_inline)) {
             const uint32_t bc = b_at + (uint32_t)(c0 + s * PER) * 16u;
@@ -188,7 +198,7 @@ struct LoraTile {
   // ... for accumulators that matrix instructions alone may touch: each adapter with the rows of the others set to zero.
   // multiply(b, a, mi, ni): accumulator (mi, ni) plus the product of the weight rows b and the rows a, both bf16x8.  Through
   // buffers that end with the rows and the columns: 32-bit offsets, and no branch around what is not there.
-  template <class M>
+  template <int STEPS, class M>
   AITAMD_DEVICE void add(const GemmParams& p, int row0, int col0, int lane, M&& multiply) const {
     const int fr = lane % MT, fq = lane / MT;
     const int rank = p.lora_rank, chunks = lora_chunks(rank);

@@ -6,7 +6,7 @@
 // what they have in registers.  A workgroup goes through its tokens' queries, then their keys (and values), so that a lane's weights
 // are read once for all heads.
 // Bound: memory, 4 bytes an element, as the rotation alone.  16384 x 20 x 256 in fp16, 335 MB: 69 us with half of each head turned
-// (neighbours; 72 halves), 4.9 TB/s, a copy's rate; with all of it turned 82, of which the sines are some 10.  16384 x 40 x 128 in bf16 71.
+// (neighbours; 72 halves), 4.9 TB/s, a copy's rate; with all of it turned, twice the sines, 82.  16384 x 40 x 128 in bf16 71.
 #include "../../include/aitemplate_amd_kernels.h"
 #include "device.hpp"
 #include "errors.hpp"
