@@ -34,8 +34,8 @@ class gemm_rcr_lora(Operator):
             raise RuntimeError(f"A/B shape mismatch! A: {shape}, B: {w_shape}")
         if not isinstance(w_shape[0], IntImm) or not isinstance(w_shape[1], IntImm):
             raise RuntimeError("gemm_rcr_lora: N and K must be static")
-        if len(a_shape) != 3 or a_shape[2] != w_shape[1] or not isinstance(a_shape[1], IntImm) or a_shape[1].value() < 1:
-            raise RuntimeError("gemm_rcr_lora: lora_a must be [adapters, rank, K] with a static rank")
+        if len(a_shape) != 3 or a_shape[2] != w_shape[1] or not isinstance(a_shape[1], IntImm) or not 1 <= a_shape[1].value() <= 1024:
+            raise RuntimeError("gemm_rcr_lora: lora_a must be [adapters, rank, K] with a static rank of 1 to 1024")
         if list(b_shape) != [a_shape[0], w_shape[0], a_shape[1]]:
             raise RuntimeError("gemm_rcr_lora: lora_b must be [adapters, N, rank]")
         if list(adapters._attrs["shape"]) != list(shape[:-1]):

@@ -22,7 +22,7 @@ class token_logprobs(Operator):
         self._attrs["scale"] = float(scale)
         if not 0 <= self._attrs["top"] <= MOST_TOP:
             raise RuntimeError(f"token_logprobs: top {top}: 0 to {MOST_TOP}")
-        if not 0.0 < self._attrs["scale"] < float("inf"):
+        if not 0.0 < self._attrs["scale"] < 2e38:  # (its product with log2(e) is a number of 32 bits too)
             raise RuntimeError(f"token_logprobs: scale {scale} is no positive number")
 
     def __call__(self, logits: Tensor, tokens: Tensor) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:

@@ -484,7 +484,8 @@ extern "C" int aitamd_token_logprobs(int dtype, const void* logits, const void* 
   if (rows < 0 || vocabulary < 0) return fail("%s: negative dimension", who);
   if (top < 0 || top > kMostTop || top > vocabulary)
     return fail("%s: top %lld: up to %d, and not more than there are tokens (%lld)", who, (long long)top, kMostTop, (long long)vocabulary);
-  if (!(scale > 0.0f) || !__builtin_isfinite(scale)) return fail("%s: scale %g is no positive number", who, (double)scale);
+  // (its product with log2(e) is finite too)
+  if (!(scale > 0.0f) || !__builtin_isfinite(scale * kLog2e)) return fail("%s: scale %g is no positive number of the range", who, (double)scale);
   if (rows > 0x7fffffffll / kMostSplits || vocabulary > 0x7fffffffll - 2 * kRound) return fail("%s: dimension too large", who);
   if (rows == 0) return 0;
   if (vocabulary == 0) return fail("%s: no tokens", who);

@@ -132,6 +132,18 @@ def test_token_logprobs_refusals():
     assert logprobs(rows=0, logits=None) == 0
 
 
+def test_ranges_ends():
+    """A scale whose product with log2(e) is beyond 32 bits; ranks from 1025 on."""
+    refused(logprobs(scale=3e38), "scale")
+    with pytest.raises(RuntimeError):
+        ops.token_logprobs(scale=3e38)
+    m, n = IntVar(values=[1, 64], name="m"), IntVar(values=[1, 9], name="n")
+    x, w, of = tensor("x", [m, 256]), tensor("w", [96, 256]), tensor("of", [m], "int32")
+    ops.gemm_rcr_lora()(x, w, tensor("a", [n, 1024, 256]), tensor("b", [n, 96, 1024]), of)
+    with pytest.raises(RuntimeError):
+        ops.gemm_rcr_lora()(x, w, tensor("a", [n, 1025, 256]), tensor("b", [n, 96, 1025]), of)
+
+
 def test_eager_calls_take_gpu_tensors_only():
     x = torch.zeros(2, 4, 64, dtype=torch.float16)
     with pytest.raises(ValueError, match="GPU"):
