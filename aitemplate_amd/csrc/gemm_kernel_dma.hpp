@@ -623,13 +623,14 @@ __global__ void __launch_bounds__(Tile::NT, Tile::OCC) gemm_rcr_dma_kernel(const
     }
     // Low-rank adapters: behind K.  The adapters whose operands fit into the registers that the sums and the rows leave, of few ranks or of
     // more: a column's ranks lie in one line, which is read once if they are read together (64 x 6144 x 4096, rank 64, 48 adapters at
-    // random: 57 us with two steps at a time).
+    // random, one workgroup for them: 57 us with two steps at a time, 46 with four).  Tiles of more than 16 sums a lane have no
+    // registers for four.
     if constexpr (kLora) {
       constexpr auto fit = [](int steps) {
         const int n = (512 / Tile::OCC - MI * NI * ACC_N - steps * (MI + (Lora::kHalves ? 2 * NI : 0)) * 4 - NI * ACC_N - 64) / (steps * NI * 4);
         return n < 8 ? n : 8;
       };
-      constexpr int kFew = (MI + NI) * MT <= 128 && fit(2) > 1 ? 2 : 1, kMore = MI * NI * ACC_N <= 32 && fit(4) > 0 ? 4 : kFew;
+      constexpr int kFew = (MI + NI) * MT <= 128 && fit(2) > 1 ? 2 : 1, kMore = MI * NI * ACC_N <= 16 && fit(4) > 0 ? 4 : kFew;
       if (splits == 1 || lora_alone) {
         const int row0 = m0 + wm * Tile::WTM, col0 = n0 + wn * Tile::WTN;
         const int part_of = lora_alone ? split - splits : 0, others = lora_alone ? parts - splits - 1 : 0;
