@@ -174,3 +174,26 @@ def test_refusals():
         eager.gemm_rcr_lora(**args, workspace=torch.empty(64, dtype=torch.uint8, device=DEV))
     with pytest.raises(RuntimeError, match="range"):
         eager.gemm_rcr_lora(**args, algo=999)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rank", [1, 8, 31, 33, 64, 65, 130])
+@pytest.mark.parametrize("M,N,K", [(64, 1536, 4096), (29, 2056, 2272), (200, 512, 2048), (129, 300, 4100)])
+def test_tiles_that_share_k(dtype, M, N, K, rank):
+    """Few tiles with a long K, whose adapters are split among workgroups: almost every row with its own, or all with one."""
+    args = make(dtype, M, N, K, rank, 50, seed=rank)
+    check(eager.gemm_rcr_lora(**args), args)
+    args["adapters"].fill_(49)
+    check(eager.gemm_rcr_lora(**args), args)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("M", [7, 64, 700, 2100])
+def test_a_row_that_is_no_numbers_is_alone(dtype, M):
+    args = make(dtype, M, 1024, 512, 16, 6, seed=M)
+    want = eager.gemm_rcr_lora(**args)
+    args["x"][M // 2, 5], args["x"][M - 1, 500] = float("nan"), float("inf")
+    got = eager.gemm_rcr_lora(**args)
+    others = torch.ones(M, dtype=torch.bool, device=DEV)
+    others[M // 2] = others[M - 1] = False
+    assert torch.equal(got[others], want[others]) and not torch.isfinite(got[~others]).any()
