@@ -143,8 +143,10 @@ __global__ void __launch_bounds__(kRowThreads) low_rows_kernel(const LowParams p
     if (lane == r) put_low(p.t + (int64_t)m * padded * 2, j0 + r, v[r]);
 }
 
-// Rows of prompts, neighbours of one adapter mostly: ROWS of them and NR x 16 ranks a workgroup.  Several adapters among the rows: one
-// after the other; more than kLoraFew: row by row.
+// Rows of prompts, neighbours of one adapter mostly: ROWS of them and NR x 16 ranks a workgroup.  Several adapters among the rows:
+// where the grid is kLoraFew deep, each by a workgroup of its own (8192 x 4096, rank 64, tiles with two: 38 us one after the other, 31
+// so), which leaves at once where there is none for it; more than kLoraFew: row by row, by all of them (2048 x 4096, rank 16, 48 at
+// random: 168 us by one, 50 by four).
 constexpr int kLoraFew = 4;
 struct LowTile {
   int mine, left, distinct;  // the lane's row's adapter, that or -1, how many there are among the rows
@@ -154,7 +156,8 @@ struct LowTile {
   }
   AITAMD_DEVICE void drop(int id) { left = left == id ? -1 : left; }
 };
-// Zeros where there is no adapter, and all rows where there are many adapters; false if that was all.  of: the rows' adapters, in LDS.
+// Zeros where there is no adapter, and all rows where there are many adapters; false if that was all for this workgroup.  of: the rows'
+// adapters, in LDS.
 template <class T, int THREADS>
 AITAMD_DEVICE bool low_begin(const LowParams& p, LowTile& l, int* of, int m0, int rows, int j0, int ranks, int padded) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -164,8 +167,10 @@ AITAMD_DEVICE bool low_begin(const LowParams& p, LowTile& l, int* of, int m0, in
   l.distinct = 0;
   for (int id = l.first(); id >= 0 && l.distinct <= kLoraFew; id = l.first(), ++l.distinct) l.drop(id);
   l.left = l.mine;
+  const int turn = blockIdx.z, turns = gridDim.z;
+  if (turn != 0 && l.distinct <= kLoraFew) return l.distinct > turn;
   bf16* const t = p.t + ((int64_t)m0 * padded + j0) * 2;
-  if (__builtin_amdgcn_ballot_w64(lane < rows && l.mine < 0) != 0) {
+  if (turn == 0 && __builtin_amdgcn_ballot_w64(lane < rows && l.mine < 0) != 0) {
     __syncthreads();
     const int chunks = ranks / 8;
     for (int i = tid; i < rows * chunks; i += THREADS) {
@@ -179,7 +184,7 @@ AITAMD_DEVICE bool low_begin(const LowParams& p, LowTile& l, int* of, int m0, in
   }
   if (l.distinct <= kLoraFew) return l.distinct > 0;
   // four ranks of a row at a time (those from p.rank on: of the last one, and zeros)
-  for (int i = wave; i < rows * (ranks / 4); i += THREADS / 64) {
+  for (int i = wave + turn * (THREADS / 64); i < rows * (ranks / 4); i += turns * (THREADS / 64)) {
     const int r = i / (ranks / 4), j = j0 + (i - r * (ranks / 4)) * 4;
     const int id = __builtin_amdgcn_readlane(l.mine, r);
     if (id < 0) continue;
@@ -231,12 +236,13 @@ AITAMD_DEVICE void low_end(const LowParams& p, const float* part, const int* of,
 template <class T, int NR_, int MB_>
 struct LowRing {
   static constexpr int NR = NR_, MB = MB_;
-  static constexpr int ROWS = 16 * MB, RANKS = 16 * NR, WAVES = 4, NS = 6, BK = 128;
+  static constexpr int ROWS = 16 * MB, RANKS = 16 * NR, WAVES = 4, BK = 128;
   static constexpr int LOADS = (ROWS + RANKS) / 4 / WAVES;  // of a wave for a slab, four rows each
   static constexpr int STAGE = (ROWS + RANKS) * BK;         // elements
+  static constexpr int NS = 78 * 1024 / (STAGE * 2) < 6 ? 78 * 1024 / (STAGE * 2) : 6;  // (two workgroups a CU)
   static constexpr int PITCH = RANKS + 4;
   static constexpr int kLdsBytes = NS * STAGE * 2;
-  static_assert((ROWS + RANKS) % (4 * WAVES) == 0 && WAVES * ROWS * PITCH * 4 <= kLdsBytes && kLdsBytes + ROWS * 4 <= 160 * 1024);
+  static_assert((ROWS + RANKS) % (4 * WAVES) == 0 && WAVES * ROWS * PITCH * 4 <= kLdsBytes && kLdsBytes + ROWS * 4 <= 80 * 1024);
 };
 template <class T, class R>
 __global__ void __launch_bounds__(R::WAVES * 64) low_ring_kernel(const LowParams p) {
@@ -266,9 +272,13 @@ __global__ void __launch_bounds__(R::WAVES * 64) low_ring_kernel(const LowParams
     at_k[i] = ((lane & 15) ^ (row & 15)) * 8;
     off[i] = (uint32_t)(of_x ? row * (int)p.ldx : (row - R::ROWS) * p.K) * 2u + (uint32_t)at_k[i] * 2u;
   }
-  for (;;) {
+  for (int turn = 0;; ++turn) {
     const int id = l.first();
     if (id < 0) break;
+    if (turn != (int)blockIdx.z) {
+      l.drop(id);
+      continue;
+    }
     const int there = p.rank - j0 < R::RANKS ? p.rank - j0 : R::RANKS;
     const __amdgpu_buffer_rsrc_t ra = make_rsrc(reinterpret_cast<const T*>(p.a) + ((int64_t)id * p.rank + j0) * p.K, (uint32_t)(there > 0 ? there : 0) * (uint32_t)p.K * 2u);
     auto issue = [&](int kt) __attribute__((always_inline)) {
@@ -406,11 +416,11 @@ __global__ void __launch_bounds__(kTileWaves * 64) low_tile_kernel(const LowPara
 }
 
 // tiles of `tile_rows` rows by `groups` groups of ranks, in as many launches as it takes
-hipError_t launch_tiles(void (*kernel)(const LowParams), LowParams p, int tile_rows, int64_t groups, int threads, int lds, hipStream_t stream) {
-  const int64_t tiles = ((int64_t)p.M + tile_rows - 1) / tile_rows, most = most_workgroups(threads) / groups;
+hipError_t launch_tiles(void (*kernel)(const LowParams), LowParams p, int tile_rows, int64_t groups, int turns, int threads, int lds, hipStream_t stream) {
+  const int64_t tiles = ((int64_t)p.M + tile_rows - 1) / tile_rows, most = most_workgroups(threads) / (groups * turns);
   for (int64_t at = 0; at < tiles; at += most) {
     p.first = (int32_t)(at * tile_rows);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles - at < most ? tiles - at : most), (unsigned)groups), dim3(threads), lds, stream, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles - at < most ? tiles - at : most), (unsigned)groups, (unsigned)turns), dim3(threads), lds, stream, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -431,7 +441,7 @@ hipError_t launch_ring(const LowParams& p, int64_t groups, hipStream_t stream) {
     errors[dev % kMaxDevices] = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, R::kLdsBytes);
   });
   if (errors[dev % kMaxDevices] != hipSuccess) return errors[dev % kMaxDevices];
-  return launch_tiles(kernel, p, R::ROWS, groups, R::WAVES * 64, R::kLdsBytes, stream);
+  return launch_tiles(kernel, p, R::ROWS, groups, kLoraFew, R::WAVES * 64, R::kLdsBytes, stream);
 }
 template <class T, int NR>
 hipError_t launch_ring(const LowParams& p, int64_t groups, int cus, hipStream_t stream) {
@@ -445,7 +455,7 @@ hipError_t launch_low(LowParams p, hipStream_t stream) {
   // A row by itself reads its whole adapter, from L2 mostly; a tile reads x once and an adapter once for its rows, and takes them one
   // by one where they have many adapters.  By themselves up to twice the waves that the chip holds at once, two ranks each then.  Of
   // rank 16, K = 4096, with one adapter / sixteen requests' rows in turn / 48 adapters at random: 1024 rows 15, 16 and 16 us by
-  // themselves, 9, 15 and 170 in tiles; 2048 rows 25, 25 and 24 by themselves, a tile's 9 to 16 with the first two.
+  // themselves, 9 and 15 in tiles with the first two; 2048 rows 25, 25 and 24 by themselves, 12, 10 and 50 in tiles.
   const int64_t waves = (int64_t)p.M * padded;
   constexpr int64_t kAtOnce = 8192;
   if (waves <= 2 * kAtOnce) {
@@ -462,7 +472,7 @@ hipError_t launch_low(LowParams p, hipStream_t stream) {
     return nr == 4 ? launch_ring<T, 4>(p, groups, cus, stream) : (nr == 2 ? launch_ring<T, 2>(p, groups, cus, stream) : launch_ring<T, 1>(p, groups, cus, stream));
   }
   auto kernel = nr == 4 ? low_tile_kernel<T, 4> : (nr == 2 ? low_tile_kernel<T, 2> : low_tile_kernel<T, 1>);
-  return launch_tiles(kernel, p, kTileRows, groups, kTileWaves * 64, 0, stream);
+  return launch_tiles(kernel, p, kTileRows, groups, 1, kTileWaves * 64, 0, stream);
 }
 
 constexpr int64_t kMostRank = 1024;
